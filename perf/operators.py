@@ -17,9 +17,6 @@ import torch
 
 own = False
 
-if own:
-    from picotron_amd import decoder_ops
-
 DTYPES = {"bf16": torch.bfloat16, "fp32": torch.float32}
 NORM_EPS = 1e-5
 ROPE_BASE = 500000.0
@@ -199,6 +196,8 @@ def run(state):
 
 
 def _own(state):
+    from picotron_amd import decoder_ops
+
     case = state["case"]
     if case["op"] == "embedding":
         outs = [decoder_ops.embedding(state["ids"], state["weight"], scale=case["scale"], padding_idx=case["padding"] if case["padding"] >= 0 else None)]
