@@ -30,7 +30,7 @@ extern "C" {
 #define PICOMOE_F32 0
 #define PICOMOE_BF16 1
 
-#define PICOMOE_ABI_VERSION 6
+#define PICOMOE_ABI_VERSION 7
 
 /* ABI version of the loaded library (compare with PICOMOE_ABI_VERSION). */
 int picomoe_abi_version(void);
@@ -222,6 +222,65 @@ int picomoe_ffn_kernel_family(int dtype, int64_t hidden, int64_t inter);
  * are addressed in place).  Empty experts get zeros. */
 int picomoe_ffn_wgrad(const void* lhs, int64_t ld_lhs, const void* rhs, int64_t ld_rhs, const int64_t* counts,
                       int num_experts, int64_t n_rows, int64_t p_dim, int64_t q_dim, int dtype, void* out, void* stream);
+
+/* ---- The decoder in front of the MoE layer ----------------------------------------------------------------
+ * Embedding: the reference's lookup picotron/model.py:343-360 (F.embedding) with a scale, and its gradient.
+ * out[t] = scale * weight[ids[t]] (an id outside [0, vocab): a row of NaN).  d_weight[v] = scale * the sum of d_out[t] over
+ * the tokens with ids[t] = v, in token order, in fp32, rounded once; rows that no token names, and row padding_idx
+ * (negative: none), are zeros; ids outside [0, vocab) are left out.  weight and d_weight [vocab, hidden], ids [n_tokens],
+ * out and d_out [n_tokens, hidden]; n_tokens and vocab below 2^31, hidden at most 2^20.  The backward call sorts the tokens in
+ * `workspace` (16-byte aligned, picomoe_embedding_bwd_workspace_bytes(...) bytes; -1 = bad arguments). */
+int picomoe_embedding_fwd(const void* weight, int dtype, int64_t vocab, int64_t hidden, const int64_t* ids, int64_t n_tokens,
+                          float scale, void* out, void* stream);
+int64_t picomoe_embedding_bwd_workspace_bytes(int dtype, int64_t n_tokens, int64_t vocab, int64_t hidden);
+int picomoe_embedding_bwd(const void* d_out, int dtype, const int64_t* ids, int64_t n_tokens, int64_t vocab, int64_t hidden,
+                          float scale, int64_t padding_idx, void* d_weight, void* workspace, int64_t workspace_bytes,
+                          void* stream);
+
+/* RMS norm of each query and key head and the rotate-half position rotation of picotron/model.py:29-36, one pass over both.
+ * q [batch, seq, q_heads, head_dim] and k [batch, seq, k_heads, head_dim] with element strides {batch, seq, head} (host
+ * arrays of three; last dimension dense); q_out and k_out dense, of the same shapes.  Per head row, in fp32, rounded once:
+ * y = x * rsqrt(mean(x^2) + eps) * weight (weight [head_dim] NULL: y = x), out = y * cos + rotate_half(y) * sin with the rows of
+ * cos and sin [n_positions, head_dim] (fp32) that positions [batch, seq] names (NULL: the token's index in its sequence); a
+ * position outside [0, n_positions) gives NaN.  The backward call recomputes the norm from q and k; dq_weight / dk_weight (NULL:
+ * not wanted; they need their weight and the workspace) are summed over all rows in a fixed order.  head_dim a multiple of 8,
+ * at most 256; strides multiples of 4 elements; q, k and weights aligned to 4 elements, everything else to 16 bytes. */
+int picomoe_qk_norm_rope_fwd(const void* q, const int64_t* q_strides, int q_heads, const void* k, const int64_t* k_strides,
+                             int k_heads, int dtype, int64_t batch, int64_t seq, int head_dim, const void* q_weight,
+                             const void* k_weight, float eps, const float* cos, const float* sin, int64_t n_positions,
+                             const int64_t* positions, void* q_out, void* k_out, void* stream);
+int64_t picomoe_qk_norm_rope_bwd_workspace_bytes(int dtype, int64_t batch, int64_t seq, int q_heads, int k_heads, int head_dim);
+int picomoe_qk_norm_rope_bwd(const void* dq_out, const void* dk_out, const void* q, const int64_t* q_strides, int q_heads,
+                             const void* k, const int64_t* k_strides, int k_heads, int dtype, int64_t batch, int64_t seq,
+                             int head_dim, const void* q_weight, const void* k_weight, float eps, const float* cos,
+                             const float* sin, int64_t n_positions, const int64_t* positions, void* dq, void* dk,
+                             void* dq_weight, void* dk_weight, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Attention of picotron/model.py:199-233 (softmax(q k^T / sqrt(d)) v over grouped heads, causal), with capped scores, a distance
+ * bias and document, prefix and window masks.  q [batch, q_len, q_heads, head_dim], k and v [batch, kv_len, kv_heads, head_dim]
+ * with element strides {batch, seq, head}; out dense like q; lse [batch, q_heads, q_len] fp32.  Query s stands at position
+ * p = s + kv_len - q_len and head h reads key head h / (q_heads / kv_heads).  Scores: x = scale * q . k; with softcap > 0
+ * softcap * tanh(x / softcap); with slopes [q_heads] (fp32) minus slopes[h] * |p - j|.  Key j is seen when: causal == 0 or
+ * j <= p or j < prefix_lengths[batch] (needs causal); window == 0 or |p - j| < window; document_ids [batch, kv_len] is NULL or
+ * document_ids[j] == document_ids[p] >= 0.  A query that sees nothing gets out 0 and lse -inf, and no gradient; what is not seen has no influence,
+ * NaN and infinities included.  The backward call takes the forward's out and lse; d_out, dq, dk, dv are dense.  head_dim a multiple
+ * of 8, at most 256; strides multiples of 16 bytes, pointers 16-byte aligned; lengths at most 2^28, q_len * q_heads / kv_heads at
+ * most 2^30.  Workspaces: 16-byte aligned, of the size that the _workspace_bytes call gives (-1 = bad arguments). */
+int64_t picomoe_attention_fwd_workspace_bytes(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, int kv_heads,
+                                              int head_dim);
+int picomoe_attention_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                          const int64_t* v_strides, int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads,
+                          int kv_heads, int head_dim, float scale, float softcap, int causal, int64_t window,
+                          const float* slopes, const int32_t* document_ids, const int32_t* prefix_lengths, void* out, float* lse,
+                          void* workspace, int64_t workspace_bytes, void* stream);
+int64_t picomoe_attention_bwd_workspace_bytes(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, int kv_heads,
+                                              int head_dim);
+int picomoe_attention_bwd(const void* d_out, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                          const void* v, const int64_t* v_strides, const void* out, const float* lse, int dtype, int64_t batch,
+                          int64_t q_len, int64_t kv_len, int q_heads, int kv_heads, int head_dim, float scale, float softcap,
+                          int causal, int64_t window, const float* slopes, const int32_t* document_ids,
+                          const int32_t* prefix_lengths, void* dq, void* dk, void* dv, void* workspace, int64_t workspace_bytes,
+                          void* stream);
 
 /* ---- Diagnostics -----------------------------------------------------------------------------------------
  * No counterpart in the reference and not part of the MoE path: a loop of nothing but MFMAs, to measure what the matrix

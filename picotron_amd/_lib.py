@@ -12,7 +12,7 @@ import torch
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG_DIR, "libpicomoe.so")
 HEADER_PATH = os.path.join(os.path.dirname(_PKG_DIR), "include", "picomoe.h")
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 F32, BF16 = 0, 1
 _DTYPE_CODE = {torch.float32: F32, torch.bfloat16: BF16}
@@ -49,12 +49,27 @@ _SIGNATURES = {
     "picomoe_ffn_workspace_bytes": [],
     "picomoe_ffn_kernel_family": [_i32, _i64, _i64],
     "picomoe_ffn_wgrad": [_p, _i64, _p, _i64, _p, _i32, _i64, _i64, _i64, _i32, _p, _p],
+    "picomoe_embedding_fwd": [_p, _i32, _i64, _i64, _p, _i64, _f32, _p, _p],
+    "picomoe_embedding_bwd_workspace_bytes": [_i32, _i64, _i64, _i64],
+    "picomoe_embedding_bwd": [_p, _i32, _p, _i64, _i64, _i64, _f32, _i64, _p, _p, _i64, _p],
+    "picomoe_qk_norm_rope_fwd": [_p, _p, _i32, _p, _p, _i32, _i32, _i64, _i64, _i32, _p, _p, _f32, _p, _p, _i64, _p, _p, _p, _p],
+    "picomoe_qk_norm_rope_bwd_workspace_bytes": [_i32, _i64, _i64, _i32, _i32, _i32],
+    "picomoe_qk_norm_rope_bwd": [_p, _p, _p, _p, _i32, _p, _p, _i32, _i32, _i64, _i64, _i32, _p, _p, _f32, _p, _p, _i64, _p, _p, _p, _p, _p, _p,
+                                 _i64, _p],
+    "picomoe_attention_fwd_workspace_bytes": [_i32, _i64, _i64, _i64, _i32, _i32, _i32],
+    "picomoe_attention_fwd": [_p, _p, _p, _p, _p, _p, _i32, _i64, _i64, _i64, _i32, _i32, _i32, _f32, _f32, _i32, _i64, _p, _p, _p, _p, _p, _p,
+                              _i64, _p],
+    "picomoe_attention_bwd_workspace_bytes": [_i32, _i64, _i64, _i64, _i32, _i32, _i32],
+    "picomoe_attention_bwd": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i32, _i64, _i64, _i64, _i32, _i32, _i32, _f32, _f32, _i32, _i64, _p, _p, _p,
+                              _p, _p, _p, _p, _i64, _p],
     "picomoe_diag_mfma_loop_flop": [_i32, _i64, _i32],
     "picomoe_diag_mfma_loop": [_p, _i64, _i32, _i64, _i64, _i64, _i32, _p, _p],
 }
 _RESTYPES = {"picomoe_error_string": ctypes.c_char_p, "picomoe_permute_workspace_bytes": ctypes.c_int64,
              "picomoe_permute_plan_static_max_bytes": ctypes.c_int64,
-             "picomoe_ffn_workspace_bytes": ctypes.c_int64, "picomoe_gate_bwd_workspace_bytes": ctypes.c_int64, "picomoe_diag_mfma_loop_flop": ctypes.c_int64}
+             "picomoe_ffn_workspace_bytes": ctypes.c_int64, "picomoe_gate_bwd_workspace_bytes": ctypes.c_int64, "picomoe_diag_mfma_loop_flop": ctypes.c_int64,
+             "picomoe_embedding_bwd_workspace_bytes": ctypes.c_int64, "picomoe_qk_norm_rope_bwd_workspace_bytes": ctypes.c_int64,
+             "picomoe_attention_fwd_workspace_bytes": ctypes.c_int64, "picomoe_attention_bwd_workspace_bytes": ctypes.c_int64}
 
 _lib = None
 

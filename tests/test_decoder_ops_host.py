@@ -1,0 +1,110 @@
+"""Arguments of the decoder's operators that are refused before anything reaches the GPU: through the C ABI with pointers that are
+never dereferenced on the host, and through the Python wrappers with CPU tensors."""
+
+import ctypes
+import types
+
+import pytest
+import torch
+
+from picotron_amd import _lib, decoder_ops
+
+P = ctypes.c_void_p(64)          # never dereferenced: these calls return before any launch
+ODD = ctypes.c_void_p(72)        # off the 16-byte grid
+STRIDES = (ctypes.c_int64 * 3)(4 * 4 * 64, 4 * 64, 64)
+ODD_STRIDES = (ctypes.c_int64 * 3)(4 * 4 * 64, 4 * 64 + 2, 64)
+
+
+def test_embedding_arguments():
+    lib = _lib.load()
+    assert lib.picomoe_embedding_fwd(P, 7, 10, 64, P, 4, 1.0, P, None) == 1           # dtype
+    assert lib.picomoe_embedding_fwd(P, 1, 0, 64, P, 4, 1.0, P, None) == 1            # empty table
+    assert lib.picomoe_embedding_fwd(P, 1, 1 << 31, 64, P, 4, 1.0, P, None) == 1      # table rows beyond 31 bits
+    assert lib.picomoe_embedding_fwd(P, 1, 10, (1 << 20) + 1, P, 4, 1.0, P, None) == 1
+    assert lib.picomoe_embedding_fwd(None, 1, 10, 64, P, 4, 1.0, P, None) == 1
+    assert lib.picomoe_embedding_fwd(None, 1, 10, 64, None, 0, 1.0, None, None) == 0  # no tokens
+    need = lib.picomoe_embedding_bwd_workspace_bytes(1, 5000, 100, 64)
+    # two buffers of keys and of tokens, two blocks' digit counts, two partial rows for each of 79 pieces
+    assert need == 4 * 20000 + 2 * 512 * 4 + 79 * 2 * 64 * 4
+    assert lib.picomoe_embedding_bwd_workspace_bytes(1, -1, 100, 64) == -1
+    assert lib.picomoe_embedding_bwd_workspace_bytes(1, 1 << 31, 100, 64) == -1
+    assert lib.picomoe_embedding_bwd(P, 1, P, 5000, 100, 64, 1.0, -1, P, P, need - 1, None) == 1   # workspace too small
+    assert lib.picomoe_embedding_bwd(P, 1, P, 5000, 100, 64, 1.0, -1, P, ODD, need, None) == 1
+    assert lib.picomoe_embedding_bwd(P, 1, P, 5000, 100, 64, 1.0, -1, None, P, need, None) == 1
+    assert lib.picomoe_embedding_bwd(None, 1, P, 5000, 100, 64, 1.0, -1, P, P, need, None) == 1
+
+
+def test_norm_rope_arguments():
+    lib = _lib.load()
+
+    def fwd(q=P, qs=STRIDES, heads=4, dtype=1, batch=2, seq=4, D=64, weight=None, cos=P, k=P):
+        return lib.picomoe_qk_norm_rope_fwd(q, qs, heads, k, STRIDES, 4, dtype, batch, seq, D, weight, None, 1e-5, cos, P, 8, None, P, P, None)
+
+    assert fwd(batch=0) == 0 and fwd(seq=0) == 0
+    for bad in (dict(q=None), dict(qs=None), dict(qs=ODD_STRIDES), dict(heads=0), dict(heads=5000), dict(dtype=3), dict(batch=-1), dict(D=60), dict(D=264),
+                dict(D=0), dict(cos=None), dict(cos=ODD), dict(q=ctypes.c_void_p(66)), dict(weight=ctypes.c_void_p(66)), dict(batch=1 << 16, seq=1 << 16)):
+        assert fwd(**bad) == 1, bad
+    assert lib.picomoe_qk_norm_rope_bwd_workspace_bytes(1, 2, 4, 4, 4, 60) == -1
+    need = lib.picomoe_qk_norm_rope_bwd_workspace_bytes(1, 2, 4, 4, 4, 64)
+    assert need > 0
+
+    def bwd(dq_out=P, qw=P, dqw=P, ws=P, size=need):
+        return lib.picomoe_qk_norm_rope_bwd(dq_out, P, P, STRIDES, 4, P, STRIDES, 4, 1, 2, 4, 64, qw, P, 1e-5, P, P, 8, None, P, P, dqw, None, ws, size, None)
+
+    for bad in (dict(dq_out=None), dict(dq_out=ODD), dict(qw=None), dict(ws=None), dict(size=need - 1)):
+        assert bwd(**bad) == 1, bad
+
+
+def test_attention_arguments():
+    lib = _lib.load()
+
+    def fwd(q=P, qs=STRIDES, ks=STRIDES, dtype=1, batch=2, q_len=4, kv_len=4, heads=4, kv_heads=4, D=64, scale=0.1, softcap=0.0, causal=1, window=0, prefix=None,
+            out=P, lse=P, ws=P, size=1 << 40):
+        return lib.picomoe_attention_fwd(q, qs, P, ks, P, STRIDES, dtype, batch, q_len, kv_len, heads, kv_heads, D, scale, softcap, causal, window, None, None,
+                                         prefix, out, lse, ws, size, None)
+
+    assert fwd(batch=0) == 0 and fwd(q_len=0) == 0
+    nan = float("nan")
+    for bad in (dict(q=None), dict(q=ODD), dict(qs=None), dict(qs=ODD_STRIDES), dict(ks=ODD_STRIDES), dict(dtype=2), dict(batch=-1), dict(q_len=-1), dict(kv_len=-1),
+                dict(kv_len=(1 << 28) + 1), dict(heads=6), dict(kv_heads=0), dict(heads=8192, kv_heads=1), dict(D=60), dict(D=264), dict(scale=nan),
+                dict(softcap=-1.0), dict(softcap=nan), dict(softcap=float("inf")), dict(window=-1), dict(causal=0, prefix=P), dict(out=None), dict(out=ODD),
+                dict(lse=None), dict(ws=None), dict(ws=ODD), dict(size=0), dict(q_len=1 << 28, heads=32, kv_heads=4)):
+        assert fwd(**bad) == 1, bad
+    for call in (lib.picomoe_attention_fwd_workspace_bytes, lib.picomoe_attention_bwd_workspace_bytes):
+        assert call(1, 2, 4, 4, 4, 2, 64) >= 16 and call(1, 2, 4, 4, 4, 3, 64) == -1 and call(5, 2, 4, 4, 4, 2, 64) == -1
+    need = lib.picomoe_attention_bwd_workspace_bytes(1, 2, 4, 4, 4, 4, 64)
+
+    def bwd(g=P, out=P, lse=P, dq=P, dv=P, size=need, kv_len=4, q_len=4):
+        return lib.picomoe_attention_bwd(g, P, STRIDES, P, STRIDES, P, STRIDES, out, lse, 1, 2, q_len, kv_len, 4, 4, 64, 0.1, 0.0, 1, 0, None, None, None, dq, P, dv,
+                                         P, size, None)
+
+    for bad in (dict(g=None), dict(g=ODD), dict(out=None), dict(lse=None), dict(dq=None), dict(dv=ODD), dict(size=need - 1), dict(kv_len=0), dict(q_len=0)):
+        assert bwd(**bad) == 1, bad
+
+
+def test_cpu_tensors_are_refused():
+    q = torch.zeros(1, 2, 2, 64)
+    table = torch.zeros(4, 64)
+    for call in (lambda: decoder_ops.attention(q, q, q), lambda: decoder_ops.qk_norm_rope(q, q, table, table), lambda: decoder_ops.embedding(torch.tensor([1]), table)):
+        with pytest.raises(_lib.PicomoeError):
+            call()
+
+
+def test_model_options():
+    from picotron_amd.model import Llama
+
+    base = dict(vocab_size=50, hidden_size=64, intermediate_size=32, num_attention_heads=4, num_key_value_heads=2, num_hidden_layers=1, max_position_embeddings=8,
+                rms_norm_eps=1e-5, rope_theta=10000.0)
+    plain = Llama(types.SimpleNamespace(**base))
+    attention = plain.decoder_layers[0].attention
+    assert not attention.fused and attention.q_norm is None and plain.embedding.scale is None
+    model = Llama(types.SimpleNamespace(**base, qk_norm=True, attention_bias="distance", embedding_scale=8.0))
+    attention = model.decoder_layers[0].attention
+    assert attention.fused and attention.q_norm.weight.shape == (16,) and attention.slopes.tolist() == [0.25, 0.0625, 0.015625, 0.00390625]
+    assert model.embedding.scale == 8.0
+    extra = set(n for n, _ in model.named_parameters()) - set(n for n, _ in plain.named_parameters())
+    assert extra == {"decoder_layers.0.attention.q_norm.weight", "decoder_layers.0.attention.k_norm.weight"}
+    for option in (dict(fused_attention=True), dict(attention_softcap=30.0), dict(attention_window=4)):
+        assert Llama(types.SimpleNamespace(**base, **option)).decoder_layers[0].attention.fused
+    with pytest.raises(ValueError):
+        Llama(types.SimpleNamespace(**base, attention_bias="alibi"))
