@@ -17,6 +17,8 @@ import math
 import torch
 
 U = 2.0 ** -24
+# what an exponential or a product below fp32's normal range may lose: the hardware's exponential returns zero there
+FLUSH = 2.0 ** -126
 
 
 def half_step(dtype):
@@ -142,7 +144,7 @@ def attention(q, k, v, *, causal=True, scale=None, softcap=0.0, window=0, slopes
     e_p = e_z + torch.where(m, e_z, zero).amax(-1, keepdim=True) + (Sk + 32) * U + 2 * U * top.abs()
     o = over(P, V, m)
     o_size = over(P, V.abs(), m)
-    e_o = r * o.abs() + over(P * (e_p + r), V.abs(), m) + (Sk + 8) * U * o_size
+    e_o = r * o.abs() + over(torch.where(m, P * (e_p + r) + FLUSH, zero), V.abs(), m) + (Sk + 8) * U * o_size
     back = lambda a: a.transpose(1, 2)
     found = {"out": (back(o), back(e_o))}
     if d_out is None:
@@ -157,7 +159,7 @@ def attention(q, k, v, *, causal=True, scale=None, softcap=0.0, window=0, slopes
     e_dx = raw * slope * ((D + 2) * U * pairs(g.abs(), V.abs()) + e_delta) + (e_p + 8 * U) * dx.abs()
     if softcap:
         e_dx = e_dx + raw * (dP - delta).abs() * (2 * e_z / softcap + 16 * U)
-    e_dx = torch.where(m, e_dx + r * dx.abs(), zero)
+    e_dx = torch.where(m, e_dx + r * dx.abs() + FLUSH * (1 + scale * (dP - delta).abs()), zero)
     dq = over(dx, K, m)
     e_dq = r * dq.abs() + over(e_dx + (Sk + 8) * U * dx.abs(), K.abs(), m)
     mt = m.transpose(2, 3)
@@ -166,6 +168,6 @@ def attention(q, k, v, *, causal=True, scale=None, softcap=0.0, window=0, slopes
     n = Sq * (H // G)
     e_dk = r * dk.abs() + group(over((e_dx + (n + 8) * U * dx.abs()).transpose(2, 3), Q.abs(), mt))
     dv = group(over(P.transpose(2, 3), g, mt))
-    e_dv = r * dv.abs() + group(over((P * (e_p + r + (n + 8) * U)).transpose(2, 3), g.abs(), mt))
+    e_dv = r * dv.abs() + group(over(torch.where(m, P * (e_p + r + (n + 8) * U) + FLUSH, zero).transpose(2, 3), g.abs(), mt))
     found.update(dq=(back(dq), back(e_dq)), dk=(back(dk), back(e_dk)), dv=(back(dv), back(e_dv)))
     return found

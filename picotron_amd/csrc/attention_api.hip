@@ -39,7 +39,7 @@ bool fill(AttnArgs* a, const void* q, const int64_t* qs, const void* k, const in
 extern "C" int64_t picomoe_attention_fwd_workspace_bytes(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, int kv_heads,
                                                          int head_dim) {
     if (!sizes_ok(dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim)) return -1;
-    return 16;
+    return attention_mfma_supported(head_dim) ? attention_mfma_fwd_workspace(dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim) : 16;
 }
 
 extern "C" int picomoe_attention_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
@@ -55,13 +55,15 @@ extern "C" int picomoe_attention_fwd(const void* q, const int64_t* q_strides, co
     PICOMOE_CHECK_ARG(out && lse && ((uintptr_t)out & 15) == 0 && workspace && ((uintptr_t)workspace & 15) == 0 &&
                       workspace_bytes >= picomoe_attention_fwd_workspace_bytes(dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim));
     a.out = out; a.lse = lse; a.ws = (char*)workspace;
+    if (attention_mfma_supported(head_dim)) return attention_mfma_fwd(a, (hipStream_t)stream);
     return attention_simple_fwd(a, (hipStream_t)stream);
 }
 
 extern "C" int64_t picomoe_attention_bwd_workspace_bytes(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, int kv_heads,
                                                          int head_dim) {
     if (!sizes_ok(dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim)) return -1;
-    return round16(batch * q_len * q_heads * 4) + 16;
+    const int64_t delta = round16(batch * q_len * q_heads * 4);
+    return delta + (attention_mfma_supported(head_dim) ? attention_mfma_bwd_workspace(dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim) : 16);
 }
 
 extern "C" int picomoe_attention_bwd(const void* d_out, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
@@ -80,5 +82,6 @@ extern "C" int picomoe_attention_bwd(const void* d_out, const void* q, const int
     a.out = (void*)out; a.lse = (float*)lse; a.d_out = d_out; a.dq = dq; a.dk = dk; a.dv = dv;
     a.delta = (float*)workspace;
     a.ws = (char*)workspace + round16(batch * q_len * q_heads * 4);
+    if (attention_mfma_supported(head_dim)) return attention_mfma_bwd(a, (hipStream_t)stream);
     return attention_simple_bwd(a, (hipStream_t)stream);
 }

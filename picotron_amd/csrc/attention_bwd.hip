@@ -1,0 +1,611 @@
+// Attention backward on MFMA, without atomics: dq in one kernel, dk and dv in another, P recomputed from lse in both.
+//
+// Seven products instead of the five of the formulas (S and dP are formed twice); what that buys is that every sum has one owner
+// and one order.  dq: a wavefront owns 32 rows (as in the forward), walks the key tiles: S^T = K Q^T, dP^T = V dO^T,
+// dq^T += K^T dx^T; it also forms D = dO . out, which the second kernel reads.  dk, dv: a wavefront owns 32 keys, walks the row
+// tiles of the key head -- all its query heads, so that their gradients meet in one accumulator: S = Q K^T, dP = dO V^T,
+// dv^T += dO^T P, dk^T += Q^T dx.  Where the key blocks are too few to fill the chip the rows are dealt to `splits` blocks
+// whose fp32 parts a last launch adds in order.
+#include "attention_tiles.h"
+
+namespace {
+
+// ---------------------------------------------------------------------------------------------------------------
+// dq
+// ---------------------------------------------------------------------------------------------------------------
+template <typename T, int DP>
+struct DqShape {
+    static constexpr int kTile = sizeof(T) == 2 ? 64 : 32;
+    static constexpr int kTileBytes = kTile * DP * (int)sizeof(T);
+    static constexpr int kLds = 2 * 2 * kTileBytes + 2 * kTile * 4;
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq_kernel(MfmaArgs m) {
+    typedef DqShape<T, DP> Sh;
+    typedef Tile<T, DP> Tl;
+    constexpr int kSub = Sh::kTile / 32, kSteps = DP / 16, kCols = DP / 32, kPasses = Sh::kTile / Tl::kRowsPerPass;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const AttnArgs& a = m.a;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5;
+
+    const int heads = (int)a.batch * a.kv_heads, bh = blockIdx.x % heads, tile = m.n_tiles - 1 - blockIdx.x / heads;
+    const int b = bh / a.kv_heads, kvh = bh % a.kv_heads;
+    int row = tile * 32 * kWaves + wave * 32 + (lane & 31);
+    const bool row_in = row < m.rows;
+    row = row_in ? row : m.rows - 1;
+    const int s = m.div(row), head = kvh * a.group + row - s * a.group, pos = s + a.kv_len - a.q_len;
+    const RowSpan span = row_span(a, b, s);
+    const int key_span = span.hi - span.lo;
+    const float slope2 = a.slopes ? a.slopes[head] * kLog2e : 0.f;
+    const int64_t out_row = ((int64_t)b * a.q_len + s) * a.heads + head, stat = ((int64_t)b * a.heads + head) * a.q_len + s;
+
+    Frag<T> qf[kSteps], gf[kSteps];
+    float delta = 0.f;
+    {
+        const T* q = (const T*)a.q.p + b * a.q.sb + s * a.q.ss + head * a.q.sh;
+        const T *g = (const T*)a.d_out + out_row * a.D, *out = (const T*)a.out + out_row * a.D;
+#pragma unroll
+        for (int ks = 0; ks < kSteps; ++ks) {
+            qf[ks] = load_frag<T>(q, 16 * ks + 8 * hi, a.D);
+            gf[ks] = load_frag<T>(g, 16 * ks + 8 * hi, a.D);
+            delta += frag_dot(gf[ks], load_frag<T>(out, 16 * ks + 8 * hi, a.D));
+        }
+    }
+    delta = other_sum(delta);
+    if (row_in && hi == 0) a.delta[stat] = delta;
+    float lse2 = a.lse[stat] * kLog2e;
+    lse2 = lse2 == -INFINITY ? INFINITY : lse2;  // a row without a key: P = 0
+
+    const bool some = key_span >= 0;
+    Reach w;
+    w.lo_min = wave_min_i32(some ? span.lo : 0x7FFFFFFF);
+    w.hi_max = wave_max_i32(some ? span.hi : -1);
+    w.lo_max = wave_max_i32(some ? span.lo : 0x7FFFFFFF);
+    w.hi_min = wave_min_i32(some ? span.hi : -1);
+    w.doc_min = wave_min_i32(some ? span.doc : 0x7FFFFFFF);
+    w.doc_max = wave_max_i32(some ? span.doc : -1);
+    Reach blk = w;
+    {
+        __shared__ int reach[kWaves][4];
+        if (lane == 0) {
+            reach[wave][0] = w.lo_min;
+            reach[wave][1] = w.hi_max;
+            reach[wave][2] = w.doc_min;
+            reach[wave][3] = w.doc_max;
+        }
+        __syncthreads();
+        for (int i = 0; i < kWaves; ++i) {
+            blk.lo_min = min(blk.lo_min, reach[i][0]);
+            blk.hi_max = max(blk.hi_max, reach[i][1]);
+            blk.doc_min = min(blk.doc_min, reach[i][2]);
+            blk.doc_max = max(blk.doc_max, reach[i][3]);
+        }
+        blk.lo_min = __builtin_amdgcn_readfirstlane(blk.lo_min);
+        blk.hi_max = __builtin_amdgcn_readfirstlane(blk.hi_max);
+        blk.doc_min = __builtin_amdgcn_readfirstlane(blk.doc_min);
+        blk.doc_max = __builtin_amdgcn_readfirstlane(blk.doc_max);
+    }
+    const int32_t* doc_min = a.docs ? m.doc_min + (int64_t)b * m.walked_tiles : nullptr;
+    const int32_t* doc_max = a.docs ? m.doc_max + (int64_t)b * m.walked_tiles : nullptr;
+    const bool any = blk.hi_max >= blk.lo_min;
+    const int first = any ? blk.lo_min / Sh::kTile : 0, end = any ? blk.hi_max / Sh::kTile + 1 : 0;
+
+    const T* kbase = (const T*)a.k.p + b * a.k.sb + kvh * a.k.sh;
+    const T* vbase = (const T*)a.v.p + b * a.v.sb + kvh * a.v.sh;
+    const int st_row = threadIdx.x / Tl::kChunks, st_chunk = threadIdx.x % Tl::kChunks;
+    const bool st_in = st_chunk * Tl::kPerChunk < a.D;
+    u32x4_t kreg[kPasses], vreg[kPasses];
+    int doc_reg = 0;
+    auto fetch = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            int key = t * Sh::kTile + i * Tl::kRowsPerPass + st_row;
+            key = key < a.kv_len ? key : a.kv_len - 1;
+            const u32x4_t zero = {0u, 0u, 0u, 0u};
+            kreg[i] = st_in ? *(const u32x4_t*)(kbase + (int64_t)key * a.k.ss + st_chunk * Tl::kPerChunk) : zero;
+            vreg[i] = st_in ? *(const u32x4_t*)(vbase + (int64_t)key * a.v.ss + st_chunk * Tl::kPerChunk) : zero;
+        }
+        if (a.docs && threadIdx.x < Sh::kTile) {
+            const int key = t * Sh::kTile + (int)threadIdx.x;
+            doc_reg = key < a.kv_len ? a.docs[(int64_t)b * a.kv_len + key] : -1;
+        }
+    };
+    auto stage = [&](int buf) {
+        char* kt = lds + buf * 2 * Sh::kTileBytes;
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            const uint32_t at = Tl::at(i * Tl::kRowsPerPass + st_row, st_chunk);
+            *(u32x4_t*)(kt + at) = kreg[i];
+            *(u32x4_t*)(kt + Sh::kTileBytes + at) = vreg[i];
+        }
+        if (a.docs && threadIdx.x < Sh::kTile) ((int32_t*)(lds + 4 * Sh::kTileBytes))[buf * Sh::kTile + threadIdx.x] = doc_reg;
+    };
+
+    const ScoreScale sc = score_scale<T>(a);
+    f32x16_t dq[kCols];
+    auto run = [&](auto careful) {  // CAREFUL: as in the forward, for K
+        constexpr bool kCareful = decltype(careful)::value;
+#pragma unroll
+        for (int t = 0; t < kCols; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dq[t][i] = 0.f;
+        auto active = [&](int t) { return !a.docs || (doc_max[t] >= blk.doc_min && doc_min[t] <= blk.doc_max); };
+        TileWalk<decltype(active)> walk(first, end, active);
+        int cur = walk.next(), buf = 0;
+        if (cur >= 0) fetch(cur);
+        while (cur >= 0) {
+            stage(buf);
+            const int following = walk.next();
+            if (following >= 0) fetch(following);
+            __syncthreads();
+            const char* kt = lds + buf * 2 * Sh::kTileBytes;
+            const char* vt = kt + Sh::kTileBytes;
+            const int32_t* docs = (const int32_t*)(lds + 4 * Sh::kTileBytes) + buf * Sh::kTile;
+            const int key0 = cur * Sh::kTile, key1 = key0 + Sh::kTile - 1;
+            bool in = key0 <= w.hi_max && key1 >= w.lo_min, full = key0 >= w.lo_max && key1 <= w.hi_min;
+            if (a.docs) {
+                const int d0 = doc_min[cur], d1 = doc_max[cur];
+                in = in && d1 >= w.doc_min && d0 <= w.doc_max;
+                full = full && d0 == d1 && d0 == w.doc_min && d0 == w.doc_max;
+            }
+            if (in) {
+#pragma unroll
+                for (int u = 0; u < kSub; ++u) {
+                    f32x16_t x, dp;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i] = dp[i] = 0.f;
+#pragma unroll
+                    for (int ks = 0; ks < kSteps; ++ks) {
+                        mma(x, Tl::frag(kt, u * 32 + (lane & 31), ks, hi), qf[ks]);
+                        mma(dp, Tl::frag(vt, u * 32 + (lane & 31), ks, hi), gf[ks]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) dp[i] -= delta;
+                    if (sc.cap2 > 0.f) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const float t = capped<T>(x[i], sc.mul);
+                            x[i] = sc.cap2 * t;
+                            dp[i] *= 1.f - t * t;
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) x[i] *= sc.mul;
+                    }
+                    if (a.slopes) {
+                        const float away = (float)(pos - key0 - 4 * hi);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) x[i] -= slope2 * __builtin_fabsf(away - (float)(u * 32 + 8 * (i / 4) + i % 4));
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i] = __builtin_amdgcn_exp2f(x[i] - lse2) * dp[i];
+                    if (!full) {
+                        const int from = span.lo - key0 - 4 * hi;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int at = u * 32 + 8 * (i / 4) + i % 4;
+                            bool see = key_span >= 0 && (uint32_t)(at - from) <= (uint32_t)key_span;
+                            if (a.docs) see = see && docs[at + 4 * hi] == span.doc;
+                            x[i] = see ? x[i] : 0.f;
+                        }
+                    }
+#pragma unroll
+                    for (int st = 0; st < 2; ++st) {
+                        const Frag<T> dx = to_frag<T>(x, st);
+#pragma unroll
+                        for (int t = 0; t < kCols; ++t) {
+                            Frag<T> k = Tl::frag_t(kt, u * 32 + 16 * st, t, lane);
+                            if (kCareful) zero_not_finite(k);
+                            mma(dq[t], k, dx);
+                        }
+                    }
+                }
+                if (kCareful) {
+                    bool bad = false;
+                    if (lane < Sh::kTile) bad = Tl::row_not_finite(kt, lane);
+                    for (uint64_t left = __ballot(bad); left; left &= left - 1) {
+                        const int key = __builtin_ctzll(left), j = key0 + key;
+                        const bool see = j >= span.lo && j <= span.hi && (!a.docs || docs[key] == span.doc);
+#pragma unroll
+                        for (int t = 0; t < kCols; ++t)
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const float v = Tl::element(kt, key, 32 * t + 8 * (i / 4) + 4 * hi + i % 4);
+                                if (see && !(__builtin_fabsf(v) < INFINITY)) dq[t][i] += v - v;  // its score is not finite either
+                            }
+                    }
+                }
+            }
+            cur = following;
+            buf ^= 1;
+        }
+    };
+    run(std::integral_constant<bool, false>());
+    bool bad = false;
+#pragma unroll
+    for (int t = 0; t < kCols; ++t) bad |= not_finite(dq[t]);
+    if (__syncthreads_or(bad)) run(std::integral_constant<bool, true>());
+
+    if (!row_in) return;
+    T* to = (T*)a.dq + out_row * a.D;
+#pragma unroll
+    for (int t = 0; t < kCols; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int d = 32 * t + 8 * j + 4 * hi;
+            if (d >= a.D) continue;
+            const f32x4_t v = {dq[t][4 * j] * a.scale, dq[t][4 * j + 1] * a.scale, dq[t][4 * j + 2] * a.scale, dq[t][4 * j + 3] * a.scale};
+            if constexpr (sizeof(T) == 2) *(u32x2_t*)(to + d) = u32x2_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+            else *(f32x4_t*)(to + d) = v;
+        }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// dk, dv
+// ---------------------------------------------------------------------------------------------------------------
+template <typename T, int DP>
+struct DkvShape {
+    static constexpr int kTile = 32;              // rows of a tile
+    static constexpr int kKeys = 32 * kWaves;     // keys of a block
+    static constexpr int kTileBytes = kTile * DP * (int)sizeof(T);
+    static constexpr int kStats = 7 * kTile * 4;  // lse2, delta, slope2 (floats), position, first key, keys, document (ints)
+    static constexpr int kLds = 2 * (2 * kTileBytes + kStats);
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dkv_kernel(MfmaArgs m) {
+    typedef DkvShape<T, DP> Sh;
+    typedef Tile<T, DP> Tl;
+    constexpr int kSteps = DP / 16, kCols = DP / 32, kPasses = Sh::kTile / Tl::kRowsPerPass, kBuf = 2 * Sh::kTileBytes + Sh::kStats;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const AttnArgs& a = m.a;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5;
+    const int heads = (int)a.batch * a.kv_heads, bh = blockIdx.x % heads, block = blockIdx.x / heads, split = blockIdx.y;
+    const int b = bh / a.kv_heads, kvh = bh % a.kv_heads;
+    const int block0 = block * Sh::kKeys, block1 = min(block0 + Sh::kKeys, a.kv_len) - 1;
+    const int wave0 = block0 + wave * 32, wave1 = wave0 + 31;
+    const int key = wave0 + (lane & 31), key_in = key < a.kv_len, key_at = key_in ? key : a.kv_len - 1;
+
+    Frag<T> kf[kSteps], vf[kSteps];
+    {
+        const T* k = (const T*)a.k.p + b * a.k.sb + (int64_t)key_at * a.k.ss + kvh * a.k.sh;
+        const T* v = (const T*)a.v.p + b * a.v.sb + (int64_t)key_at * a.v.ss + kvh * a.v.sh;
+#pragma unroll
+        for (int ks = 0; ks < kSteps; ++ks) {
+            kf[ks] = load_frag<T>(k, 16 * ks + 8 * hi, a.D);
+            vf[ks] = load_frag<T>(v, 16 * ks + 8 * hi, a.D);
+        }
+    }
+    // keys past the end get a document of their own; without documents every key and row has document 0
+    const int doc = a.docs ? (key_in ? a.docs[(int64_t)b * a.kv_len + key] : -1) : 0;
+    const int w_doc_min = wave_min_i32(doc), w_doc_max = wave_max_i32(doc);
+    int blk_doc_min = 0, blk_doc_max = 0;
+    if (a.docs) {
+        __shared__ int range[kWaves][2];
+        if (lane == 0) {
+            range[wave][0] = w_doc_min;
+            range[wave][1] = w_doc_max;
+        }
+        __syncthreads();
+        blk_doc_min = __builtin_amdgcn_readfirstlane(min(min(range[0][0], range[1][0]), min(range[2][0], range[3][0])));
+        blk_doc_max = __builtin_amdgcn_readfirstlane(max(max(range[0][1], range[1][1]), max(range[2][1], range[3][1])));
+    }
+    const int32_t* doc_min = a.docs ? m.doc_min + (int64_t)b * m.walked_tiles : nullptr;
+    const int32_t* doc_max = a.docs ? m.doc_max + (int64_t)b * m.walked_tiles : nullptr;
+    const int prefix = a.prefix ? a.prefix[b] : 0, off = a.kv_len - a.q_len;
+    // first and last key of the interval of query s (documents aside): both grow with s
+    auto lo_of = [&](int q) { return a.window > 0 ? max(0, q + off - a.window + 1) : 0; };
+    auto hi_of = [&](int q) {
+        int last = a.kv_len - 1;
+        if (a.causal) last = min(last, max(q + off, prefix - 1));
+        if (a.window > 0) last = min(last, q + off + a.window - 1);
+        return last;
+    };
+    auto first_query = [&](int t) { return m.div(t * Sh::kTile); };
+    auto last_query = [&](int t) { return m.div(min(t * Sh::kTile + Sh::kTile, m.rows) - 1); };
+
+    // staging: this thread's row of a tile and its chunk
+    const int st_row = threadIdx.x / Tl::kChunks, st_chunk = threadIdx.x % Tl::kChunks;
+    const bool st_in = st_chunk * Tl::kPerChunk < a.D;
+    const T* qbase = (const T*)a.q.p + b * a.q.sb + (int64_t)(kvh * a.group) * a.q.sh;
+    const T* gbase = (const T*)a.d_out + ((int64_t)b * a.q_len * a.heads + kvh * a.group) * a.D;
+    u32x4_t qreg[kPasses], greg[kPasses];
+    float stat_f[3] = {};
+    int stat_i[4] = {};
+    auto fetch = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            const int r = min(t * Sh::kTile + i * Tl::kRowsPerPass + st_row, m.rows - 1), s = m.div(r), h = r - s * a.group;
+            const u32x4_t zero = {0u, 0u, 0u, 0u};
+            qreg[i] = st_in ? *(const u32x4_t*)(qbase + s * a.q.ss + h * a.q.sh + st_chunk * Tl::kPerChunk) : zero;
+            greg[i] = st_in ? *(const u32x4_t*)(gbase + ((int64_t)s * a.heads + h) * a.D + st_chunk * Tl::kPerChunk) : zero;
+        }
+        if (threadIdx.x < Sh::kTile) {
+            const int r = t * Sh::kTile + (int)threadIdx.x, rc = min(r, m.rows - 1), s = m.div(rc), h = kvh * a.group + rc - s * a.group;
+            const int64_t stat = ((int64_t)b * a.heads + h) * a.q_len + s;
+            const RowSpan span = row_span(a, b, s);
+            const float lse = a.lse[stat];
+            stat_f[0] = lse == -INFINITY ? INFINITY : lse * kLog2e;
+            stat_f[1] = a.delta[stat];
+            stat_f[2] = a.slopes ? a.slopes[h] * kLog2e : 0.f;
+            const bool see = r < m.rows && span.hi >= span.lo;
+            stat_i[0] = s + off;
+            stat_i[1] = see ? span.lo : 0x7FFFFFFF;  // no key is that far
+            stat_i[2] = see ? span.hi - span.lo : 0;
+            stat_i[3] = span.doc;
+        }
+    };
+    auto stage = [&](int buf) {
+        char* qt = lds + buf * kBuf;
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            const uint32_t at = Tl::at(i * Tl::kRowsPerPass + st_row, st_chunk);
+            *(u32x4_t*)(qt + at) = qreg[i];
+            *(u32x4_t*)(qt + Sh::kTileBytes + at) = greg[i];
+        }
+        if (threadIdx.x < Sh::kTile) {
+            float* f = (float*)(qt + 2 * Sh::kTileBytes);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) f[i * Sh::kTile + threadIdx.x] = stat_f[i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ((int*)f)[(3 + i) * Sh::kTile + threadIdx.x] = stat_i[i];
+        }
+    };
+
+    const ScoreScale sc = score_scale<T>(a);
+    f32x16_t dk[kCols], dv[kCols];
+    auto run = [&](auto careful) {  // CAREFUL: as in the forward, for Q and dO
+        constexpr bool kCareful = decltype(careful)::value;
+#pragma unroll
+        for (int t = 0; t < kCols; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dk[t][i] = dv[t][i] = 0.f;
+        auto active = [&](int t) {
+            if (hi_of(last_query(t)) < block0 || lo_of(first_query(t)) > block1) return false;
+            return !a.docs || (doc_max[t] >= max(0, blk_doc_min) && doc_min[t] <= blk_doc_max);
+        };
+        TileWalk<decltype(active)> walk(0, m.walked_tiles, active);
+        int seen = 0;  // every splits-th active tile is this block's
+        auto next = [&]() {
+            while (true) {
+                const int t = walk.next();
+                if (t < 0 || seen++ % m.splits == split) return t;
+            }
+        };
+        int cur = next(), buf = 0;
+        if (cur >= 0) fetch(cur);
+        while (cur >= 0) {
+            stage(buf);
+            const int following = next();
+            if (following >= 0) fetch(following);
+            __syncthreads();
+            const char* qt = lds + buf * kBuf;
+            const char* gt = qt + Sh::kTileBytes;
+            const float* stats = (const float*)(gt + Sh::kTileBytes);
+            const int* stati = (const int*)(stats + 3 * Sh::kTile);
+            const int s0 = first_query(cur), s1 = last_query(cur);
+            bool in = hi_of(s1) >= wave0 && lo_of(s0) <= wave1;
+            bool full = lo_of(s1) <= wave0 && hi_of(s0) >= wave1 && (cur + 1) * Sh::kTile <= m.rows;
+            if (a.docs) {
+                const int d0 = doc_min[cur], d1 = doc_max[cur];
+                in = in && d1 >= max(0, w_doc_min) && d0 <= w_doc_max;
+                full = full && d0 == d1 && d0 == w_doc_min && d0 == w_doc_max && d0 >= 0;
+            }
+            if (in) {
+                f32x16_t x, dp;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] = dp[i] = 0.f;
+#pragma unroll
+                for (int ks = 0; ks < kSteps; ++ks) {
+                    mma(x, Tl::frag(qt, lane & 31, ks, hi), kf[ks]);
+                    mma(dp, Tl::frag(gt, lane & 31, ks, hi), vf[ks]);
+                }
+                auto stat4 = [&](int which, int j) { return *(const f32x4_t*)(stats + which * Sh::kTile + 8 * j + 4 * hi); };
+                auto stat4i = [&](int which, int j) {
+                    typedef __attribute__((ext_vector_type(4))) int i32x4_t;
+                    return *(const i32x4_t*)(stati + which * Sh::kTile + 8 * j + 4 * hi);
+                };
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const f32x4_t delta = stat4(1, j);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) dp[4 * j + i] -= delta[i];
+                }
+                if (sc.cap2 > 0.f) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float t = capped<T>(x[i], sc.mul);
+                        x[i] = sc.cap2 * t;
+                        dp[i] *= 1.f - t * t;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i] *= sc.mul;
+                }
+                if (a.slopes) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const f32x4_t slope2 = stat4(2, j);
+                        const auto pos = stat4i(0, j);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) x[4 * j + i] -= slope2[i] * __builtin_fabsf((float)(pos[i] - key));
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const f32x4_t lse2 = stat4(0, j);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[4 * j + i] = __builtin_amdgcn_exp2f(x[4 * j + i] - lse2[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) dp[i] *= x[i];
+                if (!full) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const auto lo = stat4i(1, j), keys = stat4i(2, j), row_doc = stat4i(3, j);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const bool see = (uint32_t)(key - lo[i]) <= (uint32_t)keys[i] && row_doc[i] == doc;
+                            x[4 * j + i] = see ? x[4 * j + i] : 0.f;
+                            dp[4 * j + i] = see ? dp[4 * j + i] : 0.f;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int st = 0; st < 2; ++st) {
+                    const Frag<T> p = to_frag<T>(x, st), dx = to_frag<T>(dp, st);
+#pragma unroll
+                    for (int t = 0; t < kCols; ++t) {
+                        Frag<T> g = Tl::frag_t(gt, 16 * st, t, lane), q = Tl::frag_t(qt, 16 * st, t, lane);
+                        if (kCareful) {
+                            zero_not_finite(g);
+                            zero_not_finite(q);
+                        }
+                        mma(dv[t], g, p);
+                        mma(dk[t], q, dx);
+                    }
+                }
+                if (kCareful) {
+                    const bool bad = Tl::row_not_finite(hi ? gt : qt, lane & 31);
+                    for (uint64_t left = __ballot(bad); left; left &= left - 1) {
+                        const int which = __builtin_ctzll(left), r = which & 31;
+                        const char* from = which >> 5 ? gt : qt;
+                        const bool see = (uint32_t)(key - stati[1 * Sh::kTile + r]) <= (uint32_t)stati[2 * Sh::kTile + r] && stati[3 * Sh::kTile + r] == doc;
+#pragma unroll
+                        for (int t = 0; t < kCols; ++t)
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const float v = Tl::element(from, r, 32 * t + 8 * (i / 4) + 4 * hi + i % 4);
+                                const bool add = see && !(__builtin_fabsf(v) < INFINITY);
+                                dv[t][i] += add && which >= 32 ? v : 0.f;
+                                dk[t][i] += add && which < 32 ? v - v : 0.f;
+                            }
+                    }
+                }
+            }
+            cur = following;
+            buf ^= 1;
+        }
+    };
+    run(std::integral_constant<bool, false>());
+    bool bad = false;
+#pragma unroll
+    for (int t = 0; t < kCols; ++t) bad |= not_finite(dk[t]) || not_finite(dv[t]);
+    if (__syncthreads_or(bad)) run(std::integral_constant<bool, true>());
+
+    if (!key_in) return;
+    const int64_t out_row = ((int64_t)b * a.kv_len + key) * a.kv_heads + kvh, rows = a.batch * a.kv_len * a.kv_heads;
+#pragma unroll
+    for (int t = 0; t < kCols; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int d = 32 * t + 8 * j + 4 * hi;
+            if (d >= a.D) continue;
+            const f32x4_t u = {dk[t][4 * j] * a.scale, dk[t][4 * j + 1] * a.scale, dk[t][4 * j + 2] * a.scale, dk[t][4 * j + 3] * a.scale};
+            const f32x4_t v = {dv[t][4 * j], dv[t][4 * j + 1], dv[t][4 * j + 2], dv[t][4 * j + 3]};
+            if (m.splits > 1) {
+                float* to = m.part_out + ((int64_t)split * 2 * rows + out_row) * a.D + d;
+                *(f32x4_t*)to = u;
+                *(f32x4_t*)(to + rows * a.D) = v;
+            } else if constexpr (sizeof(T) == 2) {
+                *(u32x2_t*)((T*)a.dk + out_row * a.D + d) = u32x2_t{pack_bf16x2(u[0], u[1]), pack_bf16x2(u[2], u[3])};
+                *(u32x2_t*)((T*)a.dv + out_row * a.D + d) = u32x2_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+            } else {
+                *(f32x4_t*)((T*)a.dk + out_row * a.D + d) = u;
+                *(f32x4_t*)((T*)a.dv + out_row * a.D + d) = v;
+            }
+        }
+}
+
+// dk and dv from the parts of the splits, four elements a thread
+template <typename T>
+__global__ __launch_bounds__(kThreads) void attention_dkv_join_kernel(const f32x4_t* __restrict__ parts, int splits, int64_t quads, T* dk, T* dv) {
+    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (i >= 2 * quads) return;
+    f32x4_t sum = parts[i];
+    for (int s = 1; s < splits; ++s) sum += parts[s * 2 * quads + i];
+    T* to = (i < quads ? dk : dv) + 4 * (i < quads ? i : i - quads);
+    if constexpr (sizeof(T) == 2) *(u32x2_t*)to = u32x2_t{pack_bf16x2(sum[0], sum[1]), pack_bf16x2(sum[2], sum[3])};
+    else *(f32x4_t*)to = sum;
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
+
+struct Plan {
+    int key_tile, key_tiles, row_tiles, dq_tiles, key_blocks, splits;
+    int64_t key_docs, row_docs, parts;
+};
+Plan plan(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, int kv_heads, int head_dim) {
+    Plan p;
+    const int64_t rows = q_len * (q_heads / kv_heads);
+    p.key_tile = dtype == PICOMOE_BF16 ? 64 : 32;
+    p.key_tiles = (int)((kv_len + p.key_tile - 1) / p.key_tile);
+    p.row_tiles = (int)((rows + 31) / 32);
+    p.dq_tiles = (int)((rows + 32 * kWaves - 1) / (32 * kWaves));
+    p.key_blocks = (int)((kv_len + 32 * kWaves - 1) / (32 * kWaves));
+    // Fewer blocks than two per CU: the rows are dealt to several, at least four tiles each
+    const int64_t blocks = batch * kv_heads * p.key_blocks;
+    int64_t splits = blocks > 0 ? 512 / blocks : 1;
+    if (splits > p.row_tiles / 4) splits = p.row_tiles / 4;
+    if (splits > 16) splits = 16;
+    p.splits = splits < 1 ? 1 : (int)splits;
+    p.key_docs = round16(batch * p.key_tiles * 8);
+    p.row_docs = round16(batch * p.row_tiles * 8);
+    p.parts = p.splits > 1 ? (int64_t)p.splits * 2 * batch * kv_len * kv_heads * head_dim * 4 : 0;
+    return p;
+}
+
+template <typename T, int DP>
+int launch(MfmaArgs m, const Plan& p, hipStream_t s) {
+    typedef DqShape<T, DP> Q;
+    typedef DkvShape<T, DP> K;
+    hipError_t e = hipFuncSetAttribute((const void*)attention_dq_kernel<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, Q::kLds);
+    if (e == hipSuccess) e = hipFuncSetAttribute((const void*)attention_dkv_kernel<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, K::kLds);
+    if (e != hipSuccess) return PICOMOE_ERR_HIP_BASE + (int)e;
+    const AttnArgs& a = m.a;
+    const int64_t heads = a.batch * a.kv_heads, dq_blocks = heads * p.dq_tiles, key_blocks = heads * p.key_blocks;
+    const int64_t quads = a.batch * a.kv_len * a.kv_heads * a.D / 4, join_blocks = (2 * quads + kThreads - 1) / kThreads;
+    if (dq_blocks > 0x7FFFFFFF || key_blocks > 0x7FFFFFFF || (p.splits > 1 && join_blocks > 0x7FFFFFFF)) return PICOMOE_ERR_TOO_LARGE;
+    int32_t *key_docs = (int32_t*)a.ws, *row_docs = (int32_t*)(a.ws + p.key_docs);
+    m.part_out = (float*)(a.ws + p.key_docs + p.row_docs);
+    if (a.docs) {
+        int rc = attention_mfma_documents(a, p.key_tile, p.key_tiles, a.kv_len, 0, 1, key_docs, key_docs + a.batch * p.key_tiles, s);
+        if (rc == PICOMOE_OK)
+            rc = attention_mfma_documents(a, 32, p.row_tiles, m.rows, a.kv_len - a.q_len, a.group, row_docs, row_docs + a.batch * p.row_tiles, s);
+        if (rc) return rc;
+    }
+    m.doc_min = key_docs;
+    m.doc_max = key_docs + a.batch * p.key_tiles;
+    m.walked_tiles = p.key_tiles;
+    m.n_tiles = p.dq_tiles;
+    m.splits = 1;
+    attention_dq_kernel<T, DP><<<(unsigned)dq_blocks, kThreads, Q::kLds, s>>>(m);
+    m.doc_min = row_docs;
+    m.doc_max = row_docs + a.batch * p.row_tiles;
+    m.walked_tiles = p.row_tiles;
+    m.n_tiles = p.key_blocks;
+    m.splits = p.splits;
+    attention_dkv_kernel<T, DP><<<dim3((unsigned)key_blocks, (unsigned)p.splits), kThreads, K::kLds, s>>>(m);
+    if (p.splits > 1)
+        attention_dkv_join_kernel<T><<<(unsigned)join_blocks, kThreads, 0, s>>>((const f32x4_t*)m.part_out, p.splits, quads, (T*)a.dk, (T*)a.dv);
+    return picomoe_launch_status();
+}
+
+}  // namespace
+
+int64_t attention_mfma_bwd_workspace(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, int kv_heads, int head_dim) {
+    const Plan p = plan(dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim);
+    return p.key_docs + p.row_docs + p.parts + 16;
+}
+
+int attention_mfma_bwd(const AttnArgs& a, hipStream_t s) {
+    const Plan p = plan(a.dtype, a.batch, a.q_len, a.kv_len, a.heads, a.kv_heads, a.D);
+    MfmaArgs m = {};
+    m.a = a;
+    m.div = group_div(a.group);
+    m.rows = a.q_len * a.group;
+    if (a.dtype == PICOMOE_BF16) return a.D <= 64 ? launch<__bf16, 64>(m, p, s) : launch<__bf16, 128>(m, p, s);
+    return a.D <= 64 ? launch<float, 64>(m, p, s) : launch<float, 128>(m, p, s);
+}

@@ -1,0 +1,473 @@
+// Attention forward on MFMA: one pass over the keys with the running maximum and sum of the softmax.
+//
+// The query heads of a key head are one list of rows, row r = query r / group, head r % group of the group, so that a K / V
+// tile in LDS serves all of them and one new token of a large group still fills a fragment.  A wavefront owns 32 rows, one per
+// lane pair (lane, lane + 32): S^T[key, row] = K Q^T keeps a row's scores in its two lanes -- maximum and sum need one exchange
+// between them --, and O^T[d, row] = V^T P^T takes P from registers.  Tiles are staged through registers into one of two LDS
+// buffers while the other is multiplied, one barrier per tile.
+//
+// The accumulated O is only rescaled when a row's maximum grows by more than 2^8: until then P is at most 2^8 instead of 1,
+// which costs bf16 nothing and fp32 sums nothing, and the 64 multiplications per tile fall away in all but the first tiles.
+#include "attention_tiles.h"
+
+namespace {
+
+constexpr float kLazy = 8.f;
+
+// KEYS: the four waves share 32 rows and split every tile's keys among them (few rows: one new token); otherwise every wave
+// has 32 rows of its own and all of the tile's keys.
+template <typename T, int DP, bool KEYS>
+struct FwdShape {
+    static constexpr int kTile = KEYS ? 128 : (sizeof(T) == 2 ? 64 : 32);  // keys of a tile
+    static constexpr int kWaveKeys = KEYS ? 32 : kTile;
+    static constexpr int kRows = KEYS ? 32 : 32 * kWaves;  // rows of a block
+    static constexpr int kBuffers = KEYS ? 1 : 2;
+    static constexpr int kTileBytes = kTile * DP * (int)sizeof(T);
+    static constexpr int kLds = kBuffers * 2 * kTileBytes + kBuffers * kTile * 4;  // K, V, document ids
+};
+
+template <typename T, int DP, bool KEYS>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fwd_kernel(MfmaArgs m) {
+    typedef FwdShape<T, DP, KEYS> Sh;
+    typedef Tile<T, DP> Tl;
+    constexpr int kSub = Sh::kWaveKeys / 32, kSteps = DP / 16, kCols = DP / 32, kPasses = Sh::kTile / Tl::kRowsPerPass;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const AttnArgs& a = m.a;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5;
+
+    // blocks of one key head lie on one XCD where there are 8 heads or more; those with the most keys (the last rows) go first
+    const int heads = (int)a.batch * a.kv_heads, bh = blockIdx.x % heads, tile = m.n_tiles - 1 - blockIdx.x / heads, split = blockIdx.y;
+    const int b = bh / a.kv_heads, kvh = bh % a.kv_heads;
+    const int row0 = tile * Sh::kRows + (KEYS ? 0 : wave * 32);
+    int row = row0 + (lane & 31);
+    const bool row_in = row < m.rows;
+    row = row_in ? row : m.rows - 1;  // rows past the end repeat the last one
+    const int s = m.div(row), head = kvh * a.group + row - s * a.group, pos = s + a.kv_len - a.q_len;
+    const RowSpan span = row_span(a, b, s);
+    const int key_span = span.hi - span.lo;  // negative: no keys
+    const float slope2 = a.slopes ? a.slopes[head] * kLog2e : 0.f;
+
+    Frag<T> qf[kSteps];
+    const T* q = (const T*)a.q.p + b * a.q.sb + s * a.q.ss + head * a.q.sh;
+#pragma unroll
+    for (int ks = 0; ks < kSteps; ++ks) qf[ks] = load_frag<T>(q, 16 * ks + 8 * hi, a.D);
+
+    const bool some = key_span >= 0;
+    Reach w;
+    w.lo_min = wave_min_i32(some ? span.lo : 0x7FFFFFFF);
+    w.hi_max = wave_max_i32(some ? span.hi : -1);
+    w.lo_max = wave_max_i32(some ? span.lo : 0x7FFFFFFF);
+    w.hi_min = wave_min_i32(some ? span.hi : -1);
+    w.doc_min = wave_min_i32(some ? span.doc : 0x7FFFFFFF);
+    w.doc_max = wave_max_i32(some ? span.doc : -1);
+    Reach blk = w;
+    if (!KEYS) {
+        __shared__ int reach[kWaves][4];
+        if (lane == 0) {
+            reach[wave][0] = w.lo_min;
+            reach[wave][1] = w.hi_max;
+            reach[wave][2] = w.doc_min;
+            reach[wave][3] = w.doc_max;
+        }
+        __syncthreads();
+        for (int i = 0; i < kWaves; ++i) {
+            blk.lo_min = min(blk.lo_min, reach[i][0]);
+            blk.hi_max = max(blk.hi_max, reach[i][1]);
+            blk.doc_min = min(blk.doc_min, reach[i][2]);
+            blk.doc_max = max(blk.doc_max, reach[i][3]);
+        }
+        blk.lo_min = __builtin_amdgcn_readfirstlane(blk.lo_min);
+        blk.hi_max = __builtin_amdgcn_readfirstlane(blk.hi_max);
+        blk.doc_min = __builtin_amdgcn_readfirstlane(blk.doc_min);
+        blk.doc_max = __builtin_amdgcn_readfirstlane(blk.doc_max);
+    }
+    const int32_t* doc_min = a.docs ? m.doc_min + (int64_t)b * m.walked_tiles : nullptr;
+    const int32_t* doc_max = a.docs ? m.doc_max + (int64_t)b * m.walked_tiles : nullptr;
+    // this block's share of the tiles between the first and the last key that its rows may see
+    int first = 0, end = 0;
+    if (blk.hi_max >= blk.lo_min) {
+        const int t0 = blk.lo_min / Sh::kTile, n = blk.hi_max / Sh::kTile + 1 - t0;
+        first = t0 + (int)((int64_t)n * split / m.splits);
+        end = t0 + (int)((int64_t)n * (split + 1) / m.splits);
+    }
+
+    const T* kbase = (const T*)a.k.p + b * a.k.sb + kvh * a.k.sh;
+    const T* vbase = (const T*)a.v.p + b * a.v.sb + kvh * a.v.sh;
+    const int st_row = threadIdx.x / Tl::kChunks, st_chunk = threadIdx.x % Tl::kChunks;
+    const bool st_in = st_chunk * Tl::kPerChunk < a.D;
+    u32x4_t kreg[kPasses], vreg[kPasses];
+    int doc_reg = 0;
+    auto fetch = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            int key = t * Sh::kTile + i * Tl::kRowsPerPass + st_row;
+            key = key < a.kv_len ? key : a.kv_len - 1;  // keys past the end are hidden by every row's interval
+            const u32x4_t zero = {0u, 0u, 0u, 0u};
+            kreg[i] = st_in ? *(const u32x4_t*)(kbase + (int64_t)key * a.k.ss + st_chunk * Tl::kPerChunk) : zero;
+            vreg[i] = st_in ? *(const u32x4_t*)(vbase + (int64_t)key * a.v.ss + st_chunk * Tl::kPerChunk) : zero;
+        }
+        if (a.docs && threadIdx.x < Sh::kTile) {
+            const int key = t * Sh::kTile + (int)threadIdx.x;
+            doc_reg = key < a.kv_len ? a.docs[(int64_t)b * a.kv_len + key] : -1;
+        }
+    };
+    auto stage = [&](int buf) {
+        char* kt = lds + buf * 2 * Sh::kTileBytes;
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            const uint32_t at = Tl::at(i * Tl::kRowsPerPass + st_row, st_chunk);
+            *(u32x4_t*)(kt + at) = kreg[i];
+            *(u32x4_t*)(kt + Sh::kTileBytes + at) = vreg[i];
+        }
+        if (a.docs && threadIdx.x < Sh::kTile) ((int32_t*)(lds + Sh::kBuffers * 2 * Sh::kTileBytes))[buf * Sh::kTile + threadIdx.x] = doc_reg;
+    };
+
+    const ScoreScale sc = score_scale<T>(a);
+    f32x16_t o[kCols];
+    float top = -INFINITY, total = 0.f;  // running maximum that P refers to (log2 units), this lane's share of the sum
+
+    // CAREFUL: values of V that are not finite are kept out of the products, where 0 * inf would reach rows that do not see them,
+    // and added one by one to the rows that do
+    auto run = [&](auto careful) {
+        constexpr bool kCareful = decltype(careful)::value;
+        top = -INFINITY;
+        total = 0.f;
+#pragma unroll
+        for (int t = 0; t < kCols; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
+
+        auto active = [&](int t) { return !a.docs || (doc_max[t] >= blk.doc_min && doc_min[t] <= blk.doc_max); };
+        TileWalk<decltype(active)> walk(first, end, active);
+        int cur = walk.next(), buf = 0;
+        if (cur >= 0) fetch(cur);
+        while (cur >= 0) {
+            if (Sh::kBuffers == 1) __syncthreads();
+            stage(buf);
+            const int following = walk.next();
+            if (following >= 0) fetch(following);
+            __syncthreads();
+            const char* kt = lds + buf * 2 * Sh::kTileBytes;
+            const char* vt = kt + Sh::kTileBytes;
+            const int32_t* docs = (const int32_t*)(lds + Sh::kBuffers * 2 * Sh::kTileBytes) + buf * Sh::kTile;
+            const int sub0 = KEYS ? wave * 32 : 0, key0 = cur * Sh::kTile + sub0, key1 = key0 + Sh::kWaveKeys - 1;
+            bool in = key0 <= w.hi_max && key1 >= w.lo_min, full = key0 >= w.lo_max && key1 <= w.hi_min;
+            if (a.docs) {
+                const int d0 = doc_min[cur], d1 = doc_max[cur];
+                in = in && d1 >= w.doc_min && d0 <= w.doc_max;
+                full = full && d0 == d1 && d0 == w.doc_min && d0 == w.doc_max;
+            }
+            if (in) {
+                f32x16_t x[kSub];
+#pragma unroll
+                for (int u = 0; u < kSub; ++u) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[u][i] = 0.f;
+#pragma unroll
+                    for (int ks = 0; ks < kSteps; ++ks) mma(x[u], Tl::frag(kt, sub0 + u * 32 + (lane & 31), ks, hi), qf[ks]);
+                }
+                if (sc.cap2 > 0.f) {
+#pragma unroll
+                    for (int u = 0; u < kSub; ++u)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) x[u][i] = sc.cap2 * capped<T>(x[u][i], sc.mul);
+                } else {
+#pragma unroll
+                    for (int u = 0; u < kSub; ++u)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) x[u][i] *= sc.mul;
+                }
+                if (a.slopes) {
+                    const float away = (float)(pos - key0 - 4 * hi);
+#pragma unroll
+                    for (int u = 0; u < kSub; ++u)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) x[u][i] -= slope2 * __builtin_fabsf(away - (float)(u * 32 + 8 * (i / 4) + i % 4));
+                }
+                if (!full) {
+                    const int from = span.lo - key0 - 4 * hi;  // the lane's first key is 0
+#pragma unroll
+                    for (int u = 0; u < kSub; ++u)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int at = u * 32 + 8 * (i / 4) + i % 4;
+                            bool see = key_span >= 0 && (uint32_t)(at - from) <= (uint32_t)key_span;
+                            if (a.docs) see = see && docs[sub0 + at + 4 * hi] == span.doc;
+                            x[u][i] = see ? x[u][i] : -INFINITY;
+                        }
+                }
+                float mx = x[0][0];
+#pragma unroll
+                for (int u = 0; u < kSub; ++u)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) mx = __builtin_fmaxf(mx, x[u][i]);
+                mx = other_max(mx);
+                if (__any(mx > top + kLazy)) {
+                    const float old = top;
+                    top = __builtin_fmaxf(top, mx);
+                    const float shrink = __builtin_amdgcn_exp2f(old - (top == -INFINITY ? 0.f : top));
+                    total *= shrink;
+#pragma unroll
+                    for (int t = 0; t < kCols; ++t)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[t][i] *= shrink;
+                }
+                const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+                for (int u = 0; u < kSub; ++u)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        x[u][i] = __builtin_amdgcn_exp2f(x[u][i] - base);
+                        total += x[u][i];
+                    }
+#pragma unroll
+                for (int st = 0; st < 2 * kSub; ++st) {
+                    const Frag<T> p = to_frag<T>(x[st / 2], st & 1);
+#pragma unroll
+                    for (int t = 0; t < kCols; ++t) {
+                        Frag<T> v = Tl::frag_t(vt, sub0 + 16 * st, t, lane);
+                        if (kCareful) zero_not_finite(v);
+                        mma(o[t], v, p);
+                    }
+                }
+                if (kCareful) {
+                    bool bad = false;
+                    if (lane < Sh::kWaveKeys) bad = Tl::row_not_finite(vt, sub0 + lane);
+                    for (uint64_t left = __ballot(bad); left; left &= left - 1) {
+                        const int key = __builtin_ctzll(left), j = key0 + key;
+                        const bool see = j >= span.lo && j <= span.hi && (!a.docs || docs[sub0 + key] == span.doc);
+#pragma unroll
+                        for (int t = 0; t < kCols; ++t)
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const float v = Tl::element(vt, sub0 + key, 32 * t + 8 * (i / 4) + 4 * hi + i % 4);
+                                if (see && !(__builtin_fabsf(v) < INFINITY)) o[t][i] += v;
+                            }
+                    }
+                }
+            }
+            cur = following;
+            buf = Sh::kBuffers == 2 ? buf ^ 1 : 0;
+        }
+    };
+    run(std::integral_constant<bool, false>());
+    bool bad = false;
+#pragma unroll
+    for (int t = 0; t < kCols; ++t) bad |= not_finite(o[t]);
+    if (__syncthreads_or(bad)) {
+        run(std::integral_constant<bool, true>());
+        __syncthreads();
+    }
+    total = other_sum(total);
+
+    if (KEYS) {  // the four waves' sums over their keys, through LDS (the tile is no longer needed)
+        float* part = (float*)lds;  // [wave][32 rows][DP]
+        __shared__ float part_top[kWaves][32], part_total[kWaves][32];
+#pragma unroll
+        for (int t = 0; t < kCols; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const f32x4_t v = {o[t][4 * j], o[t][4 * j + 1], o[t][4 * j + 2], o[t][4 * j + 3]};
+                *(f32x4_t*)(part + (wave * 32 + (lane & 31)) * DP + 32 * t + 8 * j + 4 * hi) = v;
+            }
+        if (lane < 32) {
+            part_top[wave][lane] = top;
+            part_total[wave][lane] = total;
+        }
+        __syncthreads();
+        if (wave != 0) return;
+        const int r = lane & 31;
+        float t0 = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) t0 = __builtin_fmaxf(t0, part_top[i][r]);
+        const float base = t0 == -INFINITY ? 0.f : t0;
+        float weight[kWaves];
+        total = 0.f;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) {
+            weight[i] = __builtin_amdgcn_exp2f(part_top[i][r] - base);
+            total += weight[i] * part_total[i][r];
+        }
+        top = t0;
+#pragma unroll
+        for (int t = 0; t < kCols; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < kWaves; ++i) sum += weight[i] * *(const f32x4_t*)(part + (i * 32 + r) * DP + 32 * t + 8 * j + 4 * hi);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[t][4 * j + e] = sum[e];
+            }
+    }
+
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    const float lse2 = total == 0.f ? -INFINITY : (top == -INFINITY ? 0.f : top) + log2f(total);
+    if (!row_in) return;
+    if (m.splits > 1) {
+        const int64_t at = ((int64_t)split * heads + bh) * m.rows + row;
+        float* to = m.part_out + at * a.D;
+        if (hi == 0) m.part_lse[at] = lse2;
+#pragma unroll
+        for (int t = 0; t < kCols; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int d = 32 * t + 8 * j + 4 * hi;
+                if (d < a.D) *(f32x4_t*)(to + d) = f32x4_t{o[t][4 * j] * inv, o[t][4 * j + 1] * inv, o[t][4 * j + 2] * inv, o[t][4 * j + 3] * inv};
+            }
+        return;
+    }
+    T* to = (T*)a.out + (((int64_t)b * a.q_len + s) * a.heads + head) * a.D;
+    if (hi == 0) a.lse[((int64_t)b * a.heads + head) * a.q_len + s] = lse2 * (1.f / kLog2e);
+#pragma unroll
+    for (int t = 0; t < kCols; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int d = 32 * t + 8 * j + 4 * hi;
+            if (d >= a.D) continue;
+            if constexpr (sizeof(T) == 2)
+                *(u32x2_t*)(to + d) = u32x2_t{pack_bf16x2(o[t][4 * j] * inv, o[t][4 * j + 1] * inv), pack_bf16x2(o[t][4 * j + 2] * inv, o[t][4 * j + 3] * inv)};
+            else
+                *(f32x4_t*)(to + d) = f32x4_t{o[t][4 * j] * inv, o[t][4 * j + 1] * inv, o[t][4 * j + 2] * inv, o[t][4 * j + 3] * inv};
+        }
+}
+
+// Joins the parts of a row: out = sum 2^(lse_i - max) out_i / sum 2^(lse_i - max).  A wavefront per row.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void attention_join_kernel(MfmaArgs m) {
+    const AttnArgs& a = m.a;
+    const int lane = threadIdx.x & 63, heads = (int)a.batch * a.kv_heads;
+    const int64_t index = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6), per_split = (int64_t)heads * m.rows;
+    if (index >= per_split) return;
+    const int bh = (int)(index / m.rows), row = (int)(index - (int64_t)bh * m.rows), b = bh / a.kv_heads, kvh = bh % a.kv_heads;
+    const int s = m.div(row), head = kvh * a.group + row - s * a.group;
+    float top = -INFINITY;
+    for (int i = lane; i < m.splits; i += 64) top = __builtin_fmaxf(top, m.part_lse[i * per_split + index]);
+    top = wave_max(top);
+    const float base = top == -INFINITY ? 0.f : top;
+    float total = 0.f, sum[4] = {};
+    for (int i = 0; i < m.splits; ++i) {
+        const float lse2 = m.part_lse[i * per_split + index];
+        if (lse2 == -INFINITY) continue;  // saw no key
+        const float weight = __builtin_amdgcn_exp2f(lse2 - base);
+        total += weight;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            if (c * 64 + lane < a.D) sum[c] += weight * m.part_out[(i * per_split + index) * a.D + c * 64 + lane];
+    }
+    T* to = (T*)a.out + (((int64_t)b * a.q_len + s) * a.heads + head) * a.D;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        if (c * 64 + lane < a.D) to[c * 64 + lane] = (T)(total == 0.f ? 0.f : sum[c] / total);
+    if (lane == 0) a.lse[((int64_t)b * a.heads + head) * a.q_len + s] = total == 0.f ? -INFINITY : (base + log2f(total)) * (1.f / kLog2e);
+}
+
+// lowest and highest document of every tile of `per` rows, row r standing for token r / group + offset; -1 where a token is none
+__global__ __launch_bounds__(kThreads) void attention_documents_kernel(const int32_t* __restrict__ docs, int kv_len, int per, int tiles, int rows,
+                                                                       int offset, GroupDiv div, int32_t* __restrict__ lowest,
+                                                                       int32_t* __restrict__ highest) {
+    const int tile_blocks = (tiles + kWaves - 1) / kWaves, b = blockIdx.x / tile_blocks, lane = threadIdx.x & 63;
+    const int tile = (blockIdx.x - b * tile_blocks) * kWaves + (threadIdx.x >> 6);
+    if (tile >= tiles) return;
+    int lo = 0x7FFFFFFF, hi = -1;
+    for (int i = lane; i < per; i += 64) {
+        const int row = tile * per + i;
+        if (row >= rows) break;
+        const int pos = div(row) + offset;
+        const int doc = pos >= 0 ? docs[(int64_t)b * kv_len + pos] : -1;
+        lo = min(lo, doc);
+        hi = max(hi, doc);
+    }
+    lo = wave_min_i32(lo);
+    hi = wave_max_i32(hi);
+    if (lane == 0) {
+        lowest[(int64_t)b * tiles + tile] = lo;
+        highest[(int64_t)b * tiles + tile] = hi;
+    }
+}
+
+template <typename T, int DP, bool KEYS>
+int launch(const MfmaArgs& m, hipStream_t s) {
+    typedef FwdShape<T, DP, KEYS> Sh;
+    const hipError_t e = hipFuncSetAttribute((const void*)attention_fwd_kernel<T, DP, KEYS>, hipFuncAttributeMaxDynamicSharedMemorySize, Sh::kLds);
+    if (e != hipSuccess) return PICOMOE_ERR_HIP_BASE + (int)e;
+    const int64_t blocks = (int64_t)m.n_tiles * m.a.batch * m.a.kv_heads;
+    if (blocks > 0x7FFFFFFF) return PICOMOE_ERR_TOO_LARGE;
+    attention_fwd_kernel<T, DP, KEYS><<<dim3((unsigned)blocks, (unsigned)m.splits), kThreads, Sh::kLds, s>>>(m);
+    if (m.splits > 1) {
+        const int64_t rows = (int64_t)m.a.batch * m.a.kv_heads * m.rows;
+        attention_join_kernel<T><<<(unsigned)((rows + kWaves - 1) / kWaves), kThreads, 0, s>>>(m);
+    }
+    return picomoe_launch_status();
+}
+
+struct Plan {
+    bool keys;      // the waves of a block share 32 rows
+    int tile, n_tiles, splits, walked_tiles;
+    int64_t doc_bytes, out_bytes, lse_bytes;
+};
+int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
+
+Plan plan(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, int kv_heads, int head_dim) {
+    Plan p;
+    const int64_t rows = q_len * (q_heads / kv_heads), heads = batch * kv_heads;
+    p.keys = rows <= 32;
+    p.tile = p.keys ? 128 : (dtype == PICOMOE_BF16 ? 64 : 32);
+    const int per = p.keys ? 32 : 32 * kWaves;
+    p.n_tiles = (int)((rows + per - 1) / per);
+    p.walked_tiles = (int)((kv_len + p.tile - 1) / p.tile);
+    // Fewer blocks than two per CU: the keys are cut until there are, down to four tiles a part
+    const int64_t blocks = heads * p.n_tiles;
+    int64_t splits = blocks > 0 ? 512 / blocks : 1;
+    if (splits > p.walked_tiles / 4) splits = p.walked_tiles / 4;
+    if (splits > 256) splits = 256;
+    p.splits = splits < 1 ? 1 : (int)splits;
+    p.doc_bytes = round16(batch * p.walked_tiles * 8);
+    p.out_bytes = p.splits > 1 ? round16((int64_t)p.splits * heads * rows * head_dim * 4) : 0;
+    p.lse_bytes = p.splits > 1 ? round16((int64_t)p.splits * heads * rows * 4) : 0;
+    return p;
+}
+
+}  // namespace
+
+bool attention_mfma_supported(int head_dim) { return head_dim <= 128; }
+
+int64_t attention_mfma_fwd_workspace(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, int kv_heads, int head_dim) {
+    const Plan p = plan(dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim);
+    return p.doc_bytes + p.out_bytes + p.lse_bytes + 16;
+}
+
+int attention_mfma_documents(const AttnArgs& a, int per, int tiles, int rows, int offset, int group, int32_t* lowest, int32_t* highest, hipStream_t s) {
+    if (tiles == 0) return PICOMOE_OK;
+    const int64_t blocks = (int64_t)((tiles + kWaves - 1) / kWaves) * a.batch;
+    if (blocks > 0x7FFFFFFF) return PICOMOE_ERR_TOO_LARGE;
+    attention_documents_kernel<<<(unsigned)blocks, kThreads, 0, s>>>(
+        a.docs, a.kv_len, per, tiles, rows, offset, group_div(group), lowest, highest);
+    return picomoe_launch_status();
+}
+
+int attention_mfma_fwd(const AttnArgs& a, hipStream_t s) {
+    const Plan p = plan(a.dtype, a.batch, a.q_len, a.kv_len, a.heads, a.kv_heads, a.D);
+    MfmaArgs m = {};
+    m.a = a;
+    m.div = group_div(a.group);
+    m.rows = a.q_len * a.group;
+    m.n_tiles = p.n_tiles;
+    m.splits = p.splits;
+    m.walked_tiles = p.walked_tiles;
+    int32_t* lowest = (int32_t*)a.ws;
+    m.doc_min = lowest;
+    m.doc_max = lowest + a.batch * p.walked_tiles;
+    m.part_out = (float*)(a.ws + p.doc_bytes);
+    m.part_lse = (float*)(a.ws + p.doc_bytes + p.out_bytes);
+    if (a.docs) {
+        const int rc = attention_mfma_documents(a, p.tile, p.walked_tiles, a.kv_len, 0, 1, lowest, lowest + a.batch * p.walked_tiles, s);
+        if (rc) return rc;
+    }
+    if (a.dtype == PICOMOE_BF16) {
+        if (a.D <= 64) return p.keys ? launch<__bf16, 64, true>(m, s) : launch<__bf16, 64, false>(m, s);
+        return p.keys ? launch<__bf16, 128, true>(m, s) : launch<__bf16, 128, false>(m, s);
+    }
+    if (a.D <= 64) return p.keys ? launch<float, 64, true>(m, s) : launch<float, 64, false>(m, s);
+    return p.keys ? launch<float, 128, true>(m, s) : launch<float, 128, false>(m, s);
+}

@@ -1,0 +1,246 @@
+// Pieces shared by the MFMA attention kernels (forward, dq, dk + dv): fragments, LDS tiles, the walk over tiles that the masks leave.
+//
+// Every product runs on 32 x 32 x 16 blocks (bf16: one v_mfma_f32_32x32x16_bf16; fp32: eight v_mfma_f32_32x32x2_f32 on the same
+// fragment layout): operand fragments hold 8 consecutive k of one row, k = 8 * (lane / 32) + e, row = lane % 32; results hold
+// column lane % 32 and rows 8 * (i / 4) + 4 * (lane / 32) + i % 4, i = 0 .. 15.  The first products of an attention are formed
+// transposed -- S^T[key, query] in the forward and dq kernels, S[query, key] in the dk / dv kernel -- so that eight consecutive
+// accumulators of a lane are, as they lie, the fragment of P (or dx) for the product that follows, with its k (keys or queries)
+// in the order 16 s + {4 hi + 0..3, 8 + 4 hi + 0..3}; the other operand is read from LDS in that order.  P never passes through LDS.
+#pragma once
+#include "attention.h"
+
+namespace {
+
+constexpr int kThreads = 256, kWaves = 4;
+
+template <typename T>
+struct Frag;
+template <>
+struct Frag<__bf16> {
+    bf16x8_t v;
+};
+template <>
+struct Frag<float> {
+    float v[8];
+};
+
+__device__ __forceinline__ void mma(f32x16_t& c, const Frag<__bf16>& a, const Frag<__bf16>& b) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b.v, c, 0, 0, 0);
+}
+__device__ __forceinline__ void mma(f32x16_t& c, const Frag<float>& a, const Frag<float>& b) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[e], b.v[e], c, 0, 0, 0);
+}
+
+// eight accumulators -> the fragment of the next product.  bf16: P in [0, 2^8] and dx are rounded to bf16 here, a relative
+// error of at most 2^-8 per term of the sums over keys (queries); the normaliser sums the unrounded P.
+template <typename T>
+__device__ __forceinline__ Frag<T> to_frag(const f32x16_t& c, int half);
+template <>
+__device__ __forceinline__ Frag<__bf16> to_frag<__bf16>(const f32x16_t& c, int half) {
+    u32x4_t w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(c[8 * half + 2 * i], c[8 * half + 2 * i + 1]);
+    return {__builtin_bit_cast(bf16x8_t, w)};
+}
+template <>
+__device__ __forceinline__ Frag<float> to_frag<float>(const f32x16_t& c, int half) {
+    Frag<float> f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f.v[i] = c[8 * half + i];
+    return f;
+}
+
+// eight elements of a global row from column col on; zeros from column D on
+template <typename T>
+__device__ __forceinline__ Frag<T> load_frag(const T* row, int col, int D) {
+    Frag<T> f;
+    if constexpr (sizeof(T) == 2) {
+        f.v = col < D ? *(const bf16x8_t*)(row + col) : bf16x8_t{};
+    } else {
+        const f32x4_t z = {0.f, 0.f, 0.f, 0.f};
+        const f32x4_t a = col < D ? *(const f32x4_t*)(row + col) : z, b = col < D ? *(const f32x4_t*)(row + col + 4) : z;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f.v[i] = a[i];
+            f.v[4 + i] = b[i];
+        }
+    }
+    return f;
+}
+
+template <typename T>
+__device__ __forceinline__ float frag_dot(const Frag<T>& a, const Frag<T>& b) {
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += (float)a.v[e] * (float)b.v[e];
+    return s;
+}
+
+// Tiles in LDS: `rows` rows of DP elements in 16-byte chunks, chunk c of a row at c ^ swizzle(row).  The 16 rows that a
+// ds_read_b128 serves at a time, and the 4 rows x 64 bytes of a transposing read, then lie on different banks.
+template <typename T, int DP>
+struct Tile {
+    static constexpr int kRowBytes = DP * (int)sizeof(T), kChunks = kRowBytes / 16, kPerChunk = 16 / (int)sizeof(T);
+    static constexpr int kRowsPerPass = kThreads / kChunks;  // rows that the block's threads stage at a time
+
+    __device__ static __forceinline__ uint32_t swizzle(int row) {
+        if (kRowBytes == 128) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+        return ((row & 3) << 2) | ((row >> 2) & 3);
+    }
+    __device__ static __forceinline__ uint32_t at(int row, uint32_t chunk) { return row * kRowBytes + ((chunk ^ swizzle(row)) << 4); }
+
+    // row `row` (a multiple of 32 plus lane % 32), elements 16 ks + 8 hi ..
+    __device__ static __forceinline__ Frag<T> frag(const char* tile, int row, int ks, int hi) {
+        Frag<T> f;
+        if constexpr (sizeof(T) == 2) {
+            f.v = *(const bf16x8_t*)(tile + at(row, 2 * ks + hi));
+        } else {
+            const f32x4_t a = *(const f32x4_t*)(tile + at(row, 4 * ks + 2 * hi)), b = *(const f32x4_t*)(tile + at(row, 4 * ks + 2 * hi + 1));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f.v[i] = a[i];
+                f.v[4 + i] = b[i];
+            }
+        }
+        return f;
+    }
+
+    // the tile transposed: column 32 t + lane % 32, rows row0 + {4 hi + 0..3, 8 + 4 hi + 0..3}
+    __device__ static __forceinline__ Frag<T> frag_t(const char* tile, int row0, int t, int lane) {
+        const int hi = lane >> 5;
+        Frag<T> f;
+        if constexpr (sizeof(T) == 2) {
+            typedef __attribute__((ext_vector_type(4))) short s16x4_t;
+            typedef __attribute__((ext_vector_type(8))) short s16x8_t;
+            // a transposing read: lane l of 16 gives the address of 4 elements of row (l / 4) and gets column l of 4 rows
+            const int row = row0 + 4 * hi + ((lane >> 2) & 3), col = 32 * t + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+            const uint32_t a0 = at(row, col >> 3) + ((col & 7) << 1), a1 = at(row + 8, col >> 3) + ((col & 7) << 1);
+            typedef __attribute__((address_space(3))) s16x4_t lds4;
+            const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(tile + a0));
+            const s16x4_t up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(tile + a1));
+            const s16x8_t v = {lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
+            f.v = __builtin_bit_cast(bf16x8_t, v);
+        } else {
+            const int col = 32 * t + (lane & 31);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int row = row0 + (e & 4) * 2 + 4 * hi + (e & 3);
+                f.v[e] = *(const float*)(tile + at(row, col >> 2) + ((col & 3) << 2));
+            }
+        }
+        return f;
+    }
+
+    __device__ static __forceinline__ float element(const char* tile, int row, int col) {
+        return to_f32(*(const T*)(tile + at(row, col / kPerChunk) + (col % kPerChunk) * (int)sizeof(T)));
+    }
+    // whether row `row` holds a value that is not finite
+    __device__ static __forceinline__ bool row_not_finite(const char* tile, int row) {
+        bool bad = false;
+        for (int c = 0; c < DP; ++c) bad |= !(__builtin_fabsf(element(tile, row, c)) < INFINITY);
+        return bad;
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ void zero_not_finite(Frag<T>& f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (!(__builtin_fabsf((float)f.v[e]) < INFINITY)) f.v[e] = (T)0.f;
+}
+
+__device__ __forceinline__ bool not_finite(const f32x16_t& c) {
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) bad |= !(__builtin_fabsf(c[i]) < INFINITY);
+    return bad;
+}
+
+// both halves of a wavefront: what lanes l and l + 32 hold
+__device__ __forceinline__ float other_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __builtin_fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float other_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ __forceinline__ int wave_min_i32(int v) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        const int o = __shfl_xor(v, off, 64);
+        v = o < v ? o : v;
+    }
+    return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ int wave_max_i32(int v) { return -wave_min_i32(-v); }
+
+// r / group for the rows of a key head, r < 2^31: a multiplication (exact: mul = floor(2^(31 + shift) / group) + 1, 2^shift >= group)
+struct GroupDiv {
+    uint32_t mul;
+    int shift;
+    __device__ __forceinline__ int operator()(int r) const { return shift == 0 ? r : (int)(__umulhi((uint32_t)r, mul) >> (shift - 1)); }
+};
+inline GroupDiv group_div(int group) {
+    int shift = 0;
+    while ((1 << shift) < group) ++shift;
+    return {shift == 0 ? 0u : (uint32_t)(((uint64_t)1 << (31 + shift)) / (uint32_t)group + 1), shift};
+}
+
+struct MfmaArgs {
+    AttnArgs a;
+    GroupDiv div;
+    int rows;                 // of a key head: q_len * group
+    int n_tiles, splits;      // tiles of the launch's blocks; parts that the walked dimension is cut into
+    const int32_t* doc_min;   // of every tile of the walked dimension: [batch, walked tiles], -1 among them where a token has no document
+    const int32_t* doc_max;
+    int walked_tiles;
+    float* part_out;          // splits > 1: partial results
+    float* part_lse;
+};
+
+// what a set of query rows may see, and which documents it has
+struct Reach {
+    int lo_min, lo_max, hi_min, hi_max, doc_min, doc_max;
+};
+
+// the walk over the walked dimension's tiles that pass `active`, 64 at a time; the same in every wave of a block
+template <typename F>
+struct TileWalk {
+    F active;
+    int base, end;
+    uint64_t mask;
+    __device__ __forceinline__ TileWalk(int first, int end_, F f) : active(f), base(first - 64), end(end_), mask(0) {}
+    __device__ __forceinline__ int next() {
+        while (mask == 0) {
+            base += 64;
+            if (base >= end) return -1;
+            const int t = base + (int)(threadIdx.x & 63);
+            mask = __ballot(t < end && active(t));
+        }
+        const int t = base + __builtin_ctzll(mask);
+        mask &= mask - 1;
+        return t;
+    }
+};
+
+// S in log2 units from q . k.  softcap > 0: cap2 * tanh(x / cap) with tanh(y) = 1 - 2 / (1 + e^(2y)); bf16 takes the hardware's
+// exponential and reciprocal (absolute error some 1e-7 of softcap), fp32 the library's tanh.
+struct ScoreScale {
+    float mul;   // log2(e) * scale, or with softcap: scale / softcap (fp32), 2 log2(e) scale / softcap (bf16)
+    float cap2;  // softcap * log2(e), 0: none
+};
+template <typename T>
+__device__ __forceinline__ ScoreScale score_scale(const AttnArgs& a) {
+    if (a.softcap > 0.f) return {a.scale / a.softcap * (sizeof(T) == 2 ? 2.f * kLog2e : 1.f), a.softcap * kLog2e};
+    return {a.scale * kLog2e, 0.f};
+}
+template <typename T>
+__device__ __forceinline__ float capped(float x, float mul) {  // tanh(x * scale / softcap)
+    if (sizeof(T) == 2) return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * mul));
+    return tanhf(x * mul);
+}
+
+}  // namespace
