@@ -263,7 +263,9 @@ int picomoe_qk_norm_rope_bwd(const void* dq_out, const void* dk_out, const void*
  * softcap * tanh(x / softcap); with slopes [q_heads] (fp32) minus slopes[h] * |p - j|.  Key j is seen when: causal == 0 or
  * j <= p or j < prefix_lengths[batch] (needs causal); window == 0 or |p - j| < window; document_ids [batch, kv_len] is NULL or
  * document_ids[j] == document_ids[p] >= 0.  A query that sees nothing gets out 0 and lse -inf, and no gradient; what is not seen has no influence,
- * NaN and infinities included.  The backward call takes the forward's out and lse; d_out, dq, dk, dv are dense.  head_dim a multiple
+ * NaN and infinities included.  The backward call takes the forward's out and lse; d_out, dq, dk, dv are dense.  out_residual (bf16, dense like
+ * out; NULL: none, ignored for fp32): what the rounding of out left, rounded to bf16; with it the backward's d_out . out is exact to
+ * 2^-16 instead of 2^-8.  head_dim a multiple
  * of 8, at most 256; strides multiples of 16 bytes, pointers 16-byte aligned; lengths at most 2^28, q_len * q_heads / kv_heads at
  * most 2^30.  Workspaces: 16-byte aligned, of the size that the _workspace_bytes call gives (-1 = bad arguments). */
 int64_t picomoe_attention_fwd_workspace_bytes(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, int kv_heads,
@@ -271,12 +273,12 @@ int64_t picomoe_attention_fwd_workspace_bytes(int dtype, int64_t batch, int64_t 
 int picomoe_attention_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
                           const int64_t* v_strides, int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads,
                           int kv_heads, int head_dim, float scale, float softcap, int causal, int64_t window,
-                          const float* slopes, const int32_t* document_ids, const int32_t* prefix_lengths, void* out, float* lse,
-                          void* workspace, int64_t workspace_bytes, void* stream);
+                          const float* slopes, const int32_t* document_ids, const int32_t* prefix_lengths, void* out, void* out_residual,
+                          float* lse, void* workspace, int64_t workspace_bytes, void* stream);
 int64_t picomoe_attention_bwd_workspace_bytes(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, int kv_heads,
                                               int head_dim);
 int picomoe_attention_bwd(const void* d_out, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
-                          const void* v, const int64_t* v_strides, const void* out, const float* lse, int dtype, int64_t batch,
+                          const void* v, const int64_t* v_strides, const void* out, const void* out_residual, const float* lse, int dtype, int64_t batch,
                           int64_t q_len, int64_t kv_len, int q_heads, int kv_heads, int head_dim, float scale, float softcap,
                           int causal, int64_t window, const float* slopes, const int32_t* document_ids,
                           const int32_t* prefix_lengths, void* dq, void* dk, void* dv, void* workspace, int64_t workspace_bytes,

@@ -58,9 +58,9 @@ _SIGNATURES = {
                                  _i64, _p],
     "picomoe_attention_fwd_workspace_bytes": [_i32, _i64, _i64, _i64, _i32, _i32, _i32],
     "picomoe_attention_fwd": [_p, _p, _p, _p, _p, _p, _i32, _i64, _i64, _i64, _i32, _i32, _i32, _f32, _f32, _i32, _i64, _p, _p, _p, _p, _p, _p,
-                              _i64, _p],
+                              _p, _i64, _p],
     "picomoe_attention_bwd_workspace_bytes": [_i32, _i64, _i64, _i64, _i32, _i32, _i32],
-    "picomoe_attention_bwd": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i32, _i64, _i64, _i64, _i32, _i32, _i32, _f32, _f32, _i32, _i64, _p, _p, _p,
+    "picomoe_attention_bwd": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i32, _i64, _i64, _i64, _i32, _i32, _i32, _f32, _f32, _i32, _i64, _p, _p, _p,
                               _p, _p, _p, _p, _i64, _p],
     "picomoe_diag_mfma_loop_flop": [_i32, _i64, _i32],
     "picomoe_diag_mfma_loop": [_p, _i64, _i32, _i64, _i64, _i64, _i32, _p, _p],

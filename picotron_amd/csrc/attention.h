@@ -9,7 +9,8 @@
 // window: |p - j| < window), and of those the ones of the query's document (equal ids, not negative).  A key outside takes no
 // part at all: NaN or infinity in its k or v (or in the q or d_out of a query that does not see the key) reaches nothing.
 //
-// Backward, g = d out:   D = g . out      dP[j] = g . v[j]      dz = P (dP - D)      dx = dz (1 - (y / softcap)^2)
+// Backward, g = d out:   D = g . out (with the residual of out, where it is bf16: D's error would reach every dx of the row)
+//       dP[j] = g . v[j]      dz = P (dP - D)      dx = dz (1 - (y / softcap)^2)
 //   dq = scale sum dx[j] k[j]      dk[j] = scale sum over queries and heads of the group of dx q      dv[j] = sum P[j] g
 #pragma once
 #include "common.h"
@@ -31,6 +32,7 @@ struct AttnArgs {
     const int32_t* prefix;                         // [batch] or NULL
     void* out;                                     // [batch, q_len, heads, D]
     float* lse;                                    // [batch, heads, q_len], natural log
+    void* residual;                                // like out: what its rounding to bf16 left, rounded to bf16; or NULL
     // backward
     const void* d_out;
     void *dq, *dk, *dv;

@@ -45,16 +45,16 @@ extern "C" int64_t picomoe_attention_fwd_workspace_bytes(int dtype, int64_t batc
 extern "C" int picomoe_attention_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
                                      const int64_t* v_strides, int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, int kv_heads,
                                      int head_dim, float scale, float softcap, int causal, int64_t window, const float* slopes,
-                                     const int32_t* document_ids, const int32_t* prefix_lengths, void* out, float* lse, void* workspace,
+                                     const int32_t* document_ids, const int32_t* prefix_lengths, void* out, void* out_residual, float* lse, void* workspace,
                                      int64_t workspace_bytes, void* stream) {
     PICOMOE_CHECK_ARG(sizes_ok(dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim));
     if (batch == 0 || q_len == 0) return PICOMOE_OK;
     AttnArgs a = {};
     PICOMOE_CHECK_ARG(fill(&a, q, q_strides, k, k_strides, v, v_strides, dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim, scale, softcap,
                            causal, window, slopes, document_ids, prefix_lengths));
-    PICOMOE_CHECK_ARG(out && lse && ((uintptr_t)out & 15) == 0 && workspace && ((uintptr_t)workspace & 15) == 0 &&
+    PICOMOE_CHECK_ARG(out && lse && (((uintptr_t)out | (uintptr_t)out_residual) & 15) == 0 && workspace && ((uintptr_t)workspace & 15) == 0 &&
                       workspace_bytes >= picomoe_attention_fwd_workspace_bytes(dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim));
-    a.out = out; a.lse = lse; a.ws = (char*)workspace;
+    a.out = out; a.residual = dtype == PICOMOE_BF16 ? out_residual : nullptr; a.lse = lse; a.ws = (char*)workspace;
     if (attention_mfma_supported(head_dim)) return attention_mfma_fwd(a, (hipStream_t)stream);
     return attention_simple_fwd(a, (hipStream_t)stream);
 }
@@ -67,7 +67,7 @@ extern "C" int64_t picomoe_attention_bwd_workspace_bytes(int dtype, int64_t batc
 }
 
 extern "C" int picomoe_attention_bwd(const void* d_out, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
-                                     const int64_t* v_strides, const void* out, const float* lse, int dtype, int64_t batch, int64_t q_len,
+                                     const int64_t* v_strides, const void* out, const void* out_residual, const float* lse, int dtype, int64_t batch, int64_t q_len,
                                      int64_t kv_len, int q_heads, int kv_heads, int head_dim, float scale, float softcap, int causal, int64_t window,
                                      const float* slopes, const int32_t* document_ids, const int32_t* prefix_lengths, void* dq, void* dk, void* dv,
                                      void* workspace, int64_t workspace_bytes, void* stream) {
@@ -77,9 +77,9 @@ extern "C" int picomoe_attention_bwd(const void* d_out, const void* q, const int
     PICOMOE_CHECK_ARG(fill(&a, q, q_strides, k, k_strides, v, v_strides, dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim, scale, softcap,
                            causal, window, slopes, document_ids, prefix_lengths));
     auto ok16 = [](const void* p) { return p && ((uintptr_t)p & 15) == 0; };
-    PICOMOE_CHECK_ARG(ok16(d_out) && ok16(out) && lse && ok16(dq) && ok16(dk) && ok16(dv) && ok16(workspace) &&
+    PICOMOE_CHECK_ARG(ok16(d_out) && ok16(out) && ((uintptr_t)out_residual & 15) == 0 && lse && ok16(dq) && ok16(dk) && ok16(dv) && ok16(workspace) &&
                       workspace_bytes >= picomoe_attention_bwd_workspace_bytes(dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim));
-    a.out = (void*)out; a.lse = (float*)lse; a.d_out = d_out; a.dq = dq; a.dk = dk; a.dv = dv;
+    a.out = (void*)out; a.residual = dtype == PICOMOE_BF16 ? (void*)out_residual : nullptr; a.lse = (float*)lse; a.d_out = d_out; a.dq = dq; a.dk = dk; a.dv = dv;
     a.delta = (float*)workspace;
     a.ws = (char*)workspace + round16(batch * q_len * q_heads * 4);
     if (attention_mfma_supported(head_dim)) return attention_mfma_bwd(a, (hipStream_t)stream);

@@ -17,14 +17,16 @@ template <typename T, int DP>
 struct DqShape {
     static constexpr int kTile = sizeof(T) == 2 ? 64 : 32;
     static constexpr int kTileBytes = kTile * DP * (int)sizeof(T);
-    static constexpr int kLds = 2 * 2 * kTileBytes + 2 * kTile * 4;
+    static constexpr int kBuf = 2 * kTileBytes + kTile * 4;  // K, V, document ids
+    static constexpr int kLds = 2 * kBuf;
 };
 
-template <typename T, int DP>
+// PLAIN: neither softcap nor slopes
+template <typename T, int DP, bool PLAIN>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq_kernel(MfmaArgs m) {
     typedef DqShape<T, DP> Sh;
     typedef Tile<T, DP> Tl;
-    constexpr int kSub = Sh::kTile / 32, kSteps = DP / 16, kCols = DP / 32, kPasses = Sh::kTile / Tl::kRowsPerPass;
+    constexpr int kSub = Sh::kTile / 32, kSteps = DP / 16, kCols = DP / 32;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const AttnArgs& a = m.a;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5;
@@ -50,6 +52,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq
             qf[ks] = load_frag<T>(q, 16 * ks + 8 * hi, a.D);
             gf[ks] = load_frag<T>(g, 16 * ks + 8 * hi, a.D);
             delta += frag_dot(gf[ks], load_frag<T>(out, 16 * ks + 8 * hi, a.D));
+            if (sizeof(T) == 2 && a.residual) delta += frag_dot(gf[ks], load_frag<T>((const T*)a.residual + out_row * a.D, 16 * ks + 8 * hi, a.D));
         }
     }
     delta = other_sum(delta);
@@ -93,33 +96,13 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq
 
     const T* kbase = (const T*)a.k.p + b * a.k.sb + kvh * a.k.sh;
     const T* vbase = (const T*)a.v.p + b * a.v.sb + kvh * a.v.sh;
-    const int st_row = threadIdx.x / Tl::kChunks, st_chunk = threadIdx.x % Tl::kChunks;
-    const bool st_in = st_chunk * Tl::kPerChunk < a.D;
-    u32x4_t kreg[kPasses], vreg[kPasses];
-    int doc_reg = 0;
-    auto fetch = [&](int t) {
-#pragma unroll
-        for (int i = 0; i < kPasses; ++i) {
-            int key = t * Sh::kTile + i * Tl::kRowsPerPass + st_row;
-            key = key < a.kv_len ? key : a.kv_len - 1;
-            const u32x4_t zero = {0u, 0u, 0u, 0u};
-            kreg[i] = st_in ? *(const u32x4_t*)(kbase + (int64_t)key * a.k.ss + st_chunk * Tl::kPerChunk) : zero;
-            vreg[i] = st_in ? *(const u32x4_t*)(vbase + (int64_t)key * a.v.ss + st_chunk * Tl::kPerChunk) : zero;
-        }
-        if (a.docs && threadIdx.x < Sh::kTile) {
-            const int key = t * Sh::kTile + (int)threadIdx.x;
-            doc_reg = key < a.kv_len ? a.docs[(int64_t)b * a.kv_len + key] : -1;
-        }
-    };
-    auto stage = [&](int buf) {
-        char* kt = lds + buf * 2 * Sh::kTileBytes;
-#pragma unroll
-        for (int i = 0; i < kPasses; ++i) {
-            const uint32_t at = Tl::at(i * Tl::kRowsPerPass + st_row, st_chunk);
-            *(u32x4_t*)(kt + at) = kreg[i];
-            *(u32x4_t*)(kt + Sh::kTileBytes + at) = vreg[i];
-        }
-        if (a.docs && threadIdx.x < Sh::kTile) ((int32_t*)(lds + 4 * Sh::kTileBytes))[buf * Sh::kTile + threadIdx.x] = doc_reg;
+    if (a.D < DP) clear_lds(lds, Sh::kLds);
+    auto fetch = [&](int t, int buf) {
+        char* kt = lds + buf * Sh::kBuf;
+        auto key_at = [&](int r) { return (int64_t)min(t * Sh::kTile + r, a.kv_len - 1); };
+        Tl::template load<Sh::kTile>(kt, a.D, [&](int r) { return kbase + key_at(r) * a.k.ss; });
+        Tl::template load<Sh::kTile>(kt + Sh::kTileBytes, a.D, [&](int r) { return vbase + key_at(r) * a.v.ss; });
+        if (a.docs && wave == 0 && lane < Sh::kTile) load4_to_lds(a.docs + (int64_t)b * a.kv_len + key_at(lane), kt + 2 * Sh::kTileBytes);
     };
 
     const ScoreScale sc = score_scale<T>(a);
@@ -133,15 +116,15 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq
         auto active = [&](int t) { return !a.docs || (doc_max[t] >= blk.doc_min && doc_min[t] <= blk.doc_max); };
         TileWalk<decltype(active)> walk(first, end, active);
         int cur = walk.next(), buf = 0;
-        if (cur >= 0) fetch(cur);
+        if (cur >= 0) fetch(cur, 0);
         while (cur >= 0) {
-            stage(buf);
-            const int following = walk.next();
-            if (following >= 0) fetch(following);
+            lds_loads_done();
             __syncthreads();
-            const char* kt = lds + buf * 2 * Sh::kTileBytes;
+            const int following = walk.next();
+            if (following >= 0) fetch(following, buf ^ 1);
+            const char* kt = lds + buf * Sh::kBuf;
             const char* vt = kt + Sh::kTileBytes;
-            const int32_t* docs = (const int32_t*)(lds + 4 * Sh::kTileBytes) + buf * Sh::kTile;
+            const int32_t* docs = (const int32_t*)(vt + Sh::kTileBytes);
             const int key0 = cur * Sh::kTile, key1 = key0 + Sh::kTile - 1;
             bool in = key0 <= w.hi_max && key1 >= w.lo_min, full = key0 >= w.lo_max && key1 <= w.hi_min;
             if (a.docs) {
@@ -162,7 +145,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq
                     }
 #pragma unroll
                     for (int i = 0; i < 16; ++i) dp[i] -= delta;
-                    if (sc.cap2 > 0.f) {
+                    if (PLAIN) {
+                    } else if (sc.cap2 > 0.f) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             const float t = capped<T>(x[i], sc.mul);
@@ -173,13 +157,13 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq
 #pragma unroll
                         for (int i = 0; i < 16; ++i) x[i] *= sc.mul;
                     }
-                    if (a.slopes) {
+                    if (!PLAIN && a.slopes) {
                         const float away = (float)(pos - key0 - 4 * hi);
 #pragma unroll
                         for (int i = 0; i < 16; ++i) x[i] -= slope2 * __builtin_fabsf(away - (float)(u * 32 + 8 * (i / 4) + i % 4));
                     }
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i] = __builtin_amdgcn_exp2f(x[i] - lse2) * dp[i];
+                    for (int i = 0; i < 16; ++i) x[i] = __builtin_amdgcn_exp2f(PLAIN ? __builtin_fmaf(x[i], sc.mul, -lse2) : x[i] - lse2) * dp[i];
                     if (!full) {
                         const int from = span.lo - key0 - 4 * hi;
 #pragma unroll
@@ -250,14 +234,18 @@ struct DkvShape {
     static constexpr int kKeys = 32 * kWaves;     // keys of a block
     static constexpr int kTileBytes = kTile * DP * (int)sizeof(T);
     static constexpr int kStats = 7 * kTile * 4;  // lse2, delta, slope2 (floats), position, first key, keys, document (ints)
-    static constexpr int kLds = 2 * (2 * kTileBytes + kStats);
+    static constexpr int kBuf = 2 * kTileBytes + kStats;
+    // V's fragments are the ones that do not fit the 256 registers of a lane at head_dim 128 (dk, dv, K, S, dP do): read from LDS
+    static constexpr bool kVInLds = DP == 128;
+    static constexpr int kVBytes = kVInLds ? kKeys * DP * (int)sizeof(T) : 0;
+    static constexpr int kLds = 2 * kBuf + kVBytes;
 };
 
-template <typename T, int DP>
+template <typename T, int DP, bool PLAIN>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dkv_kernel(MfmaArgs m) {
     typedef DkvShape<T, DP> Sh;
     typedef Tile<T, DP> Tl;
-    constexpr int kSteps = DP / 16, kCols = DP / 32, kPasses = Sh::kTile / Tl::kRowsPerPass, kBuf = 2 * Sh::kTileBytes + Sh::kStats;
+    constexpr int kSteps = DP / 16, kCols = DP / 32, kBuf = Sh::kBuf;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const AttnArgs& a = m.a;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5;
@@ -267,14 +255,20 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
     const int wave0 = block0 + wave * 32, wave1 = wave0 + 31;
     const int key = wave0 + (lane & 31), key_in = key < a.kv_len, key_at = key_in ? key : a.kv_len - 1;
 
+    if (a.D < DP) clear_lds(lds, Sh::kLds);
     Frag<T> kf[kSteps], vf[kSteps];
+    char* vtile = lds + 2 * kBuf;
+    if (Sh::kVInLds) {
+        const T* v = (const T*)a.v.p + b * a.v.sb + kvh * a.v.sh;
+        Tl::template load<Sh::kKeys>(vtile, a.D, [&](int r) { return v + (int64_t)min(block0 + r, a.kv_len - 1) * a.v.ss; });
+    }
     {
         const T* k = (const T*)a.k.p + b * a.k.sb + (int64_t)key_at * a.k.ss + kvh * a.k.sh;
         const T* v = (const T*)a.v.p + b * a.v.sb + (int64_t)key_at * a.v.ss + kvh * a.v.sh;
 #pragma unroll
         for (int ks = 0; ks < kSteps; ++ks) {
             kf[ks] = load_frag<T>(k, 16 * ks + 8 * hi, a.D);
-            vf[ks] = load_frag<T>(v, 16 * ks + 8 * hi, a.D);
+            if (!Sh::kVInLds) vf[ks] = load_frag<T>(v, 16 * ks + 8 * hi, a.D);
         }
     }
     // keys past the end get a document of their own; without documents every key and row has document 0
@@ -305,22 +299,21 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
     auto first_query = [&](int t) { return m.div(t * Sh::kTile); };
     auto last_query = [&](int t) { return m.div(min(t * Sh::kTile + Sh::kTile, m.rows) - 1); };
 
-    // staging: this thread's row of a tile and its chunk
-    const int st_row = threadIdx.x / Tl::kChunks, st_chunk = threadIdx.x % Tl::kChunks;
-    const bool st_in = st_chunk * Tl::kPerChunk < a.D;
     const T* qbase = (const T*)a.q.p + b * a.q.sb + (int64_t)(kvh * a.group) * a.q.sh;
     const T* gbase = (const T*)a.d_out + ((int64_t)b * a.q_len * a.heads + kvh * a.group) * a.D;
-    u32x4_t qreg[kPasses], greg[kPasses];
     float stat_f[3] = {};
     int stat_i[4] = {};
-    auto fetch = [&](int t) {
-#pragma unroll
-        for (int i = 0; i < kPasses; ++i) {
-            const int r = min(t * Sh::kTile + i * Tl::kRowsPerPass + st_row, m.rows - 1), s = m.div(r), h = r - s * a.group;
-            const u32x4_t zero = {0u, 0u, 0u, 0u};
-            qreg[i] = st_in ? *(const u32x4_t*)(qbase + s * a.q.ss + h * a.q.sh + st_chunk * Tl::kPerChunk) : zero;
-            greg[i] = st_in ? *(const u32x4_t*)(gbase + ((int64_t)s * a.heads + h) * a.D + st_chunk * Tl::kPerChunk) : zero;
-        }
+    auto fetch = [&](int t, int buf) {
+        char* qt = lds + buf * kBuf;
+        auto row_at = [&](int r) { return min(t * Sh::kTile + r, m.rows - 1); };
+        Tl::template load<Sh::kTile>(qt, a.D, [&](int r) {
+            const int s = m.div(row_at(r)), h = row_at(r) - s * a.group;
+            return qbase + s * a.q.ss + h * a.q.sh;
+        });
+        Tl::template load<Sh::kTile>(qt + Sh::kTileBytes, a.D, [&](int r) {
+            const int s = m.div(row_at(r)), h = row_at(r) - s * a.group;
+            return gbase + ((int64_t)s * a.heads + h) * a.D;
+        });
         if (threadIdx.x < Sh::kTile) {
             const int r = t * Sh::kTile + (int)threadIdx.x, rc = min(r, m.rows - 1), s = m.div(rc), h = kvh * a.group + rc - s * a.group;
             const int64_t stat = ((int64_t)b * a.heads + h) * a.q_len + s;
@@ -336,16 +329,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
             stat_i[3] = span.doc;
         }
     };
-    auto stage = [&](int buf) {
-        char* qt = lds + buf * kBuf;
-#pragma unroll
-        for (int i = 0; i < kPasses; ++i) {
-            const uint32_t at = Tl::at(i * Tl::kRowsPerPass + st_row, st_chunk);
-            *(u32x4_t*)(qt + at) = qreg[i];
-            *(u32x4_t*)(qt + Sh::kTileBytes + at) = greg[i];
-        }
+    auto stage_stats = [&](int buf) {
         if (threadIdx.x < Sh::kTile) {
-            float* f = (float*)(qt + 2 * Sh::kTileBytes);
+            float* f = (float*)(lds + buf * kBuf + 2 * Sh::kTileBytes);
 #pragma unroll
             for (int i = 0; i < 3; ++i) f[i * Sh::kTile + threadIdx.x] = stat_f[i];
 #pragma unroll
@@ -374,12 +360,13 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
             }
         };
         int cur = next(), buf = 0;
-        if (cur >= 0) fetch(cur);
+        if (cur >= 0) fetch(cur, 0);
         while (cur >= 0) {
-            stage(buf);
-            const int following = next();
-            if (following >= 0) fetch(following);
+            stage_stats(buf);
+            lds_loads_done();
             __syncthreads();
+            const int following = next();
+            if (following >= 0) fetch(following, buf ^ 1);
             const char* qt = lds + buf * kBuf;
             const char* gt = qt + Sh::kTileBytes;
             const float* stats = (const float*)(gt + Sh::kTileBytes);
@@ -399,7 +386,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
 #pragma unroll
                 for (int ks = 0; ks < kSteps; ++ks) {
                     mma(x, Tl::frag(qt, lane & 31, ks, hi), kf[ks]);
-                    mma(dp, Tl::frag(gt, lane & 31, ks, hi), vf[ks]);
+                    mma(dp, Tl::frag(gt, lane & 31, ks, hi), Sh::kVInLds ? Tl::frag(vtile, wave * 32 + (lane & 31), ks, hi) : vf[ks]);
                 }
                 auto stat4 = [&](int which, int j) { return *(const f32x4_t*)(stats + which * Sh::kTile + 8 * j + 4 * hi); };
                 auto stat4i = [&](int which, int j) {
@@ -412,7 +399,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
 #pragma unroll
                     for (int i = 0; i < 4; ++i) dp[4 * j + i] -= delta[i];
                 }
-                if (sc.cap2 > 0.f) {
+                if (PLAIN) {
+                } else if (sc.cap2 > 0.f) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const float t = capped<T>(x[i], sc.mul);
@@ -423,7 +411,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
 #pragma unroll
                     for (int i = 0; i < 16; ++i) x[i] *= sc.mul;
                 }
-                if (a.slopes) {
+                if (!PLAIN && a.slopes) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const f32x4_t slope2 = stat4(2, j);
@@ -436,7 +424,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
                 for (int j = 0; j < 4; ++j) {
                     const f32x4_t lse2 = stat4(0, j);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) x[4 * j + i] = __builtin_amdgcn_exp2f(x[4 * j + i] - lse2[i]);
+                    for (int i = 0; i < 4; ++i) x[4 * j + i] = __builtin_amdgcn_exp2f(PLAIN ? __builtin_fmaf(x[4 * j + i], sc.mul, -lse2[i]) : x[4 * j + i] - lse2[i]);
                 }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) dp[i] *= x[i];
@@ -545,10 +533,11 @@ Plan plan(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, 
     p.row_tiles = (int)((rows + 31) / 32);
     p.dq_tiles = (int)((rows + 32 * kWaves - 1) / (32 * kWaves));
     p.key_blocks = (int)((kv_len + 32 * kWaves - 1) / (32 * kWaves));
-    // Fewer blocks than two per CU: the rows are dealt to several, at least four tiles each
+    // A mask leaves the key blocks unequal work (causal: the first sees all rows, the last its own): the rows are dealt to
+    // several blocks until there are eight per CU to balance with, of at least 16 row tiles each
     const int64_t blocks = batch * kv_heads * p.key_blocks;
-    int64_t splits = blocks > 0 ? 512 / blocks : 1;
-    if (splits > p.row_tiles / 4) splits = p.row_tiles / 4;
+    int64_t splits = blocks > 0 ? (2048 + blocks - 1) / blocks : 1;
+    if (splits > p.row_tiles / 16) splits = p.row_tiles / 16;
     if (splits > 16) splits = 16;
     p.splits = splits < 1 ? 1 : (int)splits;
     p.key_docs = round16(batch * p.key_tiles * 8);
@@ -557,12 +546,12 @@ Plan plan(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, 
     return p;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool PLAIN>
 int launch(MfmaArgs m, const Plan& p, hipStream_t s) {
     typedef DqShape<T, DP> Q;
     typedef DkvShape<T, DP> K;
-    hipError_t e = hipFuncSetAttribute((const void*)attention_dq_kernel<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, Q::kLds);
-    if (e == hipSuccess) e = hipFuncSetAttribute((const void*)attention_dkv_kernel<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, K::kLds);
+    hipError_t e = hipFuncSetAttribute((const void*)attention_dq_kernel<T, DP, PLAIN>, hipFuncAttributeMaxDynamicSharedMemorySize, Q::kLds);
+    if (e == hipSuccess) e = hipFuncSetAttribute((const void*)attention_dkv_kernel<T, DP, PLAIN>, hipFuncAttributeMaxDynamicSharedMemorySize, K::kLds);
     if (e != hipSuccess) return PICOMOE_ERR_HIP_BASE + (int)e;
     const AttnArgs& a = m.a;
     const int64_t heads = a.batch * a.kv_heads, dq_blocks = heads * p.dq_tiles, key_blocks = heads * p.key_blocks;
@@ -581,16 +570,21 @@ int launch(MfmaArgs m, const Plan& p, hipStream_t s) {
     m.walked_tiles = p.key_tiles;
     m.n_tiles = p.dq_tiles;
     m.splits = 1;
-    attention_dq_kernel<T, DP><<<(unsigned)dq_blocks, kThreads, Q::kLds, s>>>(m);
+    attention_dq_kernel<T, DP, PLAIN><<<(unsigned)dq_blocks, kThreads, Q::kLds, s>>>(m);
     m.doc_min = row_docs;
     m.doc_max = row_docs + a.batch * p.row_tiles;
     m.walked_tiles = p.row_tiles;
     m.n_tiles = p.key_blocks;
     m.splits = p.splits;
-    attention_dkv_kernel<T, DP><<<dim3((unsigned)key_blocks, (unsigned)p.splits), kThreads, K::kLds, s>>>(m);
+    attention_dkv_kernel<T, DP, PLAIN><<<dim3((unsigned)key_blocks, (unsigned)p.splits), kThreads, K::kLds, s>>>(m);
     if (p.splits > 1)
         attention_dkv_join_kernel<T><<<(unsigned)join_blocks, kThreads, 0, s>>>((const f32x4_t*)m.part_out, p.splits, quads, (T*)a.dk, (T*)a.dv);
     return picomoe_launch_status();
+}
+
+template <typename T, int DP>
+int launch_for(const MfmaArgs& m, const Plan& p, hipStream_t s) {
+    return m.a.softcap == 0.f && !m.a.slopes ? launch<T, DP, true>(m, p, s) : launch<T, DP, false>(m, p, s);
 }
 
 }  // namespace
@@ -606,6 +600,6 @@ int attention_mfma_bwd(const AttnArgs& a, hipStream_t s) {
     m.a = a;
     m.div = group_div(a.group);
     m.rows = a.q_len * a.group;
-    if (a.dtype == PICOMOE_BF16) return a.D <= 64 ? launch<__bf16, 64>(m, p, s) : launch<__bf16, 128>(m, p, s);
-    return a.D <= 64 ? launch<float, 64>(m, p, s) : launch<float, 128>(m, p, s);
+    if (a.dtype == PICOMOE_BF16) return a.D <= 64 ? launch_for<__bf16, 64>(m, p, s) : launch_for<__bf16, 128>(m, p, s);
+    return a.D <= 64 ? launch_for<float, 64>(m, p, s) : launch_for<float, 128>(m, p, s);
 }

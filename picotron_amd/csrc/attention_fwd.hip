@@ -3,8 +3,8 @@
 // The query heads of a key head are one list of rows, row r = query r / group, head r % group of the group, so that a K / V
 // tile in LDS serves all of them and one new token of a large group still fills a fragment.  A wavefront owns 32 rows, one per
 // lane pair (lane, lane + 32): S^T[key, row] = K Q^T keeps a row's scores in its two lanes -- maximum and sum need one exchange
-// between them --, and O^T[d, row] = V^T P^T takes P from registers.  Tiles are staged through registers into one of two LDS
-// buffers while the other is multiplied, one barrier per tile.
+// between them --, and O^T[d, row] = V^T P^T takes P from registers.  Tiles are loaded straight into one of two LDS buffers while
+// the other is multiplied, one barrier per tile.
 //
 // The accumulated O is only rescaled when a row's maximum grows by more than 2^8: until then P is at most 2^8 instead of 1,
 // which costs bf16 nothing and fp32 sums nothing, and the 64 multiplications per tile fall away in all but the first tiles.
@@ -21,16 +21,18 @@ struct FwdShape {
     static constexpr int kTile = KEYS ? 128 : (sizeof(T) == 2 ? 64 : 32);  // keys of a tile
     static constexpr int kWaveKeys = KEYS ? 32 : kTile;
     static constexpr int kRows = KEYS ? 32 : 32 * kWaves;  // rows of a block
-    static constexpr int kBuffers = KEYS ? 1 : 2;
     static constexpr int kTileBytes = kTile * DP * (int)sizeof(T);
-    static constexpr int kLds = kBuffers * 2 * kTileBytes + kBuffers * kTile * 4;  // K, V, document ids
+    static constexpr int kBuffers = kTileBytes <= 32768 ? 2 : 1;  // two of 128 KB do not fit
+    static constexpr int kBuf = 2 * kTileBytes + kTile * 4;       // K, V, document ids
+    static constexpr int kLds = kBuffers * kBuf;
 };
 
-template <typename T, int DP, bool KEYS>
+// PLAIN: neither softcap nor slopes, scale > 0: the scale goes into the exponent's multiply-add.
+template <typename T, int DP, bool KEYS, bool PLAIN>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fwd_kernel(MfmaArgs m) {
     typedef FwdShape<T, DP, KEYS> Sh;
     typedef Tile<T, DP> Tl;
-    constexpr int kSub = Sh::kWaveKeys / 32, kSteps = DP / 16, kCols = DP / 32, kPasses = Sh::kTile / Tl::kRowsPerPass;
+    constexpr int kSub = Sh::kWaveKeys / 32, kSteps = DP / 16, kCols = DP / 32;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const AttnArgs& a = m.a;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5;
@@ -93,33 +95,16 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
 
     const T* kbase = (const T*)a.k.p + b * a.k.sb + kvh * a.k.sh;
     const T* vbase = (const T*)a.v.p + b * a.v.sb + kvh * a.v.sh;
-    const int st_row = threadIdx.x / Tl::kChunks, st_chunk = threadIdx.x % Tl::kChunks;
-    const bool st_in = st_chunk * Tl::kPerChunk < a.D;
-    u32x4_t kreg[kPasses], vreg[kPasses];
-    int doc_reg = 0;
-    auto fetch = [&](int t) {
-#pragma unroll
-        for (int i = 0; i < kPasses; ++i) {
-            int key = t * Sh::kTile + i * Tl::kRowsPerPass + st_row;
-            key = key < a.kv_len ? key : a.kv_len - 1;  // keys past the end are hidden by every row's interval
-            const u32x4_t zero = {0u, 0u, 0u, 0u};
-            kreg[i] = st_in ? *(const u32x4_t*)(kbase + (int64_t)key * a.k.ss + st_chunk * Tl::kPerChunk) : zero;
-            vreg[i] = st_in ? *(const u32x4_t*)(vbase + (int64_t)key * a.v.ss + st_chunk * Tl::kPerChunk) : zero;
-        }
-        if (a.docs && threadIdx.x < Sh::kTile) {
-            const int key = t * Sh::kTile + (int)threadIdx.x;
-            doc_reg = key < a.kv_len ? a.docs[(int64_t)b * a.kv_len + key] : -1;
-        }
-    };
-    auto stage = [&](int buf) {
-        char* kt = lds + buf * 2 * Sh::kTileBytes;
-#pragma unroll
-        for (int i = 0; i < kPasses; ++i) {
-            const uint32_t at = Tl::at(i * Tl::kRowsPerPass + st_row, st_chunk);
-            *(u32x4_t*)(kt + at) = kreg[i];
-            *(u32x4_t*)(kt + Sh::kTileBytes + at) = vreg[i];
-        }
-        if (a.docs && threadIdx.x < Sh::kTile) ((int32_t*)(lds + Sh::kBuffers * 2 * Sh::kTileBytes))[buf * Sh::kTile + threadIdx.x] = doc_reg;
+    if (a.D < DP) clear_lds(lds, Sh::kLds);
+    auto fetch = [&](int t, int buf) {
+        char* kt = lds + buf * Sh::kBuf;
+        // keys past the end are hidden by every row's interval
+        auto key_at = [&](int r) { return (int64_t)min(t * Sh::kTile + r, a.kv_len - 1); };
+        Tl::template load<Sh::kTile>(kt, a.D, [&](int r) { return kbase + key_at(r) * a.k.ss; });
+        Tl::template load<Sh::kTile>(kt + Sh::kTileBytes, a.D, [&](int r) { return vbase + key_at(r) * a.v.ss; });
+        if (a.docs && wave < Sh::kTile / 64)
+            load4_to_lds(a.docs + (int64_t)b * a.kv_len + key_at(wave * 64 + lane), kt + 2 * Sh::kTileBytes + wave * 256);
+        if (a.docs && Sh::kTile < 64 && wave == 0 && lane < Sh::kTile) load4_to_lds(a.docs + (int64_t)b * a.kv_len + key_at(lane), kt + 2 * Sh::kTileBytes);
     };
 
     const ScoreScale sc = score_scale<T>(a);
@@ -140,16 +125,15 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
         auto active = [&](int t) { return !a.docs || (doc_max[t] >= blk.doc_min && doc_min[t] <= blk.doc_max); };
         TileWalk<decltype(active)> walk(first, end, active);
         int cur = walk.next(), buf = 0;
-        if (cur >= 0) fetch(cur);
+        if (cur >= 0) fetch(cur, 0);
         while (cur >= 0) {
-            if (Sh::kBuffers == 1) __syncthreads();
-            stage(buf);
+            lds_loads_done();
+            __syncthreads();  // the tile is there, and every wave is done with the other buffer
             const int following = walk.next();
-            if (following >= 0) fetch(following);
-            __syncthreads();
-            const char* kt = lds + buf * 2 * Sh::kTileBytes;
+            if (Sh::kBuffers == 2 && following >= 0) fetch(following, buf ^ 1);
+            const char* kt = lds + buf * Sh::kBuf;
             const char* vt = kt + Sh::kTileBytes;
-            const int32_t* docs = (const int32_t*)(lds + Sh::kBuffers * 2 * Sh::kTileBytes) + buf * Sh::kTile;
+            const int32_t* docs = (const int32_t*)(vt + Sh::kTileBytes);
             const int sub0 = KEYS ? wave * 32 : 0, key0 = cur * Sh::kTile + sub0, key1 = key0 + Sh::kWaveKeys - 1;
             bool in = key0 <= w.hi_max && key1 >= w.lo_min, full = key0 >= w.lo_max && key1 <= w.hi_min;
             if (a.docs) {
@@ -166,7 +150,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
 #pragma unroll
                     for (int ks = 0; ks < kSteps; ++ks) mma(x[u], Tl::frag(kt, sub0 + u * 32 + (lane & 31), ks, hi), qf[ks]);
                 }
-                if (sc.cap2 > 0.f) {
+                if (PLAIN) {
+                } else if (sc.cap2 > 0.f) {
 #pragma unroll
                     for (int u = 0; u < kSub; ++u)
 #pragma unroll
@@ -177,7 +162,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
 #pragma unroll
                         for (int i = 0; i < 16; ++i) x[u][i] *= sc.mul;
                 }
-                if (a.slopes) {
+                if (!PLAIN && a.slopes) {
                     const float away = (float)(pos - key0 - 4 * hi);
 #pragma unroll
                     for (int u = 0; u < kSub; ++u)
@@ -201,7 +186,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
                 for (int u = 0; u < kSub; ++u)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) mx = __builtin_fmaxf(mx, x[u][i]);
-                mx = other_max(mx);
+                mx = other_max(mx) * (PLAIN ? sc.mul : 1.f);
                 if (__any(mx > top + kLazy)) {
                     const float old = top;
                     top = __builtin_fmaxf(top, mx);
@@ -217,7 +202,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
                 for (int u = 0; u < kSub; ++u)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        x[u][i] = __builtin_amdgcn_exp2f(x[u][i] - base);
+                        x[u][i] = __builtin_amdgcn_exp2f(PLAIN ? __builtin_fmaf(x[u][i], sc.mul, -base) : x[u][i] - base);
                         total += x[u][i];
                     }
 #pragma unroll
@@ -247,7 +232,12 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
                 }
             }
             cur = following;
-            buf = Sh::kBuffers == 2 ? buf ^ 1 : 0;
+            if (Sh::kBuffers == 2) {
+                buf ^= 1;
+            } else if (cur >= 0) {
+                __syncthreads();
+                fetch(cur, 0);
+            }
         }
     };
     run(std::integral_constant<bool, false>());
@@ -325,10 +315,19 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
         for (int j = 0; j < 4; ++j) {
             const int d = 32 * t + 8 * j + 4 * hi;
             if (d >= a.D) continue;
-            if constexpr (sizeof(T) == 2)
-                *(u32x2_t*)(to + d) = u32x2_t{pack_bf16x2(o[t][4 * j] * inv, o[t][4 * j + 1] * inv), pack_bf16x2(o[t][4 * j + 2] * inv, o[t][4 * j + 3] * inv)};
-            else
-                *(f32x4_t*)(to + d) = f32x4_t{o[t][4 * j] * inv, o[t][4 * j + 1] * inv, o[t][4 * j + 2] * inv, o[t][4 * j + 3] * inv};
+            const f32x4_t v = {o[t][4 * j] * inv, o[t][4 * j + 1] * inv, o[t][4 * j + 2] * inv, o[t][4 * j + 3] * inv};
+            if constexpr (sizeof(T) == 2) {
+                const u32x2_t w = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+                *(u32x2_t*)(to + d) = w;
+                if (a.residual) {
+                    f32x4_t rest;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) rest[e] = v[e] - __uint_as_float(e & 1 ? w[e / 2] & 0xFFFF0000u : w[e / 2] << 16);
+                    *(u32x2_t*)((T*)a.residual + (to - (T*)a.out) + d) = u32x2_t{pack_bf16x2(rest[0], rest[1]), pack_bf16x2(rest[2], rest[3])};
+                }
+            } else {
+                *(f32x4_t*)(to + d) = v;
+            }
         }
 }
 
@@ -358,7 +357,11 @@ __global__ __launch_bounds__(kThreads) void attention_join_kernel(MfmaArgs m) {
     T* to = (T*)a.out + (((int64_t)b * a.q_len + s) * a.heads + head) * a.D;
 #pragma unroll
     for (int c = 0; c < 4; ++c)
-        if (c * 64 + lane < a.D) to[c * 64 + lane] = (T)(total == 0.f ? 0.f : sum[c] / total);
+        if (c * 64 + lane < a.D) {
+            const float v = total == 0.f ? 0.f : sum[c] / total;
+            to[c * 64 + lane] = (T)v;
+            if (sizeof(T) == 2 && a.residual) ((T*)a.residual)[(to - (T*)a.out) + c * 64 + lane] = (T)(v - (float)(T)v);
+        }
     if (lane == 0) a.lse[((int64_t)b * a.heads + head) * a.q_len + s] = total == 0.f ? -INFINITY : (base + log2f(total)) * (1.f / kLog2e);
 }
 
@@ -386,19 +389,25 @@ __global__ __launch_bounds__(kThreads) void attention_documents_kernel(const int
     }
 }
 
-template <typename T, int DP, bool KEYS>
+template <typename T, int DP, bool KEYS, bool PLAIN>
 int launch(const MfmaArgs& m, hipStream_t s) {
     typedef FwdShape<T, DP, KEYS> Sh;
-    const hipError_t e = hipFuncSetAttribute((const void*)attention_fwd_kernel<T, DP, KEYS>, hipFuncAttributeMaxDynamicSharedMemorySize, Sh::kLds);
+    const hipError_t e = hipFuncSetAttribute((const void*)attention_fwd_kernel<T, DP, KEYS, PLAIN>, hipFuncAttributeMaxDynamicSharedMemorySize, Sh::kLds);
     if (e != hipSuccess) return PICOMOE_ERR_HIP_BASE + (int)e;
     const int64_t blocks = (int64_t)m.n_tiles * m.a.batch * m.a.kv_heads;
     if (blocks > 0x7FFFFFFF) return PICOMOE_ERR_TOO_LARGE;
-    attention_fwd_kernel<T, DP, KEYS><<<dim3((unsigned)blocks, (unsigned)m.splits), kThreads, Sh::kLds, s>>>(m);
+    attention_fwd_kernel<T, DP, KEYS, PLAIN><<<dim3((unsigned)blocks, (unsigned)m.splits), kThreads, Sh::kLds, s>>>(m);
     if (m.splits > 1) {
         const int64_t rows = (int64_t)m.a.batch * m.a.kv_heads * m.rows;
         attention_join_kernel<T><<<(unsigned)((rows + kWaves - 1) / kWaves), kThreads, 0, s>>>(m);
     }
     return picomoe_launch_status();
+}
+template <typename T, int DP>
+int launch_for(const MfmaArgs& m, bool keys, hipStream_t s) {
+    const bool plain = m.a.softcap == 0.f && !m.a.slopes && m.a.scale > 0.f;
+    if (keys) return plain ? launch<T, DP, true, true>(m, s) : launch<T, DP, true, false>(m, s);
+    return plain ? launch<T, DP, false, true>(m, s) : launch<T, DP, false, false>(m, s);
 }
 
 struct Plan {
@@ -464,10 +473,6 @@ int attention_mfma_fwd(const AttnArgs& a, hipStream_t s) {
         const int rc = attention_mfma_documents(a, p.tile, p.walked_tiles, a.kv_len, 0, 1, lowest, lowest + a.batch * p.walked_tiles, s);
         if (rc) return rc;
     }
-    if (a.dtype == PICOMOE_BF16) {
-        if (a.D <= 64) return p.keys ? launch<__bf16, 64, true>(m, s) : launch<__bf16, 64, false>(m, s);
-        return p.keys ? launch<__bf16, 128, true>(m, s) : launch<__bf16, 128, false>(m, s);
-    }
-    if (a.D <= 64) return p.keys ? launch<float, 64, true>(m, s) : launch<float, 64, false>(m, s);
-    return p.keys ? launch<float, 128, true>(m, s) : launch<float, 128, false>(m, s);
+    if (a.dtype == PICOMOE_BF16) return a.D <= 64 ? launch_for<__bf16, 64>(m, p.keys, s) : launch_for<__bf16, 128>(m, p.keys, s);
+    return a.D <= 64 ? launch_for<float, 64>(m, p.keys, s) : launch_for<float, 128>(m, p.keys, s);
 }

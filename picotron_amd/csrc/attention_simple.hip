@@ -95,7 +95,11 @@ __global__ __launch_bounds__(kThreads) void attention_simple_fwd_kernel(AttnArgs
     // NaN scores leave top at -inf: total is NaN then, and so are the sums
     T* out = (T*)a.out + row * a.D;
     for (int c = 0; c < kCols; ++c)
-        if (c * 64 + lane < a.D) out[c * 64 + lane] = (T)(total == 0.f ? 0.f : o[c] / total);
+        if (c * 64 + lane < a.D) {
+            const float v = total == 0.f ? 0.f : o[c] / total;
+            out[c * 64 + lane] = (T)v;
+            if (sizeof(T) == 2 && a.residual) ((T*)a.residual)[row * a.D + c * 64 + lane] = (T)(v - (float)(T)v);
+        }
     if (lane == 0) a.lse[(r.b * a.heads + r.h) * a.q_len + r.s] = total == 0.f ? -INFINITY : top + logf(total);
 }
 
@@ -112,7 +116,9 @@ __global__ __launch_bounds__(kThreads) void attention_simple_dq_kernel(AttnArgs 
     for (int d = lane; d < a.D; d += 64) {
         qs[wave][d] = to_f32(q[d]);
         gs[wave][d] = to_f32(g[d]);
-        delta += gs[wave][d] * to_f32(out[d]);
+        float o = to_f32(out[d]);
+        if (sizeof(T) == 2 && a.residual) o += to_f32(((const T*)a.residual)[(r.in ? row : 0) * a.D + d]);
+        delta += gs[wave][d] * o;
     }
     delta = wave_sum(delta);
     __syncthreads();

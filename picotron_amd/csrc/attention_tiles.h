@@ -77,6 +77,28 @@ __device__ __forceinline__ float frag_dot(const Frag<T>& a, const Frag<T>& b) {
     return s;
 }
 
+// A 16-byte (4-byte) direct-to-LDS load as an instruction sequence that the compiler does not look into: lane l lands at
+// lds + 16 l (4 l); lanes that are switched off leave their place alone.  With the builtin the compiler waits for all loads in
+// front of every LDS read that it cannot prove disjoint, so that nothing would be in flight under the products.  The kernels
+// wait themselves, with lds_loads_done() and a barrier.  M0 is written here and cannot be named as clobbered: nothing else in
+// these kernels may use it (the Makefile looks).
+__device__ __forceinline__ uint32_t lds_address(const char* l) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)l; }
+__device__ __forceinline__ void load16_to_lds(const void* from, char* lds) {
+    const uint32_t at = __builtin_amdgcn_readfirstlane(lds_address(lds));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory");
+}
+__device__ __forceinline__ void load4_to_lds(const void* from, char* lds) {
+    const uint32_t at = __builtin_amdgcn_readfirstlane(lds_address(lds));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(at), "v"(from) : "memory");
+}
+__device__ __forceinline__ void lds_loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// zeros over a block's dynamic LDS: rows narrower than DP are padded by what no load writes
+__device__ __forceinline__ void clear_lds(char* lds, int bytes) {
+    for (int i = threadIdx.x * 16; i < bytes; i += kThreads * 16) *(u32x4_t*)(lds + i) = u32x4_t{0u, 0u, 0u, 0u};
+    __syncthreads();
+}
+
 // Tiles in LDS: `rows` rows of DP elements in 16-byte chunks, chunk c of a row at c ^ swizzle(row).  The 16 rows that a
 // ds_read_b128 serves at a time, and the 4 rows x 64 bytes of a transposing read, then lie on different banks.
 template <typename T, int DP>
@@ -132,6 +154,19 @@ struct Tile {
         return f;
     }
 
+    // Stages `kRows` rows with direct-to-LDS loads, 64 chunks per wavefront and instruction: chunk p of row r of the tile comes from
+    // chunk p ^ swizzle(r) of row_of(r).  Chunks past D are left as they are (zeros: clear_lds).
+    template <int kRows, typename F>
+    __device__ static __forceinline__ void load(char* tile, int D, F row_of) {
+        constexpr int kRowsPerWave = 64 / kChunks;
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+        for (int i = 0; i < kRows / kRowsPerPass; ++i) {
+            const int first = (i * kWaves + wave) * kRowsPerWave, row = first + lane / kChunks;
+            const uint32_t chunk = (uint32_t)(lane % kChunks) ^ swizzle(row);
+            if ((int)chunk * kPerChunk < D) load16_to_lds((const char*)row_of(row) + chunk * 16, tile + first * kRowBytes);
+        }
+    }
     __device__ static __forceinline__ float element(const char* tile, int row, int col) {
         return to_f32(*(const T*)(tile + at(row, col / kPerChunk) + (col % kPerChunk) * (int)sizeof(T)));
     }

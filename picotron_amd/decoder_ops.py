@@ -221,23 +221,25 @@ class _Attention(torch.autograd.Function):
             q, k, v = _rows16(q), _rows16(k), _rows16(v)
             out = _empty((B, Sq, H, D), q)
             lse = _empty((B, H, Sq), q, torch.float32)
+            # what out's rounding left makes the backward's d_out . out exact; nothing else reads it
+            residual = _empty(q.shape, q) if q.dtype == torch.bfloat16 and any(ctx.needs_input_grad[:3]) else None
             ws = _workspace(lib.picomoe_attention_fwd_workspace_bytes(dt, B, Sq, Sk, H, G, D), q, "attention")
             _lib.check(
                 lib.picomoe_attention_fwd(
                     _lib.ptr(q), _strides(q), _lib.ptr(k), _strides(k), _lib.ptr(v), _strides(v), dt, B, Sq, Sk, H, G, D, scale, softcap, causal,
-                    window, _lib.ptr(slopes), _lib.ptr(document_ids), _lib.ptr(prefix_lengths), _lib.ptr(out), _lib.ptr(lse), _lib.ptr(ws),
-                    ws.numel(), _lib.stream_ptr(),
+                    window, _lib.ptr(slopes), _lib.ptr(document_ids), _lib.ptr(prefix_lengths), _lib.ptr(out), _lib.ptr(residual),
+                    _lib.ptr(lse), _lib.ptr(ws), ws.numel(), _lib.stream_ptr(),
                 ),
                 "picomoe_attention_fwd",
             )
-        ctx.save_for_backward(q, k, v, out, lse, slopes, document_ids, prefix_lengths)
+        ctx.save_for_backward(q, k, v, out, residual, lse, slopes, document_ids, prefix_lengths)
         ctx.meta = (scale, softcap, causal, window)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
-        q, k, v, out, lse, slopes, document_ids, prefix_lengths = ctx.saved_tensors
+        q, k, v, out, residual, lse, slopes, document_ids, prefix_lengths = ctx.saved_tensors
         scale, softcap, causal, window = ctx.meta
         lib = _lib.load()
         B, Sq, H, D = q.shape
@@ -251,8 +253,8 @@ class _Attention(torch.autograd.Function):
             ws = _workspace(lib.picomoe_attention_bwd_workspace_bytes(dt, B, Sq, Sk, H, G, D), q, "attention")
             _lib.check(
                 lib.picomoe_attention_bwd(
-                    _lib.ptr(d_out), _lib.ptr(q), _strides(q), _lib.ptr(k), _strides(k), _lib.ptr(v), _strides(v), _lib.ptr(out), _lib.ptr(lse),
-                    dt, B, Sq, Sk, H, G, D, scale, softcap, causal, window, _lib.ptr(slopes), _lib.ptr(document_ids), _lib.ptr(prefix_lengths),
+                    _lib.ptr(d_out), _lib.ptr(q), _strides(q), _lib.ptr(k), _strides(k), _lib.ptr(v), _strides(v), _lib.ptr(out), _lib.ptr(residual),
+                    _lib.ptr(lse), dt, B, Sq, Sk, H, G, D, scale, softcap, causal, window, _lib.ptr(slopes), _lib.ptr(document_ids), _lib.ptr(prefix_lengths),
                     _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), _lib.ptr(ws), ws.numel(), _lib.stream_ptr(),
                 ),
                 "picomoe_attention_bwd",

@@ -61,7 +61,7 @@ def test_attention_arguments():
     def fwd(q=P, qs=STRIDES, ks=STRIDES, dtype=1, batch=2, q_len=4, kv_len=4, heads=4, kv_heads=4, D=64, scale=0.1, softcap=0.0, causal=1, window=0, prefix=None,
             out=P, lse=P, ws=P, size=1 << 40):
         return lib.picomoe_attention_fwd(q, qs, P, ks, P, STRIDES, dtype, batch, q_len, kv_len, heads, kv_heads, D, scale, softcap, causal, window, None, None,
-                                         prefix, out, lse, ws, size, None)
+                                         prefix, out, None, lse, ws, size, None)
 
     assert fwd(batch=0) == 0 and fwd(q_len=0) == 0
     nan = float("nan")
@@ -75,7 +75,7 @@ def test_attention_arguments():
     need = lib.picomoe_attention_bwd_workspace_bytes(1, 2, 4, 4, 4, 4, 64)
 
     def bwd(g=P, out=P, lse=P, dq=P, dv=P, size=need, kv_len=4, q_len=4):
-        return lib.picomoe_attention_bwd(g, P, STRIDES, P, STRIDES, P, STRIDES, out, lse, 1, 2, q_len, kv_len, 4, 4, 64, 0.1, 0.0, 1, 0, None, None, None, dq, P, dv,
+        return lib.picomoe_attention_bwd(g, P, STRIDES, P, STRIDES, P, STRIDES, out, None, lse, 1, 2, q_len, kv_len, 4, 4, 64, 0.1, 0.0, 1, 0, None, None, None, dq, P, dv,
                                          P, size, None)
 
     for bad in (dict(g=None), dict(g=ODD), dict(out=None), dict(lse=None), dict(dq=None), dict(dv=ODD), dict(size=need - 1), dict(kv_len=0), dict(q_len=0)):
