@@ -86,7 +86,5 @@ int attention_simple_bwd(const AttnArgs& a, hipStream_t s);
 bool attention_mfma_supported(int head_dim);
 int64_t attention_mfma_fwd_workspace(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, int kv_heads, int head_dim);
 int attention_mfma_fwd(const AttnArgs& a, hipStream_t s);
-// lowest and highest document id of every `per` rows, row r standing for position r / group + offset
-int attention_mfma_documents(const AttnArgs& a, int per, int tiles, int rows, int offset, int group, int32_t* lowest, int32_t* highest, hipStream_t s);
 int64_t attention_mfma_bwd_workspace(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, int kv_heads, int head_dim);
 int attention_mfma_bwd(const AttnArgs& a, hipStream_t s);

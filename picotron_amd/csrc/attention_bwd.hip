@@ -1,11 +1,11 @@
-// Attention backward on MFMA, without atomics: dq in one kernel, dk and dv in another, P recomputed from lse in both.
+// Attention backward on MFMA, without atomics: one launch forms dq, another dk and dv, P recomputed from lse in both.
 //
 // Seven products instead of the five of the formulas (S and dP are formed twice); what that buys is that every sum has one owner
 // and one order.  dq: a wavefront owns 32 rows (as in the forward), walks the key tiles: S^T = K Q^T, dP^T = V dO^T,
-// dq^T += K^T dx^T; it also forms D = dO . out, which the second kernel reads.  dk, dv: a wavefront owns 32 keys, walks the row
-// tiles of the key head -- all its query heads, so that their gradients meet in one accumulator: S = Q K^T, dP = dO V^T,
-// dv^T += dO^T P, dk^T += Q^T dx.  Where the key blocks are too few to fill the chip the rows are dealt to `splits` blocks
-// whose fp32 parts a last launch adds in order.
+// dq^T += K^T dx^T.  dk, dv: a wavefront owns 32 keys, walks the row tiles of the key head -- all its query heads, so that their
+// gradients meet in one accumulator: S = Q K^T, dP = dO V^T, dv^T += dO^T P, dk^T += Q^T dx.  Blocks with long walks are cut
+// into parts (MfmaArgs) whose fp32 sums a last launch adds in order; a first one forms D = dO . out.  Both kinds of blocks in one
+// launch were slower (16384 tokens, 16 heads: 8.3 ms against 4.7 + 2.3): the registers of the two spill more together.
 #include "attention_tiles.h"
 
 namespace {
@@ -24,14 +24,14 @@ struct DqShape {
 // PLAIN: neither softcap nor slopes
 template <typename T, int DP, bool PLAIN>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq_kernel(MfmaArgs m) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
     typedef DqShape<T, DP> Sh;
     typedef Tile<T, DP> Tl;
     constexpr int kSub = Sh::kTile / 32, kSteps = DP / 16, kCols = DP / 32;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
     const AttnArgs& a = m.a;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5;
 
-    const int heads = (int)a.batch * a.kv_heads, bh = blockIdx.x % heads, tile = m.n_tiles - 1 - blockIdx.x / heads;
+    const int heads = (int)a.batch * a.kv_heads, bh = blockIdx.x % heads, split = blockIdx.y, tile = m.blocks - 1 - blockIdx.x / heads;
     const int b = bh / a.kv_heads, kvh = bh % a.kv_heads;
     int row = tile * 32 * kWaves + wave * 32 + (lane & 31);
     const bool row_in = row < m.rows;
@@ -41,24 +41,6 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq
     const int key_span = span.hi - span.lo;
     const float slope2 = a.slopes ? a.slopes[head] * kLog2e : 0.f;
     const int64_t out_row = ((int64_t)b * a.q_len + s) * a.heads + head, stat = ((int64_t)b * a.heads + head) * a.q_len + s;
-
-    Frag<T> qf[kSteps], gf[kSteps];
-    float delta = 0.f;
-    {
-        const T* q = (const T*)a.q.p + b * a.q.sb + s * a.q.ss + head * a.q.sh;
-        const T *g = (const T*)a.d_out + out_row * a.D, *out = (const T*)a.out + out_row * a.D;
-#pragma unroll
-        for (int ks = 0; ks < kSteps; ++ks) {
-            qf[ks] = load_frag<T>(q, 16 * ks + 8 * hi, a.D);
-            gf[ks] = load_frag<T>(g, 16 * ks + 8 * hi, a.D);
-            delta += frag_dot(gf[ks], load_frag<T>(out, 16 * ks + 8 * hi, a.D));
-            if (sizeof(T) == 2 && a.residual) delta += frag_dot(gf[ks], load_frag<T>((const T*)a.residual + out_row * a.D, 16 * ks + 8 * hi, a.D));
-        }
-    }
-    delta = other_sum(delta);
-    if (row_in && hi == 0) a.delta[stat] = delta;
-    float lse2 = a.lse[stat] * kLog2e;
-    lse2 = lse2 == -INFINITY ? INFINITY : lse2;  // a row without a key: P = 0
 
     const bool some = key_span >= 0;
     Reach w;
@@ -89,10 +71,32 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq
         blk.doc_min = __builtin_amdgcn_readfirstlane(blk.doc_min);
         blk.doc_max = __builtin_amdgcn_readfirstlane(blk.doc_max);
     }
-    const int32_t* doc_min = a.docs ? m.doc_min + (int64_t)b * m.walked_tiles : nullptr;
-    const int32_t* doc_max = a.docs ? m.doc_max + (int64_t)b * m.walked_tiles : nullptr;
+    const int32_t* doc_min = a.docs ? m.key_docs.lowest + (int64_t)b * m.key_docs.tiles : nullptr;
+    const int32_t* doc_max = a.docs ? m.key_docs.highest + (int64_t)b * m.key_docs.tiles : nullptr;
     const bool any = blk.hi_max >= blk.lo_min;
     const int first = any ? blk.lo_min / Sh::kTile : 0, end = any ? blk.hi_max / Sh::kTile + 1 : 0;
+
+    auto active = [&](int t) { return !a.docs || (doc_max[t] >= blk.doc_min && doc_min[t] <= blk.doc_max); };
+    Share share = {1, 0, 0x7FFFFFFF};
+    if (m.splits > 1) {
+        share = share_of(a.docs ? count_tiles(first, end, active) : end - first, split, m);
+        if (split == 0 && threadIdx.x == 0) m.parts[bh * m.blocks + tile] = share.parts;
+        if (split >= share.parts) return;
+    }
+
+    Frag<T> qf[kSteps], gf[kSteps];
+    {
+        const T* q = (const T*)a.q.p + b * a.q.sb + s * a.q.ss + head * a.q.sh;
+        const T* g = (const T*)a.d_out + out_row * a.D;
+#pragma unroll
+        for (int ks = 0; ks < kSteps; ++ks) {
+            qf[ks] = load_frag<T>(q, 16 * ks + 8 * hi, a.D);
+            gf[ks] = load_frag<T>(g, 16 * ks + 8 * hi, a.D);
+        }
+    }
+    const float delta = a.delta[stat];
+    float lse2 = a.lse[stat] * kLog2e;
+    lse2 = lse2 == -INFINITY ? INFINITY : lse2;  // a row without a key: P = 0
 
     const T* kbase = (const T*)a.k.p + b * a.k.sb + kvh * a.k.sh;
     const T* vbase = (const T*)a.v.p + b * a.v.sb + kvh * a.v.sh;
@@ -113,8 +117,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq
         for (int t = 0; t < kCols; ++t)
 #pragma unroll
             for (int i = 0; i < 16; ++i) dq[t][i] = 0.f;
-        auto active = [&](int t) { return !a.docs || (doc_max[t] >= blk.doc_min && doc_min[t] <= blk.doc_max); };
-        TileWalk<decltype(active)> walk(first, end, active);
+        TileWalk<decltype(active)> walk(first, end, active, share.skip, share.left);
         int cur = walk.next(), buf = 0;
         if (cur >= 0) fetch(cur, 0);
         while (cur >= 0) {
@@ -206,6 +209,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq
         }
     };
     run(std::integral_constant<bool, false>());
+    lds_loads_done();  // also where no tile was walked: nothing may land in LDS after the block is gone
     bool bad = false;
 #pragma unroll
     for (int t = 0; t < kCols; ++t) bad |= not_finite(dq[t]);
@@ -220,7 +224,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq
             const int d = 32 * t + 8 * j + 4 * hi;
             if (d >= a.D) continue;
             const f32x4_t v = {dq[t][4 * j] * a.scale, dq[t][4 * j + 1] * a.scale, dq[t][4 * j + 2] * a.scale, dq[t][4 * j + 3] * a.scale};
-            if constexpr (sizeof(T) == 2) *(u32x2_t*)(to + d) = u32x2_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+            if (share.parts > 1) *(f32x4_t*)(m.part_out + ((int64_t)split * a.batch * a.q_len * a.heads + out_row) * a.D + d) = v;
+            else if constexpr (sizeof(T) == 2) *(u32x2_t*)(to + d) = u32x2_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
             else *(f32x4_t*)(to + d) = v;
         }
 }
@@ -243,17 +248,57 @@ struct DkvShape {
 
 template <typename T, int DP, bool PLAIN>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dkv_kernel(MfmaArgs m) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
     typedef DkvShape<T, DP> Sh;
     typedef Tile<T, DP> Tl;
     constexpr int kSteps = DP / 16, kCols = DP / 32, kBuf = Sh::kBuf;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
     const AttnArgs& a = m.a;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5;
-    const int heads = (int)a.batch * a.kv_heads, bh = blockIdx.x % heads, block = blockIdx.x / heads, split = blockIdx.y;
+    const int heads = (int)a.batch * a.kv_heads, bh = blockIdx.x % heads, split = blockIdx.y, block = blockIdx.x / heads;
     const int b = bh / a.kv_heads, kvh = bh % a.kv_heads;
     const int block0 = block * Sh::kKeys, block1 = min(block0 + Sh::kKeys, a.kv_len) - 1;
     const int wave0 = block0 + wave * 32, wave1 = wave0 + 31;
     const int key = wave0 + (lane & 31), key_in = key < a.kv_len, key_at = key_in ? key : a.kv_len - 1;
+
+    // keys past the end get a document of their own; without documents every key and row has document 0
+    const int doc = a.docs ? (key_in ? a.docs[(int64_t)b * a.kv_len + key] : -1) : 0;
+    const int w_doc_min = wave_min_i32(doc), w_doc_max = wave_max_i32(doc);
+    int blk_doc_min = 0, blk_doc_max = 0;
+    if (a.docs) {
+        __shared__ int range[kWaves][2];
+        if (lane == 0) {
+            range[wave][0] = w_doc_min;
+            range[wave][1] = w_doc_max;
+        }
+        __syncthreads();
+        blk_doc_min = __builtin_amdgcn_readfirstlane(min(min(range[0][0], range[1][0]), min(range[2][0], range[3][0])));
+        blk_doc_max = __builtin_amdgcn_readfirstlane(max(max(range[0][1], range[1][1]), max(range[2][1], range[3][1])));
+    }
+    const int32_t* doc_min = a.docs ? m.row_docs.lowest + (int64_t)b * m.row_docs.tiles : nullptr;
+    const int32_t* doc_max = a.docs ? m.row_docs.highest + (int64_t)b * m.row_docs.tiles : nullptr;
+    const int prefix = a.prefix ? a.prefix[b] : 0, off = a.kv_len - a.q_len;
+    // first and last key of the interval of query s (documents aside): both grow with s
+    auto lo_of = [&](int q) { return a.window > 0 ? max(0, q + off - a.window + 1) : 0; };
+    auto hi_of = [&](int q) {
+        int last = a.kv_len - 1;
+        if (a.causal) last = min(last, max(q + off, prefix - 1));
+        if (a.window > 0) last = min(last, q + off + a.window - 1);
+        return last;
+    };
+    auto first_query = [&](int t) { return m.div(t * Sh::kTile); };
+    auto last_query = [&](int t) { return m.div(min(t * Sh::kTile + Sh::kTile, m.rows) - 1); };
+
+    const int row_tiles = (m.rows + Sh::kTile - 1) / Sh::kTile;
+    auto active = [&](int t) {
+        if (hi_of(last_query(t)) < block0 || lo_of(first_query(t)) > block1) return false;
+        return !a.docs || (doc_max[t] >= max(0, blk_doc_min) && doc_min[t] <= blk_doc_max);
+    };
+    Share share = {1, 0, 0x7FFFFFFF};
+    if (m.splits > 1) {
+        share = share_of(count_tiles(0, row_tiles, active), split, m);
+        if (split == 0 && threadIdx.x == 0) m.parts[bh * m.blocks + block] = share.parts;
+        if (split >= share.parts) return;
+    }
 
     if (a.D < DP) clear_lds(lds, Sh::kLds);
     Frag<T> kf[kSteps], vf[kSteps];
@@ -271,34 +316,6 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
             if (!Sh::kVInLds) vf[ks] = load_frag<T>(v, 16 * ks + 8 * hi, a.D);
         }
     }
-    // keys past the end get a document of their own; without documents every key and row has document 0
-    const int doc = a.docs ? (key_in ? a.docs[(int64_t)b * a.kv_len + key] : -1) : 0;
-    const int w_doc_min = wave_min_i32(doc), w_doc_max = wave_max_i32(doc);
-    int blk_doc_min = 0, blk_doc_max = 0;
-    if (a.docs) {
-        __shared__ int range[kWaves][2];
-        if (lane == 0) {
-            range[wave][0] = w_doc_min;
-            range[wave][1] = w_doc_max;
-        }
-        __syncthreads();
-        blk_doc_min = __builtin_amdgcn_readfirstlane(min(min(range[0][0], range[1][0]), min(range[2][0], range[3][0])));
-        blk_doc_max = __builtin_amdgcn_readfirstlane(max(max(range[0][1], range[1][1]), max(range[2][1], range[3][1])));
-    }
-    const int32_t* doc_min = a.docs ? m.doc_min + (int64_t)b * m.walked_tiles : nullptr;
-    const int32_t* doc_max = a.docs ? m.doc_max + (int64_t)b * m.walked_tiles : nullptr;
-    const int prefix = a.prefix ? a.prefix[b] : 0, off = a.kv_len - a.q_len;
-    // first and last key of the interval of query s (documents aside): both grow with s
-    auto lo_of = [&](int q) { return a.window > 0 ? max(0, q + off - a.window + 1) : 0; };
-    auto hi_of = [&](int q) {
-        int last = a.kv_len - 1;
-        if (a.causal) last = min(last, max(q + off, prefix - 1));
-        if (a.window > 0) last = min(last, q + off + a.window - 1);
-        return last;
-    };
-    auto first_query = [&](int t) { return m.div(t * Sh::kTile); };
-    auto last_query = [&](int t) { return m.div(min(t * Sh::kTile + Sh::kTile, m.rows) - 1); };
-
     const T* qbase = (const T*)a.q.p + b * a.q.sb + (int64_t)(kvh * a.group) * a.q.sh;
     const T* gbase = (const T*)a.d_out + ((int64_t)b * a.q_len * a.heads + kvh * a.group) * a.D;
     float stat_f[3] = {};
@@ -347,25 +364,14 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
         for (int t = 0; t < kCols; ++t)
 #pragma unroll
             for (int i = 0; i < 16; ++i) dk[t][i] = dv[t][i] = 0.f;
-        auto active = [&](int t) {
-            if (hi_of(last_query(t)) < block0 || lo_of(first_query(t)) > block1) return false;
-            return !a.docs || (doc_max[t] >= max(0, blk_doc_min) && doc_min[t] <= blk_doc_max);
-        };
-        TileWalk<decltype(active)> walk(0, m.walked_tiles, active);
-        int seen = 0;  // every splits-th active tile is this block's
-        auto next = [&]() {
-            while (true) {
-                const int t = walk.next();
-                if (t < 0 || seen++ % m.splits == split) return t;
-            }
-        };
-        int cur = next(), buf = 0;
+        TileWalk<decltype(active)> walk(0, row_tiles, active, share.skip, share.left);
+        int cur = walk.next(), buf = 0;
         if (cur >= 0) fetch(cur, 0);
         while (cur >= 0) {
             stage_stats(buf);
             lds_loads_done();
             __syncthreads();
-            const int following = next();
+            const int following = walk.next();
             if (following >= 0) fetch(following, buf ^ 1);
             const char* qt = lds + buf * kBuf;
             const char* gt = qt + Sh::kTileBytes;
@@ -477,6 +483,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
         }
     };
     run(std::integral_constant<bool, false>());
+    lds_loads_done();  // also where no tile was walked: nothing may land in LDS after the block is gone
     bool bad = false;
 #pragma unroll
     for (int t = 0; t < kCols; ++t) bad |= not_finite(dk[t]) || not_finite(dv[t]);
@@ -492,7 +499,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
             if (d >= a.D) continue;
             const f32x4_t u = {dk[t][4 * j] * a.scale, dk[t][4 * j + 1] * a.scale, dk[t][4 * j + 2] * a.scale, dk[t][4 * j + 3] * a.scale};
             const f32x4_t v = {dv[t][4 * j], dv[t][4 * j + 1], dv[t][4 * j + 2], dv[t][4 * j + 3]};
-            if (m.splits > 1) {
+            if (share.parts > 1) {
                 float* to = m.part_out + ((int64_t)split * 2 * rows + out_row) * a.D + d;
                 *(f32x4_t*)to = u;
                 *(f32x4_t*)(to + rows * a.D) = v;
@@ -506,43 +513,105 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
         }
 }
 
-// dk and dv from the parts of the splits, four elements a thread
+struct JoinArgs {  // blockIdx.y: one of dq, dk, dv; the parts of its quads of elements
+    void* to[3];
+    const float* from[3];
+    const int32_t* parts[3];
+    int64_t quads[3], stride[3];  // stride: between the parts of one, in quads
+    int length[3], heads[3], group[3], rows[3], blocks[3];  // rows: of a block
+};
+
+// the gradients of the blocks that were cut, four elements a thread
 template <typename T>
-__global__ __launch_bounds__(kThreads) void attention_dkv_join_kernel(const f32x4_t* __restrict__ parts, int splits, int64_t quads, T* dk, T* dv) {
+__global__ __launch_bounds__(kThreads) void attention_grad_join_kernel(JoinArgs j, int quads_per_row, int kv_heads) {
+    const int w = blockIdx.y;
     const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (i >= 2 * quads) return;
-    f32x4_t sum = parts[i];
-    for (int s = 1; s < splits; ++s) sum += parts[s * 2 * quads + i];
-    T* to = (i < quads ? dk : dv) + 4 * (i < quads ? i : i - quads);
+    if (i >= j.quads[w]) return;
+    const int64_t row = i / quads_per_row, token = row / j.heads[w], b = token / j.length[w];
+    const int head = (int)(row - token * j.heads[w]), at = (int)(token - b * j.length[w]);  // row of the key head: at * group + head % group
+    const int block = (at * j.group[w] + head % j.group[w]) / j.rows[w];
+    const int parts = j.parts[w][(b * kv_heads + head / j.group[w]) * j.blocks[w] + block];
+    if (parts == 1) return;  // written by its block
+    const f32x4_t* from = (const f32x4_t*)j.from[w] + i;
+    f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int p = 0; p < parts; ++p) sum += from[p * j.stride[w]];
+    T* to = (T*)j.to[w] + 4 * i;
     if constexpr (sizeof(T) == 2) *(u32x2_t*)to = u32x2_t{pack_bf16x2(sum[0], sum[1]), pack_bf16x2(sum[2], sum[3])};
     else *(f32x4_t*)to = sum;
+}
+
+// D = dO . (out + residual) of every row, a group of lanes per row and 16 bytes a lane; and the document ranges of the tiles
+template <typename T>
+__global__ __launch_bounds__(kThreads) void attention_prepare_kernel(MfmaArgs m, int64_t out_rows, int delta_blocks, int key_tile, int row_tile,
+                                                                     int key_blocks) {
+    const AttnArgs& a = m.a;
+    constexpr int kPer = 16 / (int)sizeof(T), kLanes = 128 / kPer;
+    if ((int)blockIdx.x < delta_blocks) {
+        const int64_t row = (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
+        const int col = threadIdx.x % kLanes * kPer;
+        float sum = 0.f;
+        if (row < out_rows && col < a.D) {
+            const T *g = (const T*)a.d_out + row * a.D + col, *o = (const T*)a.out + row * a.D + col;
+            typedef __attribute__((ext_vector_type(kPer))) T vec;
+            const vec gv = *(const vec*)g, ov = *(const vec*)o;
+            vec rv = {};
+            if (sizeof(T) == 2 && a.residual) rv = *(const vec*)((const T*)a.residual + row * a.D + col);
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) sum += (float)gv[e] * ((float)ov[e] + (float)rv[e]);
+        }
+#pragma unroll
+        for (int off = kLanes / 2; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+        if (row < out_rows && threadIdx.x % kLanes == 0) {
+            const int64_t token = row / a.heads, b = token / a.q_len;
+            a.delta[(b * a.heads + (row - token * a.heads)) * a.q_len + (token - b * a.q_len)] = sum;
+        }
+        return;
+    }
+    const int block = blockIdx.x - delta_blocks;
+    if (block < key_blocks)
+        document_range(a.docs, a.kv_len, block, key_tile, m.key_docs.tiles, a.kv_len, 0, GroupDiv{0u, 0}, (int32_t*)m.key_docs.lowest,
+                       (int32_t*)m.key_docs.highest);
+    else
+        document_range(a.docs, a.kv_len, block - key_blocks, row_tile, m.row_docs.tiles, m.rows, a.kv_len - a.q_len, m.div,
+                       (int32_t*)m.row_docs.lowest, (int32_t*)m.row_docs.highest);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
 int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 
+struct Cut {
+    int blocks, splits, target;
+};
+// A mask leaves the blocks unequal walks (causal: the last rows see all keys, the first one).  Walks longer than an eighth of what
+// each of the 512 blocks that the chip holds would get without a mask are cut, into parts of `shortest` tiles or more -- a part costs
+// its sums in fp32 each way -- and 16 parts at most.
+Cut cut(int64_t heads, int64_t blocks, int64_t tiles, int64_t shortest) {
+    const int64_t share = (heads * blocks * tiles + 4095) / 4096, longest = (tiles + 15) / 16;
+    int64_t target = share > shortest ? share : shortest;
+    target = target > longest ? target : longest;
+    return {(int)blocks, tiles > target ? (int)((tiles + target - 1) / target) : 1, (int)target};
+}
+
 struct Plan {
-    int key_tile, key_tiles, row_tiles, dq_tiles, key_blocks, splits;
-    int64_t key_docs, row_docs, parts;
+    int key_tile, key_tiles, row_tiles;
+    Cut dq, dkv;
+    int64_t key_docs, row_docs, dq_parts, dkv_parts, dq_bytes, dkv_bytes;
 };
 Plan plan(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, int kv_heads, int head_dim) {
     Plan p;
-    const int64_t rows = q_len * (q_heads / kv_heads);
+    const int64_t rows = q_len * (q_heads / kv_heads), heads = batch * kv_heads, per = 32 * kWaves;
     p.key_tile = dtype == PICOMOE_BF16 ? 64 : 32;
     p.key_tiles = (int)((kv_len + p.key_tile - 1) / p.key_tile);
     p.row_tiles = (int)((rows + 31) / 32);
-    p.dq_tiles = (int)((rows + 32 * kWaves - 1) / (32 * kWaves));
-    p.key_blocks = (int)((kv_len + 32 * kWaves - 1) / (32 * kWaves));
-    // A mask leaves the key blocks unequal work (causal: the first sees all rows, the last its own): the rows are dealt to
-    // several blocks until there are eight per CU to balance with, of at least 16 row tiles each
-    const int64_t blocks = batch * kv_heads * p.key_blocks;
-    int64_t splits = blocks > 0 ? (2048 + blocks - 1) / blocks : 1;
-    if (splits > p.row_tiles / 16) splits = p.row_tiles / 16;
-    if (splits > 16) splits = 16;
-    p.splits = splits < 1 ? 1 : (int)splits;
+    p.dq = cut(heads, (rows + per - 1) / per, p.key_tiles, 8);
+    p.dkv = cut(heads, (kv_len + per - 1) / per, p.row_tiles, 16);
     p.key_docs = round16(batch * p.key_tiles * 8);
     p.row_docs = round16(batch * p.row_tiles * 8);
-    p.parts = p.splits > 1 ? (int64_t)p.splits * 2 * batch * kv_len * kv_heads * head_dim * 4 : 0;
+    p.dq_parts = p.dq.splits > 1 ? round16(heads * p.dq.blocks * 4) : 0;
+    p.dkv_parts = p.dkv.splits > 1 ? round16(heads * p.dkv.blocks * 4) : 0;
+    p.dq_bytes = p.dq.splits > 1 ? p.dq.splits * batch * q_len * q_heads * head_dim * 4 : 0;
+    p.dkv_bytes = p.dkv.splits > 1 ? p.dkv.splits * 2 * batch * kv_len * kv_heads * head_dim * 4 : 0;
     return p;
 }
 
@@ -550,35 +619,55 @@ template <typename T, int DP, bool PLAIN>
 int launch(MfmaArgs m, const Plan& p, hipStream_t s) {
     typedef DqShape<T, DP> Q;
     typedef DkvShape<T, DP> K;
-    hipError_t e = hipFuncSetAttribute((const void*)attention_dq_kernel<T, DP, PLAIN>, hipFuncAttributeMaxDynamicSharedMemorySize, Q::kLds);
-    if (e == hipSuccess) e = hipFuncSetAttribute((const void*)attention_dkv_kernel<T, DP, PLAIN>, hipFuncAttributeMaxDynamicSharedMemorySize, K::kLds);
+    hipError_t e = allow_lds<attention_dq_kernel<T, DP, PLAIN>>(Q::kLds);
+    if (e == hipSuccess) e = allow_lds<attention_dkv_kernel<T, DP, PLAIN>>(K::kLds);
     if (e != hipSuccess) return PICOMOE_ERR_HIP_BASE + (int)e;
     const AttnArgs& a = m.a;
-    const int64_t heads = a.batch * a.kv_heads, dq_blocks = heads * p.dq_tiles, key_blocks = heads * p.key_blocks;
-    const int64_t quads = a.batch * a.kv_len * a.kv_heads * a.D / 4, join_blocks = (2 * quads + kThreads - 1) / kThreads;
-    if (dq_blocks > 0x7FFFFFFF || key_blocks > 0x7FFFFFFF || (p.splits > 1 && join_blocks > 0x7FFFFFFF)) return PICOMOE_ERR_TOO_LARGE;
-    int32_t *key_docs = (int32_t*)a.ws, *row_docs = (int32_t*)(a.ws + p.key_docs);
-    m.part_out = (float*)(a.ws + p.key_docs + p.row_docs);
-    if (a.docs) {
-        int rc = attention_mfma_documents(a, p.key_tile, p.key_tiles, a.kv_len, 0, 1, key_docs, key_docs + a.batch * p.key_tiles, s);
-        if (rc == PICOMOE_OK)
-            rc = attention_mfma_documents(a, 32, p.row_tiles, m.rows, a.kv_len - a.q_len, a.group, row_docs, row_docs + a.batch * p.row_tiles, s);
-        if (rc) return rc;
+    const int64_t heads = a.batch * a.kv_heads, q_quads = a.batch * a.q_len * a.heads * (a.D / 4), k_quads = a.batch * a.kv_len * a.kv_heads * (a.D / 4);
+    const int64_t join_blocks = ((q_quads > k_quads ? q_quads : k_quads) + kThreads - 1) / kThreads;
+    const int64_t out_rows = a.batch * a.q_len * a.heads, per_block = sizeof(T) == 2 ? 16 : 8, delta_blocks = (out_rows + per_block - 1) / per_block;
+    const int64_t key_ranges = a.docs ? a.batch * range_blocks(p.key_tiles) : 0, row_ranges = a.docs ? a.batch * range_blocks(p.row_tiles) : 0;
+    if (heads * p.dq.blocks > 0x7FFFFFFF || heads * p.dkv.blocks > 0x7FFFFFFF || join_blocks > 0x7FFFFFFF ||
+        delta_blocks + key_ranges + row_ranges > 0x7FFFFFFF)
+        return PICOMOE_ERR_TOO_LARGE;
+    char* ws = a.ws;
+    auto take = [&](int64_t bytes) {
+        char* at = ws;
+        ws += bytes;
+        return at;
+    };
+    int32_t *key_docs = (int32_t*)take(p.key_docs), *row_docs = (int32_t*)take(p.row_docs);
+    int32_t *dq_parts = (int32_t*)take(p.dq_parts), *dkv_parts = (int32_t*)take(p.dkv_parts);
+    float *dq_sums = (float*)take(p.dq_bytes), *dkv_sums = (float*)take(p.dkv_bytes);
+    m.key_docs = {key_docs, key_docs + a.batch * p.key_tiles, p.key_tiles};
+    m.row_docs = {row_docs, row_docs + a.batch * p.row_tiles, p.row_tiles};
+    attention_prepare_kernel<T><<<(unsigned)(delta_blocks + key_ranges + row_ranges), kThreads, 0, s>>>(m, out_rows, (int)delta_blocks, p.key_tile, 32,
+                                                                                                        (int)key_ranges);
+    auto use = [&](const Cut& c, int32_t* parts, float* sums) {
+        m.blocks = c.blocks;
+        m.splits = c.splits;
+        m.target = c.target;
+        m.parts = parts;
+        m.part_out = sums;
+        return dim3((unsigned)(heads * c.blocks), (unsigned)c.splits);
+    };
+    const dim3 dkv_grid = use(p.dkv, dkv_parts, dkv_sums);
+    attention_dkv_kernel<T, DP, PLAIN><<<dkv_grid, kThreads, K::kLds, s>>>(m);
+    const dim3 dq_grid = use(p.dq, dq_parts, dq_sums);
+    attention_dq_kernel<T, DP, PLAIN><<<dq_grid, kThreads, Q::kLds, s>>>(m);
+    JoinArgs j = {};
+    unsigned n = 0;
+    auto join = [&](void* to, const float* from, const int32_t* parts, int64_t quads, int64_t stride, int length, int of_heads, int group, int rows, int blocks) {
+        j.to[n] = to; j.from[n] = from; j.parts[n] = parts; j.quads[n] = quads; j.stride[n] = stride;
+        j.length[n] = length; j.heads[n] = of_heads; j.group[n] = group; j.rows[n] = rows; j.blocks[n] = blocks;
+        ++n;
+    };
+    if (p.dq.splits > 1) join(a.dq, dq_sums, dq_parts, q_quads, q_quads, a.q_len, a.heads, a.group, 32 * kWaves, p.dq.blocks);
+    if (p.dkv.splits > 1) {
+        join(a.dk, dkv_sums, dkv_parts, k_quads, 2 * k_quads, a.kv_len, a.kv_heads, 1, 32 * kWaves, p.dkv.blocks);
+        join(a.dv, dkv_sums + 4 * k_quads, dkv_parts, k_quads, 2 * k_quads, a.kv_len, a.kv_heads, 1, 32 * kWaves, p.dkv.blocks);
     }
-    m.doc_min = key_docs;
-    m.doc_max = key_docs + a.batch * p.key_tiles;
-    m.walked_tiles = p.key_tiles;
-    m.n_tiles = p.dq_tiles;
-    m.splits = 1;
-    attention_dq_kernel<T, DP, PLAIN><<<(unsigned)dq_blocks, kThreads, Q::kLds, s>>>(m);
-    m.doc_min = row_docs;
-    m.doc_max = row_docs + a.batch * p.row_tiles;
-    m.walked_tiles = p.row_tiles;
-    m.n_tiles = p.key_blocks;
-    m.splits = p.splits;
-    attention_dkv_kernel<T, DP, PLAIN><<<dim3((unsigned)key_blocks, (unsigned)p.splits), kThreads, K::kLds, s>>>(m);
-    if (p.splits > 1)
-        attention_dkv_join_kernel<T><<<(unsigned)join_blocks, kThreads, 0, s>>>((const f32x4_t*)m.part_out, p.splits, quads, (T*)a.dk, (T*)a.dv);
+    if (n > 0) attention_grad_join_kernel<T><<<dim3((unsigned)join_blocks, n), kThreads, 0, s>>>(j, a.D / 4, a.kv_heads);
     return picomoe_launch_status();
 }
 
@@ -591,7 +680,7 @@ int launch_for(const MfmaArgs& m, const Plan& p, hipStream_t s) {
 
 int64_t attention_mfma_bwd_workspace(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, int kv_heads, int head_dim) {
     const Plan p = plan(dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim);
-    return p.key_docs + p.row_docs + p.parts + 16;
+    return p.key_docs + p.row_docs + p.dq_parts + p.dkv_parts + p.dq_bytes + p.dkv_bytes + 16;
 }
 
 int attention_mfma_bwd(const AttnArgs& a, hipStream_t s) {

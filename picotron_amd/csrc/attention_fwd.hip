@@ -27,6 +27,23 @@ struct FwdShape {
     static constexpr int kLds = kBuffers * kBuf;
 };
 
+// four elements of out, and of its residual where it is wanted
+template <typename T>
+__device__ __forceinline__ void store_out(const AttnArgs& a, int64_t at, f32x4_t v) {
+    if constexpr (sizeof(T) == 2) {
+        const u32x2_t w = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+        *(u32x2_t*)((T*)a.out + at) = w;
+        if (a.residual) {
+            f32x4_t rest;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) rest[e] = v[e] - __uint_as_float(e & 1 ? w[e / 2] & 0xFFFF0000u : w[e / 2] << 16);
+            *(u32x2_t*)((T*)a.residual + at) = u32x2_t{pack_bf16x2(rest[0], rest[1]), pack_bf16x2(rest[2], rest[3])};
+        }
+    } else {
+        *(f32x4_t*)((T*)a.out + at) = v;
+    }
+}
+
 // PLAIN: neither softcap nor slopes, scale > 0: the scale goes into the exponent's multiply-add.
 template <typename T, int DP, bool KEYS, bool PLAIN>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fwd_kernel(MfmaArgs m) {
@@ -38,7 +55,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5;
 
     // blocks of one key head lie on one XCD where there are 8 heads or more; those with the most keys (the last rows) go first
-    const int heads = (int)a.batch * a.kv_heads, bh = blockIdx.x % heads, tile = m.n_tiles - 1 - blockIdx.x / heads, split = blockIdx.y;
+    const int heads = (int)a.batch * a.kv_heads, bh = blockIdx.x % heads, tile = m.blocks - 1 - blockIdx.x / heads, split = blockIdx.y;
     const int b = bh / a.kv_heads, kvh = bh % a.kv_heads;
     const int row0 = tile * Sh::kRows + (KEYS ? 0 : wave * 32);
     int row = row0 + (lane & 31);
@@ -83,14 +100,16 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
         blk.doc_min = __builtin_amdgcn_readfirstlane(blk.doc_min);
         blk.doc_max = __builtin_amdgcn_readfirstlane(blk.doc_max);
     }
-    const int32_t* doc_min = a.docs ? m.doc_min + (int64_t)b * m.walked_tiles : nullptr;
-    const int32_t* doc_max = a.docs ? m.doc_max + (int64_t)b * m.walked_tiles : nullptr;
-    // this block's share of the tiles between the first and the last key that its rows may see
-    int first = 0, end = 0;
-    if (blk.hi_max >= blk.lo_min) {
-        const int t0 = blk.lo_min / Sh::kTile, n = blk.hi_max / Sh::kTile + 1 - t0;
-        first = t0 + (int)((int64_t)n * split / m.splits);
-        end = t0 + (int)((int64_t)n * (split + 1) / m.splits);
+    const int32_t* doc_min = a.docs ? m.key_docs.lowest + (int64_t)b * m.key_docs.tiles : nullptr;
+    const int32_t* doc_max = a.docs ? m.key_docs.highest + (int64_t)b * m.key_docs.tiles : nullptr;
+    const bool any = blk.hi_max >= blk.lo_min;
+    const int first = any ? blk.lo_min / Sh::kTile : 0, end = any ? blk.hi_max / Sh::kTile + 1 : 0;
+    auto active = [&](int t) { return !a.docs || (doc_max[t] >= blk.doc_min && doc_min[t] <= blk.doc_max); };
+    Share share = {1, 0, 0x7FFFFFFF};
+    if (m.splits > 1) {
+        share = share_of(a.docs ? count_tiles(first, end, active) : end - first, split, m);
+        if (split == 0 && threadIdx.x == 0) m.parts[bh * m.blocks + tile] = share.parts;
+        if (split >= share.parts) return;
     }
 
     const T* kbase = (const T*)a.k.p + b * a.k.sb + kvh * a.k.sh;
@@ -122,8 +141,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
 
-        auto active = [&](int t) { return !a.docs || (doc_max[t] >= blk.doc_min && doc_min[t] <= blk.doc_max); };
-        TileWalk<decltype(active)> walk(first, end, active);
+        TileWalk<decltype(active)> walk(first, end, active, share.skip, share.left);
         int cur = walk.next(), buf = 0;
         if (cur >= 0) fetch(cur, 0);
         while (cur >= 0) {
@@ -241,6 +259,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
         }
     };
     run(std::integral_constant<bool, false>());
+    lds_loads_done();  // also where no tile was walked: nothing may land in LDS after the block is gone
     bool bad = false;
 #pragma unroll
     for (int t = 0; t < kCols; ++t) bad |= not_finite(o[t]);
@@ -294,7 +313,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
     const float inv = total == 0.f ? 0.f : 1.f / total;
     const float lse2 = total == 0.f ? -INFINITY : (top == -INFINITY ? 0.f : top) + log2f(total);
     if (!row_in) return;
-    if (m.splits > 1) {
+    if (share.parts > 1) {
         const int64_t at = ((int64_t)split * heads + bh) * m.rows + row;
         float* to = m.part_out + at * a.D;
         if (hi == 0) m.part_lse[at] = lse2;
@@ -315,91 +334,55 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
         for (int j = 0; j < 4; ++j) {
             const int d = 32 * t + 8 * j + 4 * hi;
             if (d >= a.D) continue;
-            const f32x4_t v = {o[t][4 * j] * inv, o[t][4 * j + 1] * inv, o[t][4 * j + 2] * inv, o[t][4 * j + 3] * inv};
-            if constexpr (sizeof(T) == 2) {
-                const u32x2_t w = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-                *(u32x2_t*)(to + d) = w;
-                if (a.residual) {
-                    f32x4_t rest;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) rest[e] = v[e] - __uint_as_float(e & 1 ? w[e / 2] & 0xFFFF0000u : w[e / 2] << 16);
-                    *(u32x2_t*)((T*)a.residual + (to - (T*)a.out) + d) = u32x2_t{pack_bf16x2(rest[0], rest[1]), pack_bf16x2(rest[2], rest[3])};
-                }
-            } else {
-                *(f32x4_t*)(to + d) = v;
-            }
+            store_out<T>(a, (to - (T*)a.out) + d, f32x4_t{o[t][4 * j] * inv, o[t][4 * j + 1] * inv, o[t][4 * j + 2] * inv, o[t][4 * j + 3] * inv});
         }
 }
 
-// Joins the parts of a row: out = sum 2^(lse_i - max) out_i / sum 2^(lse_i - max).  A wavefront per row.
+// Joins the parts of a row: out = sum 2^(lse_i - max) out_i / sum 2^(lse_i - max).  32 lanes per row, four columns a lane.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void attention_join_kernel(MfmaArgs m) {
+__global__ __launch_bounds__(kThreads) void attention_join_kernel(MfmaArgs m, int block_rows) {
     const AttnArgs& a = m.a;
-    const int lane = threadIdx.x & 63, heads = (int)a.batch * a.kv_heads;
-    const int64_t index = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6), per_split = (int64_t)heads * m.rows;
+    const int lane = threadIdx.x & 31, heads = (int)a.batch * a.kv_heads, d = 4 * lane;
+    const int64_t index = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), per_split = (int64_t)heads * m.rows;
     if (index >= per_split) return;
-    const int bh = (int)(index / m.rows), row = (int)(index - (int64_t)bh * m.rows), b = bh / a.kv_heads, kvh = bh % a.kv_heads;
+    const int bh = (int)(index / m.rows), row = (int)(index - (int64_t)bh * m.rows), b = bh / a.kv_heads, kvh = bh - b * a.kv_heads;
+    const int parts = m.parts[bh * m.blocks + row / block_rows];
+    if (parts == 1) return;  // written by its block
     const int s = m.div(row), head = kvh * a.group + row - s * a.group;
     float top = -INFINITY;
-    for (int i = lane; i < m.splits; i += 64) top = __builtin_fmaxf(top, m.part_lse[i * per_split + index]);
-    top = wave_max(top);
+    for (int i = 0; i < parts; ++i) top = __builtin_fmaxf(top, m.part_lse[i * per_split + index]);
     const float base = top == -INFINITY ? 0.f : top;
-    float total = 0.f, sum[4] = {};
-    for (int i = 0; i < m.splits; ++i) {
-        const float lse2 = m.part_lse[i * per_split + index];
-        if (lse2 == -INFINITY) continue;  // saw no key
+    float total = 0.f;
+    f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) {
+        const float lse2 = m.part_lse[i * per_split + index];  // -inf: saw no key
         const float weight = __builtin_amdgcn_exp2f(lse2 - base);
         total += weight;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-            if (c * 64 + lane < a.D) sum[c] += weight * m.part_out[(i * per_split + index) * a.D + c * 64 + lane];
+        if (d < a.D) sum += weight * *(const f32x4_t*)(m.part_out + (i * per_split + index) * a.D + d);
     }
-    T* to = (T*)a.out + (((int64_t)b * a.q_len + s) * a.heads + head) * a.D;
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-        if (c * 64 + lane < a.D) {
-            const float v = total == 0.f ? 0.f : sum[c] / total;
-            to[c * 64 + lane] = (T)v;
-            if (sizeof(T) == 2 && a.residual) ((T*)a.residual)[(to - (T*)a.out) + c * 64 + lane] = (T)(v - (float)(T)v);
-        }
     if (lane == 0) a.lse[((int64_t)b * a.heads + head) * a.q_len + s] = total == 0.f ? -INFINITY : (base + log2f(total)) * (1.f / kLog2e);
+    if (d >= a.D) return;
+    const int64_t at = (((int64_t)b * a.q_len + s) * a.heads + head) * a.D + d;
+    store_out<T>(a, at, sum * (total == 0.f ? 0.f : 1.f / total));
 }
 
-// lowest and highest document of every tile of `per` rows, row r standing for token r / group + offset; -1 where a token is none
-__global__ __launch_bounds__(kThreads) void attention_documents_kernel(const int32_t* __restrict__ docs, int kv_len, int per, int tiles, int rows,
-                                                                       int offset, GroupDiv div, int32_t* __restrict__ lowest,
-                                                                       int32_t* __restrict__ highest) {
-    const int tile_blocks = (tiles + kWaves - 1) / kWaves, b = blockIdx.x / tile_blocks, lane = threadIdx.x & 63;
-    const int tile = (blockIdx.x - b * tile_blocks) * kWaves + (threadIdx.x >> 6);
-    if (tile >= tiles) return;
-    int lo = 0x7FFFFFFF, hi = -1;
-    for (int i = lane; i < per; i += 64) {
-        const int row = tile * per + i;
-        if (row >= rows) break;
-        const int pos = div(row) + offset;
-        const int doc = pos >= 0 ? docs[(int64_t)b * kv_len + pos] : -1;
-        lo = min(lo, doc);
-        hi = max(hi, doc);
-    }
-    lo = wave_min_i32(lo);
-    hi = wave_max_i32(hi);
-    if (lane == 0) {
-        lowest[(int64_t)b * tiles + tile] = lo;
-        highest[(int64_t)b * tiles + tile] = hi;
-    }
+__global__ __launch_bounds__(kThreads) void attention_documents_kernel(const int32_t* __restrict__ docs, int kv_len, int tile, int tiles,
+                                                                       int32_t* __restrict__ lowest, int32_t* __restrict__ highest) {
+    document_range(docs, kv_len, blockIdx.x, tile, tiles, kv_len, 0, GroupDiv{0u, 0}, lowest, highest);
 }
 
 template <typename T, int DP, bool KEYS, bool PLAIN>
 int launch(const MfmaArgs& m, hipStream_t s) {
     typedef FwdShape<T, DP, KEYS> Sh;
-    const hipError_t e = hipFuncSetAttribute((const void*)attention_fwd_kernel<T, DP, KEYS, PLAIN>, hipFuncAttributeMaxDynamicSharedMemorySize, Sh::kLds);
+    const hipError_t e = allow_lds<attention_fwd_kernel<T, DP, KEYS, PLAIN>>(Sh::kLds);
     if (e != hipSuccess) return PICOMOE_ERR_HIP_BASE + (int)e;
-    const int64_t blocks = (int64_t)m.n_tiles * m.a.batch * m.a.kv_heads;
+    const int64_t blocks = (int64_t)m.blocks * m.a.batch * m.a.kv_heads;
     if (blocks > 0x7FFFFFFF) return PICOMOE_ERR_TOO_LARGE;
     attention_fwd_kernel<T, DP, KEYS, PLAIN><<<dim3((unsigned)blocks, (unsigned)m.splits), kThreads, Sh::kLds, s>>>(m);
     if (m.splits > 1) {
         const int64_t rows = (int64_t)m.a.batch * m.a.kv_heads * m.rows;
-        attention_join_kernel<T><<<(unsigned)((rows + kWaves - 1) / kWaves), kThreads, 0, s>>>(m);
+        attention_join_kernel<T><<<(unsigned)((rows + 7) / 8), kThreads, 0, s>>>(m, Sh::kRows);
     }
     return picomoe_launch_status();
 }
@@ -411,9 +394,9 @@ int launch_for(const MfmaArgs& m, bool keys, hipStream_t s) {
 }
 
 struct Plan {
-    bool keys;      // the waves of a block share 32 rows
-    int tile, n_tiles, splits, walked_tiles;
-    int64_t doc_bytes, out_bytes, lse_bytes;
+    bool keys;  // the waves of a block share 32 rows
+    int tile, blocks, key_tiles, splits, target;
+    int64_t doc_bytes, parts_bytes, out_bytes, lse_bytes;
 };
 int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 
@@ -423,15 +406,16 @@ Plan plan(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, 
     p.keys = rows <= 32;
     p.tile = p.keys ? 128 : (dtype == PICOMOE_BF16 ? 64 : 32);
     const int per = p.keys ? 32 : 32 * kWaves;
-    p.n_tiles = (int)((rows + per - 1) / per);
-    p.walked_tiles = (int)((kv_len + p.tile - 1) / p.tile);
-    // Fewer blocks than two per CU: the keys are cut until there are, down to four tiles a part
-    const int64_t blocks = heads * p.n_tiles;
-    int64_t splits = blocks > 0 ? 512 / blocks : 1;
-    if (splits > p.walked_tiles / 4) splits = p.walked_tiles / 4;
-    if (splits > 256) splits = 256;
-    p.splits = splits < 1 ? 1 : (int)splits;
-    p.doc_bytes = round16(batch * p.walked_tiles * 8);
+    p.blocks = (int)((rows + per - 1) / per);
+    p.key_tiles = (int)((kv_len + p.tile - 1) / p.tile);
+    // Walks are cut where they are longer than what each of the 512 blocks that the chip holds gets of all rows x all keys
+    const int64_t share = (heads * p.blocks * p.key_tiles + 511) / 512, shortest = p.keys ? 2 : 4, longest = (p.key_tiles + 255) / 256;
+    int64_t target = share > shortest ? share : shortest;
+    target = target > longest ? target : longest;
+    p.target = (int)(target < p.key_tiles || p.key_tiles == 0 ? target : p.key_tiles);
+    p.splits = p.key_tiles > p.target ? (p.key_tiles + p.target - 1) / p.target : 1;
+    p.doc_bytes = round16(batch * p.key_tiles * 8);
+    p.parts_bytes = p.splits > 1 ? round16(heads * p.blocks * 4) : 0;
     p.out_bytes = p.splits > 1 ? round16((int64_t)p.splits * heads * rows * head_dim * 4) : 0;
     p.lse_bytes = p.splits > 1 ? round16((int64_t)p.splits * heads * rows * 4) : 0;
     return p;
@@ -443,16 +427,7 @@ bool attention_mfma_supported(int head_dim) { return head_dim <= 128; }
 
 int64_t attention_mfma_fwd_workspace(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, int kv_heads, int head_dim) {
     const Plan p = plan(dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim);
-    return p.doc_bytes + p.out_bytes + p.lse_bytes + 16;
-}
-
-int attention_mfma_documents(const AttnArgs& a, int per, int tiles, int rows, int offset, int group, int32_t* lowest, int32_t* highest, hipStream_t s) {
-    if (tiles == 0) return PICOMOE_OK;
-    const int64_t blocks = (int64_t)((tiles + kWaves - 1) / kWaves) * a.batch;
-    if (blocks > 0x7FFFFFFF) return PICOMOE_ERR_TOO_LARGE;
-    attention_documents_kernel<<<(unsigned)blocks, kThreads, 0, s>>>(
-        a.docs, a.kv_len, per, tiles, rows, offset, group_div(group), lowest, highest);
-    return picomoe_launch_status();
+    return p.doc_bytes + p.parts_bytes + p.out_bytes + p.lse_bytes + 16;
 }
 
 int attention_mfma_fwd(const AttnArgs& a, hipStream_t s) {
@@ -461,17 +436,18 @@ int attention_mfma_fwd(const AttnArgs& a, hipStream_t s) {
     m.a = a;
     m.div = group_div(a.group);
     m.rows = a.q_len * a.group;
-    m.n_tiles = p.n_tiles;
+    m.blocks = p.blocks;
     m.splits = p.splits;
-    m.walked_tiles = p.walked_tiles;
+    m.target = p.target;
     int32_t* lowest = (int32_t*)a.ws;
-    m.doc_min = lowest;
-    m.doc_max = lowest + a.batch * p.walked_tiles;
-    m.part_out = (float*)(a.ws + p.doc_bytes);
-    m.part_lse = (float*)(a.ws + p.doc_bytes + p.out_bytes);
-    if (a.docs) {
-        const int rc = attention_mfma_documents(a, p.tile, p.walked_tiles, a.kv_len, 0, 1, lowest, lowest + a.batch * p.walked_tiles, s);
-        if (rc) return rc;
+    m.key_docs = {lowest, lowest + a.batch * p.key_tiles, p.key_tiles};
+    m.parts = (int32_t*)(a.ws + p.doc_bytes);
+    m.part_out = (float*)(a.ws + p.doc_bytes + p.parts_bytes);
+    m.part_lse = (float*)(a.ws + p.doc_bytes + p.parts_bytes + p.out_bytes);
+    if (a.docs && p.key_tiles > 0) {
+        const int64_t blocks = a.batch * range_blocks(p.key_tiles);
+        if (blocks > 0x7FFFFFFF) return PICOMOE_ERR_TOO_LARGE;
+        attention_documents_kernel<<<(unsigned)blocks, kThreads, 0, s>>>(a.docs, a.kv_len, p.tile, p.key_tiles, lowest, lowest + a.batch * p.key_tiles);
     }
     if (a.dtype == PICOMOE_BF16) return a.D <= 64 ? launch_for<__bf16, 64>(m, p.keys, s) : launch_for<__bf16, 128>(m, p.keys, s);
     return a.D <= 64 ? launch_for<float, 64>(m, p.keys, s) : launch_for<float, 128>(m, p.keys, s);

@@ -7,6 +7,8 @@
 // accumulators of a lane are, as they lie, the fragment of P (or dx) for the product that follows, with its k (keys or queries)
 // in the order 16 s + {4 hi + 0..3, 8 + 4 hi + 0..3}; the other operand is read from LDS in that order.  P never passes through LDS.
 #pragma once
+#include <atomic>
+
 #include "attention.h"
 
 namespace {
@@ -224,16 +226,22 @@ inline GroupDiv group_div(int group) {
     return {shift == 0 ? 0u : (uint32_t)(((uint64_t)1 << (31 + shift)) / (uint32_t)group + 1), shift};
 }
 
+struct DocRanges {  // lowest and highest document of every tile: [batch, tiles], -1 among them where a token has no document
+    const int32_t *lowest, *highest;
+    int tiles;
+};
+
 struct MfmaArgs {
     AttnArgs a;
     GroupDiv div;
-    int rows;                 // of a key head: q_len * group
-    int n_tiles, splits;      // tiles of the launch's blocks; parts that the walked dimension is cut into
-    const int32_t* doc_min;   // of every tile of the walked dimension: [batch, walked tiles], -1 among them where a token has no document
-    const int32_t* doc_max;
-    int walked_tiles;
-    float* part_out;          // splits > 1: partial results
+    int rows;  // of a key head: q_len * group
+    // Forward and dq: row blocks that walk key tiles; dk / dv: key blocks that walk row tiles.  A block whose walk is longer than
+    // `target` tiles is cut into at most `splits` parts of consecutive tiles; how many is noted in parts.
+    int blocks, splits, target;
+    int32_t* parts;
+    float* part_out;
     float* part_lse;
+    DocRanges key_docs, row_docs;
 };
 
 // what a set of query rows may see, and which documents it has
@@ -241,25 +249,83 @@ struct Reach {
     int lo_min, lo_max, hi_min, hi_max, doc_min, doc_max;
 };
 
-// the walk over the walked dimension's tiles that pass `active`, 64 at a time; the same in every wave of a block
+// The walk over the tiles of [first, end) that pass `active`, 64 at a time, the first `skip` of those left out and `left` taken; the
+// same in every wave of a block.
 template <typename F>
 struct TileWalk {
     F active;
-    int base, end;
+    int base, end, skip, left;
     uint64_t mask;
-    __device__ __forceinline__ TileWalk(int first, int end_, F f) : active(f), base(first - 64), end(end_), mask(0) {}
+    __device__ __forceinline__ TileWalk(int first, int end_, F f, int skip_, int left_)
+        : active(f), base(first - 64), end(end_), skip(skip_), left(left_), mask(0) {}
     __device__ __forceinline__ int next() {
+        if (left <= 0) return -1;
         while (mask == 0) {
             base += 64;
             if (base >= end) return -1;
             const int t = base + (int)(threadIdx.x & 63);
             mask = __ballot(t < end && active(t));
+            const int here = __builtin_popcountll(mask);
+            if (skip >= here) {
+                skip -= here;
+                mask = 0;
+            }
+            for (; skip > 0 && mask; --skip) mask &= mask - 1;
         }
         const int t = base + __builtin_ctzll(mask);
         mask &= mask - 1;
+        --left;
         return t;
     }
 };
+
+// Lowest and highest document of the tiles of `per` rows that block `block` of a launch looks at, a wavefront a tile; row r
+// stands for token r / group + offset, -1 where that is none.  range_blocks(tiles) blocks per batch element.
+__host__ __device__ inline int range_blocks(int tiles) { return (tiles + kWaves - 1) / kWaves; }
+__device__ __forceinline__ void document_range(const int32_t* __restrict__ docs, int kv_len, int block, int per, int tiles, int rows, int offset,
+                                               const GroupDiv& div, int32_t* __restrict__ lowest, int32_t* __restrict__ highest) {
+    const int b = block / range_blocks(tiles), lane = threadIdx.x & 63;
+    const int tile = (block - b * range_blocks(tiles)) * kWaves + (threadIdx.x >> 6);
+    if (tile >= tiles) return;
+    int lo = 0x7FFFFFFF, hi = -1;
+    for (int i = lane; i < per; i += 64) {
+        const int row = tile * per + i;
+        if (row >= rows) break;
+        const int pos = div(row) + offset;
+        const int doc = pos >= 0 ? docs[(int64_t)b * kv_len + pos] : -1;
+        lo = min(lo, doc);
+        hi = max(hi, doc);
+    }
+    lo = wave_min_i32(lo);
+    hi = wave_max_i32(hi);
+    if (lane == 0) {
+        lowest[(int64_t)b * tiles + tile] = lo;
+        highest[(int64_t)b * tiles + tile] = hi;
+    }
+}
+
+// the tiles that a walk passes
+template <typename F>
+__device__ __forceinline__ int count_tiles(int first, int end, F active) {
+    int n = 0;
+    for (int base = first; base < end; base += 64) {
+        const int t = base + (int)(threadIdx.x & 63);
+        n += __builtin_popcountll(__ballot(t < end && active(t)));
+    }
+    return n;
+}
+// a block's share of its walk: tiles skip .. skip + left - 1 of those that the walk passes
+struct Share {
+    int parts, skip, left;
+};
+__device__ __forceinline__ Share share_of(int tiles, int split, const MfmaArgs& m) {
+    Share s;
+    s.parts = (tiles + m.target - 1) / m.target;
+    s.parts = s.parts < 1 ? 1 : (s.parts < m.splits ? s.parts : m.splits);
+    s.skip = (int)((int64_t)tiles * split / s.parts);
+    s.left = (int)((int64_t)tiles * (split + 1) / s.parts) - s.skip;
+    return s;
+}
 
 // S in log2 units from q . k.  softcap > 0: cap2 * tanh(x / cap) with tanh(y) = 1 - 2 / (1 + e^(2y)); bf16 takes the hardware's
 // exponential and reciprocal (absolute error some 1e-7 of softcap), fp32 the library's tanh.
@@ -276,6 +342,20 @@ template <typename T>
 __device__ __forceinline__ float capped(float x, float mul) {  // tanh(x * scale / softcap)
     if (sizeof(T) == 2) return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * mul));
     return tanhf(x * mul);
+}
+
+// lets a kernel have `bytes` of dynamic LDS; asked once per device
+template <auto KERNEL>
+inline hipError_t allow_lds(int bytes) {
+    static std::atomic<uint64_t> allowed{0};
+    int device = 0;
+    const hipError_t e = hipGetDevice(&device);
+    if (e != hipSuccess) return e;
+    const uint64_t bit = device < 64 ? 1ull << device : 0;
+    if (allowed.load(std::memory_order_relaxed) & bit) return hipSuccess;
+    const hipError_t set = hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (set == hipSuccess) allowed.fetch_or(bit, std::memory_order_relaxed);
+    return set;
 }
 
 }  // namespace
