@@ -16,7 +16,8 @@ namespace {
 template <typename T, int DP>
 struct DqShape {
     static constexpr int kTile = sizeof(T) == 2 ? 64 : 32;
-    static constexpr int kTileBytes = kTile * DP * (int)sizeof(T);
+    typedef Tile<T, DP, kTile> Tl;
+    static constexpr int kTileBytes = Tl::kBytes;
     static constexpr int kBuf = 2 * kTileBytes + kTile * 4;  // K, V, document ids
     static constexpr int kLds = 2 * kBuf;
 };
@@ -26,7 +27,7 @@ template <typename T, int DP, bool PLAIN>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq_kernel(MfmaArgs m) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     typedef DqShape<T, DP> Sh;
-    typedef Tile<T, DP> Tl;
+    typedef typename Sh::Tl Tl;
     constexpr int kSub = Sh::kTile / 32, kSteps = DP / 16, kCols = DP / 32;
     const AttnArgs& a = m.a;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5;
@@ -104,11 +105,12 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq
     auto fetch = [&](int t, int buf) {
         char* kt = lds + buf * Sh::kBuf;
         auto key_at = [&](int r) { return (int64_t)min(t * Sh::kTile + r, a.kv_len - 1); };
-        Tl::template load<Sh::kTile>(kt, a.D, [&](int r) { return kbase + key_at(r) * a.k.ss; });
-        Tl::template load<Sh::kTile>(kt + Sh::kTileBytes, a.D, [&](int r) { return vbase + key_at(r) * a.v.ss; });
+        Tl::load(kt, a.D, [&](int r) { return kbase + key_at(r) * a.k.ss; });
+        Tl::load(kt + Sh::kTileBytes, a.D, [&](int r) { return vbase + key_at(r) * a.v.ss; });
         if (a.docs && wave == 0 && lane < Sh::kTile) load4_to_lds(a.docs + (int64_t)b * a.kv_len + key_at(lane), kt + 2 * Sh::kTileBytes);
     };
 
+    const typename Tl::Lane ln;
     const ScoreScale sc = score_scale<T>(a);
     f32x16_t dq[kCols];
     auto run = [&](auto careful) {  // CAREFUL: as in the forward, for K
@@ -128,6 +130,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq
             const char* kt = lds + buf * Sh::kBuf;
             const char* vt = kt + Sh::kTileBytes;
             const int32_t* docs = (const int32_t*)(vt + Sh::kTileBytes);
+            const uint32_t ka = lds_address(kt), va = ka + Sh::kTileBytes;
             const int key0 = cur * Sh::kTile, key1 = key0 + Sh::kTile - 1;
             bool in = key0 <= w.hi_max && key1 >= w.lo_min, full = key0 >= w.lo_max && key1 <= w.hi_min;
             if (a.docs) {
@@ -143,8 +146,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq
                     for (int i = 0; i < 16; ++i) x[i] = dp[i] = 0.f;
 #pragma unroll
                     for (int ks = 0; ks < kSteps; ++ks) {
-                        mma(x, Tl::frag(kt, u * 32 + (lane & 31), ks, hi), qf[ks]);
-                        mma(dp, Tl::frag(vt, u * 32 + (lane & 31), ks, hi), gf[ks]);
+                        mma(x, Tl::frag(ka, ln, u * 32, ks), qf[ks]);
+                        mma(dp, Tl::frag(va, ln, u * 32, ks), gf[ks]);
                     }
 #pragma unroll
                     for (int i = 0; i < 16; ++i) dp[i] -= delta;
@@ -182,7 +185,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq
                         const Frag<T> dx = to_frag<T>(x, st);
 #pragma unroll
                         for (int t = 0; t < kCols; ++t) {
-                            Frag<T> k = Tl::frag_t(kt, u * 32 + 16 * st, t, lane);
+                            Frag<T> k = Tl::frag_t(ka, ln, u * 32 + 16 * st, t);
                             if (kCareful) zero_not_finite(k);
                             mma(dq[t], k, dx);
                         }
@@ -237,12 +240,14 @@ template <typename T, int DP>
 struct DkvShape {
     static constexpr int kTile = 32;              // rows of a tile
     static constexpr int kKeys = 32 * kWaves;     // keys of a block
-    static constexpr int kTileBytes = kTile * DP * (int)sizeof(T);
+    typedef Tile<T, DP, kTile> Tl;
+    typedef Tile<T, DP, kKeys> VTl;
+    static constexpr int kTileBytes = Tl::kBytes;
     static constexpr int kStats = 7 * kTile * 4;  // lse2, delta, slope2 (floats), position, first key, keys, document (ints)
     static constexpr int kBuf = 2 * kTileBytes + kStats;
     // V's fragments are the ones that do not fit the 256 registers of a lane at head_dim 128 (dk, dv, K, S, dP do): read from LDS
     static constexpr bool kVInLds = DP == 128;
-    static constexpr int kVBytes = kVInLds ? kKeys * DP * (int)sizeof(T) : 0;
+    static constexpr int kVBytes = kVInLds ? VTl::kBytes : 0;
     static constexpr int kLds = 2 * kBuf + kVBytes;
 };
 
@@ -250,7 +255,7 @@ template <typename T, int DP, bool PLAIN>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dkv_kernel(MfmaArgs m) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     typedef DkvShape<T, DP> Sh;
-    typedef Tile<T, DP> Tl;
+    typedef typename Sh::Tl Tl;
     constexpr int kSteps = DP / 16, kCols = DP / 32, kBuf = Sh::kBuf;
     const AttnArgs& a = m.a;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5;
@@ -305,7 +310,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
     char* vtile = lds + 2 * kBuf;
     if (Sh::kVInLds) {
         const T* v = (const T*)a.v.p + b * a.v.sb + kvh * a.v.sh;
-        Tl::template load<Sh::kKeys>(vtile, a.D, [&](int r) { return v + (int64_t)min(block0 + r, a.kv_len - 1) * a.v.ss; });
+        Sh::VTl::load(vtile, a.D, [&](int r) { return v + (int64_t)min(block0 + r, a.kv_len - 1) * a.v.ss; });
     }
     {
         const T* k = (const T*)a.k.p + b * a.k.sb + (int64_t)key_at * a.k.ss + kvh * a.k.sh;
@@ -323,11 +328,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
     auto fetch = [&](int t, int buf) {
         char* qt = lds + buf * kBuf;
         auto row_at = [&](int r) { return min(t * Sh::kTile + r, m.rows - 1); };
-        Tl::template load<Sh::kTile>(qt, a.D, [&](int r) {
+        Tl::load(qt, a.D, [&](int r) {
             const int s = m.div(row_at(r)), h = row_at(r) - s * a.group;
             return qbase + s * a.q.ss + h * a.q.sh;
         });
-        Tl::template load<Sh::kTile>(qt + Sh::kTileBytes, a.D, [&](int r) {
+        Tl::load(qt + Sh::kTileBytes, a.D, [&](int r) {
             const int s = m.div(row_at(r)), h = row_at(r) - s * a.group;
             return gbase + ((int64_t)s * a.heads + h) * a.D;
         });
@@ -356,6 +361,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
         }
     };
 
+    const typename Tl::Lane ln;
+    const uint32_t v_rows = lds_address(vtile) + wave * 32 * Tl::kRowBytes;
     const ScoreScale sc = score_scale<T>(a);
     f32x16_t dk[kCols], dv[kCols];
     auto run = [&](auto careful) {  // CAREFUL: as in the forward, for Q and dO
@@ -375,6 +382,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
             if (following >= 0) fetch(following, buf ^ 1);
             const char* qt = lds + buf * kBuf;
             const char* gt = qt + Sh::kTileBytes;
+            const uint32_t qa = lds_address(qt), ga = qa + Sh::kTileBytes;
             const float* stats = (const float*)(gt + Sh::kTileBytes);
             const int* stati = (const int*)(stats + 3 * Sh::kTile);
             const int s0 = first_query(cur), s1 = last_query(cur);
@@ -391,8 +399,15 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
                 for (int i = 0; i < 16; ++i) x[i] = dp[i] = 0.f;
 #pragma unroll
                 for (int ks = 0; ks < kSteps; ++ks) {
-                    mma(x, Tl::frag(qt, lane & 31, ks, hi), kf[ks]);
-                    mma(dp, Tl::frag(gt, lane & 31, ks, hi), Sh::kVInLds ? Tl::frag(vtile, wave * 32 + (lane & 31), ks, hi) : vf[ks]);
+                    mma(x, Tl::frag(qa, ln, 0, ks), kf[ks]);
+                    if constexpr (Sh::kVInLds) {
+                        typename Sh::VTl::Lane vl;
+                        vl.row = ln.row;
+                        vl.row2 = ln.row2;
+                        mma(dp, Tl::frag(ga, ln, 0, ks), Sh::VTl::frag(v_rows, vl, 0, ks));
+                    } else {
+                        mma(dp, Tl::frag(ga, ln, 0, ks), vf[ks]);
+                    }
                 }
                 auto stat4 = [&](int which, int j) { return *(const f32x4_t*)(stats + which * Sh::kTile + 8 * j + 4 * hi); };
                 auto stat4i = [&](int which, int j) {
@@ -451,7 +466,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
                     const Frag<T> p = to_frag<T>(x, st), dx = to_frag<T>(dp, st);
 #pragma unroll
                     for (int t = 0; t < kCols; ++t) {
-                        Frag<T> g = Tl::frag_t(gt, 16 * st, t, lane), q = Tl::frag_t(qt, 16 * st, t, lane);
+                        Frag<T> g = Tl::frag_t(ga, ln, 16 * st, t), q = Tl::frag_t(qa, ln, 16 * st, t);
                         if (kCareful) {
                             zero_not_finite(g);
                             zero_not_finite(q);

@@ -21,8 +21,9 @@ struct FwdShape {
     static constexpr int kTile = KEYS ? 128 : (sizeof(T) == 2 ? 64 : 32);  // keys of a tile
     static constexpr int kWaveKeys = KEYS ? 32 : kTile;
     static constexpr int kRows = KEYS ? 32 : 32 * kWaves;  // rows of a block
-    static constexpr int kTileBytes = kTile * DP * (int)sizeof(T);
-    static constexpr int kBuffers = kTileBytes <= 32768 ? 2 : 1;  // two of 128 KB do not fit
+    typedef Tile<T, DP, kTile> Tl;
+    static constexpr int kTileBytes = Tl::kBytes;
+    static constexpr int kBuffers = kTileBytes <= 36 * 1024 ? 2 : 1;  // two of 128 KB do not fit
     static constexpr int kBuf = 2 * kTileBytes + kTile * 4;       // K, V, document ids
     static constexpr int kLds = kBuffers * kBuf;
 };
@@ -48,7 +49,7 @@ __device__ __forceinline__ void store_out(const AttnArgs& a, int64_t at, f32x4_t
 template <typename T, int DP, bool KEYS, bool PLAIN>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fwd_kernel(MfmaArgs m) {
     typedef FwdShape<T, DP, KEYS> Sh;
-    typedef Tile<T, DP> Tl;
+    typedef typename Sh::Tl Tl;
     constexpr int kSub = Sh::kWaveKeys / 32, kSteps = DP / 16, kCols = DP / 32;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const AttnArgs& a = m.a;
@@ -119,13 +120,14 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
         char* kt = lds + buf * Sh::kBuf;
         // keys past the end are hidden by every row's interval
         auto key_at = [&](int r) { return (int64_t)min(t * Sh::kTile + r, a.kv_len - 1); };
-        Tl::template load<Sh::kTile>(kt, a.D, [&](int r) { return kbase + key_at(r) * a.k.ss; });
-        Tl::template load<Sh::kTile>(kt + Sh::kTileBytes, a.D, [&](int r) { return vbase + key_at(r) * a.v.ss; });
+        Tl::load(kt, a.D, [&](int r) { return kbase + key_at(r) * a.k.ss; });
+        Tl::load(kt + Sh::kTileBytes, a.D, [&](int r) { return vbase + key_at(r) * a.v.ss; });
         if (a.docs && wave < Sh::kTile / 64)
             load4_to_lds(a.docs + (int64_t)b * a.kv_len + key_at(wave * 64 + lane), kt + 2 * Sh::kTileBytes + wave * 256);
         if (a.docs && Sh::kTile < 64 && wave == 0 && lane < Sh::kTile) load4_to_lds(a.docs + (int64_t)b * a.kv_len + key_at(lane), kt + 2 * Sh::kTileBytes);
     };
 
+    const typename Tl::Lane ln;
     const ScoreScale sc = score_scale<T>(a);
     f32x16_t o[kCols];
     float top = -INFINITY, total = 0.f;  // running maximum that P refers to (log2 units), this lane's share of the sum
@@ -152,6 +154,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
             const char* kt = lds + buf * Sh::kBuf;
             const char* vt = kt + Sh::kTileBytes;
             const int32_t* docs = (const int32_t*)(vt + Sh::kTileBytes);
+            const uint32_t ka = lds_address(kt) + (KEYS ? wave * 32 * Tl::kRowBytes : 0), va = ka + Sh::kTileBytes;
             const int sub0 = KEYS ? wave * 32 : 0, key0 = cur * Sh::kTile + sub0, key1 = key0 + Sh::kWaveKeys - 1;
             bool in = key0 <= w.hi_max && key1 >= w.lo_min, full = key0 >= w.lo_max && key1 <= w.hi_min;
             if (a.docs) {
@@ -166,7 +169,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
 #pragma unroll
                     for (int i = 0; i < 16; ++i) x[u][i] = 0.f;
 #pragma unroll
-                    for (int ks = 0; ks < kSteps; ++ks) mma(x[u], Tl::frag(kt, sub0 + u * 32 + (lane & 31), ks, hi), qf[ks]);
+                    for (int ks = 0; ks < kSteps; ++ks) mma(x[u], Tl::frag(ka, ln, u * 32, ks), qf[ks]);
                 }
                 if (PLAIN) {
                 } else if (sc.cap2 > 0.f) {
@@ -228,7 +231,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
                     const Frag<T> p = to_frag<T>(x[st / 2], st & 1);
 #pragma unroll
                     for (int t = 0; t < kCols; ++t) {
-                        Frag<T> v = Tl::frag_t(vt, sub0 + 16 * st, t, lane);
+                        Frag<T> v = Tl::frag_t(va, ln, 16 * st, t);
                         if (kCareful) zero_not_finite(v);
                         mma(o[t], v, p);
                     }

@@ -7,8 +7,6 @@
 // accumulators of a lane are, as they lie, the fragment of P (or dx) for the product that follows, with its k (keys or queries)
 // in the order 16 s + {4 hi + 0..3, 8 + 4 hi + 0..3}; the other operand is read from LDS in that order.  P never passes through LDS.
 #pragma once
-#include <atomic>
-
 #include "attention.h"
 
 namespace {
@@ -101,26 +99,50 @@ __device__ __forceinline__ void clear_lds(char* lds, int bytes) {
     __syncthreads();
 }
 
-// Tiles in LDS: `rows` rows of DP elements in 16-byte chunks, chunk c of a row at c ^ swizzle(row).  The 16 rows that a
-// ds_read_b128 serves at a time, and the 4 rows x 64 bytes of a transposing read, then lie on different banks.
-template <typename T, int DP>
+// Tiles in LDS: panels of 16 columns, in a panel ROWS rows of 32 (fp32: 64) bytes in 16-byte chunks, chunk c of a row at
+// c ^ swizzle(row); 128 bytes between panels.  The 16 rows that a ds_read_b128 serves at a time, and the 4 rows of two neighbouring
+// panels of a transposing read, then lie on different banks, and every fragment of a tile is at a constant distance from a lane's
+// first: three address registers a tile, where swizzled rows of the whole width took one per fragment -- with dk and dv in
+// registers those spilled, and a reload from scratch waits for the tile in flight.
+template <typename T, int DP, int ROWS>
 struct Tile {
-    static constexpr int kRowBytes = DP * (int)sizeof(T), kChunks = kRowBytes / 16, kPerChunk = 16 / (int)sizeof(T);
-    static constexpr int kRowsPerPass = kThreads / kChunks;  // rows that the block's threads stage at a time
+    static constexpr int kSize = (int)sizeof(T), kPerChunk = 16 / kSize, kRowBytes = 16 * kSize, kRowChunks = kSize;  // of a panel
+    static constexpr int kPanels = DP / 16, kStride = ROWS * kRowBytes + 128, kBytes = kPanels * kStride;
+    typedef __attribute__((address_space(3))) const bf16x8_t lds_bf16x8;
+    typedef __attribute__((address_space(3))) const f32x4_t lds_f32x4;
+    typedef __attribute__((address_space(3))) const float lds_f32;
 
-    __device__ static __forceinline__ uint32_t swizzle(int row) {
-        if (kRowBytes == 128) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
-        return ((row & 3) << 2) | ((row >> 2) & 3);
+    __device__ static __forceinline__ uint32_t swizzle(int row) { return kSize == 2 ? (row >> 3) & 1 : (row >> 2) & 3; }
+    __device__ static __forceinline__ uint32_t at(int row, int col) {
+        return col / 16 * kStride + row * kRowBytes + (((uint32_t)(col % 16 / kPerChunk) ^ swizzle(row)) << 4) + col % kPerChunk * kSize;
     }
-    __device__ static __forceinline__ uint32_t at(int row, uint32_t chunk) { return row * kRowBytes + ((chunk ^ swizzle(row)) << 4); }
 
-    // row `row` (a multiple of 32 plus lane % 32), elements 16 ks + 8 hi ..
-    __device__ static __forceinline__ Frag<T> frag(const char* tile, int row, int ks, int hi) {
+    // this lane's offsets: fragments of rows lane % 32, and of the transposed tile
+    struct Lane {
+        uint32_t row, row2, col, col2;
+        __device__ __forceinline__ Lane() {
+            const int lane = threadIdx.x & 63, hi = lane >> 5;
+            row = at(lane & 31, hi * 8);
+            row2 = row ^ 16;  // fp32: the second half of the eight
+            if (kSize == 2) {
+                // a transposing read: lane l of 16 gives the address of 4 elements of row l / 4 and gets column l of the 4 rows
+                col = at(4 * hi + ((lane >> 2) & 3), 16 * ((lane >> 4) & 1) + 4 * (lane & 3));
+                col2 = at(4 * hi + ((lane >> 2) & 3) + 8, 16 * ((lane >> 4) & 1) + 4 * (lane & 3));
+            } else {
+                col = at(4 * hi, lane & 31);
+                col2 = at(4 * hi + 8, lane & 31);
+            }
+        }
+    };
+
+    // rows row0 (a multiple of 32) + lane % 32, elements 16 ks + 8 hi ..; tile: its LDS address
+    __device__ static __forceinline__ Frag<T> frag(uint32_t tile, const Lane& l, int row0, int ks) {
         Frag<T> f;
-        if constexpr (sizeof(T) == 2) {
-            f.v = *(const bf16x8_t*)(tile + at(row, 2 * ks + hi));
+        const uint32_t off = row0 * kRowBytes + ks * kStride;
+        if constexpr (kSize == 2) {
+            f.v = *(lds_bf16x8*)(uintptr_t)(tile + l.row + off);
         } else {
-            const f32x4_t a = *(const f32x4_t*)(tile + at(row, 4 * ks + 2 * hi)), b = *(const f32x4_t*)(tile + at(row, 4 * ks + 2 * hi + 1));
+            const f32x4_t a = *(lds_f32x4*)(uintptr_t)(tile + l.row + off), b = *(lds_f32x4*)(uintptr_t)(tile + l.row2 + off);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 f.v[i] = a[i];
@@ -130,48 +152,47 @@ struct Tile {
         return f;
     }
 
-    // the tile transposed: column 32 t + lane % 32, rows row0 + {4 hi + 0..3, 8 + 4 hi + 0..3}
-    __device__ static __forceinline__ Frag<T> frag_t(const char* tile, int row0, int t, int lane) {
-        const int hi = lane >> 5;
+    // the tile transposed: column 32 t + lane % 32, rows row0 (a multiple of 16) + {4 hi + 0..3, 8 + 4 hi + 0..3}
+    __device__ static __forceinline__ Frag<T> frag_t(uint32_t tile, const Lane& l, int row0, int t) {
         Frag<T> f;
-        if constexpr (sizeof(T) == 2) {
+        const uint32_t off = row0 * kRowBytes + 2 * t * kStride;
+        if constexpr (kSize == 2) {
             typedef __attribute__((ext_vector_type(4))) short s16x4_t;
             typedef __attribute__((ext_vector_type(8))) short s16x8_t;
-            // a transposing read: lane l of 16 gives the address of 4 elements of row (l / 4) and gets column l of 4 rows
-            const int row = row0 + 4 * hi + ((lane >> 2) & 3), col = 32 * t + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-            const uint32_t a0 = at(row, col >> 3) + ((col & 7) << 1), a1 = at(row + 8, col >> 3) + ((col & 7) << 1);
             typedef __attribute__((address_space(3))) s16x4_t lds4;
-            const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(tile + a0));
-            const s16x4_t up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(tile + a1));
+            const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(uintptr_t)(tile + l.col + off));
+            const s16x4_t up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(uintptr_t)(tile + l.col2 + off));
             const s16x8_t v = {lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
             f.v = __builtin_bit_cast(bf16x8_t, v);
         } else {
-            const int col = 32 * t + (lane & 31);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int row = row0 + (e & 4) * 2 + 4 * hi + (e & 3);
-                f.v[e] = *(const float*)(tile + at(row, col >> 2) + ((col & 3) << 2));
+            for (int e = 0; e < 4; ++e) {
+                f.v[e] = *(lds_f32*)(uintptr_t)(tile + l.col + off + e * kRowBytes);
+                f.v[4 + e] = *(lds_f32*)(uintptr_t)(tile + l.col2 + off + e * kRowBytes);
             }
         }
         return f;
     }
 
-    // Stages `kRows` rows with direct-to-LDS loads, 64 chunks per wavefront and instruction: chunk p of row r of the tile comes from
-    // chunk p ^ swizzle(r) of row_of(r).  Chunks past D are left as they are (zeros: clear_lds).
-    template <int kRows, typename F>
+    // Stages the tile with direct-to-LDS loads of 1 KB, a panel's next 32 (fp32: 16) rows each; a wavefront takes neighbouring
+    // panels, so that the lines it touches are used whole.  Columns from D on are left as they are (zeros: clear_lds).
+    template <typename F>
     __device__ static __forceinline__ void load(char* tile, int D, F row_of) {
-        constexpr int kRowsPerWave = 64 / kChunks;
+        constexpr int kRows = 64 / kRowChunks, kMine = kPanels / kWaves;
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
-        for (int i = 0; i < kRows / kRowsPerPass; ++i) {
-            const int first = (i * kWaves + wave) * kRowsPerWave, row = first + lane / kChunks;
-            const uint32_t chunk = (uint32_t)(lane % kChunks) ^ swizzle(row);
-            if ((int)chunk * kPerChunk < D) load16_to_lds((const char*)row_of(row) + chunk * 16, tile + first * kRowBytes);
+        for (int r0 = 0; r0 < ROWS; r0 += kRows) {
+            const int row = r0 + lane / kRowChunks;
+            const uint32_t chunk = (uint32_t)(lane % kRowChunks) ^ swizzle(row);
+            const char* from = (const char*)row_of(row) + chunk * 16;
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+                const int panel = wave * kMine + i;
+                if (panel * 16 + (int)chunk * kPerChunk < D) load16_to_lds(from + panel * kRowBytes, tile + panel * kStride + r0 * kRowBytes);
+            }
         }
     }
-    __device__ static __forceinline__ float element(const char* tile, int row, int col) {
-        return to_f32(*(const T*)(tile + at(row, col / kPerChunk) + (col % kPerChunk) * (int)sizeof(T)));
-    }
+    __device__ static __forceinline__ float element(const char* tile, int row, int col) { return to_f32(*(const T*)(tile + at(row, col))); }
     // whether row `row` holds a value that is not finite
     __device__ static __forceinline__ bool row_not_finite(const char* tile, int row) {
         bool bad = false;
@@ -342,20 +363,6 @@ template <typename T>
 __device__ __forceinline__ float capped(float x, float mul) {  // tanh(x * scale / softcap)
     if (sizeof(T) == 2) return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * mul));
     return tanhf(x * mul);
-}
-
-// lets a kernel have `bytes` of dynamic LDS; asked once per device
-template <auto KERNEL>
-inline hipError_t allow_lds(int bytes) {
-    static std::atomic<uint64_t> allowed{0};
-    int device = 0;
-    const hipError_t e = hipGetDevice(&device);
-    if (e != hipSuccess) return e;
-    const uint64_t bit = device < 64 ? 1ull << device : 0;
-    if (allowed.load(std::memory_order_relaxed) & bit) return hipSuccess;
-    const hipError_t set = hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (set == hipSuccess) allowed.fetch_or(bit, std::memory_order_relaxed);
-    return set;
 }
 
 }  // namespace

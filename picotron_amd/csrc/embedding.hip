@@ -5,8 +5,8 @@
 //
 // Both are bound by memory: the forward reads and writes one row per token, the backward reads one row per token and writes
 // the whole table once.  The sums must not depend on the order in which blocks run, so nothing is added with atomics: the
-// tokens are sorted by id with a stable radix sort (digits of up to 9 bits, two launches per digit), every table row then
-// owns a run of the sorted order and is summed in token order, in fp32, and rounded once.  Frequent tokens would leave one
+// tokens are sorted by id with a stable radix sort (digits of up to 9 bits; up to kSmall tokens in the LDS of one block, more with
+// two launches per digit), every table row then owns a run of the sorted order and is summed in token order, in fp32, and rounded once.  Frequent tokens would leave one
 // block with thousands of rows: runs longer than kChunk are cut at the multiples of kChunk of the sorted order, the pieces
 // are summed by blocks of their own into fp32 partial rows and joined in order by a last launch.
 #include "common.h"
@@ -98,10 +98,11 @@ __global__ __launch_bounds__(kThreads) void embedding_fwd_kernel(const typename 
 
 // ---------------------------------------------------------------------------------------------------------------
 // Stable radix sort of (id, token) by id.  Ids outside the table and the padding id become the key `vocab`, which sorts
-// behind every row.  One block ranks kTile tokens; a wave owns kTile / 16 consecutive ones.
+// behind every row.  A block ranks 1024 * ROUNDS tokens, a wave 64 * ROUNDS consecutive ones of them.
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64, kSortRounds = 4, kTile = kSortThreads * kSortRounds;
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
 constexpr int kMaxDigitBits = 9, kMaxDigits = 1 << kMaxDigitBits;
+constexpr int kSmallRounds = 8, kSmall = kSortThreads * kSmallRounds;
 
 __device__ __forceinline__ uint32_t id_key(int64_t id, int64_t vocab, int64_t padding) {
     return id < 0 || id >= vocab || id == padding ? (uint32_t)vocab : (uint32_t)id;
@@ -129,38 +130,26 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-__global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortPass p) {
-    __shared__ int32_t count[kMaxDigits];
-    const int digits = 1 << p.bits;
-    for (int d = threadIdx.x; d < digits; d += kSortThreads) count[d] = 0;
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < kSortRounds; ++r) {
-        const int64_t i = (int64_t)blockIdx.x * kTile + r * kSortThreads + threadIdx.x;
-        if (i < p.n) atomicAdd(&count[(load_key(p, i) >> p.shift) & (digits - 1)], 1);
+// the rank of a lane's token among the wave's tokens of its digit: those counted in `seen` so far and those of lanes below
+__device__ __forceinline__ int32_t wave_rank(int32_t* seen, uint32_t digit, int bits, bool in, int lane) {
+    uint64_t same = __ballot(in);
+    if (!in) same = ~same;
+    for (int bit = 0; bit < bits; ++bit) {
+        const bool set = (digit >> bit) & 1u;
+        const uint64_t with = __ballot(set);
+        same &= set ? with : ~with;
     }
-    __syncthreads();
-    for (int d = threadIdx.x; d < digits; d += kSortThreads) p.hist[(int64_t)blockIdx.x * digits + d] = count[d];
+    const int below = __popcll(same & ((1ull << lane) - 1));
+    const int32_t had = in ? seen[digit] : 0;
+    wave_sync();  // every lane has read the count before the first of its peers moves it on, ...
+    if (in && below == 0) seen[digit] = had + __popcll(same);
+    wave_sync();  // ... and it has moved before the next round reads it
+    return had + below;
 }
 
-__global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortPass p) {
-    __shared__ int32_t base[kMaxDigits];                // where the block's first token of a digit goes
-    __shared__ int32_t seen[kSortWaves][kMaxDigits];    // tokens of a digit that a wave has ranked; then: those of the waves before
-    __shared__ int32_t wave_total[kSortWaves];
-    const int digits = 1 << p.bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int w = 0; w < kSortWaves; ++w)
-        for (int d = threadIdx.x; d < digits; d += kSortThreads) seen[w][d] = 0;
-
-    // tokens with a smaller digit, and those of the same digit in earlier blocks
-    int32_t all = 0, before = 0;
-    if ((int)threadIdx.x < digits) {
-        for (int b = 0; b < (int)gridDim.x; ++b) {
-            const int32_t c = p.hist[(int64_t)b * digits + threadIdx.x];
-            all += c;
-            before += b < (int)blockIdx.x ? c : 0;
-        }
-    }
-    int32_t scan = all;
+// exclusive sums of `v` over the first `digits` threads of the block
+__device__ __forceinline__ int32_t block_scan(int32_t v, int32_t* wave_total, int lane, int wave) {
+    int32_t scan = v;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
         const int32_t o = __shfl_up(scan, off, 64);
@@ -168,32 +157,105 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortPass p) 
     }
     if (lane == 63) wave_total[wave] = scan;
     __syncthreads();
-    int32_t smaller = scan - all;
-    for (int w = 0; w < wave; ++w) smaller += wave_total[w];
+    int32_t before = scan - v;
+    for (int w = 0; w < wave; ++w) before += wave_total[w];
+    return before;
+}
+
+// Up to kSmall tokens: every pass in one block, keys and tokens in LDS between the passes.
+__global__ __launch_bounds__(kSortThreads) void sort_small_kernel(SortPass p, int passes) {
+    extern __shared__ int32_t lds[];
+    uint32_t* keys = (uint32_t*)lds;                 // [kSmall]
+    int32_t* vals = lds + kSmall;                    // [kSmall]
+    int32_t* seen_all = lds + 2 * kSmall;            // [waves][digits]
+    int32_t* wave_total = seen_all + kSortWaves * kMaxDigits;
+    const int digits = 1 << p.bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rounds = (int)((p.n + kSortThreads - 1) / kSortThreads);
+    int32_t* seen = seen_all + wave * kMaxDigits;
+    uint32_t key[kSmallRounds];
+    int32_t val[kSmallRounds], rank[kSmallRounds];
+    for (int pass = 0; pass < passes; ++pass) {
+        for (int d = lane; d < digits; d += 64) seen[d] = 0;
+        wave_sync();
+#pragma unroll
+        for (int r = 0; r < kSmallRounds; ++r) {
+            if (r >= rounds) break;
+            const int i = wave * (64 * rounds) + r * 64 + lane;
+            const bool in = i < p.n;
+            key[r] = in ? (pass == 0 ? id_key(p.ids[i], p.vocab, p.padding) : keys[i]) : 0xFFFFFFFFu;
+            val[r] = in ? (pass == 0 ? i : vals[i]) : -1;
+            rank[r] = wave_rank(seen, (key[r] >> (pass * p.bits)) & (uint32_t)(digits - 1), p.bits, in, lane);
+        }
+        __syncthreads();
+        int32_t all = 0;  // thread d: the waves' counts of digit d become what comes before each wave's tokens
+        if ((int)threadIdx.x < digits) {
+            for (int w = 0; w < kSortWaves; ++w) {
+                const int32_t c = seen_all[w * kMaxDigits + threadIdx.x];
+                seen_all[w * kMaxDigits + threadIdx.x] = all;
+                all += c;
+            }
+        }
+        const int32_t base = block_scan(all, wave_total, lane, wave);
+        if ((int)threadIdx.x < digits)
+            for (int w = 0; w < kSortWaves; ++w) seen_all[w * kMaxDigits + threadIdx.x] += base;
+        __syncthreads();
+        const bool last = pass == passes - 1;
+#pragma unroll
+        for (int r = 0; r < kSmallRounds; ++r) {
+            if (r >= rounds || val[r] < 0) continue;
+            const int to = seen[(key[r] >> (pass * p.bits)) & (uint32_t)(digits - 1)] + rank[r];
+            (last ? p.keys_out : keys)[to] = key[r];
+            (last ? p.vals_out : vals)[to] = val[r];
+        }
+        __syncthreads();
+    }
+}
+
+template <int ROUNDS>
+__global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortPass p) {
+    __shared__ int32_t count[kMaxDigits];
+    const int digits = 1 << p.bits;
+    for (int d = threadIdx.x; d < digits; d += kSortThreads) count[d] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        const int64_t i = (int64_t)blockIdx.x * (kSortThreads * ROUNDS) + r * kSortThreads + threadIdx.x;
+        if (i < p.n) atomicAdd(&count[(load_key(p, i) >> p.shift) & (digits - 1)], 1);
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < digits; d += kSortThreads) p.hist[(int64_t)blockIdx.x * digits + d] = count[d];
+}
+
+template <int ROUNDS>
+__global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortPass p) {
+    __shared__ int32_t base[kMaxDigits];                // where the block's first token of a digit goes
+    __shared__ int32_t seen[kSortWaves][kMaxDigits];    // tokens of a digit that a wave has ranked; then: those of the waves before
+    __shared__ int32_t wave_total[kSortWaves];
+    const int digits = 1 << p.bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int d = lane; d < digits; d += 64) seen[wave][d] = 0;
+    wave_sync();
+
+    // tokens of the same digit in all blocks and in earlier ones
+    int32_t all = 0, before = 0;
+    if ((int)threadIdx.x < digits) {
+#pragma unroll 8
+        for (int b = 0; b < (int)gridDim.x; ++b) {
+            const int32_t c = p.hist[(int64_t)b * digits + threadIdx.x];
+            all += c;
+            before += b < (int)blockIdx.x ? c : 0;
+        }
+    }
+    const int32_t smaller = block_scan(all, wave_total, lane, wave);
     if ((int)threadIdx.x < digits) base[threadIdx.x] = smaller + before;
 
-    uint32_t key[kSortRounds];
-    int32_t val[kSortRounds], rank[kSortRounds];
+    uint32_t key[ROUNDS];
+    int32_t val[ROUNDS], rank[ROUNDS];
 #pragma unroll
-    for (int r = 0; r < kSortRounds; ++r) {
-        const int64_t i = (int64_t)blockIdx.x * kTile + wave * (64 * kSortRounds) + r * 64 + lane;
+    for (int r = 0; r < ROUNDS; ++r) {
+        const int64_t i = (int64_t)blockIdx.x * (kSortThreads * ROUNDS) + wave * (64 * ROUNDS) + r * 64 + lane;
         const bool in = i < p.n;
         key[r] = in ? load_key(p, i) : 0xFFFFFFFFu;
         val[r] = in ? (p.ids ? (int32_t)i : p.vals[i]) : -1;
-        const uint32_t digit = (key[r] >> p.shift) & (uint32_t)(digits - 1);
-        uint64_t same = __ballot(in);
-        if (!in) same = ~same;
-        for (int bit = 0; bit < p.bits; ++bit) {
-            const bool set = (digit >> bit) & 1u;
-            const uint64_t with = __ballot(set);
-            same &= set ? with : ~with;
-        }
-        const int below = __popcll(same & ((1ull << lane) - 1));
-        const int32_t had = in ? seen[wave][digit] : 0;
-        rank[r] = had + below;
-        wave_sync();  // every lane has read the count before the first of its peers moves it on, ...
-        if (in && below == 0) seen[wave][digit] = had + __popcll(same);
-        wave_sync();  // ... and it has moved before the next round reads it
+        rank[r] = wave_rank(seen[wave], (key[r] >> p.shift) & (uint32_t)(digits - 1), p.bits, in, lane);
     }
     __syncthreads();
     if ((int)threadIdx.x < digits) {
@@ -206,7 +268,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortPass p) 
     }
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < kSortRounds; ++r) {
+    for (int r = 0; r < ROUNDS; ++r) {
         if (val[r] < 0) continue;
         const uint32_t digit = (key[r] >> p.shift) & (uint32_t)(digits - 1);
         const int64_t to = (int64_t)base[digit] + seen[wave][digit] + rank[r];
@@ -219,7 +281,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortPass p) 
 // Sums over the runs of the sorted order
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int kChunk = 64;       // longest run that one group sums in one go, and the piece of a longer one
-constexpr int kRowsPerGroup = 8;  // table rows that a group of threads walks
+constexpr int kRowsPerGroup = 16;  // table rows that a group of threads walks
 
 struct SumArgs {
     const uint32_t* keys;  // sorted
@@ -230,25 +292,34 @@ struct SumArgs {
     float* partial;  // [chunks][2][row_chunks * kVec]: the sums of the runs that hold a chunk's first and last position
 };
 
-__device__ __forceinline__ int64_t first_at_least(const uint32_t* keys, int64_t n, uint32_t key) {
-    int64_t lo = 0, hi = n;
-    while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (keys[mid] < key) lo = mid + 1;
-        else hi = mid;
+// The first of the sorted keys from `lo` on that is at least `key`, looked up by a wavefront: 64 places are probed at a time, so that
+// a lookup among n keys waits for log64(n) loads in a row, not log2(n).
+__device__ __forceinline__ int64_t first_at_least(const uint32_t* __restrict__ keys, int64_t lo, int64_t n, uint32_t key) {
+    const int lane = threadIdx.x & 63;
+    int64_t hi = n;  // the answer is in [lo, hi]
+    while (hi > lo) {
+        const int64_t step = (hi - lo + 63) / 64, at = lo + lane * step;
+        const uint64_t less = __ballot(at < hi && keys[at < hi ? at : lo] < key);  // a prefix of the lanes
+        const int k = __popcll(less);
+        if (k == 0) return lo;
+        if (step == 1) return lo + k;
+        const int64_t from = lo + (int64_t)(k - 1) * step + 1;  // behind the last probe that is less, up to the next one
+        hi = lo + k * step < hi ? lo + k * step : hi;
+        lo = from;
     }
     return lo;
 }
 
-template <typename R>
-__device__ __forceinline__ void add_rows(const typename R::raw* __restrict__ d_out, const SumArgs& a, int64_t from, int64_t to, uint32_t col,
+// adds the rows of places [from, to) of the sorted order; token(i): the token at place i, the same in every lane
+template <typename R, typename F>
+__device__ __forceinline__ void add_rows(const typename R::raw* __restrict__ d_out, const SumArgs& a, int64_t from, int64_t to, uint32_t col, F token,
                                          float (&sum)[R::kVec]) {
-    constexpr int kAhead = 4;
+    constexpr int kAhead = 8;
     for (int64_t i = from; i < to; i += kAhead) {
         typename R::raw v[kAhead];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u)
-            if (i + u < to) v[u] = d_out[(int64_t)a.vals[i + u] * a.row_chunks + col];
+            if (i + u < to) v[u] = d_out[(int64_t)token(i + u) * a.row_chunks + col];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
             if (i + u >= to) continue;
@@ -260,42 +331,77 @@ __device__ __forceinline__ void add_rows(const typename R::raw* __restrict__ d_o
     }
 }
 
-// Groups of `group` threads (64 or 256) hold the columns of a row, blockIdx.y steps over wider rows.  The first row_blocks
-// blocks write the table rows whose run is at most kChunk long, the others sum the pieces of the longer ones.
+// kVec fp32 sums of a partial row
 template <typename R>
-__global__ __launch_bounds__(kThreads) void sum_runs_kernel(const typename R::raw* __restrict__ d_out, SumArgs a, int group, int64_t row_blocks,
+__device__ __forceinline__ void load_sums(const float* slot, float (&f)[R::kVec]) {
+    if constexpr (R::kVec >= 4) {
+#pragma unroll
+        for (int i = 0; i < R::kVec; i += 4) {
+            const f32x4_t v = *(const f32x4_t*)(slot + i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[i + j] = v[j];
+        }
+    } else {
+        f[0] = slot[0];
+    }
+}
+
+// Groups of `group` threads (64 or 256) hold the columns of a row, blockIdx.y steps over wider rows.  The first
+// chunk_blocks blocks sum the pieces of the runs longer than kChunk, which take the longest, the others write the table rows of the
+// shorter ones.
+template <typename R>
+__global__ __launch_bounds__(kThreads) void sum_runs_kernel(const typename R::raw* __restrict__ d_out, SumArgs a, int group, int64_t chunk_blocks,
                                                             typename R::raw* __restrict__ d_weight) {
     const int groups = kThreads / group, g = threadIdx.x / group;
     const uint32_t col = blockIdx.y * group + threadIdx.x % group;
     const int lane = threadIdx.x & 63;
-    if (blockIdx.x < row_blocks) {
-        const int64_t row0 = ((int64_t)blockIdx.x * groups + g) * kRowsPerGroup;
-        // lane i < kRowsPerGroup + 1 looks up where row0 + i begins
-        const int64_t mine = row0 + (lane < kRowsPerGroup ? lane : kRowsPerGroup);
-        const int64_t begins = first_at_least(a.keys, a.n, (uint32_t)(mine < a.vocab ? mine : a.vocab));
+    if (blockIdx.x >= chunk_blocks) {
+        const int64_t row0 = (((int64_t)blockIdx.x - chunk_blocks) * groups + g) * kRowsPerGroup;
+        if (row0 >= a.vocab) return;
+        // the sorted keys and their tokens from `window` on, one a lane
+        int64_t at = first_at_least(a.keys, 0, a.n, (uint32_t)row0), window = at;
+        uint32_t ahead = window + lane < a.n ? a.keys[window + lane] : 0xFFFFFFFFu;
+        int32_t tokens = window + lane < a.n ? a.vals[window + lane] : 0;
         for (int r = 0; r < kRowsPerGroup; ++r) {
-            const int64_t from = __shfl(begins, r, 64), to = __shfl(begins, r + 1, 64);
-            if (row0 + r >= a.vocab || to - from > kChunk || col >= a.row_chunks) continue;
+            const uint32_t row = (uint32_t)row0 + r;
+            if (row >= a.vocab) break;
+            const int64_t from = at;
+            const uint64_t behind = __ballot(ahead > row);
             float sum[R::kVec] = {};
-            add_rows<R>(d_out, a, from, to, col, sum);
+            if (behind) {
+                at = window + (__ffsll((unsigned long long)behind) - 1);
+                if (col < a.row_chunks)
+                    add_rows<R>(d_out, a, from, at, col,
+                                [&](int64_t i) { return __builtin_amdgcn_readlane(tokens, __builtin_amdgcn_readfirstlane((int)(i - window))); }, sum);
+            } else {
+                at = window = first_at_least(a.keys, window + 64, a.n, row + 1);
+                ahead = window + lane < a.n ? a.keys[window + lane] : 0xFFFFFFFFu;
+                tokens = window + lane < a.n ? a.vals[window + lane] : 0;
+                if (at - from > kChunk) continue;
+                if (col < a.row_chunks) add_rows<R>(d_out, a, from, at, col, [&](int64_t i) { return a.vals[i]; }, sum);
+            }
+            if (col >= a.row_chunks) continue;
 #pragma unroll
             for (int e = 0; e < R::kVec; ++e) sum[e] *= a.scale;
-            d_weight[(row0 + r) * (int64_t)a.row_chunks + col] = R::pack(sum);
+            d_weight[(int64_t)row * a.row_chunks + col] = R::pack(sum);
         }
         return;
     }
-    const int64_t chunk = ((int64_t)blockIdx.x - row_blocks) * groups + g, begin = chunk * kChunk;
+    const int64_t chunk = (int64_t)blockIdx.x * groups + g, begin = chunk * kChunk;
     if (begin >= a.n) return;
     const int64_t end = begin + kChunk < a.n ? begin + kChunk : a.n;
-    const uint32_t key0 = a.keys[begin], key1 = a.keys[end - 1];
+    const uint32_t mine = a.keys[begin + lane < end ? begin + lane : end - 1];  // kChunk is a wavefront's width
+    const int32_t tokens = a.vals[begin + lane < end ? begin + lane : end - 1];
+    const uint32_t key0 = __builtin_amdgcn_readfirstlane(mine), key1 = __builtin_amdgcn_readlane(mine, 63);
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
         const uint32_t key = side ? key1 : key0;
         if (key >= a.vocab || (side && key1 == key0)) continue;
-        const int64_t from = first_at_least(a.keys, a.n, key), to = first_at_least(a.keys, a.n, key + 1);
+        const int64_t from = first_at_least(a.keys, 0, a.n, key), to = first_at_least(a.keys, from, a.n, key + 1);
         if (to - from <= kChunk || col >= a.row_chunks) continue;
         float sum[R::kVec] = {};
-        add_rows<R>(d_out, a, from > begin ? from : begin, to < end ? to : end, col, sum);
+        add_rows<R>(d_out, a, from > begin ? from : begin, to < end ? to : end, col,
+                    [&](int64_t i) { return __builtin_amdgcn_readlane(tokens, __builtin_amdgcn_readfirstlane((int)(i - begin))); }, sum);
         float* slot = a.partial + ((chunk * 2 + side) * (int64_t)a.row_chunks + col) * R::kVec;
 #pragma unroll
         for (int e = 0; e < R::kVec; ++e) slot[e] = sum[e];
@@ -308,20 +414,29 @@ __global__ __launch_bounds__(kThreads) void join_runs_kernel(SumArgs a, int grou
     const int groups = kThreads / group, g = threadIdx.x / group;
     const uint32_t col = blockIdx.y * group + threadIdx.x % group;
     const int64_t chunk = (int64_t)blockIdx.x * groups + g, begin = chunk * kChunk;
-    if (begin >= a.n || col >= a.row_chunks) return;
+    if (begin >= a.n) return;
     const int64_t end = begin + kChunk < a.n ? begin + kChunk : a.n;
     // a run that begins here and is longer than a chunk holds the chunk's last position
     const uint32_t key = a.keys[end - 1];
     if (key >= a.vocab || (begin > 0 && a.keys[begin - 1] == key)) return;
-    const int64_t from = first_at_least(a.keys, a.n, key), to = first_at_least(a.keys, a.n, key + 1);
+    const int64_t from = first_at_least(a.keys, begin, a.n, key), to = first_at_least(a.keys, from, a.n, key + 1);
     if (to - from <= kChunk) return;
+    if (col >= a.row_chunks) return;
     float sum[R::kVec] = {};
     const int64_t last = (to - 1) / kChunk;
-    for (int64_t c = chunk; c <= last; ++c) {
-        const int side = c == chunk && from > begin;
-        const float* slot = a.partial + ((c * 2 + side) * (int64_t)a.row_chunks + col) * R::kVec;
+    constexpr int kAhead = 8;
+    for (int64_t c0 = chunk; c0 <= last; c0 += kAhead) {
+        float v[kAhead][R::kVec];
 #pragma unroll
-        for (int e = 0; e < R::kVec; ++e) sum[e] += slot[e];
+        for (int u = 0; u < kAhead; ++u) {
+            const int64_t c = c0 + u < last ? c0 + u : last;
+            const int side = c == chunk && from > begin;
+            load_sums<R>(a.partial + ((c * 2 + side) * (int64_t)a.row_chunks + col) * R::kVec, v[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+            for (int e = 0; e < R::kVec; ++e) sum[e] += c0 + u <= last ? v[u][e] : 0.f;
     }
 #pragma unroll
     for (int e = 0; e < R::kVec; ++e) sum[e] *= a.scale;
@@ -336,11 +451,15 @@ int key_bits(int64_t vocab) {
 }
 
 bool sizes_fit(int dtype, int64_t n_tokens, int64_t vocab, int64_t hidden) {
-    return (dtype == PICOMOE_F32 || dtype == PICOMOE_BF16) && n_tokens >= 0 && n_tokens < (1ll << 31) - kTile && vocab >= 1 && vocab < (1ll << 31) &&
+    return (dtype == PICOMOE_F32 || dtype == PICOMOE_BF16) && n_tokens >= 0 && n_tokens < (1ll << 31) - (1 << 16) && vocab >= 1 && vocab < (1ll << 31) &&
            hidden >= 1 && hidden <= (1 << 20);
 }
 
 int64_t round16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
+
+// Every block of a scatter reads all blocks' counts, so blocks are few: 64 up to a million tokens; below that, rounds are few
+int sort_rounds(int64_t n) { return n <= 64 * kSortThreads ? 1 : (n <= 256 * kSortThreads ? 4 : 16); }
+int64_t sort_blocks(int64_t n) { return (n + sort_rounds(n) * kSortThreads - 1) / (sort_rounds(n) * kSortThreads); }
 
 struct BwdLayout {
     int64_t keys[2], vals[2], hist, partial, bytes;
@@ -355,7 +474,7 @@ BwdLayout bwd_layout(int64_t n, int64_t hidden) {
         at += round16(n * 4);
     }
     l.hist = at;
-    at += (n + kTile - 1) / kTile * kMaxDigits * 4;
+    at += n > kSmall ? sort_blocks(n) * kMaxDigits * 4 : 0;
     l.partial = at;
     at += (n + kChunk - 1) / kChunk * 2 * hidden * 4;
     l.bytes = round16(at);
@@ -385,7 +504,7 @@ int launch_sum(const void* d_out, SumArgs a, int64_t hidden, void* d_weight, hip
     const int64_t chunks = (a.n + kChunk - 1) / kChunk, chunk_blocks = (chunks + groups - 1) / groups;
     if (row_blocks + chunk_blocks > 0x7FFFFFFF) return PICOMOE_ERR_TOO_LARGE;
     sum_runs_kernel<R><<<dim3((unsigned)(row_blocks + chunk_blocks), slabs), kThreads, 0, stream>>>((const typename R::raw*)d_out, a, group,
-                                                                                                  row_blocks, (typename R::raw*)d_weight);
+                                                                                                  chunk_blocks, (typename R::raw*)d_weight);
     if (a.n > kChunk) join_runs_kernel<R><<<dim3((unsigned)chunk_blocks, slabs), kThreads, 0, stream>>>(a, group, (typename R::raw*)d_weight);
     return picomoe_launch_status();
 }
@@ -419,7 +538,6 @@ extern "C" int picomoe_embedding_bwd(const void* d_out, int dtype, const int64_t
     hipStream_t s = (hipStream_t)stream;
     char* ws = (char*)workspace;
     const int bits = key_bits(vocab), passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits, digit_bits = (bits + passes - 1) / passes;
-    const unsigned blocks = (unsigned)((n_tokens + kTile - 1) / kTile);
     SumArgs a = {};
     for (int pass = 0; pass < passes && n_tokens > 0; ++pass) {
         SortPass p;
@@ -431,10 +549,27 @@ extern "C" int picomoe_embedding_bwd(const void* d_out, int dtype, const int64_t
         p.hist = (int32_t*)(ws + l.hist);
         p.n = n_tokens; p.vocab = vocab; p.padding = padding_idx;
         p.shift = pass * digit_bits; p.bits = digit_bits;
-        sort_count_kernel<<<blocks, kSortThreads, 0, s>>>(p);
-        sort_scatter_kernel<<<blocks, kSortThreads, 0, s>>>(p);
         a.keys = p.keys_out;
         a.vals = p.vals_out;
+        if (n_tokens <= kSmall) {
+            constexpr int kLds = (2 * kSmall + kSortWaves * kMaxDigits + kSortWaves) * 4;
+            const hipError_t e = allow_lds<sort_small_kernel>(kLds);
+            if (e != hipSuccess) return PICOMOE_ERR_HIP_BASE + (int)e;
+            sort_small_kernel<<<1, kSortThreads, kLds, s>>>(p, passes);
+            break;
+        }
+        const unsigned blocks = (unsigned)sort_blocks(n_tokens);
+        const int rounds = sort_rounds(n_tokens);
+        if (rounds == 1) {
+            sort_count_kernel<1><<<blocks, kSortThreads, 0, s>>>(p);
+            sort_scatter_kernel<1><<<blocks, kSortThreads, 0, s>>>(p);
+        } else if (rounds == 4) {
+            sort_count_kernel<4><<<blocks, kSortThreads, 0, s>>>(p);
+            sort_scatter_kernel<4><<<blocks, kSortThreads, 0, s>>>(p);
+        } else {
+            sort_count_kernel<16><<<blocks, kSortThreads, 0, s>>>(p);
+            sort_scatter_kernel<16><<<blocks, kSortThreads, 0, s>>>(p);
+        }
     }
     a.n = n_tokens; a.vocab = vocab; a.scale = scale;
     a.partial = n_tokens > 0 ? (float*)(ws + l.partial) : nullptr;

@@ -12,8 +12,9 @@
 // Everything is computed in fp32 and rounded once, at the store.  Both passes are bound by memory: forward one read and one
 // write of the heads, backward two reads (x and g; r is recomputed, nothing is saved) and one write.  A lane holds kVec values
 // of the first half and the kVec values they are rotated with, so the rotation needs no exchange and the sum of squares one
-// butterfly over the lanes of a head.  Queries and keys go through one launch.  dw is summed in registers over the rows a
-// group of lanes walks, joined per block in LDS and over the blocks by a second launch, in a fixed order.
+// butterfly over the lanes of a head.  A group of lanes takes some heads of one token, whose table rows it reads once -- in fp32
+// they are twice a bf16 head --, and has the loads of all of them in flight.  Queries and keys go through one launch.  dw is summed
+// in registers over the rows a group walks, joined per block in LDS and over the blocks by a second launch, in a fixed order.
 #include "common.h"
 
 namespace {
@@ -77,13 +78,19 @@ struct Args {
     float* partial;  // backward: [blocks][2][D] sums of dw
 };
 
-// Rows are (token, head of q then k), numbered token by token; a group of `lanes` lanes works on one row at a time.
+// field by field: a reference to one of the two would put the arguments into scratch memory
+__device__ __forceinline__ Heads pick(const Args& a, bool k) {
+    return {k ? a.k.x : a.q.x, k ? a.k.grad : a.q.grad, k ? a.k.weight : a.q.weight, k ? a.k.out : a.q.out, k ? a.k.sb : a.q.sb,
+            k ? a.k.ss : a.q.ss, k ? a.k.sh : a.q.sh, k ? a.k.heads : a.q.heads};
+}
+
+// A group of `lanes` lanes holds a head.
 template <typename T, int VEC>
 struct Lane {
     typedef Vec<T, VEC> V;
     typedef typename V::raw raw;
     int half, col;   // this lane's first column, below half
-    bool in;         // lanes past half / VEC of a group hold zeros
+    bool in;         // lanes past half / VEC of a group read the first lane's and hold zeros
 
     __device__ Lane(int D, int lanes) {
         half = D / 2;
@@ -92,12 +99,12 @@ struct Lane {
         col = in ? l * VEC : 0;
     }
     __device__ void load(const T* p, float (&a)[VEC], float (&b)[VEC]) const {
-        if (in) {
-            V::get(*(const raw*)(p + col), a);
-            V::get(*(const raw*)(p + half + col), b);
-        } else {
+        V::get(*(const raw*)(p + col), a);
+        V::get(*(const raw*)(p + half + col), b);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) a[i] = b[i] = 0.f;
+        for (int i = 0; i < VEC; ++i) {
+            a[i] = in ? a[i] : 0.f;
+            b[i] = in ? b[i] : 0.f;
         }
     }
     __device__ void store(T* p, const float (&a)[VEC], const float (&b)[VEC]) const {
@@ -129,12 +136,17 @@ template <typename T, int VEC>
 __device__ __forceinline__ void table_rows(const Args& a, const Lane<T, VEC>& ln, int64_t token, float (&c0)[VEC], float (&c1)[VEC],
                                            float (&s0)[VEC], float (&s1)[VEC]) {
     const int64_t pos = a.positions ? a.positions[token] : token % a.seq;
-    if (pos >= 0 && pos < a.n_positions) {
-        ln.load_f32(a.cos + pos * a.D, c0, c1);
-        ln.load_f32(a.sin + pos * a.D, s0, s1);
-    } else {
+    const bool good = pos >= 0 && pos < a.n_positions;
+    const int64_t at = good ? pos * a.D : 0;
+    ln.load_f32(a.cos + at, c0, c1);
+    ln.load_f32(a.sin + at, s0, s1);
+    const float nan = __builtin_nanf("");
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) c0[i] = c1[i] = s0[i] = s1[i] = __builtin_nanf("");
+    for (int i = 0; i < VEC; ++i) {
+        c0[i] = good ? c0[i] : nan;
+        c1[i] = good ? c1[i] : nan;
+        s0[i] = good ? s0[i] : nan;
+        s1[i] = good ? s1[i] : nan;
     }
 }
 
@@ -146,85 +158,106 @@ __device__ __forceinline__ float row_rms(const float (&a)[VEC], const float (&b)
     return 1.0f / sqrtf(group_sum(sq, lanes) / (float)D + eps);
 }
 
+// Heads that a group has in flight.  The backward, which loads two rows a head, takes 59 us with one at 8192 tokens x (32 + 8) heads of
+// 128, 78 with two and 80 with four: the registers cost it more waves than the loads in flight bring.
+constexpr int kFwdHeads = 4, kBwdHeads = 1;
+
+// Work is numbered token by token, and in a token by sets of kFwdHeads query heads, then of key heads.
 template <typename T, int VEC>
 __global__ __launch_bounds__(kThreads) void qk_norm_rope_fwd_kernel(Args a, int lanes) {
     const Lane<T, VEC> ln(a.D, lanes);
-    const int heads = a.q.heads + a.k.heads, groups = kThreads / lanes;
-    const int64_t row = (int64_t)blockIdx.x * groups + threadIdx.x / lanes, token = row / heads;
+    const int q_sets = (a.q.heads + kFwdHeads - 1) / kFwdHeads, sets = q_sets + (a.k.heads + kFwdHeads - 1) / kFwdHeads;
+    const int64_t set = (int64_t)blockIdx.x * (kThreads / lanes) + threadIdx.x / lanes, token = set / sets;
     if (token >= a.tokens) return;
-    const int vh = (int)(row - token * heads);
-    const bool is_k = vh >= a.q.heads;
-    const Heads& t = is_k ? a.k : a.q;
-    const int h = is_k ? vh - a.q.heads : vh;
+    const int in_token = (int)(set - token * sets);
+    const bool is_k = in_token >= q_sets;
+    const Heads t = pick(a, is_k);
+    const int h0 = (is_k ? in_token - q_sets : in_token) * kFwdHeads, n = min(kFwdHeads, t.heads - h0);
     const int64_t b = token / a.seq, s = token - b * a.seq;
-    float x0[VEC], x1[VEC], c0[VEC], c1[VEC], s0[VEC], s1[VEC];
-    ln.load((const T*)t.x + b * t.sb + s * t.ss + h * t.sh, x0, x1);
+    const T* x = (const T*)t.x + b * t.sb + s * t.ss + h0 * t.sh;
+    float x0[kFwdHeads][VEC], x1[kFwdHeads][VEC], c0[VEC], c1[VEC], s0[VEC], s1[VEC], w0[VEC], w1[VEC];
+#pragma unroll
+    for (int h = 0; h < kFwdHeads; ++h)
+        if (h < n) ln.load(x + h * t.sh, x0[h], x1[h]);
     table_rows<T, VEC>(a, ln, token, c0, c1, s0, s1);
-    if (t.weight) {
-        float w0[VEC], w1[VEC];
-        ln.load((const T*)t.weight, w0, w1);
-        const float r = row_rms<T, VEC>(x0, x1, lanes, a.D, a.eps);
+    if (t.weight) ln.load((const T*)t.weight, w0, w1);
+#pragma unroll
+    for (int h = 0; h < kFwdHeads; ++h) {
+        if (h >= n) break;
+        if (t.weight) {
+            const float r = row_rms<T, VEC>(x0[h], x1[h], lanes, a.D, a.eps);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                x0[h][i] = x0[h][i] * r * w0[i];
+                x1[h][i] = x1[h][i] * r * w1[i];
+            }
+        }
+        float o0[VEC], o1[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            x0[i] = x0[i] * r * w0[i];
-            x1[i] = x1[i] * r * w1[i];
+            o0[i] = x0[h][i] * c0[i] - x1[h][i] * s0[i];
+            o1[i] = x1[h][i] * c1[i] + x0[h][i] * s1[i];
         }
+        ln.store((T*)t.out + (token * t.heads + h0 + h) * a.D, o0, o1);
     }
-    float o0[VEC], o1[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-        o0[i] = x0[i] * c0[i] - x1[i] * s0[i];
-        o1[i] = x1[i] * c1[i] + x0[i] * s1[i];
-    }
-    ln.store((T*)t.out + (token * t.heads + h) * a.D, o0, o1);
 }
 
-// A group walks rows of one tensor only -- the first q_blocks blocks the queries, the others the keys -- and keeps its columns of dw.
+// A group walks sets of one tensor only -- the first q_blocks blocks the queries, the others the keys -- and keeps its columns of dw.
 template <typename T, int VEC>
 __global__ __launch_bounds__(kThreads) void qk_norm_rope_bwd_kernel(Args a, int lanes, int q_blocks) {
     const Lane<T, VEC> ln(a.D, lanes);
     const bool is_k = (int)blockIdx.x >= q_blocks;
-    const Heads& t = is_k ? a.k : a.q;
-    const int groups = kThreads / lanes, group = threadIdx.x / lanes;
+    const Heads t = pick(a, is_k);
+    const int groups = kThreads / lanes, group = threadIdx.x / lanes, sets = (t.heads + kBwdHeads - 1) / kBwdHeads;
     const int64_t block = is_k ? blockIdx.x - q_blocks : blockIdx.x, blocks = is_k ? gridDim.x - q_blocks : q_blocks;
-    const int64_t rows = a.tokens * t.heads;
     float w0[VEC], w1[VEC], dw0[VEC], dw1[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) dw0[i] = dw1[i] = 0.f;
     if (t.weight) ln.load((const T*)t.weight, w0, w1);
-    for (int64_t row = block * groups + group; row < rows; row += blocks * groups) {
-        const int64_t token = row / t.heads, b = token / a.seq, s = token - b * a.seq;
-        const int h = (int)(row - token * t.heads);
-        float x0[VEC], x1[VEC], g0[VEC], g1[VEC], c0[VEC], c1[VEC], s0[VEC], s1[VEC], y0[VEC], y1[VEC];
-        ln.load((const T*)t.grad + row * a.D, g0, g1);
-        if (t.weight) ln.load((const T*)t.x + b * t.sb + s * t.ss + h * t.sh, x0, x1);
+    for (int64_t set = block * groups + group; set < a.tokens * sets; set += blocks * groups) {
+        const int64_t token = set / sets, b = token / a.seq, s = token - b * a.seq;
+        const int h0 = (int)(set - token * sets) * kBwdHeads, n = min(kBwdHeads, t.heads - h0);
+        const int64_t row = token * t.heads + h0;
+        const T* x = (const T*)t.x + b * t.sb + s * t.ss + h0 * t.sh;
+        float x0[kBwdHeads][VEC], x1[kBwdHeads][VEC], g0[kBwdHeads][VEC], g1[kBwdHeads][VEC], c0[VEC], c1[VEC], s0[VEC], s1[VEC];
+#pragma unroll
+        for (int h = 0; h < kBwdHeads; ++h) {
+            if (h >= n) break;
+            ln.load((const T*)t.grad + (row + h) * a.D, g0[h], g1[h]);
+            if (t.weight) ln.load(x + h * t.sh, x0[h], x1[h]);
+        }
         table_rows<T, VEC>(a, ln, token, c0, c1, s0, s1);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            y0[i] = g0[i] * c0[i] + g1[i] * s1[i];
-            y1[i] = g1[i] * c1[i] - g0[i] * s0[i];
-        }
-        if (t.weight) {
-            const float r = row_rms<T, VEC>(x0, x1, lanes, a.D, a.eps);
-            float dot = 0.f;
+        for (int h = 0; h < kBwdHeads; ++h) {
+            if (h >= n) break;
+            float y0[VEC], y1[VEC];
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                x0[i] *= r;
-                x1[i] *= r;
-                dw0[i] += y0[i] * x0[i];
-                dw1[i] += y1[i] * x1[i];
-                y0[i] *= w0[i];
-                y1[i] *= w1[i];
-                dot += y0[i] * x0[i] + y1[i] * x1[i];
+                y0[i] = g0[h][i] * c0[i] + g1[h][i] * s1[i];
+                y1[i] = g1[h][i] * c1[i] - g0[h][i] * s0[i];
             }
-            dot = group_sum(ln.in ? dot : 0.f, lanes) / (float)a.D;
+            if (t.weight) {
+                const float r = row_rms<T, VEC>(x0[h], x1[h], lanes, a.D, a.eps);
+                float dot = 0.f;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                y0[i] = r * (y0[i] - x0[i] * dot);
-                y1[i] = r * (y1[i] - x1[i] * dot);
+                for (int i = 0; i < VEC; ++i) {
+                    x0[h][i] *= r;
+                    x1[h][i] *= r;
+                    dw0[i] += y0[i] * x0[h][i];
+                    dw1[i] += y1[i] * x1[h][i];
+                    y0[i] *= w0[i];
+                    y1[i] *= w1[i];
+                    dot += y0[i] * x0[h][i] + y1[i] * x1[h][i];
+                }
+                dot = group_sum(ln.in ? dot : 0.f, lanes) / (float)a.D;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    y0[i] = r * (y0[i] - x0[h][i] * dot);
+                    y1[i] = r * (y1[i] - x1[h][i] * dot);
+                }
             }
+            ln.store((T*)t.out + (row + h) * a.D, y0, y1);
         }
-        ln.store((T*)t.out + row * a.D, y0, y1);
     }
     if (!a.partial || !t.weight) return;
     extern __shared__ float sums[];  // [groups][D]
@@ -243,29 +276,29 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_bwd_kernel(Args a, int 
     }
 }
 
-// dw of the queries (block 0) and of the keys (block 1): the blocks' sums in order, by kThreads / 64 waves of consecutive blocks
+// dw: blockIdx.y 0 for the queries, 1 for the keys, 16 columns a block; 64 threads per column sum consecutive blocks' parts
+constexpr int kGradColumns = 16;
 template <typename T>
 __global__ __launch_bounds__(1024) void qk_weight_grad_kernel(const float* __restrict__ partial, int D, int q_blocks, int k_blocks, T* dq_weight,
                                                               T* dk_weight) {
-    __shared__ float part[16][256];
-    T* out = blockIdx.x ? dk_weight : dq_weight;
+    __shared__ float part[64][kGradColumns + 1];
+    T* out = blockIdx.y ? dk_weight : dq_weight;
     if (!out) return;
-    const int first = blockIdx.x ? q_blocks : 0, count = blockIdx.x ? k_blocks : q_blocks;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, per = (count + 15) / 16;
-    const int from = wave * per, to = from + per < count ? from + per : count;
-    for (int c = lane; c < D; c += 64) {
-        float sum = 0.f;
+    const int first = blockIdx.y ? q_blocks : 0, count = blockIdx.y ? k_blocks : q_blocks;
+    const int c = threadIdx.x % kGradColumns, col = blockIdx.x * kGradColumns + c, slice = threadIdx.x / kGradColumns, per = (count + 63) / 64;
+    const int from = slice * per, to = min(from + per, count);
+    float sum = 0.f;
+    if (col < D) {
 #pragma unroll 8
-        for (int b = from; b < to; ++b) sum += partial[(int64_t)(first + b) * D + c];
-        part[wave][c] = sum;
+        for (int b = from; b < to; ++b) sum += partial[(int64_t)(first + b) * D + col];
     }
+    part[slice][c] = sum;
     __syncthreads();
-    for (int c = threadIdx.x; c < D; c += 1024) {
-        float sum = 0.f;
+    if (slice != 0 || col >= D) return;
+    sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < 16; ++w) sum += part[w][c];
-        out[c] = (T)sum;
-    }
+    for (int i = 0; i < 64; ++i) sum += part[i][c];
+    out[col] = (T)sum;
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -300,11 +333,12 @@ bool heads_ok(const Heads& t, int dtype, bool backward) {
 struct Blocks {
     int q, k;
 };
+int64_t head_sets(int heads, int per) { return (heads + per - 1) / per; }
 Blocks bwd_blocks(int64_t tokens, int q_heads, int k_heads, int lanes) {
-    const int groups = kThreads / lanes;
-    const int64_t q_need = (tokens * q_heads + groups - 1) / groups, k_need = (tokens * k_heads + groups - 1) / groups;
+    const int64_t groups = kThreads / lanes, q_sets = head_sets(q_heads, kBwdHeads), k_sets = head_sets(k_heads, kBwdHeads);
+    const int64_t q_need = (tokens * q_sets + groups - 1) / groups, k_need = (tokens * k_sets + groups - 1) / groups;
     if (q_need + k_need <= kMaxBlocks) return {(int)q_need, (int)k_need};
-    int q = (int)((int64_t)kMaxBlocks * q_heads / (q_heads + k_heads));
+    int q = (int)(kMaxBlocks * q_sets / (q_sets + k_sets));
     q = q < 1 ? 1 : (q > kMaxBlocks - 1 ? kMaxBlocks - 1 : q);
     return {q, kMaxBlocks - q};
 }
@@ -312,7 +346,7 @@ Blocks bwd_blocks(int64_t tokens, int q_heads, int k_heads, int lanes) {
 template <typename T, int VEC>
 int launch_fwd(const Args& a, hipStream_t s) {
     const int lanes = lanes_for(a.D, VEC), groups = kThreads / lanes;
-    const int64_t blocks = (a.tokens * (a.q.heads + a.k.heads) + groups - 1) / groups;
+    const int64_t blocks = (a.tokens * (head_sets(a.q.heads, kFwdHeads) + head_sets(a.k.heads, kFwdHeads)) + groups - 1) / groups;
     if (blocks > 0x7FFFFFFF) return PICOMOE_ERR_TOO_LARGE;
     qk_norm_rope_fwd_kernel<T, VEC><<<(unsigned)blocks, kThreads, 0, s>>>(a, lanes);
     return picomoe_launch_status();
@@ -324,7 +358,7 @@ int launch_bwd(const Args& a, void* dq_weight, void* dk_weight, hipStream_t s) {
     const Blocks n = bwd_blocks(a.tokens, a.q.heads, a.k.heads, lanes);
     if (n.q + n.k > 0)
         qk_norm_rope_bwd_kernel<T, VEC><<<(unsigned)(n.q + n.k), kThreads, kThreads / lanes * a.D * sizeof(float), s>>>(a, lanes, n.q);
-    if (dq_weight || dk_weight) qk_weight_grad_kernel<T><<<2, 1024, 0, s>>>(a.partial, a.D, n.q, n.k, (T*)dq_weight, (T*)dk_weight);
+    if (dq_weight || dk_weight) qk_weight_grad_kernel<T><<<dim3((unsigned)((a.D + kGradColumns - 1) / kGradColumns), 2), 1024, 0, s>>>(a.partial, a.D, n.q, n.k, (T*)dq_weight, (T*)dk_weight);
     return picomoe_launch_status();
 }
 
@@ -339,7 +373,7 @@ extern "C" int picomoe_qk_norm_rope_fwd(const void* q, const int64_t* q_strides,
     Args a = {};
     a.q = {q, nullptr, q_weight, q_out, q_strides[0], q_strides[1], q_strides[2], q_heads};
     a.k = {k, nullptr, k_weight, k_out, k_strides[0], k_strides[1], k_strides[2], k_heads};
-    PICOMOE_CHECK_ARG(heads_ok(a.q, dtype, false) && heads_ok(a.k, dtype, false) && cos && sin && aligned(cos, 16) && aligned(sin, 16));
+    PICOMOE_CHECK_ARG(heads_ok(a.q, dtype, false) && heads_ok(a.k, dtype, false) && cos && sin && n_positions > 0 && aligned(cos, 16) && aligned(sin, 16));
     a.cos = cos; a.sin = sin; a.positions = positions; a.n_positions = n_positions;
     a.tokens = batch * seq; a.seq = seq; a.eps = eps; a.D = head_dim;
     if (dtype == PICOMOE_F32) return launch_fwd<float, 4>(a, (hipStream_t)stream);
@@ -363,7 +397,7 @@ extern "C" int picomoe_qk_norm_rope_bwd(const void* dq_out, const void* dk_out, 
     a.q = {q, dq_out, q_weight, dq, q_strides[0], q_strides[1], q_strides[2], q_heads};
     a.k = {k, dk_out, k_weight, dk, k_strides[0], k_strides[1], k_strides[2], k_heads};
     const bool empty = batch == 0 || seq == 0;
-    PICOMOE_CHECK_ARG(empty || (heads_ok(a.q, dtype, true) && heads_ok(a.k, dtype, true) && cos && sin && aligned(cos, 16) && aligned(sin, 16)));
+    PICOMOE_CHECK_ARG(empty || (heads_ok(a.q, dtype, true) && heads_ok(a.k, dtype, true) && cos && sin && n_positions > 0 && aligned(cos, 16) && aligned(sin, 16)));
     if (dq_weight || dk_weight) {
         PICOMOE_CHECK_ARG(empty || (workspace && aligned(workspace, 16) &&
                                     workspace_bytes >= picomoe_qk_norm_rope_bwd_workspace_bytes(dtype, batch, seq, q_heads, k_heads, head_dim)));

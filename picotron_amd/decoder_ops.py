@@ -12,10 +12,13 @@ HIP graph.  Arguments that the kernels do not take raise ``PicomoeError``; value
 host: token ids and positions outside their tables give NaN rows.
 """
 
+import contextlib
 import ctypes
+import functools
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from picotron_amd import _lib
 
@@ -25,17 +28,39 @@ def _fail(message):
 
 
 def _same_device(what, first, *others):
-    _lib.require_cuda(first, *others)
+    if not first.is_cuda:
+        _lib.require_cuda(first)
     for t in others:
         if t is not None and t.device != first.device:
+            _lib.require_cuda(t)
             _fail(f"{what}: tensors on {first.device} and {t.device}")
 
 
-def _rows16(t, *sizes):
+def _on(t):
+    """Context in which t's device is the current one (the calls below are short: entering one costs as much as a launch)."""
+    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _rows16(t):
     """t, or a copy of it, with a dense last dimension and rows that start on 16-byte boundaries."""
-    step = 16 // t.element_size()
-    fits = t.data_ptr() % 16 == 0 and t.stride(-1) == 1 and all(n == 1 or s % step == 0 for n, s in zip(t.shape[:-1], t.stride()[:-1]))
-    return t if fits else t.clone(memory_format=torch.contiguous_format)
+    if t.data_ptr() % 16 == 0 and (t.is_contiguous() or _strided16(t.shape, t.stride(), 16 // t.element_size())):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _strided16(shape, stride, step):
+    return stride[-1] == 1 and all(n == 1 or s % step == 0 for n, s in zip(shape[:-1], stride[:-1]))
 
 
 def _dense16(t):
@@ -45,17 +70,20 @@ def _dense16(t):
 
 def _strides(t):
     """{batch, length, head} strides for the C ABI; a dimension of one element has none."""
-    return (ctypes.c_int64 * 3)(*(0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3])))
+    return _stride_array(tuple(t.shape[:3]), t.stride()[:3])
+
+
+@functools.lru_cache(maxsize=256)
+def _stride_array(shape, stride):
+    return (ctypes.c_int64 * 3)(*(0 if n == 1 else s for n, s in zip(shape, stride)))
 
 
 def _integer(what, t):
-    if t.dtype not in (torch.int32, torch.int64):
+    if t.dtype == torch.int64:
+        return t.contiguous()
+    if t.dtype != torch.int32:
         _fail(f"{what} must be int32 or int64, got {t.dtype}")
     return t.to(torch.int64).contiguous()
-
-
-def _empty(shape, like, dtype=None):
-    return torch.empty(shape, dtype=dtype or like.dtype, device=like.device)
 
 
 def _workspace(n_bytes, like, what):
@@ -73,11 +101,11 @@ class _Embedding(torch.autograd.Function):
         lib = _lib.load()
         dt = _lib.dtype_code(weight.dtype)
         vocab, hidden = weight.shape
-        with torch.cuda.device(weight.device):
+        with _on(weight):
             table = weight.contiguous()
-            out = _empty((ids.numel(), hidden), weight)
+            out = table.new_empty((ids.numel(), hidden))
             _lib.check(
-                lib.picomoe_embedding_fwd(_lib.ptr(table), dt, vocab, hidden, _lib.ptr(ids), ids.numel(), scale, _lib.ptr(out), _lib.stream_ptr()),
+                lib.picomoe_embedding_fwd(_ptr(table), dt, vocab, hidden, _ptr(ids), ids.numel(), scale, _ptr(out), _stream()),
                 "picomoe_embedding_fwd",
             )
         ctx.save_for_backward(ids)
@@ -85,19 +113,19 @@ class _Embedding(torch.autograd.Function):
         return out.view(*ids.shape, hidden)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_differentiable
     def backward(ctx, d_out):
         (ids,) = ctx.saved_tensors
         vocab, hidden, scale, padding_idx = ctx.meta
         lib = _lib.load()
         dt = _lib.dtype_code(d_out.dtype)
-        with torch.cuda.device(d_out.device):
+        with _on(d_out):
             d_out = d_out.contiguous()
-            d_weight = _empty((vocab, hidden), d_out)
+            d_weight = d_out.new_empty((vocab, hidden))
             ws = _workspace(lib.picomoe_embedding_bwd_workspace_bytes(dt, ids.numel(), vocab, hidden), d_out, "embedding")
             _lib.check(
-                lib.picomoe_embedding_bwd(_lib.ptr(d_out), dt, _lib.ptr(ids), ids.numel(), vocab, hidden, scale, padding_idx, _lib.ptr(d_weight),
-                                          _lib.ptr(ws), ws.numel(), _lib.stream_ptr()),
+                lib.picomoe_embedding_bwd(_ptr(d_out), dt, _ptr(ids), ids.numel(), vocab, hidden, scale, padding_idx, _ptr(d_weight),
+                                          _ptr(ws), ws.numel(), _stream()),
                 "picomoe_embedding_bwd",
             )
         return d_weight, None, None, None
@@ -127,14 +155,14 @@ class _QkNormRope(torch.autograd.Function):
     def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps):
         lib = _lib.load()
         B, S, _, D = q.shape
-        with torch.cuda.device(q.device):
+        with _on(q):
             q, k = _rows16(q), _rows16(k)
-            q_out, k_out = _empty(q.shape, q), _empty(k.shape, k)
+            q_out, k_out = q.new_empty(q.shape), k.new_empty(k.shape)
             _lib.check(
                 lib.picomoe_qk_norm_rope_fwd(
-                    _lib.ptr(q), _strides(q), q.shape[2], _lib.ptr(k), _strides(k), k.shape[2], _lib.dtype_code(q.dtype), B, S, D,
-                    _lib.ptr(q_weight), _lib.ptr(k_weight), eps, _lib.ptr(cos), _lib.ptr(sin), cos.shape[0], _lib.ptr(positions),
-                    _lib.ptr(q_out), _lib.ptr(k_out), _lib.stream_ptr(),
+                    _ptr(q), _strides(q), q.shape[2], _ptr(k), _strides(k), k.shape[2], _lib.dtype_code(q.dtype), B, S, D,
+                    _ptr(q_weight), _ptr(k_weight), eps, _ptr(cos), _ptr(sin), cos.shape[0], _ptr(positions),
+                    _ptr(q_out), _ptr(k_out), _stream(),
                 ),
                 "picomoe_qk_norm_rope_fwd",
             )
@@ -143,23 +171,23 @@ class _QkNormRope(torch.autograd.Function):
         return q_out, k_out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_differentiable
     def backward(ctx, dq_out, dk_out):
         q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
         lib = _lib.load()
         B, S, _, D = q.shape
         dt = _lib.dtype_code(q.dtype)
-        with torch.cuda.device(q.device):
+        with _on(q):
             dq_out, dk_out = _dense16(dq_out), _dense16(dk_out)
-            dq, dk = _empty(q.shape, q), _empty(k.shape, k)
-            dqw = _empty((D,), q) if q_weight is not None and ctx.needs_input_grad[2] else None
-            dkw = _empty((D,), q) if k_weight is not None and ctx.needs_input_grad[3] else None
+            dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
+            dqw = q.new_empty((D,)) if q_weight is not None and ctx.needs_input_grad[2] else None
+            dkw = q.new_empty((D,)) if k_weight is not None and ctx.needs_input_grad[3] else None
             ws = _workspace(lib.picomoe_qk_norm_rope_bwd_workspace_bytes(dt, B, S, q.shape[2], k.shape[2], D), q, "qk_norm_rope")
             _lib.check(
                 lib.picomoe_qk_norm_rope_bwd(
-                    _lib.ptr(dq_out), _lib.ptr(dk_out), _lib.ptr(q), _strides(q), q.shape[2], _lib.ptr(k), _strides(k), k.shape[2], dt, B, S, D,
-                    _lib.ptr(q_weight), _lib.ptr(k_weight), ctx.eps, _lib.ptr(cos), _lib.ptr(sin), cos.shape[0], _lib.ptr(positions),
-                    _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dqw), _lib.ptr(dkw), _lib.ptr(ws), ws.numel(), _lib.stream_ptr(),
+                    _ptr(dq_out), _ptr(dk_out), _ptr(q), _strides(q), q.shape[2], _ptr(k), _strides(k), k.shape[2], dt, B, S, D,
+                    _ptr(q_weight), _ptr(k_weight), ctx.eps, _ptr(cos), _ptr(sin), cos.shape[0], _ptr(positions),
+                    _ptr(dq), _ptr(dk), _ptr(dqw), _ptr(dkw), _ptr(ws), ws.numel(), _stream(),
                 ),
                 "picomoe_qk_norm_rope_bwd",
             )
@@ -217,18 +245,18 @@ class _Attention(torch.autograd.Function):
         B, Sq, H, D = q.shape
         Sk, G = k.shape[1:3]
         dt = _lib.dtype_code(q.dtype)
-        with torch.cuda.device(q.device):
+        with _on(q):
             q, k, v = _rows16(q), _rows16(k), _rows16(v)
-            out = _empty((B, Sq, H, D), q)
-            lse = _empty((B, H, Sq), q, torch.float32)
+            out = q.new_empty((B, Sq, H, D))
+            lse = q.new_empty((B, H, Sq), dtype=torch.float32)
             # what out's rounding left makes the backward's d_out . out exact; nothing else reads it
-            residual = _empty(q.shape, q) if q.dtype == torch.bfloat16 and any(ctx.needs_input_grad[:3]) else None
+            residual = q.new_empty(q.shape) if q.dtype == torch.bfloat16 and any(ctx.needs_input_grad[:3]) else None
             ws = _workspace(lib.picomoe_attention_fwd_workspace_bytes(dt, B, Sq, Sk, H, G, D), q, "attention")
             _lib.check(
                 lib.picomoe_attention_fwd(
-                    _lib.ptr(q), _strides(q), _lib.ptr(k), _strides(k), _lib.ptr(v), _strides(v), dt, B, Sq, Sk, H, G, D, scale, softcap, causal,
-                    window, _lib.ptr(slopes), _lib.ptr(document_ids), _lib.ptr(prefix_lengths), _lib.ptr(out), _lib.ptr(residual),
-                    _lib.ptr(lse), _lib.ptr(ws), ws.numel(), _lib.stream_ptr(),
+                    _ptr(q), _strides(q), _ptr(k), _strides(k), _ptr(v), _strides(v), dt, B, Sq, Sk, H, G, D, scale, softcap, causal,
+                    window, _ptr(slopes), _ptr(document_ids), _ptr(prefix_lengths), _ptr(out), _ptr(residual),
+                    _ptr(lse), _ptr(ws), ws.numel(), _stream(),
                 ),
                 "picomoe_attention_fwd",
             )
@@ -237,7 +265,7 @@ class _Attention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_differentiable
     def backward(ctx, d_out):
         q, k, v, out, residual, lse, slopes, document_ids, prefix_lengths = ctx.saved_tensors
         scale, softcap, causal, window = ctx.meta
@@ -245,17 +273,17 @@ class _Attention(torch.autograd.Function):
         B, Sq, H, D = q.shape
         Sk, G = k.shape[1:3]
         dt = _lib.dtype_code(q.dtype)
-        with torch.cuda.device(q.device):
+        with _on(q):
             if Sq == 0 or Sk == 0:
                 return tuple(torch.zeros(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)) + (None,) * 7
             d_out = _dense16(d_out)
-            dq, dk, dv = _empty(q.shape, q), _empty(k.shape, k), _empty(v.shape, v)
+            dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
             ws = _workspace(lib.picomoe_attention_bwd_workspace_bytes(dt, B, Sq, Sk, H, G, D), q, "attention")
             _lib.check(
                 lib.picomoe_attention_bwd(
-                    _lib.ptr(d_out), _lib.ptr(q), _strides(q), _lib.ptr(k), _strides(k), _lib.ptr(v), _strides(v), _lib.ptr(out), _lib.ptr(residual),
-                    _lib.ptr(lse), dt, B, Sq, Sk, H, G, D, scale, softcap, causal, window, _lib.ptr(slopes), _lib.ptr(document_ids), _lib.ptr(prefix_lengths),
-                    _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), _lib.ptr(ws), ws.numel(), _lib.stream_ptr(),
+                    _ptr(d_out), _ptr(q), _strides(q), _ptr(k), _strides(k), _ptr(v), _strides(v), _ptr(out), _ptr(residual),
+                    _ptr(lse), dt, B, Sq, Sk, H, G, D, scale, softcap, causal, window, _ptr(slopes), _ptr(document_ids), _ptr(prefix_lengths),
+                    _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), ws.numel(), _stream(),
                 ),
                 "picomoe_attention_bwd",
             )

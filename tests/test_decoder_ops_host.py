@@ -24,8 +24,8 @@ def test_embedding_arguments():
     assert lib.picomoe_embedding_fwd(None, 1, 10, 64, P, 4, 1.0, P, None) == 1
     assert lib.picomoe_embedding_fwd(None, 1, 10, 64, None, 0, 1.0, None, None) == 0  # no tokens
     need = lib.picomoe_embedding_bwd_workspace_bytes(1, 5000, 100, 64)
-    # two buffers of keys and of tokens, two blocks' digit counts, two partial rows for each of 79 pieces
-    assert need == 4 * 20000 + 2 * 512 * 4 + 79 * 2 * 64 * 4
+    # two buffers of keys and of tokens, two partial rows for each of 79 pieces
+    assert need == 4 * 20000 + 79 * 2 * 64 * 4
     assert lib.picomoe_embedding_bwd_workspace_bytes(1, -1, 100, 64) == -1
     assert lib.picomoe_embedding_bwd_workspace_bytes(1, 1 << 31, 100, 64) == -1
     assert lib.picomoe_embedding_bwd(P, 1, P, 5000, 100, 64, 1.0, -1, P, P, need - 1, None) == 1   # workspace too small
