@@ -36,8 +36,8 @@ struct AttnArgs {
     // backward
     const void* d_out;
     void *dq, *dk, *dv;
-    float* delta;  // [batch, heads, q_len]: D above
-    char* ws;      // what is left of the workspace
+    float* delta;  // the simple kernels' workspace, [batch, heads, q_len]: D above
+    char* ws;      // the MFMA kernels' workspace
 };
 
 namespace {

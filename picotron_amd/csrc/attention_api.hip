@@ -62,8 +62,8 @@ extern "C" int picomoe_attention_fwd(const void* q, const int64_t* q_strides, co
 extern "C" int64_t picomoe_attention_bwd_workspace_bytes(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, int kv_heads,
                                                          int head_dim) {
     if (!sizes_ok(dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim)) return -1;
-    const int64_t delta = round16(batch * q_len * q_heads * 4);
-    return delta + (attention_mfma_supported(head_dim) ? attention_mfma_bwd_workspace(dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim) : 16);
+    if (attention_mfma_supported(head_dim)) return attention_mfma_bwd_workspace(dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim);
+    return round16(batch * q_len * q_heads * 4) + 16;  // D of the rows
 }
 
 extern "C" int picomoe_attention_bwd(const void* d_out, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
@@ -81,7 +81,7 @@ extern "C" int picomoe_attention_bwd(const void* d_out, const void* q, const int
                       workspace_bytes >= picomoe_attention_bwd_workspace_bytes(dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim));
     a.out = (void*)out; a.residual = dtype == PICOMOE_BF16 ? (void*)out_residual : nullptr; a.lse = (float*)lse; a.d_out = d_out; a.dq = dq; a.dk = dk; a.dv = dv;
     a.delta = (float*)workspace;
-    a.ws = (char*)workspace + round16(batch * q_len * q_heads * 4);
+    a.ws = (char*)workspace;
     if (attention_mfma_supported(head_dim)) return attention_mfma_bwd(a, (hipStream_t)stream);
     return attention_simple_bwd(a, (hipStream_t)stream);
 }

@@ -16,7 +16,7 @@ namespace {
 template <typename T, int DP>
 struct DqShape {
     static constexpr int kTile = sizeof(T) == 2 ? 64 : 32;
-    typedef Tile<T, DP, kTile> Tl;
+    typedef PanelTile<T, DP, kTile> Tl;
     static constexpr int kTileBytes = Tl::kBytes;
     static constexpr int kBuf = 2 * kTileBytes + kTile * 4;  // K, V, document ids
     static constexpr int kLds = 2 * kBuf;
@@ -41,7 +41,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq
     const RowSpan span = row_span(a, b, s);
     const int key_span = span.hi - span.lo;
     const float slope2 = a.slopes ? a.slopes[head] * kLog2e : 0.f;
-    const int64_t out_row = ((int64_t)b * a.q_len + s) * a.heads + head, stat = ((int64_t)b * a.heads + head) * a.q_len + s;
+    const int64_t out_row = ((int64_t)b * a.q_len + s) * a.heads + head;
 
     const bool some = key_span >= 0;
     Reach w;
@@ -95,9 +95,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq
             gf[ks] = load_frag<T>(g, 16 * ks + 8 * hi, a.D);
         }
     }
-    const float delta = a.delta[stat];
-    float lse2 = a.lse[stat] * kLog2e;
-    lse2 = lse2 == -INFINITY ? INFINITY : lse2;  // a row without a key: P = 0
+    const float* stats = m.stats + ((int64_t)bh * m.row_docs.tiles + row / 32) * (kStats * 32) + row % 32;
+    const float delta = stats[kDelta * 32], lse2 = stats[kLse2 * 32];
 
     const T* kbase = (const T*)a.k.p + b * a.k.sb + kvh * a.k.sh;
     const T* vbase = (const T*)a.v.p + b * a.v.sb + kvh * a.v.sh;
@@ -240,11 +239,10 @@ template <typename T, int DP>
 struct DkvShape {
     static constexpr int kTile = 32;              // rows of a tile
     static constexpr int kKeys = 32 * kWaves;     // keys of a block
-    typedef Tile<T, DP, kTile> Tl;
-    typedef Tile<T, DP, kKeys> VTl;
+    typedef PanelTile<T, DP, kTile> Tl;
+    typedef PanelTile<T, DP, kKeys> VTl;
     static constexpr int kTileBytes = Tl::kBytes;
-    static constexpr int kStats = 7 * kTile * 4;  // lse2, delta, slope2 (floats), position, first key, keys, document (ints)
-    static constexpr int kBuf = 2 * kTileBytes + kStats;
+    static constexpr int kBuf = 2 * kTileBytes + kStats * kTile * 4;
     // V's fragments are the ones that do not fit the 256 registers of a lane at head_dim 128 (dk, dv, K, S, dP do): read from LDS
     static constexpr bool kVInLds = DP == 128;
     static constexpr int kVBytes = kVInLds ? VTl::kBytes : 0;
@@ -323,8 +321,6 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
     }
     const T* qbase = (const T*)a.q.p + b * a.q.sb + (int64_t)(kvh * a.group) * a.q.sh;
     const T* gbase = (const T*)a.d_out + ((int64_t)b * a.q_len * a.heads + kvh * a.group) * a.D;
-    float stat_f[3] = {};
-    int stat_i[4] = {};
     auto fetch = [&](int t, int buf) {
         char* qt = lds + buf * kBuf;
         auto row_at = [&](int r) { return min(t * Sh::kTile + r, m.rows - 1); };
@@ -336,29 +332,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
             const int s = m.div(row_at(r)), h = row_at(r) - s * a.group;
             return gbase + ((int64_t)s * a.heads + h) * a.D;
         });
-        if (threadIdx.x < Sh::kTile) {
-            const int r = t * Sh::kTile + (int)threadIdx.x, rc = min(r, m.rows - 1), s = m.div(rc), h = kvh * a.group + rc - s * a.group;
-            const int64_t stat = ((int64_t)b * a.heads + h) * a.q_len + s;
-            const RowSpan span = row_span(a, b, s);
-            const float lse = a.lse[stat];
-            stat_f[0] = lse == -INFINITY ? INFINITY : lse * kLog2e;
-            stat_f[1] = a.delta[stat];
-            stat_f[2] = a.slopes ? a.slopes[h] * kLog2e : 0.f;
-            const bool see = r < m.rows && span.hi >= span.lo;
-            stat_i[0] = s + off;
-            stat_i[1] = see ? span.lo : 0x7FFFFFFF;  // no key is that far
-            stat_i[2] = see ? span.hi - span.lo : 0;
-            stat_i[3] = span.doc;
-        }
-    };
-    auto stage_stats = [&](int buf) {
-        if (threadIdx.x < Sh::kTile) {
-            float* f = (float*)(lds + buf * kBuf + 2 * Sh::kTileBytes);
-#pragma unroll
-            for (int i = 0; i < 3; ++i) f[i * Sh::kTile + threadIdx.x] = stat_f[i];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) ((int*)f)[(3 + i) * Sh::kTile + threadIdx.x] = stat_i[i];
-        }
+        if (wave == 0) load16_to_lds(m.stats + ((int64_t)bh * row_tiles + t) * (kStats * 32) + lane * 4, qt + 2 * Sh::kTileBytes);
     };
 
     const typename Tl::Lane ln;
@@ -375,7 +349,6 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
         int cur = walk.next(), buf = 0;
         if (cur >= 0) fetch(cur, 0);
         while (cur >= 0) {
-            stage_stats(buf);
             lds_loads_done();
             __syncthreads();
             const int following = walk.next();
@@ -384,7 +357,6 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
             const char* gt = qt + Sh::kTileBytes;
             const uint32_t qa = lds_address(qt), ga = qa + Sh::kTileBytes;
             const float* stats = (const float*)(gt + Sh::kTileBytes);
-            const int* stati = (const int*)(stats + 3 * Sh::kTile);
             const int s0 = first_query(cur), s1 = last_query(cur);
             bool in = hi_of(s1) >= wave0 && lo_of(s0) <= wave1;
             bool full = lo_of(s1) <= wave0 && hi_of(s0) >= wave1 && (cur + 1) * Sh::kTile <= m.rows;
@@ -401,22 +373,17 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
                 for (int ks = 0; ks < kSteps; ++ks) {
                     mma(x, Tl::frag(qa, ln, 0, ks), kf[ks]);
                     if constexpr (Sh::kVInLds) {
-                        typename Sh::VTl::Lane vl;
-                        vl.row = ln.row;
-                        vl.row2 = ln.row2;
-                        mma(dp, Tl::frag(ga, ln, 0, ks), Sh::VTl::frag(v_rows, vl, 0, ks));
+                        mma(dp, Tl::frag(ga, ln, 0, ks), Tl::template frag_of<Sh::kKeys>(v_rows, ln, ks));
                     } else {
                         mma(dp, Tl::frag(ga, ln, 0, ks), vf[ks]);
                     }
                 }
-                auto stat4 = [&](int which, int j) { return *(const f32x4_t*)(stats + which * Sh::kTile + 8 * j + 4 * hi); };
-                auto stat4i = [&](int which, int j) {
-                    typedef __attribute__((ext_vector_type(4))) int i32x4_t;
-                    return *(const i32x4_t*)(stati + which * Sh::kTile + 8 * j + 4 * hi);
-                };
+                typedef __attribute__((ext_vector_type(4))) int i32x4_t;
+                auto stat4 = [&](RowStat which, int j) { return *(const f32x4_t*)(stats + which * Sh::kTile + 8 * j + 4 * hi); };
+                auto stat4i = [&](RowStat which, int j) { return *(const i32x4_t*)(stats + which * Sh::kTile + 8 * j + 4 * hi); };
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const f32x4_t delta = stat4(1, j);
+                    const f32x4_t delta = stat4(kDelta, j);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) dp[4 * j + i] -= delta[i];
                 }
@@ -435,15 +402,15 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
                 if (!PLAIN && a.slopes) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const f32x4_t slope2 = stat4(2, j);
-                        const auto pos = stat4i(0, j);
+                        const f32x4_t slope2 = stat4(kSlope2, j);
+                        const auto pos = stat4i(kPos, j);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) x[4 * j + i] -= slope2[i] * __builtin_fabsf((float)(pos[i] - key));
                     }
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const f32x4_t lse2 = stat4(0, j);
+                    const f32x4_t lse2 = stat4(kLse2, j);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) x[4 * j + i] = __builtin_amdgcn_exp2f(PLAIN ? __builtin_fmaf(x[4 * j + i], sc.mul, -lse2[i]) : x[4 * j + i] - lse2[i]);
                 }
@@ -452,7 +419,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
                 if (!full) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const auto lo = stat4i(1, j), keys = stat4i(2, j), row_doc = stat4i(3, j);
+                        const auto lo = stat4i(kFirst, j), keys = stat4i(kKeys, j), row_doc = stat4i(kDoc, j);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const bool see = (uint32_t)(key - lo[i]) <= (uint32_t)keys[i] && row_doc[i] == doc;
@@ -480,7 +447,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
                     for (uint64_t left = __ballot(bad); left; left &= left - 1) {
                         const int which = __builtin_ctzll(left), r = which & 31;
                         const char* from = which >> 5 ? gt : qt;
-                        const bool see = (uint32_t)(key - stati[1 * Sh::kTile + r]) <= (uint32_t)stati[2 * Sh::kTile + r] && stati[3 * Sh::kTile + r] == doc;
+                        const int32_t* of = (const int32_t*)stats + r;
+                        const bool see = (uint32_t)(key - of[kFirst * 32]) <= (uint32_t)of[kKeys * 32] && of[kDoc * 32] == doc;
 #pragma unroll
                         for (int t = 0; t < kCols; ++t)
 #pragma unroll
@@ -556,30 +524,42 @@ __global__ __launch_bounds__(kThreads) void attention_grad_join_kernel(JoinArgs 
     else *(f32x4_t*)to = sum;
 }
 
-// D = dO . (out + residual) of every row, a group of lanes per row and 16 bytes a lane; and the document ranges of the tiles
+// What the two kernels want to know of the rows, D = dO . (out + residual) among it -- a group of lanes per row of a key head, 16 bytes a
+// lane -- and the document ranges of the tiles
 template <typename T>
-__global__ __launch_bounds__(kThreads) void attention_prepare_kernel(MfmaArgs m, int64_t out_rows, int delta_blocks, int key_tile, int row_tile,
-                                                                     int key_blocks) {
+__global__ __launch_bounds__(kThreads) void attention_prepare_kernel(MfmaArgs m, int delta_blocks, int key_tile, int row_tile, int key_blocks) {
     const AttnArgs& a = m.a;
-    constexpr int kPer = 16 / (int)sizeof(T), kLanes = 128 / kPer;
+    constexpr int kPer = 16 / (int)sizeof(T), kLanes = 128 / kPer, kRows = kThreads / kLanes;
     if ((int)blockIdx.x < delta_blocks) {
-        const int64_t row = (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
-        const int col = threadIdx.x % kLanes * kPer;
-        float sum = 0.f;
-        if (row < out_rows && col < a.D) {
-            const T *g = (const T*)a.d_out + row * a.D + col, *o = (const T*)a.out + row * a.D + col;
+        const int blocks = m.row_docs.tiles * 32 / kRows;  // of a key head
+        const int bh = blockIdx.x / blocks, row = (blockIdx.x - bh * blocks) * kRows + threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
+        const int at = row < m.rows ? row : m.rows - 1, b = bh / a.kv_heads, s = m.div(at), head = (bh - b * a.kv_heads) * a.group + at - s * a.group;
+        const int64_t from = (((int64_t)b * a.q_len + s) * a.heads + head) * a.D + lane * kPer;
+        float delta = 0.f;
+        if (lane * kPer < a.D) {
             typedef __attribute__((ext_vector_type(kPer))) T vec;
-            const vec gv = *(const vec*)g, ov = *(const vec*)o;
+            const vec gv = *(const vec*)((const T*)a.d_out + from), ov = *(const vec*)((const T*)a.out + from);
             vec rv = {};
-            if (sizeof(T) == 2 && a.residual) rv = *(const vec*)((const T*)a.residual + row * a.D + col);
+            if (sizeof(T) == 2 && a.residual) rv = *(const vec*)((const T*)a.residual + from);
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) sum += (float)gv[e] * ((float)ov[e] + (float)rv[e]);
+            for (int e = 0; e < kPer; ++e) delta += (float)gv[e] * ((float)ov[e] + (float)rv[e]);
         }
 #pragma unroll
-        for (int off = kLanes / 2; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-        if (row < out_rows && threadIdx.x % kLanes == 0) {
-            const int64_t token = row / a.heads, b = token / a.q_len;
-            a.delta[(b * a.heads + (row - token * a.heads)) * a.q_len + (token - b * a.q_len)] = sum;
+        for (int off = kLanes / 2; off > 0; off >>= 1) delta += __shfl_xor(delta, off, 64);
+        if (lane < kStats) {
+            const RowSpan span = row_span(a, b, s);
+            const bool some = row < m.rows && span.hi >= span.lo;
+            float v = delta;
+            if (lane == kLse2) {
+                const float lse = a.lse[((int64_t)b * a.heads + head) * a.q_len + s];
+                v = !some || lse == -INFINITY ? INFINITY : lse * kLog2e;
+            }
+            if (lane == kSlope2) v = a.slopes ? a.slopes[head] * kLog2e : 0.f;
+            if (lane == kPos) v = __int_as_float(s + a.kv_len - a.q_len);
+            if (lane == kFirst) v = __int_as_float(some ? span.lo : 0x7FFFFFFF);
+            if (lane == kKeys) v = __int_as_float(some ? span.hi - span.lo : 0);
+            if (lane == kDoc) v = __int_as_float(span.doc);
+            m.stats[((int64_t)bh * m.row_docs.tiles + row / 32) * (kStats * 32) + lane * 32 + row % 32] = v;
         }
         return;
     }
@@ -611,7 +591,7 @@ Cut cut(int64_t heads, int64_t blocks, int64_t tiles, int64_t shortest) {
 struct Plan {
     int key_tile, key_tiles, row_tiles;
     Cut dq, dkv;
-    int64_t key_docs, row_docs, dq_parts, dkv_parts, dq_bytes, dkv_bytes;
+    int64_t key_docs, row_docs, stats_bytes, dq_parts, dkv_parts, dq_bytes, dkv_bytes;
 };
 Plan plan(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, int kv_heads, int head_dim) {
     Plan p;
@@ -623,6 +603,7 @@ Plan plan(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, 
     p.dkv = cut(heads, (kv_len + per - 1) / per, p.row_tiles, 16);
     p.key_docs = round16(batch * p.key_tiles * 8);
     p.row_docs = round16(batch * p.row_tiles * 8);
+    p.stats_bytes = heads * p.row_tiles * (kStats * 32 * 4);
     p.dq_parts = p.dq.splits > 1 ? round16(heads * p.dq.blocks * 4) : 0;
     p.dkv_parts = p.dkv.splits > 1 ? round16(heads * p.dkv.blocks * 4) : 0;
     p.dq_bytes = p.dq.splits > 1 ? p.dq.splits * batch * q_len * q_heads * head_dim * 4 : 0;
@@ -640,7 +621,7 @@ int launch(MfmaArgs m, const Plan& p, hipStream_t s) {
     const AttnArgs& a = m.a;
     const int64_t heads = a.batch * a.kv_heads, q_quads = a.batch * a.q_len * a.heads * (a.D / 4), k_quads = a.batch * a.kv_len * a.kv_heads * (a.D / 4);
     const int64_t join_blocks = ((q_quads > k_quads ? q_quads : k_quads) + kThreads - 1) / kThreads;
-    const int64_t out_rows = a.batch * a.q_len * a.heads, per_block = sizeof(T) == 2 ? 16 : 8, delta_blocks = (out_rows + per_block - 1) / per_block;
+    const int64_t delta_blocks = heads * p.row_tiles * 32 / (sizeof(T) == 2 ? 16 : 8);
     const int64_t key_ranges = a.docs ? a.batch * range_blocks(p.key_tiles) : 0, row_ranges = a.docs ? a.batch * range_blocks(p.row_tiles) : 0;
     if (heads * p.dq.blocks > 0x7FFFFFFF || heads * p.dkv.blocks > 0x7FFFFFFF || join_blocks > 0x7FFFFFFF ||
         delta_blocks + key_ranges + row_ranges > 0x7FFFFFFF)
@@ -653,10 +634,11 @@ int launch(MfmaArgs m, const Plan& p, hipStream_t s) {
     };
     int32_t *key_docs = (int32_t*)take(p.key_docs), *row_docs = (int32_t*)take(p.row_docs);
     int32_t *dq_parts = (int32_t*)take(p.dq_parts), *dkv_parts = (int32_t*)take(p.dkv_parts);
+    m.stats = (float*)take(p.stats_bytes);
     float *dq_sums = (float*)take(p.dq_bytes), *dkv_sums = (float*)take(p.dkv_bytes);
     m.key_docs = {key_docs, key_docs + a.batch * p.key_tiles, p.key_tiles};
     m.row_docs = {row_docs, row_docs + a.batch * p.row_tiles, p.row_tiles};
-    attention_prepare_kernel<T><<<(unsigned)(delta_blocks + key_ranges + row_ranges), kThreads, 0, s>>>(m, out_rows, (int)delta_blocks, p.key_tile, 32,
+    attention_prepare_kernel<T><<<(unsigned)(delta_blocks + key_ranges + row_ranges), kThreads, 0, s>>>(m, (int)delta_blocks, p.key_tile, 32,
                                                                                                         (int)key_ranges);
     auto use = [&](const Cut& c, int32_t* parts, float* sums) {
         m.blocks = c.blocks;
@@ -695,7 +677,7 @@ int launch_for(const MfmaArgs& m, const Plan& p, hipStream_t s) {
 
 int64_t attention_mfma_bwd_workspace(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, int kv_heads, int head_dim) {
     const Plan p = plan(dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim);
-    return p.key_docs + p.row_docs + p.dq_parts + p.dkv_parts + p.dq_bytes + p.dkv_bytes + 16;
+    return p.key_docs + p.row_docs + p.stats_bytes + p.dq_parts + p.dkv_parts + p.dq_bytes + p.dkv_bytes + 16;
 }
 
 int attention_mfma_bwd(const AttnArgs& a, hipStream_t s) {

@@ -99,13 +99,109 @@ __device__ __forceinline__ void clear_lds(char* lds, int bytes) {
     __syncthreads();
 }
 
-// Tiles in LDS: panels of 16 columns, in a panel ROWS rows of 32 (fp32: 64) bytes in 16-byte chunks, chunk c of a row at
-// c ^ swizzle(row); 128 bytes between panels.  The 16 rows that a ds_read_b128 serves at a time, and the 4 rows of two neighbouring
-// panels of a transposing read, then lie on different banks, and every fragment of a tile is at a constant distance from a lane's
-// first: three address registers a tile, where swizzled rows of the whole width took one per fragment -- with dk and dv in
-// registers those spilled, and a reload from scratch waits for the tile in flight.
+// Tiles in LDS: groups of columns 128 bytes wide (64 bf16, 32 fp32), in a group ROWS rows of eight 16-byte chunks, chunk c of a row at
+// c ^ swizzle(row).  The 16 rows that a ds_read_b128 serves at a time, and the 4 rows x 64 bytes of a transposing read, then lie on
+// different banks; the fragments of a tile are at constant distances from eight addresses of a lane (rows of the tile's whole width: from
+// sixteen).  For the forward, which has the registers: with the panels below one new token over 32768 keys took 239 us, not 205.
 template <typename T, int DP, int ROWS>
 struct Tile {
+    static constexpr int kSize = (int)sizeof(T), kPerChunk = 16 / kSize, kRowBytes = 128, kGroupCols = 128 / kSize;
+    static constexpr int kGroups = DP / kGroupCols, kStride = ROWS * kRowBytes, kBytes = kGroups * kStride;
+    typedef __attribute__((address_space(3))) const bf16x8_t lds_bf16x8;
+    typedef __attribute__((address_space(3))) const f32x4_t lds_f32x4;
+    typedef __attribute__((address_space(3))) const float lds_f32;
+
+    __device__ static __forceinline__ uint32_t swizzle(int row) { return (((row >> 1) & 1) << 2) | ((row >> 2) & 3); }
+    __device__ static __forceinline__ uint32_t at(int row, int col) {
+        return col / kGroupCols * kStride + row * kRowBytes + (((uint32_t)(col % kGroupCols / kPerChunk) ^ swizzle(row)) << 4) + col % kPerChunk * kSize;
+    }
+
+    // this lane's offsets: [16 columns of a group][half of eight elements] of row lane % 32; of the transposed tile
+    struct Lane {
+        uint32_t row[kGroupCols / 16][kSize / 2], col[2][2];
+        __device__ __forceinline__ Lane() {
+            const int lane = threadIdx.x & 63, hi = lane >> 5;
+#pragma unroll
+            for (int g = 0; g < kGroupCols / 16; ++g)
+#pragma unroll
+                for (int h = 0; h < kSize / 2; ++h) row[g][h] = at(lane & 31, 16 * g + 8 * hi + 4 * h);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int up = 0; up < 2; ++up) {
+                    if (kSize == 2)  // [32 columns of a group][rows + 8]; a transposing read: lane l of 16 gives the address of 4 elements
+                                     // of row l / 4 and gets column l of the 4 rows
+                        col[i][up] = at(4 * hi + ((lane >> 2) & 3) + 8 * up, 32 * i + 16 * ((lane >> 4) & 1) + 4 * (lane & 3));
+                    else             // [rows + 2][rows + 8]
+                        col[i][up] = at(4 * hi + 2 * i + 8 * up, lane & 31);
+                }
+        }
+    };
+
+    // rows row0 (a multiple of 32) + lane % 32, elements 16 ks + 8 hi ..; tile: its LDS address
+    __device__ static __forceinline__ Frag<T> frag(uint32_t tile, const Lane& l, int row0, int ks) {
+        constexpr int kPer = kGroupCols / 16;
+        Frag<T> f;
+        const uint32_t off = row0 * kRowBytes + ks / kPer * kStride;
+        if constexpr (kSize == 2) {
+            f.v = *(lds_bf16x8*)(uintptr_t)(tile + l.row[ks % kPer][0] + off);
+        } else {
+            const f32x4_t a = *(lds_f32x4*)(uintptr_t)(tile + l.row[ks % kPer][0] + off), b = *(lds_f32x4*)(uintptr_t)(tile + l.row[ks % kPer][1] + off);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f.v[i] = a[i];
+                f.v[4 + i] = b[i];
+            }
+        }
+        return f;
+    }
+
+    // the tile transposed: column 32 t + lane % 32, rows row0 (a multiple of 16) + {4 hi + 0..3, 8 + 4 hi + 0..3}
+    __device__ static __forceinline__ Frag<T> frag_t(uint32_t tile, const Lane& l, int row0, int t) {
+        constexpr int kPer = kGroupCols / 32;
+        Frag<T> f;
+        const uint32_t off = row0 * kRowBytes + t / kPer * kStride;
+        if constexpr (kSize == 2) {
+            typedef __attribute__((ext_vector_type(4))) short s16x4_t;
+            typedef __attribute__((ext_vector_type(8))) short s16x8_t;
+            typedef __attribute__((address_space(3))) s16x4_t lds4;
+            const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(uintptr_t)(tile + l.col[t % kPer][0] + off));
+            const s16x4_t up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(uintptr_t)(tile + l.col[t % kPer][1] + off));
+            const s16x8_t v = {lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
+            f.v = __builtin_bit_cast(bf16x8_t, v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f.v[e] = *(lds_f32*)(uintptr_t)(tile + l.col[(e >> 1) & 1][e >> 2] + off + (e & 1) * kRowBytes);
+        }
+        return f;
+    }
+
+    // Stages the tile with direct-to-LDS loads of 1 KB: 8 rows of a group.  Columns from D on are left as they are (zeros: clear_lds).
+    template <typename F>
+    __device__ static __forceinline__ void load(char* tile, int D, F row_of) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+        for (int i = 0; i < kGroups * ROWS / 8 / kWaves; ++i) {
+            const int unit = i * kWaves + wave, group = unit % kGroups, r0 = unit / kGroups * 8, row = r0 + lane / 8;
+            const int chunk = (int)((uint32_t)(lane % 8) ^ swizzle(row)), col = group * kGroupCols + chunk * kPerChunk;
+            if (col < D) load16_to_lds(row_of(row) + col, tile + group * kStride + r0 * kRowBytes);
+        }
+    }
+    __device__ static __forceinline__ float element(const char* tile, int row, int col) { return to_f32(*(const T*)(tile + at(row, col))); }
+    // whether row `row` holds a value that is not finite
+    __device__ static __forceinline__ bool row_not_finite(const char* tile, int row) {
+        bool bad = false;
+        for (int c = 0; c < DP; ++c) bad |= !(__builtin_fabsf(element(tile, row, c)) < INFINITY);
+        return bad;
+    }
+};
+
+// The same tiles in panels of 16 columns, in a panel ROWS rows of 32 (fp32: 64) bytes in 16-byte chunks, chunk c of a row at
+// c ^ swizzle(row); 128 bytes between panels.  Every fragment is at a constant distance from a lane's first: three address registers
+// instead of eight.  For the backward, where the eight spill -- and a reload from scratch waits for the tile in flight -- although the
+// loads touch 32-byte pieces of rows: dk / dv of 16384 tokens x 16 heads took 3.9 ms against 4.3.
+template <typename T, int DP, int ROWS>
+struct PanelTile {
     static constexpr int kSize = (int)sizeof(T), kPerChunk = 16 / kSize, kRowBytes = 16 * kSize, kRowChunks = kSize;  // of a panel
     static constexpr int kPanels = DP / 16, kStride = ROWS * kRowBytes + 128, kBytes = kPanels * kStride;
     typedef __attribute__((address_space(3))) const bf16x8_t lds_bf16x8;
@@ -150,6 +246,12 @@ struct Tile {
             }
         }
         return f;
+    }
+
+    // the same of a tile of OTHER rows, from row 0 on: rows lie alike in all of them
+    template <int OTHER>
+    __device__ static __forceinline__ Frag<T> frag_of(uint32_t tile, const Lane& l, int ks) {
+        return frag(tile + ks * (OTHER - ROWS) * kRowBytes, l, 0, ks);
     }
 
     // the tile transposed: column 32 t + lane % 32, rows row0 (a multiple of 16) + {4 hi + 0..3, 8 + 4 hi + 0..3}
@@ -263,7 +365,12 @@ struct MfmaArgs {
     float* part_out;
     float* part_lse;
     DocRanges key_docs, row_docs;
+    float* stats;  // backward: [key heads][row tiles of 32][kStats][32], see RowStat
 };
+
+// What the backward knows of a row, in LDS by a kind and a row of the tile.  Rows that see nothing, and those past the end: kFirst is
+// INT_MAX, kKeys 0 -- no key is that far -- and kLse2 +inf, which makes P zero.
+enum RowStat { kLse2, kDelta, kSlope2, kPos, kFirst, kKeys, kDoc, kStats = 8 };  // from kPos on: int32
 
 // what a set of query rows may see, and which documents it has
 struct Reach {
