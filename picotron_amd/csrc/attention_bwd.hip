@@ -30,7 +30,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq
     typedef typename Sh::Tl Tl;
     constexpr int kSub = Sh::kTile / 32, kSteps = DP / 16, kCols = DP / 32;
     const AttnArgs& a = m.a;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = wave_index(), hi = lane >> 5;
 
     const int heads = (int)a.batch * a.kv_heads, bh = blockIdx.x % heads, split = blockIdx.y, tile = m.blocks - 1 - blockIdx.x / heads;
     const int b = bh / a.kv_heads, kvh = bh % a.kv_heads;
@@ -77,10 +77,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq
     const bool any = blk.hi_max >= blk.lo_min;
     const int first = any ? blk.lo_min / Sh::kTile : 0, end = any ? blk.hi_max / Sh::kTile + 1 : 0;
 
-    auto active = [&](int t) { return !a.docs || (doc_max[t] >= blk.doc_min && doc_min[t] <= blk.doc_max); };
+    auto active = [&](int, int d0, int d1) { return !a.docs || (d1 >= blk.doc_min && d0 <= blk.doc_max); };
     Share share = {1, 0, 0x7FFFFFFF};
     if (m.splits > 1) {
-        share = share_of(a.docs ? count_tiles(first, end, active) : end - first, split, m);
+        share = share_of(a.docs ? count_tiles(first, end, doc_min, doc_max, active) : end - first, split, m);
         if (split == 0 && threadIdx.x == 0) m.parts[bh * m.blocks + tile] = share.parts;
         if (split >= share.parts) return;
     }
@@ -101,43 +101,53 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq
     const T* kbase = (const T*)a.k.p + b * a.k.sb + kvh * a.k.sh;
     const T* vbase = (const T*)a.v.p + b * a.v.sb + kvh * a.v.sh;
     if (a.D < DP) clear_lds(lds, Sh::kLds);
-    auto fetch = [&](int t, int buf) {
-        char* kt = lds + buf * Sh::kBuf;
+    const uint32_t k_step = (uint32_t)(a.k.ss * (int)sizeof(T)), v_step = (uint32_t)(a.v.ss * (int)sizeof(T));
+    const bool even = a.D == DP && a.k.ss < (1 << 22) && a.v.ss < (1 << 22);  // as in the forward
+    const uint32_t k_off = Tl::lane_offset(Tl::lane_row() * k_step), v_off = Tl::lane_offset(Tl::lane_row() * v_step);
+    auto fetch = [&](int t, int buf) __attribute__((always_inline)) {
+        const uint32_t kt = lds_address(lds) + buf * Sh::kBuf;
         auto key_at = [&](int r) { return (int64_t)min(t * Sh::kTile + r, a.kv_len - 1); };
-        Tl::load(kt, a.D, [&](int r) { return kbase + key_at(r) * a.k.ss; });
-        Tl::load(kt + Sh::kTileBytes, a.D, [&](int r) { return vbase + key_at(r) * a.v.ss; });
+        if (even && (t + 1) * Sh::kTile <= a.kv_len) {
+            Tl::load_even(kt, (const char*)(kbase + (int64_t)t * Sh::kTile * a.k.ss), k_off, [&](int r) { return (uint64_t)(r * k_step); });
+            Tl::load_even(kt + Sh::kTileBytes, (const char*)(vbase + (int64_t)t * Sh::kTile * a.v.ss), v_off, [&](int r) { return (uint64_t)(r * v_step); });
+        } else {
+            Tl::load(kt, a.D, [&](int r) { return kbase + key_at(r) * a.k.ss; });
+            Tl::load(kt + Sh::kTileBytes, a.D, [&](int r) { return vbase + key_at(r) * a.v.ss; });
+        }
         if (a.docs && wave == 0 && lane < Sh::kTile) load4_to_lds(a.docs + (int64_t)b * a.kv_len + key_at(lane), kt + 2 * Sh::kTileBytes);
     };
 
     const typename Tl::Lane ln;
     const ScoreScale sc = score_scale<T>(a);
     f32x16_t dq[kCols];
-    auto run = [&](auto careful) {  // CAREFUL: as in the forward, for K
+    auto run = [&](auto careful) __attribute__((always_inline)) {  // CAREFUL: as in the forward, for K
         constexpr bool kCareful = decltype(careful)::value;
 #pragma unroll
         for (int t = 0; t < kCols; ++t)
 #pragma unroll
             for (int i = 0; i < 16; ++i) dq[t][i] = 0.f;
-        TileWalk<decltype(active)> walk(first, end, active, share.skip, share.left);
-        int cur = walk.next(), buf = 0;
-        if (cur >= 0) fetch(cur, 0);
-        while (cur >= 0) {
+        TileWalk<decltype(active)> walk(first, end, doc_min, doc_max, active, share.skip, share.left);
+        WalkTile cur = walk.next();
+        int buf = 0;
+        if (cur.t >= 0) fetch(cur.t, 0);
+        while (cur.t >= 0) {
             lds_loads_done();
             __syncthreads();
-            const int following = walk.next();
-            if (following >= 0) fetch(following, buf ^ 1);
+            const WalkTile following = walk.next();
+            if (following.t >= 0) fetch(following.t, buf ^ 1);
             const char* kt = lds + buf * Sh::kBuf;
             const char* vt = kt + Sh::kTileBytes;
             const int32_t* docs = (const int32_t*)(vt + Sh::kTileBytes);
             const uint32_t ka = lds_address(kt), va = ka + Sh::kTileBytes;
-            const int key0 = cur * Sh::kTile, key1 = key0 + Sh::kTile - 1;
+            const int key0 = cur.t * Sh::kTile, key1 = key0 + Sh::kTile - 1;
             bool in = key0 <= w.hi_max && key1 >= w.lo_min, full = key0 >= w.lo_max && key1 <= w.hi_min;
             if (a.docs) {
-                const int d0 = doc_min[cur], d1 = doc_max[cur];
-                in = in && d1 >= w.doc_min && d0 <= w.doc_max;
-                full = full && d0 == d1 && d0 == w.doc_min && d0 == w.doc_max;
+                in = in && cur.doc_max >= w.doc_min && cur.doc_min <= w.doc_max;
+                full = full && cur.doc_min == cur.doc_max && cur.doc_min == w.doc_min && cur.doc_min == w.doc_max;
             }
             if (in) {
+                const typename Tl::Rows k_rows(ln, ka), v_rows(ln, va);
+                const typename Tl::Cols k_cols(ln, ka);
 #pragma unroll
                 for (int u = 0; u < kSub; ++u) {
                     f32x16_t x, dp;
@@ -145,9 +155,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq
                     for (int i = 0; i < 16; ++i) x[i] = dp[i] = 0.f;
 #pragma unroll
                     for (int ks = 0; ks < kSteps; ++ks) {
-                        mma(x, Tl::frag(ka, ln, u * 32, ks), qf[ks]);
-                        mma(dp, Tl::frag(va, ln, u * 32, ks), gf[ks]);
+                        mma(x, Tl::frag(k_rows, u * 32, ks), qf[ks]);
+                        mma(dp, Tl::frag(v_rows, u * 32, ks), gf[ks]);
                     }
+                    if (sizeof(T) == 2) read_ahead<2, 2, kSteps, 2>();
 #pragma unroll
                     for (int i = 0; i < 16; ++i) dp[i] -= delta;
                     if (PLAIN) {
@@ -171,12 +182,18 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq
                     for (int i = 0; i < 16; ++i) x[i] = __builtin_amdgcn_exp2f(PLAIN ? __builtin_fmaf(x[i], sc.mul, -lse2) : x[i] - lse2) * dp[i];
                     if (!full) {
                         const int from = span.lo - key0 - 4 * hi;
+                        const uint32_t seen_keys = (uint32_t)key_span;
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int at = u * 32 + 8 * (i / 4) + i % 4;
-                            bool see = key_span >= 0 && (uint32_t)(at - from) <= (uint32_t)key_span;
-                            if (a.docs) see = see && docs[at + 4 * hi] == span.doc;
-                            x[i] = see ? x[i] : 0.f;
+                        for (int i = 0; i < 16; ++i)
+                            x[i] = (uint32_t)(u * 32 + 8 * (i / 4) + i % 4 - from) <= seen_keys && key_span >= 0 ? x[i] : 0.f;
+                        if (a.docs) {
+                            typedef __attribute__((ext_vector_type(4))) int i32x4_t;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const i32x4_t d = *(const i32x4_t*)(docs + u * 32 + 8 * j + 4 * hi);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) x[4 * j + i] = d[i] == span.doc ? x[4 * j + i] : 0.f;
+                            }
                         }
                     }
 #pragma unroll
@@ -184,11 +201,12 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq
                         const Frag<T> dx = to_frag<T>(x, st);
 #pragma unroll
                         for (int t = 0; t < kCols; ++t) {
-                            Frag<T> k = Tl::frag_t(ka, ln, u * 32 + 16 * st, t);
+                            Frag<T> k = Tl::frag_t(k_cols, u * 32 + 16 * st, t);
                             if (kCareful) zero_not_finite(k);
                             mma(dq[t], k, dx);
                         }
                     }
+                    if (sizeof(T) == 2 && !kCareful) read_ahead<2, 1, 2 * kCols, 3>();
                 }
                 if (kCareful) {
                     bool bad = false;
@@ -256,7 +274,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
     typedef typename Sh::Tl Tl;
     constexpr int kSteps = DP / 16, kCols = DP / 32, kBuf = Sh::kBuf;
     const AttnArgs& a = m.a;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = wave_index(), hi = lane >> 5;
     const int heads = (int)a.batch * a.kv_heads, bh = blockIdx.x % heads, split = blockIdx.y, block = blockIdx.x / heads;
     const int b = bh / a.kv_heads, kvh = bh % a.kv_heads;
     const int block0 = block * Sh::kKeys, block1 = min(block0 + Sh::kKeys, a.kv_len) - 1;
@@ -292,20 +310,20 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
     auto last_query = [&](int t) { return m.div(min(t * Sh::kTile + Sh::kTile, m.rows) - 1); };
 
     const int row_tiles = (m.rows + Sh::kTile - 1) / Sh::kTile;
-    auto active = [&](int t) {
+    auto active = [&](int t, int d0, int d1) {
         if (hi_of(last_query(t)) < block0 || lo_of(first_query(t)) > block1) return false;
-        return !a.docs || (doc_max[t] >= max(0, blk_doc_min) && doc_min[t] <= blk_doc_max);
+        return !a.docs || (d1 >= max(0, blk_doc_min) && d0 <= blk_doc_max);
     };
     Share share = {1, 0, 0x7FFFFFFF};
     if (m.splits > 1) {
-        share = share_of(count_tiles(0, row_tiles, active), split, m);
+        share = share_of(count_tiles(0, row_tiles, doc_min, doc_max, active), split, m);
         if (split == 0 && threadIdx.x == 0) m.parts[bh * m.blocks + block] = share.parts;
         if (split >= share.parts) return;
     }
 
     if (a.D < DP) clear_lds(lds, Sh::kLds);
     Frag<T> kf[kSteps], vf[kSteps];
-    char* vtile = lds + 2 * kBuf;
+    const uint32_t vtile = lds_address(lds) + 2 * kBuf;
     if (Sh::kVInLds) {
         const T* v = (const T*)a.v.p + b * a.v.sb + kvh * a.v.sh;
         Sh::VTl::load(vtile, a.D, [&](int r) { return v + (int64_t)min(block0 + r, a.kv_len - 1) * a.v.ss; });
@@ -321,63 +339,81 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
     }
     const T* qbase = (const T*)a.q.p + b * a.q.sb + (int64_t)(kvh * a.group) * a.q.sh;
     const T* gbase = (const T*)a.d_out + ((int64_t)b * a.q_len * a.heads + kvh * a.group) * a.D;
-    auto fetch = [&](int t, int buf) {
-        char* qt = lds + buf * kBuf;
-        auto row_at = [&](int r) { return min(t * Sh::kTile + r, m.rows - 1); };
-        Tl::load(qt, a.D, [&](int r) {
-            const int s = m.div(row_at(r)), h = row_at(r) - s * a.group;
-            return qbase + s * a.q.ss + h * a.q.sh;
-        });
-        Tl::load(qt + Sh::kTileBytes, a.D, [&](int r) {
-            const int s = m.div(row_at(r)), h = row_at(r) - s * a.group;
-            return gbase + ((int64_t)s * a.heads + h) * a.D;
-        });
+    // 32 rows of a tile that are whole queries, at constant offsets within 2^31 bytes from the first: as in the forward
+    const bool even = a.D == DP && 32 % a.group == 0 && a.q.ss < (1 << 22) && a.q.sh < (1 << 22) && a.heads * a.D < (1 << 22);
+    const int per_tile = 32 / a.group, lane_s = Tl::lane_row() / a.group, lane_h = Tl::lane_row() % a.group;
+    const uint32_t q_off = Tl::lane_offset((uint32_t)(lane_s * a.q.ss + lane_h * a.q.sh) * (uint32_t)sizeof(T));
+    const uint32_t g_off = Tl::lane_offset((uint32_t)((lane_s * a.heads + lane_h) * a.D) * (uint32_t)sizeof(T));
+    auto fetch = [&](int t, int buf) __attribute__((always_inline)) {
+        const uint32_t qt = lds_address(lds) + buf * kBuf;
+        if (even && (t + 1) * Sh::kTile <= m.rows && Tl::kLoadRows % a.group == 0) {
+            const int64_t s0 = (int64_t)t * per_tile;
+            Tl::load_even(qt, (const char*)(qbase + s0 * a.q.ss), q_off, [&](int r) { return (uint64_t)(r / a.group * a.q.ss * (int)sizeof(T)); });
+            Tl::load_even(qt + Sh::kTileBytes, (const char*)(gbase + s0 * a.heads * a.D), g_off,
+                          [&](int r) { return (uint64_t)(r / a.group * a.heads * a.D * (int)sizeof(T)); });
+        } else {
+            auto row_at = [&](int r) { return min(t * Sh::kTile + r, m.rows - 1); };
+            Tl::load(qt, a.D, [&](int r) {
+                const int s = m.div(row_at(r)), h = row_at(r) - s * a.group;
+                return qbase + s * a.q.ss + h * a.q.sh;
+            });
+            Tl::load(qt + Sh::kTileBytes, a.D, [&](int r) {
+                const int s = m.div(row_at(r)), h = row_at(r) - s * a.group;
+                return gbase + ((int64_t)s * a.heads + h) * a.D;
+            });
+        }
         if (wave == 0) load16_to_lds(m.stats + ((int64_t)bh * row_tiles + t) * (kStats * 32) + lane * 4, qt + 2 * Sh::kTileBytes);
     };
 
     const typename Tl::Lane ln;
-    const uint32_t v_rows = lds_address(vtile) + wave * 32 * Tl::kRowBytes;
+    typename Sh::VTl::Lane vl;
+    vl.row = ln.row;
+    vl.row2 = ln.row2;
+    const typename Sh::VTl::Rows v_rows(vl, vtile + wave * 32 * Tl::kRowBytes);
     const ScoreScale sc = score_scale<T>(a);
     f32x16_t dk[kCols], dv[kCols];
-    auto run = [&](auto careful) {  // CAREFUL: as in the forward, for Q and dO
+    auto run = [&](auto careful) __attribute__((always_inline)) {  // CAREFUL: as in the forward, for Q and dO
         constexpr bool kCareful = decltype(careful)::value;
 #pragma unroll
         for (int t = 0; t < kCols; ++t)
 #pragma unroll
             for (int i = 0; i < 16; ++i) dk[t][i] = dv[t][i] = 0.f;
-        TileWalk<decltype(active)> walk(0, row_tiles, active, share.skip, share.left);
-        int cur = walk.next(), buf = 0;
-        if (cur >= 0) fetch(cur, 0);
-        while (cur >= 0) {
+        TileWalk<decltype(active)> walk(0, row_tiles, doc_min, doc_max, active, share.skip, share.left);
+        WalkTile cur = walk.next();
+        int buf = 0;
+        if (cur.t >= 0) fetch(cur.t, 0);
+        while (cur.t >= 0) {
             lds_loads_done();
             __syncthreads();
-            const int following = walk.next();
-            if (following >= 0) fetch(following, buf ^ 1);
+            const WalkTile following = walk.next();
+            if (following.t >= 0) fetch(following.t, buf ^ 1);
             const char* qt = lds + buf * kBuf;
             const char* gt = qt + Sh::kTileBytes;
             const uint32_t qa = lds_address(qt), ga = qa + Sh::kTileBytes;
             const float* stats = (const float*)(gt + Sh::kTileBytes);
-            const int s0 = first_query(cur), s1 = last_query(cur);
+            const int s0 = first_query(cur.t), s1 = last_query(cur.t);
             bool in = hi_of(s1) >= wave0 && lo_of(s0) <= wave1;
-            bool full = lo_of(s1) <= wave0 && hi_of(s0) >= wave1 && (cur + 1) * Sh::kTile <= m.rows;
+            bool full = lo_of(s1) <= wave0 && hi_of(s0) >= wave1 && (cur.t + 1) * Sh::kTile <= m.rows;
             if (a.docs) {
-                const int d0 = doc_min[cur], d1 = doc_max[cur];
-                in = in && d1 >= max(0, w_doc_min) && d0 <= w_doc_max;
-                full = full && d0 == d1 && d0 == w_doc_min && d0 == w_doc_max && d0 >= 0;
+                in = in && cur.doc_max >= max(0, w_doc_min) && cur.doc_min <= w_doc_max;
+                full = full && cur.doc_min == cur.doc_max && cur.doc_min == w_doc_min && cur.doc_min == w_doc_max && cur.doc_min >= 0;
             }
             if (in) {
+                const typename Tl::Rows q_rows(ln, qa), g_rows(ln, ga);
+                const typename Tl::Cols q_cols(ln, qa), g_cols(ln, ga);
                 f32x16_t x, dp;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) x[i] = dp[i] = 0.f;
 #pragma unroll
                 for (int ks = 0; ks < kSteps; ++ks) {
-                    mma(x, Tl::frag(qa, ln, 0, ks), kf[ks]);
+                    mma(x, Tl::frag(q_rows, 0, ks), kf[ks]);
                     if constexpr (Sh::kVInLds) {
-                        mma(dp, Tl::frag(ga, ln, 0, ks), Tl::template frag_of<Sh::kKeys>(v_rows, ln, ks));
+                        mma(dp, Tl::frag(g_rows, 0, ks), Sh::VTl::frag(v_rows, 0, ks));
                     } else {
-                        mma(dp, Tl::frag(ga, ln, 0, ks), vf[ks]);
+                        mma(dp, Tl::frag(g_rows, 0, ks), vf[ks]);
                     }
                 }
+                if (sizeof(T) == 2) read_ahead<Sh::kVInLds ? 3 : 2, 2, kSteps, 2>();
                 typedef __attribute__((ext_vector_type(4))) int i32x4_t;
                 auto stat4 = [&](RowStat which, int j) { return *(const f32x4_t*)(stats + which * Sh::kTile + 8 * j + 4 * hi); };
                 auto stat4i = [&](RowStat which, int j) { return *(const i32x4_t*)(stats + which * Sh::kTile + 8 * j + 4 * hi); };
@@ -433,7 +469,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
                     const Frag<T> p = to_frag<T>(x, st), dx = to_frag<T>(dp, st);
 #pragma unroll
                     for (int t = 0; t < kCols; ++t) {
-                        Frag<T> g = Tl::frag_t(ga, ln, 16 * st, t), q = Tl::frag_t(qa, ln, 16 * st, t);
+                        Frag<T> g = Tl::frag_t(g_cols, 16 * st, t), q = Tl::frag_t(q_cols, 16 * st, t);
                         if (kCareful) {
                             zero_not_finite(g);
                             zero_not_finite(q);
@@ -442,6 +478,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
                         mma(dk[t], q, dx);
                     }
                 }
+                if (sizeof(T) == 2 && !kCareful) read_ahead<4, 2, 2 * kCols, 2>();
                 if (kCareful) {
                     const bool bad = Tl::row_not_finite(hi ? gt : qt, lane & 31);
                     for (uint64_t left = __ballot(bad); left; left &= left - 1) {

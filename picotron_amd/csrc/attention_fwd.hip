@@ -18,7 +18,7 @@ constexpr float kLazy = 8.f;
 // has 32 rows of its own and all of the tile's keys.
 template <typename T, int DP, bool KEYS>
 struct FwdShape {
-    static constexpr int kTile = KEYS ? 128 : (sizeof(T) == 2 ? 64 : 32);  // keys of a tile
+    static constexpr int kTile = KEYS ? 32 * kWaves : (sizeof(T) == 2 ? 64 : 32);  // keys of a tile
     static constexpr int kWaveKeys = KEYS ? 32 : kTile;
     static constexpr int kRows = KEYS ? 32 : 32 * kWaves;  // rows of a block
     typedef Tile<T, DP, kTile> Tl;
@@ -53,7 +53,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
     constexpr int kSub = Sh::kWaveKeys / 32, kSteps = DP / 16, kCols = DP / 32;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const AttnArgs& a = m.a;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = wave_index(), hi = lane >> 5;
 
     // blocks of one key head lie on one XCD where there are 8 heads or more; those with the most keys (the last rows) go first
     const int heads = (int)a.batch * a.kv_heads, bh = blockIdx.x % heads, tile = m.blocks - 1 - blockIdx.x / heads, split = blockIdx.y;
@@ -105,10 +105,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
     const int32_t* doc_max = a.docs ? m.key_docs.highest + (int64_t)b * m.key_docs.tiles : nullptr;
     const bool any = blk.hi_max >= blk.lo_min;
     const int first = any ? blk.lo_min / Sh::kTile : 0, end = any ? blk.hi_max / Sh::kTile + 1 : 0;
-    auto active = [&](int t) { return !a.docs || (doc_max[t] >= blk.doc_min && doc_min[t] <= blk.doc_max); };
+    auto active = [&](int, int d0, int d1) { return !a.docs || (d1 >= blk.doc_min && d0 <= blk.doc_max); };
     Share share = {1, 0, 0x7FFFFFFF};
     if (m.splits > 1) {
-        share = share_of(a.docs ? count_tiles(first, end, active) : end - first, split, m);
+        share = share_of(a.docs ? count_tiles(first, end, doc_min, doc_max, active) : end - first, split, m);
         if (split == 0 && threadIdx.x == 0) m.parts[bh * m.blocks + tile] = share.parts;
         if (split >= share.parts) return;
     }
@@ -116,12 +116,21 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
     const T* kbase = (const T*)a.k.p + b * a.k.sb + kvh * a.k.sh;
     const T* vbase = (const T*)a.v.p + b * a.v.sb + kvh * a.v.sh;
     if (a.D < DP) clear_lds(lds, Sh::kLds);
-    auto fetch = [&](int t, int buf) {
-        char* kt = lds + buf * Sh::kBuf;
+    // rows of a tile within 2^31 bytes, whole tiles: no vector arithmetic for the addresses
+    const uint32_t k_step = (uint32_t)(a.k.ss * (int)sizeof(T)), v_step = (uint32_t)(a.v.ss * (int)sizeof(T));
+    const bool even = a.D == DP && a.k.ss < (1 << 22) && a.v.ss < (1 << 22);
+    const typename Tl::Source k_src(k_step), v_src(v_step);
+    auto fetch = [&](int t, int buf) __attribute__((always_inline)) {
+        const uint32_t kt = lds_address(lds) + buf * Sh::kBuf;
         // keys past the end are hidden by every row's interval
         auto key_at = [&](int r) { return (int64_t)min(t * Sh::kTile + r, a.kv_len - 1); };
-        Tl::load(kt, a.D, [&](int r) { return kbase + key_at(r) * a.k.ss; });
-        Tl::load(kt + Sh::kTileBytes, a.D, [&](int r) { return vbase + key_at(r) * a.v.ss; });
+        if (even && (t + 1) * Sh::kTile <= a.kv_len) {
+            Tl::load_even(kt, (const char*)(kbase + (int64_t)t * Sh::kTile * a.k.ss), k_step, k_src);
+            Tl::load_even(kt + Sh::kTileBytes, (const char*)(vbase + (int64_t)t * Sh::kTile * a.v.ss), v_step, v_src);
+        } else {
+            Tl::load(kt, a.D, [&](int r) { return kbase + key_at(r) * a.k.ss; });
+            Tl::load(kt + Sh::kTileBytes, a.D, [&](int r) { return vbase + key_at(r) * a.v.ss; });
+        }
         if (a.docs && wave < Sh::kTile / 64)
             load4_to_lds(a.docs + (int64_t)b * a.kv_len + key_at(wave * 64 + lane), kt + 2 * Sh::kTileBytes + wave * 256);
         if (a.docs && Sh::kTile < 64 && wave == 0 && lane < Sh::kTile) load4_to_lds(a.docs + (int64_t)b * a.kv_len + key_at(lane), kt + 2 * Sh::kTileBytes);
@@ -134,7 +143,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
 
     // CAREFUL: values of V that are not finite are kept out of the products, where 0 * inf would reach rows that do not see them,
     // and added one by one to the rows that do
-    auto run = [&](auto careful) {
+    auto run = [&](auto careful) __attribute__((always_inline)) {
         constexpr bool kCareful = decltype(careful)::value;
         top = -INFINITY;
         total = 0.f;
@@ -143,34 +152,37 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
 
-        TileWalk<decltype(active)> walk(first, end, active, share.skip, share.left);
-        int cur = walk.next(), buf = 0;
-        if (cur >= 0) fetch(cur, 0);
-        while (cur >= 0) {
+        TileWalk<decltype(active)> walk(first, end, doc_min, doc_max, active, share.skip, share.left);
+        WalkTile cur = walk.next();
+        int buf = 0;
+        if (cur.t >= 0) fetch(cur.t, 0);
+        while (cur.t >= 0) {
             lds_loads_done();
             __syncthreads();  // the tile is there, and every wave is done with the other buffer
-            const int following = walk.next();
-            if (Sh::kBuffers == 2 && following >= 0) fetch(following, buf ^ 1);
+            const WalkTile following = walk.next();
+            if (Sh::kBuffers == 2 && following.t >= 0) fetch(following.t, buf ^ 1);
             const char* kt = lds + buf * Sh::kBuf;
             const char* vt = kt + Sh::kTileBytes;
             const int32_t* docs = (const int32_t*)(vt + Sh::kTileBytes);
             const uint32_t ka = lds_address(kt) + (KEYS ? wave * 32 * Tl::kRowBytes : 0), va = ka + Sh::kTileBytes;
-            const int sub0 = KEYS ? wave * 32 : 0, key0 = cur * Sh::kTile + sub0, key1 = key0 + Sh::kWaveKeys - 1;
+            const int sub0 = KEYS ? wave * 32 : 0, key0 = cur.t * Sh::kTile + sub0, key1 = key0 + Sh::kWaveKeys - 1;
             bool in = key0 <= w.hi_max && key1 >= w.lo_min, full = key0 >= w.lo_max && key1 <= w.hi_min;
             if (a.docs) {
-                const int d0 = doc_min[cur], d1 = doc_max[cur];
-                in = in && d1 >= w.doc_min && d0 <= w.doc_max;
-                full = full && d0 == d1 && d0 == w.doc_min && d0 == w.doc_max;
+                in = in && cur.doc_max >= w.doc_min && cur.doc_min <= w.doc_max;
+                full = full && cur.doc_min == cur.doc_max && cur.doc_min == w.doc_min && cur.doc_min == w.doc_max;
             }
             if (in) {
+                const typename Tl::Rows k_rows(ln, ka);
+                const typename Tl::Cols v_cols(ln, va);
                 f32x16_t x[kSub];
 #pragma unroll
                 for (int u = 0; u < kSub; ++u) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) x[u][i] = 0.f;
 #pragma unroll
-                    for (int ks = 0; ks < kSteps; ++ks) mma(x[u], Tl::frag(ka, ln, u * 32, ks), qf[ks]);
+                    for (int ks = 0; ks < kSteps; ++ks) mma(x[u], Tl::frag(k_rows, u * 32, ks), qf[ks]);
                 }
+                if (sizeof(T) == 2) read_ahead<1, 1, kSub * kSteps, 2>();
                 if (PLAIN) {
                 } else if (sc.cap2 > 0.f) {
 #pragma unroll
@@ -192,15 +204,29 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
                 }
                 if (!full) {
                     const int from = span.lo - key0 - 4 * hi;  // the lane's first key is 0
+                    const uint32_t seen_keys = (uint32_t)key_span;
 #pragma unroll
                     for (int u = 0; u < kSub; ++u)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int at = u * 32 + 8 * (i / 4) + i % 4;
-                            bool see = key_span >= 0 && (uint32_t)(at - from) <= (uint32_t)key_span;
-                            if (a.docs) see = see && docs[sub0 + at + 4 * hi] == span.doc;
-                            x[u][i] = see ? x[u][i] : -INFINITY;
-                        }
+                        for (int i = 0; i < 16; ++i)
+                            x[u][i] = (uint32_t)(u * 32 + 8 * (i / 4) + i % 4 - from) <= seen_keys ? x[u][i] : -INFINITY;
+                    if (key_span < 0) {
+#pragma unroll
+                        for (int u = 0; u < kSub; ++u)
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) x[u][i] = -INFINITY;
+                    }
+                    if (a.docs) {
+                        typedef __attribute__((ext_vector_type(4))) int i32x4_t;
+#pragma unroll
+                        for (int u = 0; u < kSub; ++u)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const i32x4_t d = *(const i32x4_t*)(docs + sub0 + u * 32 + 8 * j + 4 * hi);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) x[u][4 * j + i] = d[i] == span.doc ? x[u][4 * j + i] : -INFINITY;
+                            }
+                    }
                 }
                 float mx = x[0][0];
 #pragma unroll
@@ -231,11 +257,12 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
                     const Frag<T> p = to_frag<T>(x[st / 2], st & 1);
 #pragma unroll
                     for (int t = 0; t < kCols; ++t) {
-                        Frag<T> v = Tl::frag_t(va, ln, 16 * st, t);
+                        Frag<T> v = Tl::frag_t(v_cols, 16 * st, t);
                         if (kCareful) zero_not_finite(v);
                         mma(o[t], v, p);
                     }
                 }
+                if (sizeof(T) == 2 && !kCareful) read_ahead<2, 1, 2 * kSub * kCols, 2>();
                 if (kCareful) {
                     bool bad = false;
                     if (lane < Sh::kWaveKeys) bad = Tl::row_not_finite(vt, sub0 + lane);
@@ -255,9 +282,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
             cur = following;
             if (Sh::kBuffers == 2) {
                 buf ^= 1;
-            } else if (cur >= 0) {
+            } else if (cur.t >= 0) {
                 __syncthreads();
-                fetch(cur, 0);
+                fetch(cur.t, 0);
             }
         }
     };

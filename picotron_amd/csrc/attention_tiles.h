@@ -32,6 +32,20 @@ __device__ __forceinline__ void mma(f32x16_t& c, const Frag<float>& a, const Fra
     for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[e], b.v[e], c, 0, 0, 0);
 }
 
+// Order of a run of STEPS steps of READS LDS reads and MFMAS products each: the reads AHEAD steps in front of the products that take
+// them.  Left to itself the compiler reads, waits and multiplies step by step, and two wavefronts per SIMD do not hide that.
+template <int READS, int MFMAS, int STEPS, int AHEAD>
+__device__ __forceinline__ void read_ahead() {
+    constexpr int kRead = 0x100, kMfma = 0x8;
+    __builtin_amdgcn_sched_group_barrier(kRead, READS * AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < STEPS - AHEAD; ++i) {
+        __builtin_amdgcn_sched_group_barrier(kMfma, MFMAS, 0);
+        __builtin_amdgcn_sched_group_barrier(kRead, READS, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(kMfma, MFMAS * AHEAD, 0);
+}
+
 // eight accumulators -> the fragment of the next product.  bf16: P in [0, 2^8] and dx are rounded to bf16 here, a relative
 // error of at most 2^-8 per term of the sums over keys (queries); the normaliser sums the unrounded P.
 template <typename T>
@@ -77,19 +91,34 @@ __device__ __forceinline__ float frag_dot(const Frag<T>& a, const Frag<T>& b) {
     return s;
 }
 
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
+__device__ __forceinline__ const char* uniform(const void* p) {
+    const uint64_t v = (uint64_t)(uintptr_t)p;
+    return (const char*)(uintptr_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
+                                    (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v));
+}
+// keeps the compiler from taking an address apart into what is uniform and what is not, one addition per LDS read
+__device__ __forceinline__ uint32_t whole(uint32_t v) {
+    asm("" : "+v"(v));
+    return v;
+}
+
 // A 16-byte (4-byte) direct-to-LDS load as an instruction sequence that the compiler does not look into: lane l lands at
 // lds + 16 l (4 l); lanes that are switched off leave their place alone.  With the builtin the compiler waits for all loads in
 // front of every LDS read that it cannot prove disjoint, so that nothing would be in flight under the products.  The kernels
 // wait themselves, with lds_loads_done() and a barrier.  M0 is written here and cannot be named as clobbered: nothing else in
 // these kernels may use it (the Makefile looks).
 __device__ __forceinline__ uint32_t lds_address(const char* l) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)l; }
-__device__ __forceinline__ void load16_to_lds(const void* from, char* lds) {
-    const uint32_t at = __builtin_amdgcn_readfirstlane(lds_address(lds));
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory");
+__device__ __forceinline__ void load16_to_lds(const void* from, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(from) : "memory");
 }
-__device__ __forceinline__ void load4_to_lds(const void* from, char* lds) {
-    const uint32_t at = __builtin_amdgcn_readfirstlane(lds_address(lds));
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(at), "v"(from) : "memory");
+__device__ __forceinline__ void load4_to_lds(const void* from, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(from) : "memory");
+}
+// a uniform base and 32 bits of offset per lane: no vector arithmetic for the address
+__device__ __forceinline__ void load16_to_lds(const char* base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(offset), "s"(base) : "memory");
 }
 __device__ __forceinline__ void lds_loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
@@ -138,15 +167,33 @@ struct Tile {
         }
     };
 
-    // rows row0 (a multiple of 32) + lane % 32, elements 16 ks + 8 hi ..; tile: its LDS address
-    __device__ static __forceinline__ Frag<T> frag(uint32_t tile, const Lane& l, int row0, int ks) {
+    // the same in the tile at LDS address `tile`
+    struct Rows {
+        uint32_t at[kGroupCols / 16][kSize / 2];
+        __device__ __forceinline__ Rows(const Lane& l, uint32_t tile) {
+#pragma unroll
+            for (int g = 0; g < kGroupCols / 16; ++g)
+#pragma unroll
+                for (int h = 0; h < kSize / 2; ++h) at[g][h] = whole(l.row[g][h] + tile);
+        }
+    };
+    struct Cols {
+        uint32_t at[2][2];
+        __device__ __forceinline__ Cols(const Lane& l, uint32_t tile) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) at[i / 2][i % 2] = whole(l.col[i / 2][i % 2] + tile);
+        }
+    };
+
+    // rows row0 (a multiple of 32) + lane % 32, elements 16 ks + 8 hi ..
+    __device__ static __forceinline__ Frag<T> frag(const Rows& r, int row0, int ks) {
         constexpr int kPer = kGroupCols / 16;
         Frag<T> f;
         const uint32_t off = row0 * kRowBytes + ks / kPer * kStride;
         if constexpr (kSize == 2) {
-            f.v = *(lds_bf16x8*)(uintptr_t)(tile + l.row[ks % kPer][0] + off);
+            f.v = *(lds_bf16x8*)(uintptr_t)(r.at[ks % kPer][0] + off);
         } else {
-            const f32x4_t a = *(lds_f32x4*)(uintptr_t)(tile + l.row[ks % kPer][0] + off), b = *(lds_f32x4*)(uintptr_t)(tile + l.row[ks % kPer][1] + off);
+            const f32x4_t a = *(lds_f32x4*)(uintptr_t)(r.at[ks % kPer][0] + off), b = *(lds_f32x4*)(uintptr_t)(r.at[ks % kPer][1] + off);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 f.v[i] = a[i];
@@ -157,7 +204,7 @@ struct Tile {
     }
 
     // the tile transposed: column 32 t + lane % 32, rows row0 (a multiple of 16) + {4 hi + 0..3, 8 + 4 hi + 0..3}
-    __device__ static __forceinline__ Frag<T> frag_t(uint32_t tile, const Lane& l, int row0, int t) {
+    __device__ static __forceinline__ Frag<T> frag_t(const Cols& c, int row0, int t) {
         constexpr int kPer = kGroupCols / 32;
         Frag<T> f;
         const uint32_t off = row0 * kRowBytes + t / kPer * kStride;
@@ -165,26 +212,50 @@ struct Tile {
             typedef __attribute__((ext_vector_type(4))) short s16x4_t;
             typedef __attribute__((ext_vector_type(8))) short s16x8_t;
             typedef __attribute__((address_space(3))) s16x4_t lds4;
-            const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(uintptr_t)(tile + l.col[t % kPer][0] + off));
-            const s16x4_t up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(uintptr_t)(tile + l.col[t % kPer][1] + off));
+            const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(uintptr_t)(c.at[t % kPer][0] + off));
+            const s16x4_t up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(uintptr_t)(c.at[t % kPer][1] + off));
             const s16x8_t v = {lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
             f.v = __builtin_bit_cast(bf16x8_t, v);
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f.v[e] = *(lds_f32*)(uintptr_t)(tile + l.col[(e >> 1) & 1][e >> 2] + off + (e & 1) * kRowBytes);
+            for (int e = 0; e < 8; ++e) f.v[e] = *(lds_f32*)(uintptr_t)(c.at[(e >> 1) & 1][e >> 2] + off + (e & 1) * kRowBytes);
         }
         return f;
     }
 
-    // Stages the tile with direct-to-LDS loads of 1 KB: 8 rows of a group.  Columns from D on are left as they are (zeros: clear_lds).
+    // Staging with direct-to-LDS loads of 1 KB, 8 rows of a group each.  Columns from D on are left as they are (zeros: clear_lds).
+    // row_of(r): where row r of the tile is.
     template <typename F>
-    __device__ static __forceinline__ void load(char* tile, int D, F row_of) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __device__ static __forceinline__ void load(uint32_t tile, int D, F row_of) {
+        const int lane = threadIdx.x & 63, wave = wave_index();
 #pragma unroll
         for (int i = 0; i < kGroups * ROWS / 8 / kWaves; ++i) {
             const int unit = i * kWaves + wave, group = unit % kGroups, r0 = unit / kGroups * 8, row = r0 + lane / 8;
             const int chunk = (int)((uint32_t)(lane % 8) ^ swizzle(row)), col = group * kGroupCols + chunk * kPerChunk;
             if (col < D) load16_to_lds(row_of(row) + col, tile + group * kStride + r0 * kRowBytes);
+        }
+    }
+    // The same for rows `stride` bytes apart from base on, D == DP; rows of a tile lie within 2^31 bytes.  A lane's offset depends on the
+    // half of 16 rows, which a wavefront keeps from load to load (kGroups < kWaves) or changes with each.
+    struct Source {
+        uint32_t off[kGroups < kWaves ? 1 : 2];
+        __device__ __forceinline__ explicit Source(uint32_t stride) {
+            const int lane = threadIdx.x & 63;
+#pragma unroll
+            for (int i = 0; i < (kGroups < kWaves ? 1 : 2); ++i) {
+                const int half = kGroups < kWaves ? wave_index() / kGroups & 1 : i;
+                off[i] = lane / 8 * stride + (((uint32_t)(lane % 8) ^ swizzle(8 * half + lane / 8)) << 4);
+            }
+        }
+    };
+    __device__ static __forceinline__ void load_even(uint32_t tile, const char* base, uint32_t stride, const Source& src) {
+        static_assert((kWaves % kGroups == 0 && (kWaves / kGroups) % 2 == 0) || kGroups == kWaves, "a wavefront's half of 16 rows");
+        const int wave = wave_index();
+#pragma unroll
+        for (int i = 0; i < kGroups * ROWS / 8 / kWaves; ++i) {
+            const int unit = i * kWaves + wave, group = unit % kGroups, r0 = unit / kGroups * 8;
+            load16_to_lds(uniform(base + (uint64_t)(r0 * stride) + group * kRowBytes), src.off[kGroups < kWaves ? 0 : i & 1],
+                          tile + group * kStride + r0 * kRowBytes);
         }
     }
     __device__ static __forceinline__ float element(const char* tile, int row, int col) { return to_f32(*(const T*)(tile + at(row, col))); }
@@ -231,14 +302,24 @@ struct PanelTile {
         }
     };
 
-    // rows row0 (a multiple of 32) + lane % 32, elements 16 ks + 8 hi ..; tile: its LDS address
-    __device__ static __forceinline__ Frag<T> frag(uint32_t tile, const Lane& l, int row0, int ks) {
+    // the same in the tile at LDS address `tile`
+    struct Rows {
+        uint32_t at, at2;
+        __device__ __forceinline__ Rows(const Lane& l, uint32_t tile) : at(whole(l.row + tile)), at2(kSize == 2 ? 0 : whole(l.row2 + tile)) {}
+    };
+    struct Cols {
+        uint32_t at, at2;
+        __device__ __forceinline__ Cols(const Lane& l, uint32_t tile) : at(whole(l.col + tile)), at2(whole(l.col2 + tile)) {}
+    };
+
+    // rows row0 (a multiple of 32) + lane % 32, elements 16 ks + 8 hi ..
+    __device__ static __forceinline__ Frag<T> frag(const Rows& r, int row0, int ks) {
         Frag<T> f;
         const uint32_t off = row0 * kRowBytes + ks * kStride;
         if constexpr (kSize == 2) {
-            f.v = *(lds_bf16x8*)(uintptr_t)(tile + l.row + off);
+            f.v = *(lds_bf16x8*)(uintptr_t)(r.at + off);
         } else {
-            const f32x4_t a = *(lds_f32x4*)(uintptr_t)(tile + l.row + off), b = *(lds_f32x4*)(uintptr_t)(tile + l.row2 + off);
+            const f32x4_t a = *(lds_f32x4*)(uintptr_t)(r.at + off), b = *(lds_f32x4*)(uintptr_t)(r.at2 + off);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 f.v[i] = a[i];
@@ -248,42 +329,36 @@ struct PanelTile {
         return f;
     }
 
-    // the same of a tile of OTHER rows, from row 0 on: rows lie alike in all of them
-    template <int OTHER>
-    __device__ static __forceinline__ Frag<T> frag_of(uint32_t tile, const Lane& l, int ks) {
-        return frag(tile + ks * (OTHER - ROWS) * kRowBytes, l, 0, ks);
-    }
-
     // the tile transposed: column 32 t + lane % 32, rows row0 (a multiple of 16) + {4 hi + 0..3, 8 + 4 hi + 0..3}
-    __device__ static __forceinline__ Frag<T> frag_t(uint32_t tile, const Lane& l, int row0, int t) {
+    __device__ static __forceinline__ Frag<T> frag_t(const Cols& c, int row0, int t) {
         Frag<T> f;
         const uint32_t off = row0 * kRowBytes + 2 * t * kStride;
         if constexpr (kSize == 2) {
             typedef __attribute__((ext_vector_type(4))) short s16x4_t;
             typedef __attribute__((ext_vector_type(8))) short s16x8_t;
             typedef __attribute__((address_space(3))) s16x4_t lds4;
-            const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(uintptr_t)(tile + l.col + off));
-            const s16x4_t up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(uintptr_t)(tile + l.col2 + off));
+            const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(uintptr_t)(c.at + off));
+            const s16x4_t up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(uintptr_t)(c.at2 + off));
             const s16x8_t v = {lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
             f.v = __builtin_bit_cast(bf16x8_t, v);
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                f.v[e] = *(lds_f32*)(uintptr_t)(tile + l.col + off + e * kRowBytes);
-                f.v[4 + e] = *(lds_f32*)(uintptr_t)(tile + l.col2 + off + e * kRowBytes);
+                f.v[e] = *(lds_f32*)(uintptr_t)(c.at + off + e * kRowBytes);
+                f.v[4 + e] = *(lds_f32*)(uintptr_t)(c.at2 + off + e * kRowBytes);
             }
         }
         return f;
     }
 
-    // Stages the tile with direct-to-LDS loads of 1 KB, a panel's next 32 (fp32: 16) rows each; a wavefront takes neighbouring
-    // panels, so that the lines it touches are used whole.  Columns from D on are left as they are (zeros: clear_lds).
+    // Staging with direct-to-LDS loads of 1 KB, a panel's next 32 (fp32: 16) rows each; a wavefront takes neighbouring panels, so
+    // that the lines it touches are used whole.  Columns from D on are left as they are (zeros: clear_lds).  row_of(r): where row r is.
+    static constexpr int kLoadRows = 64 / kRowChunks, kMine = kPanels / kWaves;
     template <typename F>
-    __device__ static __forceinline__ void load(char* tile, int D, F row_of) {
-        constexpr int kRows = 64 / kRowChunks, kMine = kPanels / kWaves;
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __device__ static __forceinline__ void load(uint32_t tile, int D, F row_of) {
+        const int lane = threadIdx.x & 63, wave = wave_index();
 #pragma unroll
-        for (int r0 = 0; r0 < ROWS; r0 += kRows) {
+        for (int r0 = 0; r0 < ROWS; r0 += kLoadRows) {
             const int row = r0 + lane / kRowChunks;
             const uint32_t chunk = (uint32_t)(lane % kRowChunks) ^ swizzle(row);
             const char* from = (const char*)row_of(row) + chunk * 16;
@@ -293,6 +368,24 @@ struct PanelTile {
                 if (panel * 16 + (int)chunk * kPerChunk < D) load16_to_lds(from + panel * kRowBytes, tile + panel * kStride + r0 * kRowBytes);
             }
         }
+    }
+    // The same for D == DP and rows at constant offsets from a uniform base: `off(lane's row of the first kLoadRows)`, and r0 rows on
+    // `step(r0)` bytes further.
+    __device__ static __forceinline__ uint32_t lane_offset(uint32_t row_offset) {
+        const int lane = threadIdx.x & 63;
+        return row_offset + (((uint32_t)(lane % kRowChunks) ^ swizzle(lane / kRowChunks)) << 4);
+    }
+    __device__ static __forceinline__ int lane_row() { return (int)(threadIdx.x & 63) / kRowChunks; }
+    template <typename F>
+    __device__ static __forceinline__ void load_even(uint32_t tile, const char* base, uint32_t offset, F step) {
+        const int wave = wave_index();
+#pragma unroll
+        for (int r0 = 0; r0 < ROWS; r0 += kLoadRows)
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+                const int panel = wave * kMine + i;
+                load16_to_lds(uniform(base + step(r0) + panel * kRowBytes), offset, tile + panel * kStride + r0 * kRowBytes);
+            }
     }
     __device__ static __forceinline__ float element(const char* tile, int row, int col) { return to_f32(*(const T*)(tile + at(row, col))); }
     // whether row `row` holds a value that is not finite
@@ -377,22 +470,31 @@ struct Reach {
     int lo_min, lo_max, hi_min, hi_max, doc_min, doc_max;
 };
 
-// The walk over the tiles of [first, end) that pass `active`, 64 at a time, the first `skip` of those left out and `left` taken; the
-// same in every wave of a block.
+// The walk over the tiles of [first, end) that pass `active(t, lowest document, highest document)`, 64 at a time, the first `skip` of
+// those left out and `left` taken; the same in every wave of a block.  The documents of a tile come with it: a load of them where
+// they are needed would wait for the next tile, which is in flight by then.
+struct WalkTile {
+    int t, doc_min, doc_max;  // t < 0: none
+};
 template <typename F>
 struct TileWalk {
     F active;
-    int base, end, skip, left;
+    const int32_t *lowest, *highest;  // NULL: no documents
+    int base, end, skip, left, doc_min, doc_max;
     uint64_t mask;
-    __device__ __forceinline__ TileWalk(int first, int end_, F f, int skip_, int left_)
-        : active(f), base(first - 64), end(end_), skip(skip_), left(left_), mask(0) {}
-    __device__ __forceinline__ int next() {
-        if (left <= 0) return -1;
+    __device__ __forceinline__ TileWalk(int first, int end_, const int32_t* lowest_, const int32_t* highest_, F f, int skip_, int left_)
+        : active(f), lowest(lowest_), highest(highest_), base(first - 64), end(end_), skip(skip_), left(left_), doc_min(0), doc_max(0), mask(0) {}
+    __device__ __forceinline__ WalkTile next() {
+        if (left <= 0) return {-1, 0, 0};
         while (mask == 0) {
             base += 64;
-            if (base >= end) return -1;
-            const int t = base + (int)(threadIdx.x & 63);
-            mask = __ballot(t < end && active(t));
+            if (base >= end) return {-1, 0, 0};
+            const int t = min(base + (int)(threadIdx.x & 63), end - 1);
+            if (lowest) {
+                doc_min = lowest[t];
+                doc_max = highest[t];
+            }
+            mask = __ballot(base + (int)(threadIdx.x & 63) < end && active(t, doc_min, doc_max));
             const int here = __builtin_popcountll(mask);
             if (skip >= here) {
                 skip -= here;
@@ -400,10 +502,10 @@ struct TileWalk {
             }
             for (; skip > 0 && mask; --skip) mask &= mask - 1;
         }
-        const int t = base + __builtin_ctzll(mask);
+        const int lane = __builtin_ctzll(mask);
         mask &= mask - 1;
         --left;
-        return t;
+        return {base + lane, __builtin_amdgcn_readlane(doc_min, lane), __builtin_amdgcn_readlane(doc_max, lane)};
     }
 };
 
@@ -434,13 +536,10 @@ __device__ __forceinline__ void document_range(const int32_t* __restrict__ docs,
 
 // the tiles that a walk passes
 template <typename F>
-__device__ __forceinline__ int count_tiles(int first, int end, F active) {
-    int n = 0;
-    for (int base = first; base < end; base += 64) {
-        const int t = base + (int)(threadIdx.x & 63);
-        n += __builtin_popcountll(__ballot(t < end && active(t)));
-    }
-    return n;
+__device__ __forceinline__ int count_tiles(int first, int end, const int32_t* lowest, const int32_t* highest, F active) {
+    TileWalk<F> walk(first, end, lowest, highest, active, 0x7FFFFFFF, 1);
+    walk.next();
+    return 0x7FFFFFFF - walk.skip;
 }
 // a block's share of its walk: tiles skip .. skip + left - 1 of those that the walk passes
 struct Share {
