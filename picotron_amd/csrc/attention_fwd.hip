@@ -47,7 +47,7 @@ __device__ __forceinline__ void store_out(const AttnArgs& a, int64_t at, f32x4_t
 
 // PLAIN: neither softcap nor slopes, scale > 0: the scale goes into the exponent's multiply-add.
 template <typename T, int DP, bool KEYS, bool PLAIN>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fwd_kernel(MfmaArgs m) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? (DP == 64 && !KEYS ? 3 : 2) : 1) void attention_fwd_kernel(MfmaArgs m) {
     typedef FwdShape<T, DP, KEYS> Sh;
     typedef typename Sh::Tl Tl;
     constexpr int kSub = Sh::kWaveKeys / 32, kSteps = DP / 16, kCols = DP / 32;

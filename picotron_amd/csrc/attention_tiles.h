@@ -547,7 +547,7 @@ struct Share {
 };
 __device__ __forceinline__ Share share_of(int tiles, int split, const MfmaArgs& m) {
     Share s;
-    s.parts = (tiles + m.target - 1) / m.target;
+    s.parts = (tiles + m.target / 2) / m.target;  // a walk a little longer than the target stays whole
     s.parts = s.parts < 1 ? 1 : (s.parts < m.splits ? s.parts : m.splits);
     s.skip = (int)((int64_t)tiles * split / s.parts);
     s.left = (int)((int64_t)tiles * (split + 1) / s.parts) - s.skip;
