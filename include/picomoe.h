@@ -266,7 +266,7 @@ int picomoe_qk_norm_rope_bwd(const void* dq_out, const void* dk_out, const void*
  * NaN and infinities included.  The backward call takes the forward's out and lse; d_out, dq, dk, dv are dense.  out_residual (bf16, dense like
  * out; NULL: none, ignored for fp32): what the rounding of out left, rounded to bf16; with it the backward's d_out . out is exact to
  * 2^-16 instead of 2^-8.  head_dim a multiple
- * of 8, at most 256; strides multiples of 16 bytes, pointers 16-byte aligned; lengths at most 2^28, q_len * q_heads / kv_heads at
+ * of 8, at most 256; strides not negative and multiples of 16 bytes, pointers 16-byte aligned; lengths at most 2^28, q_len * q_heads / kv_heads at
  * most 2^30.  Workspaces: 16-byte aligned, of the size that the _workspace_bytes call gives (-1 = bad arguments). */
 int64_t picomoe_attention_fwd_workspace_bytes(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, int kv_heads,
                                               int head_dim);

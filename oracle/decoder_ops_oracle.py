@@ -125,15 +125,18 @@ def attention(q, k, v, *, causal=True, scale=None, softcap=0.0, window=0, slopes
         return torch.where(mask[..., None], w[..., None] * b[:, :, None], zero).sum(-2)
 
     x = pairs(Q, K) * scale
-    e_z = (D + 4) * U * scale * pairs(Q.abs(), K.abs())
+    size = abs(scale)
+    e_z = (D + 4) * U * size * pairs(Q.abs(), K.abs())
     t = torch.tanh(x / softcap) if softcap else None
     z = softcap * t if softcap else x
     if softcap:
-        e_z = e_z + 16 * U * softcap        # tanh from an exponential and a quotient: absolute error of some steps at 1
+        # tanh from an exponential and a quotient: absolute error of some steps at 1; for large caps, whose scores that would
+        # swamp, tanh itself: some steps of the value
+        e_z = e_z + (16 * U * softcap if softcap <= 1024 else 8 * U * z.abs())
     if slopes is not None:
         away = (torch.arange(Sq, device=q.device)[:, None] + (Sk - Sq) - torch.arange(Sk, device=q.device)[None]).abs().double()
         z = z - slopes.double()[:, None, None] * away
-        e_z = e_z + 2 * U * slopes.double()[:, None, None] * away
+        e_z = e_z + 2 * U * slopes.double().abs()[:, None, None] * away
     e_z = e_z + 6 * U * z.abs()
     top = torch.where(m, z, zero - math.inf).amax(-1, keepdim=True)
     top = torch.where(top == -math.inf, zero, top)
@@ -155,11 +158,11 @@ def attention(q, k, v, *, causal=True, scale=None, softcap=0.0, window=0, slopes
     e_delta = (g.abs() * e_o).sum(-1, keepdim=True) + (D + 2) * U * (g.abs() * o.abs()).sum(-1, keepdim=True)
     slope = (1 - t * t) if softcap else torch.ones_like(x)
     dx = torch.where(m, P * (dP - delta) * slope * scale, zero)
-    raw = torch.where(m, P * scale, zero)
+    raw = torch.where(m, P * size, zero)
     e_dx = raw * slope * ((D + 2) * U * pairs(g.abs(), V.abs()) + e_delta) + (e_p + 8 * U) * dx.abs()
     if softcap:
         e_dx = e_dx + raw * (dP - delta).abs() * (2 * e_z / softcap + 16 * U)
-    e_dx = torch.where(m, e_dx + r * dx.abs() + FLUSH * (1 + scale * (dP - delta).abs()), zero)
+    e_dx = torch.where(m, e_dx + r * dx.abs() + FLUSH * (1 + size * (dP - delta).abs()), zero)
     dq = over(dx, K, m)
     e_dq = r * dq.abs() + over(e_dx + (Sk + 8) * U * dx.abs(), K.abs(), m)
     mt = m.transpose(2, 3)

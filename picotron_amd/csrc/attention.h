@@ -55,7 +55,7 @@ __device__ __forceinline__ RowSpan row_span(const AttnArgs& a, int64_t b, int s)
     if (a.causal) {
         int last = pos;
         if (a.prefix) {
-            const int pre = a.prefix[b] - 1;
+            const int pre = (a.prefix[b] > 0 ? a.prefix[b] : 0) - 1;
             last = pre > last ? pre : last;
         }
         r.hi = last < r.hi ? last : r.hi;

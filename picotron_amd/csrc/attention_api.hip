@@ -16,6 +16,7 @@ bool sizes_ok(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_hea
 bool tensor(AttnTensor* t, const void* p, const int64_t* strides, int dtype) {
     const int64_t vec = dtype == PICOMOE_BF16 ? 8 : 4;  // elements of a 16-byte access
     if (!p || !strides || ((uintptr_t)p & 15) || strides[0] % vec || strides[1] % vec || strides[2] % vec) return false;
+    if (strides[0] < 0 || strides[1] < 0 || strides[2] < 0) return false;  // offsets inside a tile are unsigned
     *t = {p, strides[0], strides[1], strides[2]};
     return true;
 }
@@ -23,7 +24,8 @@ bool tensor(AttnTensor* t, const void* p, const int64_t* strides, int dtype) {
 bool fill(AttnArgs* a, const void* q, const int64_t* qs, const void* k, const int64_t* ks, const void* v, const int64_t* vs, int dtype, int64_t batch,
           int64_t q_len, int64_t kv_len, int q_heads, int kv_heads, int head_dim, float scale, float softcap, int causal, int64_t window,
           const float* slopes, const int32_t* docs, const int32_t* prefix) {
-    if (!(softcap >= 0.f) || softcap > 3e38f || !(scale == scale) || window < 0 || (prefix && !causal)) return false;
+    if (!(softcap >= 0.f) || softcap > 3e38f || !(scale >= -3e38f && scale <= 3e38f) || window < 0 || (prefix && !causal)) return false;
+    if (softcap > 0.f && !((scale < 0.f ? -scale : scale) / softcap < 1e38f)) return false;  // the factor of q . k inside the cap, times 2 log2(e)
     if (!tensor(&a->q, q, qs, dtype)) return false;
     if (kv_len > 0 && (!tensor(&a->k, k, ks, dtype) || !tensor(&a->v, v, vs, dtype))) return false;
     a->dtype = dtype; a->causal = causal != 0; a->batch = batch;

@@ -22,8 +22,7 @@ struct DqShape {
     static constexpr int kLds = 2 * kBuf;
 };
 
-// PLAIN: neither softcap nor slopes
-template <typename T, int DP, bool PLAIN>
+template <typename T, int DP, int MODE>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq_kernel(MfmaArgs m) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     typedef DqShape<T, DP> Sh;
@@ -118,7 +117,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq
     };
 
     const typename Tl::Lane ln;
-    const ScoreScale sc = score_scale<T>(a);
+    const ScoreScale sc = score_scale<MODE>(a);
     f32x16_t dq[kCols];
     auto run = [&](auto careful) __attribute__((always_inline)) {  // CAREFUL: as in the forward, for K
         constexpr bool kCareful = decltype(careful)::value;
@@ -161,11 +160,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq
                     if (sizeof(T) == 2) read_ahead<2, 2, kSteps, 2>();
 #pragma unroll
                     for (int i = 0; i < 16; ++i) dp[i] -= delta;
-                    if (PLAIN) {
+                    if (MODE == kPlain) {
                     } else if (sc.cap2 > 0.f) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            const float t = capped<T>(x[i], sc.mul);
+                            const float t = capped<MODE>(x[i], sc.mul);
                             x[i] = sc.cap2 * t;
                             dp[i] *= 1.f - t * t;
                         }
@@ -173,13 +172,13 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq
 #pragma unroll
                         for (int i = 0; i < 16; ++i) x[i] *= sc.mul;
                     }
-                    if (!PLAIN && a.slopes) {
+                    if (MODE != kPlain && a.slopes) {
                         const float away = (float)(pos - key0 - 4 * hi);
 #pragma unroll
                         for (int i = 0; i < 16; ++i) x[i] -= slope2 * __builtin_fabsf(away - (float)(u * 32 + 8 * (i / 4) + i % 4));
                     }
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i] = __builtin_amdgcn_exp2f(PLAIN ? __builtin_fmaf(x[i], sc.mul, -lse2) : x[i] - lse2) * dp[i];
+                    for (int i = 0; i < 16; ++i) x[i] = __builtin_amdgcn_exp2f(MODE == kPlain ? __builtin_fmaf(x[i], sc.mul, -lse2) : x[i] - lse2) * dp[i];
                     if (!full) {
                         const int from = span.lo - key0 - 4 * hi;
                         const uint32_t seen_keys = (uint32_t)key_span;
@@ -267,7 +266,7 @@ struct DkvShape {
     static constexpr int kLds = 2 * kBuf + kVBytes;
 };
 
-template <typename T, int DP, bool PLAIN>
+template <typename T, int DP, int MODE>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dkv_kernel(MfmaArgs m) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     typedef DkvShape<T, DP> Sh;
@@ -297,7 +296,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
     }
     const int32_t* doc_min = a.docs ? m.row_docs.lowest + (int64_t)b * m.row_docs.tiles : nullptr;
     const int32_t* doc_max = a.docs ? m.row_docs.highest + (int64_t)b * m.row_docs.tiles : nullptr;
-    const int prefix = a.prefix ? a.prefix[b] : 0, off = a.kv_len - a.q_len;
+    const int prefix = a.prefix && a.prefix[b] > 0 ? a.prefix[b] : 0, off = a.kv_len - a.q_len;
     // first and last key of the interval of query s (documents aside): both grow with s
     auto lo_of = [&](int q) { return a.window > 0 ? max(0, q + off - a.window + 1) : 0; };
     auto hi_of = [&](int q) {
@@ -370,7 +369,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
     vl.row = ln.row;
     vl.row2 = ln.row2;
     const typename Sh::VTl::Rows v_rows(vl, vtile + wave * 32 * Tl::kRowBytes);
-    const ScoreScale sc = score_scale<T>(a);
+    const ScoreScale sc = score_scale<MODE>(a);
     f32x16_t dk[kCols], dv[kCols];
     auto run = [&](auto careful) __attribute__((always_inline)) {  // CAREFUL: as in the forward, for Q and dO
         constexpr bool kCareful = decltype(careful)::value;
@@ -423,11 +422,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
 #pragma unroll
                     for (int i = 0; i < 4; ++i) dp[4 * j + i] -= delta[i];
                 }
-                if (PLAIN) {
+                if (MODE == kPlain) {
                 } else if (sc.cap2 > 0.f) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const float t = capped<T>(x[i], sc.mul);
+                        const float t = capped<MODE>(x[i], sc.mul);
                         x[i] = sc.cap2 * t;
                         dp[i] *= 1.f - t * t;
                     }
@@ -435,7 +434,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
 #pragma unroll
                     for (int i = 0; i < 16; ++i) x[i] *= sc.mul;
                 }
-                if (!PLAIN && a.slopes) {
+                if (MODE != kPlain && a.slopes) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const f32x4_t slope2 = stat4(kSlope2, j);
@@ -448,7 +447,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dk
                 for (int j = 0; j < 4; ++j) {
                     const f32x4_t lse2 = stat4(kLse2, j);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) x[4 * j + i] = __builtin_amdgcn_exp2f(PLAIN ? __builtin_fmaf(x[4 * j + i], sc.mul, -lse2[i]) : x[4 * j + i] - lse2[i]);
+                    for (int i = 0; i < 4; ++i) x[4 * j + i] = __builtin_amdgcn_exp2f(MODE == kPlain ? __builtin_fmaf(x[4 * j + i], sc.mul, -lse2[i]) : x[4 * j + i] - lse2[i]);
                 }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) dp[i] *= x[i];
@@ -648,12 +647,12 @@ Plan plan(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, 
     return p;
 }
 
-template <typename T, int DP, bool PLAIN>
+template <typename T, int DP, int MODE>
 int launch(MfmaArgs m, const Plan& p, hipStream_t s) {
     typedef DqShape<T, DP> Q;
     typedef DkvShape<T, DP> K;
-    hipError_t e = allow_lds<attention_dq_kernel<T, DP, PLAIN>>(Q::kLds);
-    if (e == hipSuccess) e = allow_lds<attention_dkv_kernel<T, DP, PLAIN>>(K::kLds);
+    hipError_t e = allow_lds<attention_dq_kernel<T, DP, MODE>>(Q::kLds);
+    if (e == hipSuccess) e = allow_lds<attention_dkv_kernel<T, DP, MODE>>(K::kLds);
     if (e != hipSuccess) return PICOMOE_ERR_HIP_BASE + (int)e;
     const AttnArgs& a = m.a;
     const int64_t heads = a.batch * a.kv_heads, q_quads = a.batch * a.q_len * a.heads * (a.D / 4), k_quads = a.batch * a.kv_len * a.kv_heads * (a.D / 4);
@@ -686,9 +685,9 @@ int launch(MfmaArgs m, const Plan& p, hipStream_t s) {
         return dim3((unsigned)(heads * c.blocks), (unsigned)c.splits);
     };
     const dim3 dkv_grid = use(p.dkv, dkv_parts, dkv_sums);
-    attention_dkv_kernel<T, DP, PLAIN><<<dkv_grid, kThreads, K::kLds, s>>>(m);
+    attention_dkv_kernel<T, DP, MODE><<<dkv_grid, kThreads, K::kLds, s>>>(m);
     const dim3 dq_grid = use(p.dq, dq_parts, dq_sums);
-    attention_dq_kernel<T, DP, PLAIN><<<dq_grid, kThreads, Q::kLds, s>>>(m);
+    attention_dq_kernel<T, DP, MODE><<<dq_grid, kThreads, Q::kLds, s>>>(m);
     JoinArgs j = {};
     unsigned n = 0;
     auto join = [&](void* to, const float* from, const int32_t* parts, int64_t quads, int64_t stride, int length, int of_heads, int group, int rows, int blocks) {
@@ -707,7 +706,11 @@ int launch(MfmaArgs m, const Plan& p, hipStream_t s) {
 
 template <typename T, int DP>
 int launch_for(const MfmaArgs& m, const Plan& p, hipStream_t s) {
-    return m.a.softcap == 0.f && !m.a.slopes ? launch<T, DP, true>(m, p, s) : launch<T, DP, false>(m, p, s);
+    const ScoreMode mode = score_mode(m.a, m.a.softcap == 0.f && !m.a.slopes);
+    if (mode == kPlain) return launch<T, DP, kPlain>(m, p, s);
+    if constexpr (sizeof(T) == 2)
+        if (mode == kFast) return launch<T, DP, kFast>(m, p, s);
+    return launch<T, DP, kAccurate>(m, p, s);
 }
 
 }  // namespace

@@ -45,8 +45,7 @@ __device__ __forceinline__ void store_out(const AttnArgs& a, int64_t at, f32x4_t
     }
 }
 
-// PLAIN: neither softcap nor slopes, scale > 0: the scale goes into the exponent's multiply-add.
-template <typename T, int DP, bool KEYS, bool PLAIN>
+template <typename T, int DP, bool KEYS, int MODE>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? (DP == 64 && !KEYS ? 3 : 2) : 1) void attention_fwd_kernel(MfmaArgs m) {
     typedef FwdShape<T, DP, KEYS> Sh;
     typedef typename Sh::Tl Tl;
@@ -137,7 +136,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? (DP == 64 && !KEYS ? 3 :
     };
 
     const typename Tl::Lane ln;
-    const ScoreScale sc = score_scale<T>(a);
+    const ScoreScale sc = score_scale<MODE>(a);
     f32x16_t o[kCols];
     float top = -INFINITY, total = 0.f;  // running maximum that P refers to (log2 units), this lane's share of the sum
 
@@ -183,19 +182,19 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? (DP == 64 && !KEYS ? 3 :
                     for (int ks = 0; ks < kSteps; ++ks) mma(x[u], Tl::frag(k_rows, u * 32, ks), qf[ks]);
                 }
                 if (sizeof(T) == 2) read_ahead<1, 1, kSub * kSteps, 2>();
-                if (PLAIN) {
+                if (MODE == kPlain) {
                 } else if (sc.cap2 > 0.f) {
 #pragma unroll
                     for (int u = 0; u < kSub; ++u)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) x[u][i] = sc.cap2 * capped<T>(x[u][i], sc.mul);
+                        for (int i = 0; i < 16; ++i) x[u][i] = sc.cap2 * capped<MODE>(x[u][i], sc.mul);
                 } else {
 #pragma unroll
                     for (int u = 0; u < kSub; ++u)
 #pragma unroll
                         for (int i = 0; i < 16; ++i) x[u][i] *= sc.mul;
                 }
-                if (!PLAIN && a.slopes) {
+                if (MODE != kPlain && a.slopes) {
                     const float away = (float)(pos - key0 - 4 * hi);
 #pragma unroll
                     for (int u = 0; u < kSub; ++u)
@@ -233,7 +232,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? (DP == 64 && !KEYS ? 3 :
                 for (int u = 0; u < kSub; ++u)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) mx = __builtin_fmaxf(mx, x[u][i]);
-                mx = other_max(mx) * (PLAIN ? sc.mul : 1.f);
+                mx = other_max(mx) * (MODE == kPlain ? sc.mul : 1.f);
                 if (__any(mx > top + kLazy)) {
                     const float old = top;
                     top = __builtin_fmaxf(top, mx);
@@ -249,7 +248,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? (DP == 64 && !KEYS ? 3 :
                 for (int u = 0; u < kSub; ++u)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        x[u][i] = __builtin_amdgcn_exp2f(PLAIN ? __builtin_fmaf(x[u][i], sc.mul, -base) : x[u][i] - base);
+                        x[u][i] = __builtin_amdgcn_exp2f(MODE == kPlain ? __builtin_fmaf(x[u][i], sc.mul, -base) : x[u][i] - base);
                         total += x[u][i];
                     }
 #pragma unroll
@@ -402,25 +401,32 @@ __global__ __launch_bounds__(kThreads) void attention_documents_kernel(const int
     document_range(docs, kv_len, blockIdx.x, tile, tiles, kv_len, 0, GroupDiv{0u, 0}, lowest, highest);
 }
 
-template <typename T, int DP, bool KEYS, bool PLAIN>
+template <typename T, int DP, bool KEYS, int MODE>
 int launch(const MfmaArgs& m, hipStream_t s) {
     typedef FwdShape<T, DP, KEYS> Sh;
-    const hipError_t e = allow_lds<attention_fwd_kernel<T, DP, KEYS, PLAIN>>(Sh::kLds);
+    const hipError_t e = allow_lds<attention_fwd_kernel<T, DP, KEYS, MODE>>(Sh::kLds);
     if (e != hipSuccess) return PICOMOE_ERR_HIP_BASE + (int)e;
     const int64_t blocks = (int64_t)m.blocks * m.a.batch * m.a.kv_heads;
     if (blocks > 0x7FFFFFFF) return PICOMOE_ERR_TOO_LARGE;
-    attention_fwd_kernel<T, DP, KEYS, PLAIN><<<dim3((unsigned)blocks, (unsigned)m.splits), kThreads, Sh::kLds, s>>>(m);
+    attention_fwd_kernel<T, DP, KEYS, MODE><<<dim3((unsigned)blocks, (unsigned)m.splits), kThreads, Sh::kLds, s>>>(m);
     if (m.splits > 1) {
         const int64_t rows = (int64_t)m.a.batch * m.a.kv_heads * m.rows;
         attention_join_kernel<T><<<(unsigned)((rows + 7) / 8), kThreads, 0, s>>>(m, Sh::kRows);
     }
     return picomoe_launch_status();
 }
+template <typename T, int DP, bool KEYS>
+int launch_mode(const MfmaArgs& m, hipStream_t s) {
+    // the running maximum is taken of the unscaled products: scale > 0
+    const ScoreMode mode = score_mode(m.a, m.a.softcap == 0.f && !m.a.slopes && m.a.scale > 0.f);
+    if (mode == kPlain) return launch<T, DP, KEYS, kPlain>(m, s);
+    if constexpr (sizeof(T) == 2)
+        if (mode == kFast) return launch<T, DP, KEYS, kFast>(m, s);
+    return launch<T, DP, KEYS, kAccurate>(m, s);
+}
 template <typename T, int DP>
 int launch_for(const MfmaArgs& m, bool keys, hipStream_t s) {
-    const bool plain = m.a.softcap == 0.f && !m.a.slopes && m.a.scale > 0.f;
-    if (keys) return plain ? launch<T, DP, true, true>(m, s) : launch<T, DP, true, false>(m, s);
-    return plain ? launch<T, DP, false, true>(m, s) : launch<T, DP, false, false>(m, s);
+    return keys ? launch_mode<T, DP, true>(m, s) : launch_mode<T, DP, false>(m, s);
 }
 
 struct Plan {

@@ -428,7 +428,14 @@ __device__ __forceinline__ int wave_min_i32(int v) {
     }
     return __builtin_amdgcn_readfirstlane(v);
 }
-__device__ __forceinline__ int wave_max_i32(int v) { return -wave_min_i32(-v); }
+__device__ __forceinline__ int wave_max_i32(int v) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        const int o = __shfl_xor(v, off, 64);
+        v = o > v ? o : v;
+    }
+    return __builtin_amdgcn_readfirstlane(v);
+}
 
 // r / group for the rows of a key head, r < 2^31: a multiplication (exact: mul = floor(2^(31 + shift) / group) + 1, 2^shift >= group)
 struct GroupDiv {
@@ -554,21 +561,28 @@ __device__ __forceinline__ Share share_of(int tiles, int split, const MfmaArgs& 
     return s;
 }
 
-// S in log2 units from q . k.  softcap > 0: cap2 * tanh(x / cap) with tanh(y) = 1 - 2 / (1 + e^(2y)); bf16 takes the hardware's
-// exponential and reciprocal (absolute error some 1e-7 of softcap), fp32 the library's tanh.
+// What becomes of q . k.  kPlain: scale alone, folded into the exponent's multiply-add.  kFast and kAccurate: scale, softcap and slopes,
+// with softcap tanh(y) = 1 - 2 / (1 + e^(2y)) from the hardware's exponential and reciprocal or from the library's tanh.  The first is off
+// by up to some 2^-22 of softcap, which bf16 has room for up to a softcap of 1024 (2^-12 in a score, where P is rounded to 2^-8).
+enum ScoreMode { kPlain, kFast, kAccurate };
+constexpr float kFastCap = 1024.f;
+
 struct ScoreScale {
-    float mul;   // log2(e) * scale, or with softcap: scale / softcap (fp32), 2 log2(e) scale / softcap (bf16)
+    float mul;   // log2(e) * scale, or with softcap: scale / softcap (kAccurate), 2 log2(e) scale / softcap (kFast)
     float cap2;  // softcap * log2(e), 0: none
 };
-template <typename T>
+template <int MODE>
 __device__ __forceinline__ ScoreScale score_scale(const AttnArgs& a) {
-    if (a.softcap > 0.f) return {a.scale / a.softcap * (sizeof(T) == 2 ? 2.f * kLog2e : 1.f), a.softcap * kLog2e};
+    if (MODE != kPlain && a.softcap > 0.f) return {a.scale / a.softcap * (MODE == kFast ? 2.f * kLog2e : 1.f), a.softcap * kLog2e};
     return {a.scale * kLog2e, 0.f};
 }
-template <typename T>
+template <int MODE>
 __device__ __forceinline__ float capped(float x, float mul) {  // tanh(x * scale / softcap)
-    if (sizeof(T) == 2) return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * mul));
+    if (MODE == kFast) return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * mul));
     return tanhf(x * mul);
+}
+inline ScoreMode score_mode(const AttnArgs& a, bool plain) {
+    return plain ? kPlain : (a.dtype == PICOMOE_BF16 && a.softcap <= kFastCap ? kFast : kAccurate);
 }
 
 }  // namespace

@@ -368,7 +368,7 @@ extern "C" int picomoe_qk_norm_rope_fwd(const void* q, const int64_t* q_strides,
                                         int dtype, int64_t batch, int64_t seq, int head_dim, const void* q_weight, const void* k_weight, float eps,
                                         const float* cos, const float* sin, int64_t n_positions, const int64_t* positions, void* q_out, void* k_out,
                                         void* stream) {
-    PICOMOE_CHECK_ARG(valid(dtype, batch, seq, q_heads, k_heads, head_dim) && q_strides && k_strides && n_positions >= 0);
+    PICOMOE_CHECK_ARG(valid(dtype, batch, seq, q_heads, k_heads, head_dim) && q_strides && k_strides && n_positions >= 0 && eps >= 0.f && eps <= 3e38f);
     if (batch == 0 || seq == 0) return PICOMOE_OK;
     Args a = {};
     a.q = {q, nullptr, q_weight, q_out, q_strides[0], q_strides[1], q_strides[2], q_heads};
@@ -391,7 +391,7 @@ extern "C" int picomoe_qk_norm_rope_bwd(const void* dq_out, const void* dk_out, 
                                         const void* q_weight, const void* k_weight, float eps, const float* cos, const float* sin,
                                         int64_t n_positions, const int64_t* positions, void* dq, void* dk, void* dq_weight, void* dk_weight,
                                         void* workspace, int64_t workspace_bytes, void* stream) {
-    PICOMOE_CHECK_ARG(valid(dtype, batch, seq, q_heads, k_heads, head_dim) && q_strides && k_strides && n_positions >= 0);
+    PICOMOE_CHECK_ARG(valid(dtype, batch, seq, q_heads, k_heads, head_dim) && q_strides && k_strides && n_positions >= 0 && eps >= 0.f && eps <= 3e38f);
     PICOMOE_CHECK_ARG((!dq_weight || q_weight) && (!dk_weight || k_weight));
     Args a = {};
     a.q = {q, dq_out, q_weight, dq, q_strides[0], q_strides[1], q_strides[2], q_heads};

@@ -66,7 +66,7 @@ def test_attention_arguments():
     assert fwd(batch=0) == 0 and fwd(q_len=0) == 0
     nan = float("nan")
     for bad in (dict(q=None), dict(q=ODD), dict(qs=None), dict(qs=ODD_STRIDES), dict(ks=ODD_STRIDES), dict(dtype=2), dict(batch=-1), dict(q_len=-1), dict(kv_len=-1),
-                dict(kv_len=(1 << 28) + 1), dict(heads=6), dict(kv_heads=0), dict(heads=8192, kv_heads=1), dict(D=60), dict(D=264), dict(scale=nan),
+                dict(kv_len=(1 << 28) + 1), dict(heads=6), dict(kv_heads=0), dict(heads=8192, kv_heads=1), dict(D=60), dict(D=264), dict(scale=nan), dict(scale=float("inf")),
                 dict(softcap=-1.0), dict(softcap=nan), dict(softcap=float("inf")), dict(window=-1), dict(causal=0, prefix=P), dict(out=None), dict(out=ODD),
                 dict(lse=None), dict(ws=None), dict(ws=ODD), dict(size=0), dict(q_len=1 << 28, heads=32, kv_heads=4)):
         assert fwd(**bad) == 1, bad
@@ -80,6 +80,22 @@ def test_attention_arguments():
 
     for bad in (dict(g=None), dict(g=ODD), dict(out=None), dict(lse=None), dict(dq=None), dict(dv=ODD), dict(size=need - 1), dict(kv_len=0), dict(q_len=0)):
         assert bwd(**bad) == 1, bad
+
+
+def test_values_that_reach_no_kernel():
+    """Strides below zero (offsets inside a tile are unsigned), factors that float32 does not hold, an eps that makes a norm NaN."""
+    lib = _lib.load()
+    for at in range(3):
+        back = (ctypes.c_int64 * 3)(*(-64 if i == at else 64 for i in range(3)))
+        assert lib.picomoe_attention_fwd(P, back, P, STRIDES, P, STRIDES, 1, 2, 4, 4, 4, 4, 64, 0.1, 0.0, 1, 0, None, None, None, P, None, P, P, 1 << 40, None) == 1
+        assert lib.picomoe_attention_fwd(P, STRIDES, P, STRIDES, P, back, 1, 2, 4, 4, 4, 4, 64, 0.1, 0.0, 1, 0, None, None, None, P, None, P, P, 1 << 40, None) == 1
+        assert lib.picomoe_attention_bwd(P, P, STRIDES, P, back, P, STRIDES, P, None, P, 1, 2, 4, 4, 4, 4, 64, 0.1, 0.0, 1, 0, None, None, None, P, P, P, P, 1 << 40, None) == 1
+    assert lib.picomoe_attention_fwd(P, STRIDES, P, STRIDES, P, STRIDES, 1, 2, 4, 4, 4, 4, 64, -1e10, 1e-30, 1, 0, None, None, None, P, None, P, P, 1 << 40, None) == 1
+    for eps in (-1e-5, float("nan"), float("inf")):
+        assert lib.picomoe_qk_norm_rope_fwd(P, STRIDES, 4, P, STRIDES, 4, 1, 2, 4, 64, None, None, eps, P, P, 8, None, P, P, None) == 1
+    for scale in (float("nan"), float("-inf")):
+        assert lib.picomoe_embedding_fwd(P, 1, 10, 64, P, 4, scale, P, None) == 1
+        assert lib.picomoe_embedding_bwd(P, 1, P, 4, 10, 64, scale, -1, P, P, 1 << 30, None) == 1
 
 
 def test_cpu_tensors_are_refused():

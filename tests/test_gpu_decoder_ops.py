@@ -68,6 +68,9 @@ EMBEDDINGS = [
     (BF16, 9000, 11, 2056, 1.0, None, "one"), (FP32, 64, 3, 7, 2.0, None, "one"), (FP32, 65, 3, 5, 2.0, None, "one"), (BF16, 130, 9, 13, 1.5, 8, "few"),
     (BF16, 1000, 50, 64, 1.0, 2, "bad"), (FP32, 1, 5, 4, 1.0, None, "bad"), (BF16, 20000, 511, 16, 1.0, None, "uniform"),
     (BF16, 0, 20, 16, 1.0, None, "uniform"),
+    # sorts of one block (8192 tokens), of blocks of 1, 4 and 16 rounds; digits of one to four passes
+    (BF16, 8192, 600, 8, 1.0, None, "uniform"), (FP32, 8193, 3, 4, 1.0, 1, "uniform"), (BF16, 70000, 40000, 8, 1.0, None, "uniform"),
+    (BF16, 300000, 1000, 8, 1.0, 3, "bad"), (FP32, 300000, 600000, 4, 2.0, None, "few"), (BF16, 500, 1 << 27, 1, 1.0, None, "uniform"),
 ]
 
 
@@ -199,6 +202,9 @@ ATTENTIONS = [
     (BF16, 1, 70, 70, 5, 1, 256, {"softcap": 9.0}), (FP32, 1, 50, 50, 2, 1, 200, {}), (BF16, 1, 64, 64, 2, 2, 24, {"documents": "runs"}),
     (BF16, 4, 1, 500, 8, 2, 128, {}), (FP32, 2, 1, 300, 8, 2, 64, {"window": 100}), (BF16, 2, 5, 1000, 16, 4, 64, {"softcap": 10.0, "documents": "runs"}),
     (BF16, 1, 3, 777, 40, 1, 128, {"slopes": True}), (BF16, 1, 1, 4000, 4, 4, 128, {"causal": False}), (FP32, 1, 2, 2500, 3, 3, 72, {"prefix": 2000}),
+    (BF16, 2, 90, 90, 6, 2, 64, {"softcap": 1e5}), (FP32, 1, 80, 80, 2, 1, 64, {"softcap": 1e7}), (BF16, 1, 140, 140, 2, 1, 128, {"scale": -0.2}),
+    (BF16, 1, 140, 140, 2, 1, 64, {"scale": 0.0}), (BF16, 1, 150, 150, 24, 1, 128, {"window": 33}), (FP32, 1, 1, 900, 1, 1, 128, {"slopes": True, "softcap": 3.0}),
+    (BF16, 1, 33, 3000, 1, 1, 128, {}), (BF16, 1, 1, 130, 33, 1, 64, {"window": 7}), (BF16, 2, 260, 260, 4, 2, 120, {"documents": "runs", "softcap": 6.0}),
     (BF16, 5, 7, 7, 2, 1, 128, {}), (BF16, 1, 700, 700, 12, 4, 128, {"documents": "runs"}), (FP32, 1, 520, 520, 4, 2, 128, {"softcap": 4.0}),
 ]
 
@@ -322,6 +328,84 @@ def test_strides_and_broadcasts(gpu):
     (dk,) = torch.autograd.grad(_ops().attention(q, shared.expand(B, S, G, D), v), shared, g)
     value, bound = want["dk"]
     _within("dk", dk, (value.sum(0, keepdim=True), bound.sum(0, keepdim=True) + 2.0 ** -8 * value.abs().sum(0, keepdim=True)))
+
+
+def test_document_ids_of_any_value(gpu):
+    """The lowest and highest int32 as document ids, in and out of order: negative is padding, every other value is a document."""
+    gen = _gen(6)
+    q, k, v = _qkv(gen, BF16, 1, 300, 300, 4, 2, 64)
+    ids = torch.full((1, 300), 2 ** 31 - 1, device="cuda", dtype=torch.int32)
+    ids[:, 40:90], ids[:, 90:150:3], ids[:, 200:203] = -2 ** 31, 0, -1
+    g = _randn(gen, *q.shape)
+    out = _ops().attention(q, k, v, document_ids=ids)
+    want = O.attention(q.detach(), k.detach(), v.detach(), document_ids=ids, d_out=g)
+    for name, got in zip(("out", "dq", "dk", "dv"), (out.detach(), *torch.autograd.grad(out, (q, k, v), g))):
+        _within(name, got, want[name])
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_rows_far_apart(gpu, D):
+    """Strides of 2^22 elements and more, for which the kernels' 32-bit offsets inside a tile are not used."""
+    gen = _gen(7)
+    far = (1 << 22) + 8
+    keys = _randn(gen, 70 * far // 64, 64).view(-1)
+    k = keys.as_strided((1, 70, 2, D), (0, far, D, 1))
+    v = keys.as_strided((1, 70, 2, D), (0, far, D, 1), 1024)
+    q = keys.as_strided((1, 70, 4, D), (0, D, 2 * far, 1), 4096)
+    g = _randn(gen, 1, 70, 4, D)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    out = _ops().attention(*leaves)
+    want = O.attention(q, k, v, d_out=g)
+    for name, got in zip(("out", "dq", "dk", "dv"), (out.detach(), *torch.autograd.grad(out, leaves, g))):
+        _within(name, got, want[name])
+
+
+def test_a_long_cache(gpu):
+    """Keys and values whose last rows lie beyond 2^31 elements of the tensor: the new token's attention is that of those keys alone."""
+    gen = _gen(8)
+    length, heads, D = 1_060_000, 16, 128   # 2.17e9 elements
+    if torch.cuda.get_device_properties(0).total_memory < 40 << 30:
+        pytest.skip("needs 20 GB")
+    k, v = (torch.zeros(1, length, heads, D, device="cuda", dtype=BF16) for _ in range(2))
+    last = 300
+    k[:, -last:], v[:, -last:] = _randn(gen, 1, last, heads, D), _randn(gen, 1, last, heads, D)
+    q = _randn(gen, 1, 2, 2 * heads, D)
+    got = _ops().attention(q, k, v, window=last - 1)
+    want = O.attention(q, k[:, -last:], v[:, -last:], window=last - 1)["out"]
+    _within("out", got, want)
+
+
+def test_norm_rope_of_a_strided_table(gpu):
+    gen = _gen(3)
+    q, k = _randn(gen, 2, 4, 2, 64), _randn(gen, 2, 4, 1, 64)
+    cos, sin = torch.rand(9, 128, generator=gen, device="cuda")[:, ::2], torch.rand(9, 64, generator=gen, device="cuda")
+    got = _ops().qk_norm_rope(q, k, cos, sin)       # a strided table
+    want = O.norm_rope(q, None, cos, sin, torch.arange(4, device="cuda").expand(2, 4), 1e-5, q)
+    _within("q", got[0], want["out"])
+
+
+def test_prefixes_and_windows_of_any_value(gpu):
+    """Prefix lengths from the lowest int32 to the highest; a window wider than any integer of the kernels."""
+    gen = _gen(9)
+    q, k, v = _qkv(gen, BF16, 5, 90, 130, 4, 2, 64)
+    prefix = torch.tensor([-2 ** 31, -1, 0, 100, 2 ** 31 - 1], device="cuda", dtype=torch.int32)
+    g = _randn(gen, *q.shape)
+    out = _ops().attention(q, k, v, prefix_lengths=prefix, window=1 << 70)
+    want = O.attention(q.detach(), k.detach(), v.detach(), prefix_lengths=prefix.clamp(min=0), d_out=g)
+    for name, got in zip(("out", "dq", "dk", "dv"), (out.detach(), *torch.autograd.grad(out, (q, k, v), g))):
+        _within(name, got, want[name])
+
+
+def test_refused_values(gpu):
+    from picotron_amd._lib import PicomoeError
+
+    q = torch.zeros(1, 2, 2, 64, device="cuda")
+    table = torch.zeros(4, 64, device="cuda")
+    for bad in (lambda: _ops().attention(q, q, q, scale=1e39), lambda: _ops().attention(q, q, q, softcap=1e-50), lambda: _ops().attention(q, q, q, softcap=1e39),
+                lambda: _ops().attention(q, q, q, scale=1e10, softcap=1e-30), lambda: _ops().qk_norm_rope(q, q, table, table, eps=-1e-6),
+                lambda: _ops().qk_norm_rope(q, q, table, table, eps=math.nan), lambda: _ops().embedding(torch.zeros(3, device="cuda", dtype=torch.int64), table, scale=1e39)):
+        with pytest.raises(PicomoeError):
+            bad()
 
 
 def test_refusals(gpu):
