@@ -82,8 +82,9 @@ __device__ __forceinline__ float to_f32<__bf16>(__bf16 v) { return (float)v; }
 
 int attention_simple_fwd(const AttnArgs& a, hipStream_t s);
 int attention_simple_bwd(const AttnArgs& a, hipStream_t s);
-// head_dim up to 128: the MFMA kernels (attention_fwd.hip, attention_bwd.hip)
-bool attention_mfma_supported(int head_dim);
+// The MFMA kernels (attention_fwd.hip, attention_bwd.hip): head_dim up to 128, in bf16 up to 256.  A tile of fp32 rows of 256 and what
+// goes with it are beyond a CU's LDS.
+bool attention_mfma_supported(int dtype, int head_dim);
 int64_t attention_mfma_fwd_workspace(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, int kv_heads, int head_dim);
 int attention_mfma_fwd(const AttnArgs& a, hipStream_t s);
 int64_t attention_mfma_bwd_workspace(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, int kv_heads, int head_dim);

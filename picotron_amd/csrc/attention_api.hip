@@ -41,7 +41,7 @@ bool fill(AttnArgs* a, const void* q, const int64_t* qs, const void* k, const in
 extern "C" int64_t picomoe_attention_fwd_workspace_bytes(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, int kv_heads,
                                                          int head_dim) {
     if (!sizes_ok(dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim)) return -1;
-    return attention_mfma_supported(head_dim) ? attention_mfma_fwd_workspace(dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim) : 16;
+    return attention_mfma_supported(dtype, head_dim) ? attention_mfma_fwd_workspace(dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim) : 16;
 }
 
 extern "C" int picomoe_attention_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
@@ -57,14 +57,14 @@ extern "C" int picomoe_attention_fwd(const void* q, const int64_t* q_strides, co
     PICOMOE_CHECK_ARG(out && lse && (((uintptr_t)out | (uintptr_t)out_residual) & 15) == 0 && workspace && ((uintptr_t)workspace & 15) == 0 &&
                       workspace_bytes >= picomoe_attention_fwd_workspace_bytes(dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim));
     a.out = out; a.residual = dtype == PICOMOE_BF16 ? out_residual : nullptr; a.lse = lse; a.ws = (char*)workspace;
-    if (attention_mfma_supported(head_dim)) return attention_mfma_fwd(a, (hipStream_t)stream);
+    if (attention_mfma_supported(dtype, head_dim)) return attention_mfma_fwd(a, (hipStream_t)stream);
     return attention_simple_fwd(a, (hipStream_t)stream);
 }
 
 extern "C" int64_t picomoe_attention_bwd_workspace_bytes(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, int kv_heads,
                                                          int head_dim) {
     if (!sizes_ok(dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim)) return -1;
-    if (attention_mfma_supported(head_dim)) return attention_mfma_bwd_workspace(dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim);
+    if (attention_mfma_supported(dtype, head_dim)) return attention_mfma_bwd_workspace(dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim);
     return round16(batch * q_len * q_heads * 4) + 16;  // D of the rows
 }
 
@@ -84,6 +84,6 @@ extern "C" int picomoe_attention_bwd(const void* d_out, const void* q, const int
     a.out = (void*)out; a.residual = dtype == PICOMOE_BF16 ? (void*)out_residual : nullptr; a.lse = (float*)lse; a.d_out = d_out; a.dq = dq; a.dk = dk; a.dv = dv;
     a.delta = (float*)workspace;
     a.ws = (char*)workspace;
-    if (attention_mfma_supported(head_dim)) return attention_mfma_bwd(a, (hipStream_t)stream);
+    if (attention_mfma_supported(dtype, head_dim)) return attention_mfma_bwd(a, (hipStream_t)stream);
     return attention_simple_bwd(a, (hipStream_t)stream);
 }

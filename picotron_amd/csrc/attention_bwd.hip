@@ -23,7 +23,7 @@ struct DqShape {
 };
 
 template <typename T, int DP, int MODE>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq_kernel(MfmaArgs m) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void attention_dq_kernel(MfmaArgs m) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     typedef DqShape<T, DP> Sh;
     typedef typename Sh::Tl Tl;
@@ -260,14 +260,14 @@ struct DkvShape {
     typedef PanelTile<T, DP, kKeys> VTl;
     static constexpr int kTileBytes = Tl::kBytes;
     static constexpr int kBuf = 2 * kTileBytes + kStats * kTile * 4;
-    // V's fragments are the ones that do not fit the 256 registers of a lane at head_dim 128 (dk, dv, K, S, dP do): read from LDS
-    static constexpr bool kVInLds = DP == 128;
+    // V's fragments are the ones that do not fit the registers of a lane (dk, dv, K, S, dP do; 256 at head_dim 128, 512 at 256): read from LDS
+    static constexpr bool kVInLds = DP >= 128;
     static constexpr int kVBytes = kVInLds ? VTl::kBytes : 0;
     static constexpr int kLds = 2 * kBuf + kVBytes;
 };
 
 template <typename T, int DP, int MODE>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dkv_kernel(MfmaArgs m) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void attention_dkv_kernel(MfmaArgs m) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     typedef DkvShape<T, DP> Sh;
     typedef typename Sh::Tl Tl;
@@ -562,10 +562,11 @@ __global__ __launch_bounds__(kThreads) void attention_grad_join_kernel(JoinArgs 
 
 // What the two kernels want to know of the rows, D = dO . (out + residual) among it -- a group of lanes per row of a key head, 16 bytes a
 // lane -- and the document ranges of the tiles
-template <typename T>
+constexpr int prepare_lanes(int DP, int per) { return (DP <= 128 ? 128 : DP) / per; }  // of a row
+template <typename T, int DP>
 __global__ __launch_bounds__(kThreads) void attention_prepare_kernel(MfmaArgs m, int delta_blocks, int key_tile, int row_tile, int key_blocks) {
     const AttnArgs& a = m.a;
-    constexpr int kPer = 16 / (int)sizeof(T), kLanes = 128 / kPer, kRows = kThreads / kLanes;
+    constexpr int kPer = 16 / (int)sizeof(T), kLanes = prepare_lanes(DP, kPer), kRows = kThreads / kLanes;
     if ((int)blockIdx.x < delta_blocks) {
         const int blocks = m.row_docs.tiles * 32 / kRows;  // of a key head
         const int bh = blockIdx.x / blocks, row = (blockIdx.x - bh * blocks) * kRows + threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
@@ -657,7 +658,7 @@ int launch(MfmaArgs m, const Plan& p, hipStream_t s) {
     const AttnArgs& a = m.a;
     const int64_t heads = a.batch * a.kv_heads, q_quads = a.batch * a.q_len * a.heads * (a.D / 4), k_quads = a.batch * a.kv_len * a.kv_heads * (a.D / 4);
     const int64_t join_blocks = ((q_quads > k_quads ? q_quads : k_quads) + kThreads - 1) / kThreads;
-    const int64_t delta_blocks = heads * p.row_tiles * 32 / (sizeof(T) == 2 ? 16 : 8);
+    const int64_t delta_blocks = heads * p.row_tiles * 32 / (kThreads / prepare_lanes(DP, 16 / (int)sizeof(T)));
     const int64_t key_ranges = a.docs ? a.batch * range_blocks(p.key_tiles) : 0, row_ranges = a.docs ? a.batch * range_blocks(p.row_tiles) : 0;
     if (heads * p.dq.blocks > 0x7FFFFFFF || heads * p.dkv.blocks > 0x7FFFFFFF || join_blocks > 0x7FFFFFFF ||
         delta_blocks + key_ranges + row_ranges > 0x7FFFFFFF)
@@ -674,7 +675,7 @@ int launch(MfmaArgs m, const Plan& p, hipStream_t s) {
     float *dq_sums = (float*)take(p.dq_bytes), *dkv_sums = (float*)take(p.dkv_bytes);
     m.key_docs = {key_docs, key_docs + a.batch * p.key_tiles, p.key_tiles};
     m.row_docs = {row_docs, row_docs + a.batch * p.row_tiles, p.row_tiles};
-    attention_prepare_kernel<T><<<(unsigned)(delta_blocks + key_ranges + row_ranges), kThreads, 0, s>>>(m, (int)delta_blocks, p.key_tile, 32,
+    attention_prepare_kernel<T, DP><<<(unsigned)(delta_blocks + key_ranges + row_ranges), kThreads, 0, s>>>(m, (int)delta_blocks, p.key_tile, 32,
                                                                                                         (int)key_ranges);
     auto use = [&](const Cut& c, int32_t* parts, float* sums) {
         m.blocks = c.blocks;
@@ -726,6 +727,7 @@ int attention_mfma_bwd(const AttnArgs& a, hipStream_t s) {
     m.a = a;
     m.div = group_div(a.group);
     m.rows = a.q_len * a.group;
+    if (a.D > 128) return launch_for<__bf16, 256>(m, p, s);
     if (a.dtype == PICOMOE_BF16) return a.D <= 64 ? launch_for<__bf16, 64>(m, p, s) : launch_for<__bf16, 128>(m, p, s);
     return a.D <= 64 ? launch_for<float, 64>(m, p, s) : launch_for<float, 128>(m, p, s);
 }

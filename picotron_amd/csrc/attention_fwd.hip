@@ -26,6 +26,7 @@ struct FwdShape {
     static constexpr int kBuffers = kTileBytes <= 36 * 1024 ? 2 : 1;  // two of 128 KB do not fit
     static constexpr int kBuf = 2 * kTileBytes + kTile * 4;       // K, V, document ids
     static constexpr int kLds = kBuffers * kBuf;
+    static constexpr int kWavesPerSimd = sizeof(T) == 4 || DP == 256 ? 1 : (DP == 64 && !KEYS ? 3 : 2);  // as the registers allow
 };
 
 // four elements of out, and of its residual where it is wanted
@@ -46,7 +47,7 @@ __device__ __forceinline__ void store_out(const AttnArgs& a, int64_t at, f32x4_t
 }
 
 template <typename T, int DP, bool KEYS, int MODE>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? (DP == 64 && !KEYS ? 3 : 2) : 1) void attention_fwd_kernel(MfmaArgs m) {
+__global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) void attention_fwd_kernel(MfmaArgs m) {
     typedef FwdShape<T, DP, KEYS> Sh;
     typedef typename Sh::Tl Tl;
     constexpr int kSub = Sh::kWaveKeys / 32, kSteps = DP / 16, kCols = DP / 32;
@@ -367,11 +368,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? (DP == 64 && !KEYS ? 3 :
         }
 }
 
-// Joins the parts of a row: out = sum 2^(lse_i - max) out_i / sum 2^(lse_i - max).  32 lanes per row, four columns a lane.
+// Joins the parts of a row: out = sum 2^(lse_i - max) out_i / sum 2^(lse_i - max).  32 lanes per row, four columns at a time a lane.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void attention_join_kernel(MfmaArgs m, int block_rows) {
     const AttnArgs& a = m.a;
-    const int lane = threadIdx.x & 31, heads = (int)a.batch * a.kv_heads, d = 4 * lane;
+    const int lane = threadIdx.x & 31, heads = (int)a.batch * a.kv_heads;
     const int64_t index = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), per_split = (int64_t)heads * m.rows;
     if (index >= per_split) return;
     const int bh = (int)(index / m.rows), row = (int)(index - (int64_t)bh * m.rows), b = bh / a.kv_heads, kvh = bh - b * a.kv_heads;
@@ -381,19 +382,20 @@ __global__ __launch_bounds__(kThreads) void attention_join_kernel(MfmaArgs m, in
     float top = -INFINITY;
     for (int i = 0; i < parts; ++i) top = __builtin_fmaxf(top, m.part_lse[i * per_split + index]);
     const float base = top == -INFINITY ? 0.f : top;
-    float total = 0.f;
-    f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+    for (int d = 4 * lane; d < a.D; d += 128) {
+        float total = 0.f;
+        f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int i = 0; i < parts; ++i) {
-        const float lse2 = m.part_lse[i * per_split + index];  // -inf: saw no key
-        const float weight = __builtin_amdgcn_exp2f(lse2 - base);
-        total += weight;
-        if (d < a.D) sum += weight * *(const f32x4_t*)(m.part_out + (i * per_split + index) * a.D + d);
+        for (int i = 0; i < parts; ++i) {
+            const float lse2 = m.part_lse[i * per_split + index];  // -inf: saw no key
+            const float weight = __builtin_amdgcn_exp2f(lse2 - base);
+            total += weight;
+            sum += weight * *(const f32x4_t*)(m.part_out + (i * per_split + index) * a.D + d);
+        }
+        if (d == 0) a.lse[((int64_t)b * a.heads + head) * a.q_len + s] = total == 0.f ? -INFINITY : (base + log2f(total)) * (1.f / kLog2e);
+        const int64_t at = (((int64_t)b * a.q_len + s) * a.heads + head) * a.D + d;
+        store_out<T>(a, at, sum * (total == 0.f ? 0.f : 1.f / total));
     }
-    if (lane == 0) a.lse[((int64_t)b * a.heads + head) * a.q_len + s] = total == 0.f ? -INFINITY : (base + log2f(total)) * (1.f / kLog2e);
-    if (d >= a.D) return;
-    const int64_t at = (((int64_t)b * a.q_len + s) * a.heads + head) * a.D + d;
-    store_out<T>(a, at, sum * (total == 0.f ? 0.f : 1.f / total));
 }
 
 __global__ __launch_bounds__(kThreads) void attention_documents_kernel(const int32_t* __restrict__ docs, int kv_len, int tile, int tiles,
@@ -459,7 +461,7 @@ Plan plan(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, 
 
 }  // namespace
 
-bool attention_mfma_supported(int head_dim) { return head_dim <= 128; }
+bool attention_mfma_supported(int dtype, int head_dim) { return head_dim <= (dtype == PICOMOE_BF16 ? 256 : 128); }
 
 int64_t attention_mfma_fwd_workspace(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, int kv_heads, int head_dim) {
     const Plan p = plan(dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim);
@@ -485,6 +487,7 @@ int attention_mfma_fwd(const AttnArgs& a, hipStream_t s) {
         if (blocks > 0x7FFFFFFF) return PICOMOE_ERR_TOO_LARGE;
         attention_documents_kernel<<<(unsigned)blocks, kThreads, 0, s>>>(a.docs, a.kv_len, p.tile, p.key_tiles, lowest, lowest + a.batch * p.key_tiles);
     }
+    if (a.D > 128) return launch_for<__bf16, 256>(m, p.keys, s);
     if (a.dtype == PICOMOE_BF16) return a.D <= 64 ? launch_for<__bf16, 64>(m, p.keys, s) : launch_for<__bf16, 128>(m, p.keys, s);
     return a.D <= 64 ? launch_for<float, 64>(m, p.keys, s) : launch_for<float, 128>(m, p.keys, s);
 }

@@ -205,6 +205,8 @@ ATTENTIONS = [
     (BF16, 2, 90, 90, 6, 2, 64, {"softcap": 1e5}), (FP32, 1, 80, 80, 2, 1, 64, {"softcap": 1e7}), (BF16, 1, 140, 140, 2, 1, 128, {"scale": -0.2}),
     (BF16, 1, 140, 140, 2, 1, 64, {"scale": 0.0}), (BF16, 1, 150, 150, 24, 1, 128, {"window": 33}), (FP32, 1, 1, 900, 1, 1, 128, {"slopes": True, "softcap": 3.0}),
     (BF16, 1, 33, 3000, 1, 1, 128, {}), (BF16, 1, 1, 130, 33, 1, 64, {"window": 7}), (BF16, 2, 260, 260, 4, 2, 120, {"documents": "runs", "softcap": 6.0}),
+    (BF16, 1, 300, 300, 4, 2, 256, {}), (BF16, 2, 1, 700, 8, 2, 256, {}), (BF16, 1, 150, 150, 3, 1, 200, {"documents": "runs"}),
+    (BF16, 1, 5, 2000, 4, 1, 136, {"softcap": 20.0, "slopes": True}), (BF16, 1, 1300, 1300, 2, 1, 256, {"window": 400}), (BF16, 2, 65, 129, 1, 1, 248, {"softcap": 2e3}),
     (BF16, 5, 7, 7, 2, 1, 128, {}), (BF16, 1, 700, 700, 12, 4, 128, {"documents": "runs"}), (FP32, 1, 520, 520, 4, 2, 128, {"softcap": 4.0}),
 ]
 
