@@ -252,7 +252,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void
 // ---------------------------------------------------------------------------------------------------------------
 // dk, dv
 // ---------------------------------------------------------------------------------------------------------------
-template <typename T, int DP>
+// What a launch of the kernel forms.  At head_dim 256 the 256 accumulation registers of a lane hold dk and dv and nothing else, S and dP
+// spill: one launch for each there, which forms S twice (five products instead of four; 8192 tokens, 8 heads over 4: 1.03 + 0.48 ms, together 2.7).
+enum Grads { kDk = 1, kDv = 2, kBoth = 3 };
+
+template <typename T, int DP, int GRADS>
 struct DkvShape {
     static constexpr int kTile = 32;              // rows of a tile
     static constexpr int kKeys = 32 * kWaves;     // keys of a block
@@ -261,15 +265,16 @@ struct DkvShape {
     static constexpr int kTileBytes = Tl::kBytes;
     static constexpr int kBuf = 2 * kTileBytes + kStats * kTile * 4;
     // V's fragments are the ones that do not fit the registers of a lane (dk, dv, K, S, dP do; 256 at head_dim 128, 512 at 256): read from LDS
-    static constexpr bool kVInLds = DP >= 128;
+    static constexpr bool kVInLds = DP >= 128 && (GRADS & kDk);
     static constexpr int kVBytes = kVInLds ? VTl::kBytes : 0;
     static constexpr int kLds = 2 * kBuf + kVBytes;
+    static constexpr int kWavesPerSimd = sizeof(T) == 2 && (DP <= 128 || GRADS == kDv) ? 2 : 1;
 };
 
-template <typename T, int DP, int MODE>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void attention_dkv_kernel(MfmaArgs m) {
+template <typename T, int DP, int MODE, int GRADS>
+__global__ __launch_bounds__(kThreads, (DkvShape<T, DP, GRADS>::kWavesPerSimd)) void attention_dkv_kernel(MfmaArgs m) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    typedef DkvShape<T, DP> Sh;
+    typedef DkvShape<T, DP, GRADS> Sh;
     typedef typename Sh::Tl Tl;
     constexpr int kSteps = DP / 16, kCols = DP / 32, kBuf = Sh::kBuf;
     const AttnArgs& a = m.a;
@@ -333,7 +338,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void
 #pragma unroll
         for (int ks = 0; ks < kSteps; ++ks) {
             kf[ks] = load_frag<T>(k, 16 * ks + 8 * hi, a.D);
-            if (!Sh::kVInLds) vf[ks] = load_frag<T>(v, 16 * ks + 8 * hi, a.D);
+            if (!Sh::kVInLds && (GRADS & kDk)) vf[ks] = load_frag<T>(v, 16 * ks + 8 * hi, a.D);
         }
     }
     const T* qbase = (const T*)a.q.p + b * a.q.sb + (int64_t)(kvh * a.group) * a.q.sh;
@@ -408,11 +413,12 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void
                     mma(x, Tl::frag(q_rows, 0, ks), kf[ks]);
                     if constexpr (Sh::kVInLds) {
                         mma(dp, Tl::frag(g_rows, 0, ks), Sh::VTl::frag(v_rows, 0, ks));
-                    } else {
+                    } else if constexpr (GRADS & kDk) {
                         mma(dp, Tl::frag(g_rows, 0, ks), vf[ks]);
                     }
                 }
-                if (sizeof(T) == 2) read_ahead<Sh::kVInLds ? 3 : 2, 2, kSteps, 2>();
+                constexpr int kProducts = GRADS & kDk ? 2 : 1;
+                if (sizeof(T) == 2) read_ahead<kProducts + Sh::kVInLds, kProducts, kSteps, 2>();
                 typedef __attribute__((ext_vector_type(4))) int i32x4_t;
                 auto stat4 = [&](RowStat which, int j) { return *(const f32x4_t*)(stats + which * Sh::kTile + 8 * j + 4 * hi); };
                 auto stat4i = [&](RowStat which, int j) { return *(const i32x4_t*)(stats + which * Sh::kTile + 8 * j + 4 * hi); };
@@ -468,16 +474,20 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void
                     const Frag<T> p = to_frag<T>(x, st), dx = to_frag<T>(dp, st);
 #pragma unroll
                     for (int t = 0; t < kCols; ++t) {
-                        Frag<T> g = Tl::frag_t(g_cols, 16 * st, t), q = Tl::frag_t(q_cols, 16 * st, t);
-                        if (kCareful) {
-                            zero_not_finite(g);
-                            zero_not_finite(q);
+                        if constexpr (GRADS & kDv) {
+                            Frag<T> g = Tl::frag_t(g_cols, 16 * st, t);
+                            if (kCareful) zero_not_finite(g);
+                            mma(dv[t], g, p);
                         }
-                        mma(dv[t], g, p);
-                        mma(dk[t], q, dx);
+                        if constexpr (GRADS & kDk) {
+                            Frag<T> q = Tl::frag_t(q_cols, 16 * st, t);
+                            if (kCareful) zero_not_finite(q);
+                            mma(dk[t], q, dx);
+                        }
                     }
                 }
-                if (sizeof(T) == 2 && !kCareful) read_ahead<4, 2, 2 * kCols, 2>();
+                constexpr int kGrads = GRADS == kBoth ? 2 : 1;
+                if (sizeof(T) == 2 && !kCareful) read_ahead<2 * kGrads, kGrads, 2 * kCols, 2>();
                 if (kCareful) {
                     const bool bad = Tl::row_not_finite(hi ? gt : qt, lane & 31);
                     for (uint64_t left = __ballot(bad); left; left &= left - 1) {
@@ -520,14 +530,14 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void
             const f32x4_t v = {dv[t][4 * j], dv[t][4 * j + 1], dv[t][4 * j + 2], dv[t][4 * j + 3]};
             if (share.parts > 1) {
                 float* to = m.part_out + ((int64_t)split * 2 * rows + out_row) * a.D + d;
-                *(f32x4_t*)to = u;
-                *(f32x4_t*)(to + rows * a.D) = v;
+                if (GRADS & kDk) *(f32x4_t*)to = u;
+                if (GRADS & kDv) *(f32x4_t*)(to + rows * a.D) = v;
             } else if constexpr (sizeof(T) == 2) {
-                *(u32x2_t*)((T*)a.dk + out_row * a.D + d) = u32x2_t{pack_bf16x2(u[0], u[1]), pack_bf16x2(u[2], u[3])};
-                *(u32x2_t*)((T*)a.dv + out_row * a.D + d) = u32x2_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+                if (GRADS & kDk) *(u32x2_t*)((T*)a.dk + out_row * a.D + d) = u32x2_t{pack_bf16x2(u[0], u[1]), pack_bf16x2(u[2], u[3])};
+                if (GRADS & kDv) *(u32x2_t*)((T*)a.dv + out_row * a.D + d) = u32x2_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
             } else {
-                *(f32x4_t*)((T*)a.dk + out_row * a.D + d) = u;
-                *(f32x4_t*)((T*)a.dv + out_row * a.D + d) = v;
+                if (GRADS & kDk) *(f32x4_t*)((T*)a.dk + out_row * a.D + d) = u;
+                if (GRADS & kDv) *(f32x4_t*)((T*)a.dv + out_row * a.D + d) = v;
             }
         }
 }
@@ -651,9 +661,10 @@ Plan plan(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, 
 template <typename T, int DP, int MODE>
 int launch(MfmaArgs m, const Plan& p, hipStream_t s) {
     typedef DqShape<T, DP> Q;
-    typedef DkvShape<T, DP> K;
     hipError_t e = allow_lds<attention_dq_kernel<T, DP, MODE>>(Q::kLds);
-    if (e == hipSuccess) e = allow_lds<attention_dkv_kernel<T, DP, MODE>>(K::kLds);
+    constexpr int kOne = DP == 256 ? kDk : kBoth, kTwo = DP == 256 ? kDv : kBoth;  // the same: one launch
+    if (e == hipSuccess) e = allow_lds<attention_dkv_kernel<T, DP, MODE, kOne>>(DkvShape<T, DP, kOne>::kLds);
+    if (e == hipSuccess) e = allow_lds<attention_dkv_kernel<T, DP, MODE, kTwo>>(DkvShape<T, DP, kTwo>::kLds);
     if (e != hipSuccess) return PICOMOE_ERR_HIP_BASE + (int)e;
     const AttnArgs& a = m.a;
     const int64_t heads = a.batch * a.kv_heads, q_quads = a.batch * a.q_len * a.heads * (a.D / 4), k_quads = a.batch * a.kv_len * a.kv_heads * (a.D / 4);
@@ -686,7 +697,8 @@ int launch(MfmaArgs m, const Plan& p, hipStream_t s) {
         return dim3((unsigned)(heads * c.blocks), (unsigned)c.splits);
     };
     const dim3 dkv_grid = use(p.dkv, dkv_parts, dkv_sums);
-    attention_dkv_kernel<T, DP, MODE><<<dkv_grid, kThreads, K::kLds, s>>>(m);
+    attention_dkv_kernel<T, DP, MODE, kOne><<<dkv_grid, kThreads, DkvShape<T, DP, kOne>::kLds, s>>>(m);
+    if (kTwo != kOne) attention_dkv_kernel<T, DP, MODE, kTwo><<<dkv_grid, kThreads, DkvShape<T, DP, kTwo>::kLds, s>>>(m);
     const dim3 dq_grid = use(p.dq, dq_parts, dq_sums);
     attention_dq_kernel<T, DP, MODE><<<dq_grid, kThreads, Q::kLds, s>>>(m);
     JoinArgs j = {};
