@@ -15,6 +15,8 @@
 // butterfly over the lanes of a head.  A group of lanes takes some heads of one token, whose table rows it reads once -- in fp32
 // they are twice a bf16 head --, and has the loads of all of them in flight.  Queries and keys go through one launch.  dw is summed
 // in registers over the rows a group walks, joined per block in LDS and over the blocks by a second launch, in a fixed order.
+// Measured, bf16, 8192 tokens x (32 + 8) heads of 128: forward 36 us (168 MB: 4.7 TB/s), backward 58 us (252 MB: 4.3 TB/s) + 5 us for
+// dw; a large copy runs at 4.9 TB/s.  One token of 16 sequences: 6 us, a launch.
 #include "common.h"
 
 namespace {

@@ -16,6 +16,7 @@ import contextlib
 import ctypes
 import functools
 import math
+import warnings
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -240,6 +241,9 @@ def qk_norm_rope(q, k, cos, sin, q_weight=None, k_weight=None, eps=1e-5, positio
 # ------------------------------------------------------------------------------------------------
 # Attention
 # ------------------------------------------------------------------------------------------------
+_warned_generic = set()
+
+
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, scale, softcap, causal, window, slopes, document_ids, prefix_lengths):
@@ -304,7 +308,9 @@ def attention(q, k, v, *, causal=True, scale=None, softcap=0.0, window=0, slopes
     A query sees key j when all of these hold: ``causal`` is off or ``j <= p`` or ``j < prefix_lengths[b]`` (int32 ``[batch]``); ``window``
     is 0 or ``|p - j| < window``; ``document_ids`` (int32 ``[batch, kv_len]``, in any order) is None or
     ``document_ids[b, j] == document_ids[b, p] >= 0`` (negative: padding).  A query that sees nothing gets zeros and no gradient.
-    What a query does not see has no influence on it, NaN and infinities included."""
+    What a query does not see has no influence on it, NaN and infinities included.
+
+    Runs on the matrix pipes, except float32 heads wider than 128 (generic kernels: the same results, a one-time ``RuntimeWarning``)."""
     what = "attention"
     _same_device(what, q, k, v, slopes, document_ids, prefix_lengths)
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
@@ -315,6 +321,10 @@ def attention(q, k, v, *, causal=True, scale=None, softcap=0.0, window=0, slopes
     if G < 1 or H < 1 or H % G:
         _fail(f"{what}: {H} query heads over {G} key heads")
     _check_heads(what, D, q.dtype, ("k", k), ("v", v))
+    if q.dtype == torch.float32 and D > 128 and D not in _warned_generic:
+        _warned_generic.add(D)   # once per width: the results are the same, only the speed is not
+        warnings.warn(f"picotron_amd: float32 attention with head_dim {D} runs the generic kernels, not the matrix pipes (up to 128 does)",
+                      RuntimeWarning, stacklevel=2)
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     softcap, window = float(softcap or 0.0), int(window or 0)
     if not abs(scale) <= 3e38 or not (softcap == 0 or 1e-30 <= softcap <= 3e38) or window < 0:

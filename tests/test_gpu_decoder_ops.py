@@ -398,6 +398,19 @@ def test_prefixes_and_windows_of_any_value(gpu):
         _within(name, got, want[name])
 
 
+def test_wide_float32_heads_are_reported_once(gpu):
+    import warnings
+
+    q = torch.zeros(1, 2, 2, 136, device="cuda")
+    _ops()._warned_generic.discard(136)
+    with pytest.warns(RuntimeWarning, match="head_dim 136"):
+        _ops().attention(q, q, q)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        _ops().attention(q, q, q)
+        _ops().attention(q.to(BF16), q.to(BF16), q.to(BF16))
+
+
 def test_refused_values(gpu):
     from picotron_amd._lib import PicomoeError
 
