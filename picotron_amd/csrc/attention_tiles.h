@@ -8,6 +8,7 @@
 // in the order 16 s + {4 hi + 0..3, 8 + 4 hi + 0..3}; the other operand is read from LDS in that order.  P never passes through LDS.
 #pragma once
 #include "attention.h"
+#include "lds.h"
 
 namespace {
 

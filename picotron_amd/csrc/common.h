@@ -3,8 +3,6 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
-#include <atomic>
-
 #include "../../include/picomoe.h"
 
 #define PICOMOE_CHECK_ARG(cond)                 \
@@ -16,20 +14,6 @@
 static inline int picomoe_launch_status() {
     hipError_t e = hipGetLastError();
     return e == hipSuccess ? PICOMOE_OK : PICOMOE_ERR_HIP_BASE + (int)e;
-}
-
-// lets a kernel have `bytes` of dynamic LDS; asked once per device
-template <auto KERNEL>
-static inline hipError_t allow_lds(int bytes) {
-    static std::atomic<uint64_t> allowed{0};
-    int device = 0;
-    const hipError_t e = hipGetDevice(&device);
-    if (e != hipSuccess) return e;
-    const uint64_t bit = device < 64 ? 1ull << device : 0;
-    if (allowed.load(std::memory_order_relaxed) & bit) return hipSuccess;
-    const hipError_t set = hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (set == hipSuccess) allowed.fetch_or(bit, std::memory_order_relaxed);
-    return set;
 }
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;

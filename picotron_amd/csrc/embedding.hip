@@ -12,7 +12,7 @@
 // Measured, bf16: 32768 tokens, table 131072 x 4096: forward 93 us (537 MB: 5.8 TB/s), sort 23, sums 286 (1.34 GB: 4.7 TB/s), join 16;
 // 8192 tokens, table 32000 x 2048: 11, 21, 44 (165 MB: 3.8 TB/s) and 6.  The sorts are chains of short steps that wait for each other,
 // not bytes.
-#include "common.h"
+#include "lds.h"
 
 namespace {
 
