@@ -109,8 +109,10 @@ class Attention(nn.Module):
         self.softcap = float(getattr(config, "attention_softcap", None) or 0.0)
         self.window = int(getattr(config, "attention_window", None) or 0)
         bias = getattr(config, "attention_bias", None)
-        if bias not in (None, "distance"):
-            raise ValueError(f"attention_bias {bias!r}: None or 'distance'")
+        if not isinstance(bias, str):  # Llama configurations carry a flag of this name for biases of the projections, which are not used here
+            bias = None
+        elif bias != "distance":
+            raise ValueError(f"attention_bias {bias!r}: 'distance' or none")
         # a plain attribute like the rotation tables (no state_dict entry)
         self.slopes = 2.0 ** (-8.0 * torch.arange(1, self.num_heads + 1) / self.num_heads) if bias else None
         self.q_norm = self.k_norm = None

@@ -106,6 +106,17 @@ def test_cpu_tensors_are_refused():
             call()
 
 
+@pytest.mark.parametrize("flag", [None, False, True])
+def test_a_projection_bias_flag_is_no_distance_bias(flag):
+    """Llama configurations carry attention_bias: False; such models are built as without the option."""
+    from picotron_amd.model import Llama
+
+    config = types.SimpleNamespace(vocab_size=50, hidden_size=64, intermediate_size=32, num_attention_heads=4, num_key_value_heads=2, num_hidden_layers=1,
+                                   max_position_embeddings=8, rms_norm_eps=1e-5, rope_theta=10000.0, attention_bias=flag)
+    attention = Llama(config).decoder_layers[0].attention
+    assert not attention.fused and attention.slopes is None
+
+
 def test_model_options():
     from picotron_amd.model import Llama
 
