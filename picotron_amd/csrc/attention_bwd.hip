@@ -8,8 +8,8 @@
 // launch were slower (8.3 ms for what then took 4.7 + 2.3): the registers of the two spill more together.
 //
 // Bound: dq as the forward (MFMAs 55 % of the cycles).  dk / dv, which reads three LDS fragments for two MFMAs and has a tile of 32 rows
-// between barriers, is at 40 %; of its loads, which come from the last-level cache, half the bytes would do no better (walks from the
-// last tile on, in step over an XCD's blocks: -1.5 % at 16384 tokens, +4 % with documents).  Tiles of 64 rows with eight wavefronts
+// between barriers, is at 40 %; its loads, which mostly miss the L2, are not what holds it (walks from the last
+// tile on, in step over an XCD's blocks so that they share them: -1.5 % at 16384 tokens, +4 % with documents).  Tiles of 64 rows with eight wavefronts
 // take 2 % less at 16384 tokens and 23 % more at 4096.
 // Measured, bf16, 16384 causal tokens, 16 over 4 heads of 128: prepare 0.03, dq 1.52 ms = 1085 TFLOP/s of its three products, dk / dv
 // 2.70 ms = 815 of its four, join 0.06; with softcap 1.86 and 3.33.  2048 tokens: 57 + 94 + 20 + 7 us.  2 x 8192 tokens, head_dim 64:
