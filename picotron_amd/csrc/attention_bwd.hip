@@ -50,7 +50,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void
     const float slope2 = a.slopes ? a.slopes[head] * kLog2e : 0.f;
     const int64_t out_row = ((int64_t)b * a.q_len + s) * a.heads + head;
 
-    const bool some = key_span >= 0;
+    const bool some = key_span >= 0, few = sizeof(T) == 2 && __any(some && key_span < kFewKeys - 1);
     Reach w;
     w.lo_min = wave_min_i32(some ? span.lo : 0x7FFFFFFF);
     w.hi_max = wave_max_i32(some ? span.hi : -1);
@@ -59,13 +59,15 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void
     w.doc_min = wave_min_i32(some ? span.doc : 0x7FFFFFFF);
     w.doc_max = wave_max_i32(some ? span.doc : -1);
     Reach blk = w;
+    int blk_few = few;
     {
-        __shared__ int reach[kWaves][4];
+        __shared__ int reach[kWaves][5];
         if (lane == 0) {
             reach[wave][0] = w.lo_min;
             reach[wave][1] = w.hi_max;
             reach[wave][2] = w.doc_min;
             reach[wave][3] = w.doc_max;
+            reach[wave][4] = few;
         }
         __syncthreads();
         for (int i = 0; i < kWaves; ++i) {
@@ -73,11 +75,13 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void
             blk.hi_max = max(blk.hi_max, reach[i][1]);
             blk.doc_min = min(blk.doc_min, reach[i][2]);
             blk.doc_max = max(blk.doc_max, reach[i][3]);
+            blk_few |= reach[i][4];
         }
         blk.lo_min = __builtin_amdgcn_readfirstlane(blk.lo_min);
         blk.hi_max = __builtin_amdgcn_readfirstlane(blk.hi_max);
         blk.doc_min = __builtin_amdgcn_readfirstlane(blk.doc_min);
         blk.doc_max = __builtin_amdgcn_readfirstlane(blk.doc_max);
+        blk_few = __builtin_amdgcn_readfirstlane(blk_few);
     }
     const int32_t* doc_min = a.docs ? m.key_docs.lowest + (int64_t)b * m.key_docs.tiles : nullptr;
     const int32_t* doc_max = a.docs ? m.key_docs.highest + (int64_t)b * m.key_docs.tiles : nullptr;
@@ -127,12 +131,14 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void
     const typename Tl::Lane ln;
     const ScoreScale sc = score_scale<MODE>(a);
     f32x16_t dq[kCols];
-    auto run = [&](auto careful) __attribute__((always_inline)) {  // CAREFUL: as in the forward, for K
-        constexpr bool kCareful = decltype(careful)::value;
+    auto run = [&](auto which) __attribute__((always_inline)) {
+        constexpr Walk kWalk = decltype(which)::value;
+        if (kWalk != kRest) {
 #pragma unroll
-        for (int t = 0; t < kCols; ++t)
+            for (int t = 0; t < kCols; ++t)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) dq[t][i] = 0.f;
+                for (int i = 0; i < 16; ++i) dq[t][i] = 0.f;
+        }
         TileWalk<decltype(active)> walk(first, end, doc_min, doc_max, active, share.skip, share.left);
         WalkTile cur = walk.next();
         int buf = 0;
@@ -152,6 +158,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void
                 in = in && cur.doc_max >= w.doc_min && cur.doc_min <= w.doc_max;
                 full = full && cur.doc_min == cur.doc_max && cur.doc_min == w.doc_min && cur.doc_min == w.doc_max;
             }
+            if (kWalk == kRest) in = in && few;
             if (in) {
                 const typename Tl::Rows k_rows(ln, ka), v_rows(ln, va);
                 const typename Tl::Cols k_cols(ln, ka);
@@ -203,19 +210,20 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void
                             }
                         }
                     }
+                    if constexpr (kWalk == kRest) take_rest(x);
 #pragma unroll
                     for (int st = 0; st < 2; ++st) {
                         const Frag<T> dx = to_frag<T>(x, st);
 #pragma unroll
                         for (int t = 0; t < kCols; ++t) {
                             Frag<T> k = Tl::frag_t(k_cols, u * 32 + 16 * st, t);
-                            if (kCareful) zero_not_finite(k);
+                            if (kWalk != kMain) zero_not_finite(k);
                             mma(dq[t], k, dx);
                         }
                     }
-                    if (sizeof(T) == 2 && !kCareful) read_ahead<2, 1, 2 * kCols, 3>();
+                    if (sizeof(T) == 2 && kWalk == kMain) read_ahead<2, 1, 2 * kCols, 3>();
                 }
-                if (kCareful) {
+                if (kWalk == kCareful) {
                     bool bad = false;
                     if (lane < Sh::kTile) bad = Tl::row_not_finite(kt, lane);
                     for (uint64_t left = __ballot(bad); left; left &= left - 1) {
@@ -235,12 +243,18 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void
             buf ^= 1;
         }
     };
-    run(std::integral_constant<bool, false>());
+    run(std::integral_constant<Walk, kMain>());
     lds_loads_done();  // also where no tile was walked: nothing may land in LDS after the block is gone
     bool bad = false;
 #pragma unroll
     for (int t = 0; t < kCols; ++t) bad |= not_finite(dq[t]);
-    if (__syncthreads_or(bad)) run(std::integral_constant<bool, true>());
+    if (__syncthreads_or(bad)) {
+        run(std::integral_constant<Walk, kCareful>());
+        __syncthreads();
+    }
+    if constexpr (sizeof(T) == 2) {
+        if (blk_few) run(std::integral_constant<Walk, kRest>());
+    }
 
     if (!row_in) return;
     T* to = (T*)a.dq + out_row * a.D;
@@ -384,12 +398,14 @@ __global__ __launch_bounds__(kThreads, (DkvShape<T, DP, GRADS>::kWavesPerSimd)) 
     const typename Sh::VTl::Rows v_rows(vl, vtile + wave * 32 * Tl::kRowBytes);
     const ScoreScale sc = score_scale<MODE>(a);
     f32x16_t dk[kCols], dv[kCols];
-    auto run = [&](auto careful) __attribute__((always_inline)) {  // CAREFUL: as in the forward, for Q and dO
-        constexpr bool kCareful = decltype(careful)::value;
+    auto run = [&](auto which, auto active, Share share) __attribute__((always_inline)) {
+        constexpr Walk kWalk = decltype(which)::value;
+        if (kWalk != kRest) {
 #pragma unroll
-        for (int t = 0; t < kCols; ++t)
+            for (int t = 0; t < kCols; ++t)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) dk[t][i] = dv[t][i] = 0.f;
+                for (int i = 0; i < 16; ++i) dk[t][i] = dv[t][i] = 0.f;
+        }
         TileWalk<decltype(active)> walk(0, row_tiles, doc_min, doc_max, active, share.skip, share.left);
         WalkTile cur = walk.next();
         int buf = 0;
@@ -477,6 +493,10 @@ __global__ __launch_bounds__(kThreads, (DkvShape<T, DP, GRADS>::kWavesPerSimd)) 
                         }
                     }
                 }
+                if constexpr (kWalk == kRest) {
+                    take_rest(x);
+                    take_rest(dp);
+                }
 #pragma unroll
                 for (int st = 0; st < 2; ++st) {
                     const Frag<T> p = to_frag<T>(x, st), dx = to_frag<T>(dp, st);
@@ -484,19 +504,19 @@ __global__ __launch_bounds__(kThreads, (DkvShape<T, DP, GRADS>::kWavesPerSimd)) 
                     for (int t = 0; t < kCols; ++t) {
                         if constexpr (GRADS & kDv) {
                             Frag<T> g = Tl::frag_t(g_cols, 16 * st, t);
-                            if (kCareful) zero_not_finite(g);
+                            if (kWalk != kMain) zero_not_finite(g);
                             mma(dv[t], g, p);
                         }
                         if constexpr (GRADS & kDk) {
                             Frag<T> q = Tl::frag_t(q_cols, 16 * st, t);
-                            if (kCareful) zero_not_finite(q);
+                            if (kWalk != kMain) zero_not_finite(q);
                             mma(dk[t], q, dx);
                         }
                     }
                 }
                 constexpr int kGrads = GRADS == kBoth ? 2 : 1;
-                if (sizeof(T) == 2 && !kCareful) read_ahead<2 * kGrads, kGrads, 2 * kCols, 2>();
-                if (kCareful) {
+                if (sizeof(T) == 2 && kWalk == kMain) read_ahead<2 * kGrads, kGrads, 2 * kCols, 2>();
+                if (kWalk == kCareful) {
                     const bool bad = Tl::row_not_finite(hi ? gt : qt, lane & 31);
                     for (uint64_t left = __ballot(bad); left; left &= left - 1) {
                         const int which = __builtin_ctzll(left), r = which & 31;
@@ -519,12 +539,23 @@ __global__ __launch_bounds__(kThreads, (DkvShape<T, DP, GRADS>::kWavesPerSimd)) 
             buf ^= 1;
         }
     };
-    run(std::integral_constant<bool, false>());
+    run(std::integral_constant<Walk, kMain>(), active, share);
     lds_loads_done();  // also where no tile was walked: nothing may land in LDS after the block is gone
     bool bad = false;
 #pragma unroll
     for (int t = 0; t < kCols; ++t) bad |= not_finite(dk[t]) || not_finite(dv[t]);
-    if (__syncthreads_or(bad)) run(std::integral_constant<bool, true>());
+    if (__syncthreads_or(bad)) {
+        run(std::integral_constant<Walk, kCareful>(), active, share);
+        __syncthreads();
+    }
+    if constexpr (sizeof(T) == 2) {
+        // without a narrow window only the first keys have such rows; the parts of a cut walk share them
+        if (block0 < kFewKeys || (a.window > 0 && a.window < kFewKeys)) {
+            auto few = [&](int t, int d0, int d1) { return active(t, d0, d1) && hi_of(first_query(t)) - lo_of(first_query(t)) < kFewKeys - 1; };
+            const int tiles = count_tiles(0, row_tiles, doc_min, doc_max, few), skip = tiles * split / share.parts;
+            run(std::integral_constant<Walk, kRest>(), few, Share{share.parts, skip, tiles * (split + 1) / share.parts - skip});
+        }
+    }
 
     if (!key_in) return;
     const int64_t out_row = ((int64_t)b * a.kv_len + key) * a.kv_heads + kvh, rows = a.batch * a.kv_len * a.kv_heads;

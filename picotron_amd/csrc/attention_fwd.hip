@@ -81,7 +81,7 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
 #pragma unroll
     for (int ks = 0; ks < kSteps; ++ks) qf[ks] = load_frag<T>(q, 16 * ks + 8 * hi, a.D);
 
-    const bool some = key_span >= 0;
+    const bool some = key_span >= 0, few = sizeof(T) == 2 && __any(some && key_span < kFewKeys - 1);
     Reach w;
     w.lo_min = wave_min_i32(some ? span.lo : 0x7FFFFFFF);
     w.hi_max = wave_max_i32(some ? span.hi : -1);
@@ -90,13 +90,15 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
     w.doc_min = wave_min_i32(some ? span.doc : 0x7FFFFFFF);
     w.doc_max = wave_max_i32(some ? span.doc : -1);
     Reach blk = w;
+    int blk_few = few;
     if (!KEYS) {
-        __shared__ int reach[kWaves][4];
+        __shared__ int reach[kWaves][5];
         if (lane == 0) {
             reach[wave][0] = w.lo_min;
             reach[wave][1] = w.hi_max;
             reach[wave][2] = w.doc_min;
             reach[wave][3] = w.doc_max;
+            reach[wave][4] = few;
         }
         __syncthreads();
         for (int i = 0; i < kWaves; ++i) {
@@ -104,11 +106,13 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
             blk.hi_max = max(blk.hi_max, reach[i][1]);
             blk.doc_min = min(blk.doc_min, reach[i][2]);
             blk.doc_max = max(blk.doc_max, reach[i][3]);
+            blk_few |= reach[i][4];
         }
         blk.lo_min = __builtin_amdgcn_readfirstlane(blk.lo_min);
         blk.hi_max = __builtin_amdgcn_readfirstlane(blk.hi_max);
         blk.doc_min = __builtin_amdgcn_readfirstlane(blk.doc_min);
         blk.doc_max = __builtin_amdgcn_readfirstlane(blk.doc_max);
+        blk_few = __builtin_amdgcn_readfirstlane(blk_few);
     }
     const int32_t* doc_min = a.docs ? m.key_docs.lowest + (int64_t)b * m.key_docs.tiles : nullptr;
     const int32_t* doc_max = a.docs ? m.key_docs.highest + (int64_t)b * m.key_docs.tiles : nullptr;
@@ -150,16 +154,16 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
     f32x16_t o[kCols];
     float top = -INFINITY, total = 0.f;  // running maximum that P refers to (log2 units), this lane's share of the sum
 
-    // CAREFUL: values of V that are not finite are kept out of the products, where 0 * inf would reach rows that do not see them,
-    // and added one by one to the rows that do
-    auto run = [&](auto careful) __attribute__((always_inline)) {
-        constexpr bool kCareful = decltype(careful)::value;
-        top = -INFINITY;
-        total = 0.f;
+    auto run = [&](auto which) __attribute__((always_inline)) {
+        constexpr Walk kWalk = decltype(which)::value;
+        if (kWalk != kRest) {
+            top = -INFINITY;
+            total = 0.f;
 #pragma unroll
-        for (int t = 0; t < kCols; ++t)
+            for (int t = 0; t < kCols; ++t)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
+                for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
+        }
 
         TileWalk<decltype(active)> walk(first, end, doc_min, doc_max, active, share.skip, share.left);
         WalkTile cur = walk.next();
@@ -180,6 +184,7 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
                 in = in && cur.doc_max >= w.doc_min && cur.doc_min <= w.doc_max;
                 full = full && cur.doc_min == cur.doc_max && cur.doc_min == w.doc_min && cur.doc_min == w.doc_max;
             }
+            if (kWalk == kRest) in = in && few;
             if (in) {
                 const typename Tl::Rows k_rows(ln, ka);
                 const typename Tl::Cols v_cols(ln, va);
@@ -243,7 +248,7 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
 #pragma unroll
                     for (int i = 0; i < 16; ++i) mx = __builtin_fmaxf(mx, x[u][i]);
                 mx = other_max(mx) * (MODE == kPlain ? sc.mul : 1.f);
-                if (__any(mx > top + kLazy)) {
+                if (kWalk != kRest && __any(mx > top + kLazy)) {
                     const float old = top;
                     top = __builtin_fmaxf(top, mx);
                     const float shrink = __builtin_amdgcn_exp2f(old - (top == -INFINITY ? 0.f : top));
@@ -259,20 +264,24 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         x[u][i] = __builtin_amdgcn_exp2f(MODE == kPlain ? __builtin_fmaf(x[u][i], sc.mul, -base) : x[u][i] - base);
-                        total += x[u][i];
+                        if (kWalk != kRest) total += x[u][i];
                     }
+                if constexpr (kWalk == kRest) {
+#pragma unroll
+                    for (int u = 0; u < kSub; ++u) take_rest(x[u]);
+                }
 #pragma unroll
                 for (int st = 0; st < 2 * kSub; ++st) {
                     const Frag<T> p = to_frag<T>(x[st / 2], st & 1);
 #pragma unroll
                     for (int t = 0; t < kCols; ++t) {
                         Frag<T> v = Tl::frag_t(v_cols, 16 * st, t);
-                        if (kCareful) zero_not_finite(v);
+                        if (kWalk != kMain) zero_not_finite(v);
                         mma(o[t], v, p);
                     }
                 }
-                if (sizeof(T) == 2 && !kCareful) read_ahead<2, 1, 2 * kSub * kCols, 2>();
-                if (kCareful) {
+                if (sizeof(T) == 2 && kWalk == kMain) read_ahead<2, 1, 2 * kSub * kCols, 2>();
+                if (kWalk == kCareful) {
                     bool bad = false;
                     if (lane < Sh::kWaveKeys) bad = Tl::row_not_finite(vt, sub0 + lane);
                     for (uint64_t left = __ballot(bad); left; left &= left - 1) {
@@ -297,14 +306,20 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
             }
         }
     };
-    run(std::integral_constant<bool, false>());
+    run(std::integral_constant<Walk, kMain>());
     lds_loads_done();  // also where no tile was walked: nothing may land in LDS after the block is gone
     bool bad = false;
 #pragma unroll
     for (int t = 0; t < kCols; ++t) bad |= not_finite(o[t]);
     if (__syncthreads_or(bad)) {
-        run(std::integral_constant<bool, true>());
+        run(std::integral_constant<Walk, kCareful>());
         __syncthreads();
+    }
+    if constexpr (sizeof(T) == 2) {
+        if (blk_few) {
+            run(std::integral_constant<Walk, kRest>());
+            __syncthreads();
+        }
     }
     total = other_sum(total);
 

@@ -66,6 +66,21 @@ __device__ __forceinline__ Frag<float> to_frag<float>(const f32x16_t& c, int hal
     return f;
 }
 
+// A kernel's walks over its tiles.  kMain.  kCareful, instead of it where its sums are not finite: values that are not finite are kept out
+// of the products, where 0 * inf would reach rows that do not see them, and added one by one to the rows that do.  kRest, bf16, after it:
+// rows with few keys -- the first ones of a sequence, narrow windows -- have a few large P and dx, whose rounding shows in the result as
+// it is, where the many of a long row average it out; what to_frag left of them is added.  6 batches of two tokens have dq to 0.0017 with
+// it, 0.0034 without (the rounding of dq itself: 0.0017).  Such rows have three tiles at most.
+enum Walk { kMain, kCareful, kRest };
+constexpr int kFewKeys = 128;
+__device__ __forceinline__ void take_rest(f32x16_t& c) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float v = c[i] - (float)(__bf16)c[i];
+        c[i] = __builtin_fabsf(v) < INFINITY ? v : 0.f;
+    }
+}
+
 // eight elements of a global row from column col on; zeros from column D on
 template <typename T>
 __device__ __forceinline__ Frag<T> load_frag(const T* row, int col, int D) {
