@@ -332,6 +332,27 @@ def test_strides_and_broadcasts(gpu):
     _within("dk", dk, (value.sum(0, keepdim=True), bound.sum(0, keepdim=True) + 2.0 ** -8 * value.abs().sum(0, keepdim=True)))
 
 
+@pytest.mark.parametrize("B,S,H,G,D,options", [(6, 2, 1, 1, 128, {"slopes": True}), (3, 6, 4, 1, 128, {"window": 2}), (2, 2, 16, 4, 128, {}),
+                                               (7, 15, 2, 2, 120, {"softcap": 36.5}), (2, 45, 4, 1, 24, {"softcap": 49.4}), (1, 300, 2, 1, 64, {"window": 4}),
+                                               (2, 5, 4, 2, 256, {})])
+def test_rows_with_few_keys_are_off_by_their_rounding(gpu, B, S, H, G, D, options):
+    """bf16: P and dx of rows with few keys enter the products in two parts, so that what is left is off by 2^-17 of each term, by fp32 sums and
+    by 2^-16 in d_out . out: some 2^-14 of the result, a tenth of the rms of its own rounding (some 2^-9.2).  With one part the rounding of
+    a row's one or two large dx, as large as the result's own, would add to it: 1.4 times and more."""
+    gen = _gen(12)
+    q, k, v = _qkv(gen, BF16, B, S, S, H, G, D)
+    options = dict(options)
+    if options.pop("slopes", False):
+        options["slopes"] = torch.rand(H, generator=gen, device="cuda")
+    g = _randn(gen, *q.shape)
+    out = _ops().attention(q, k, v, **options)
+    want = O.attention(q.detach(), k.detach(), v.detach(), d_out=g, **options)
+    for name, got in zip(("out", "dq", "dk", "dv"), (out.detach(), *torch.autograd.grad(out, (q, k, v), g))):
+        value = want[name][0]
+        rounding = (value.to(BF16).double() - value).norm()
+        assert (got.double() - value).norm() <= 1.2 * rounding, name
+
+
 def test_document_ids_of_any_value(gpu):
     """The lowest and highest int32 as document ids, in and out of order: negative is padding, every other value is a document."""
     gen = _gen(6)
