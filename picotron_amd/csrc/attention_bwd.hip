@@ -12,8 +12,8 @@
 // tile on, in step over an XCD's blocks so that they share them: -1.5 % at 16384 tokens, +4 % with documents).  Tiles of 64 rows with eight wavefronts
 // take 2 % less at 16384 tokens and 23 % more at 4096.
 // Measured, bf16, 16384 causal tokens, 16 over 4 heads of 128: prepare 0.03, dq 1.52 ms = 1085 TFLOP/s of its three products, dk / dv
-// 2.70 ms = 815 of its four, join 0.06; with softcap 1.86 and 3.33.  2048 tokens: 57 + 94 + 20 + 7 us.  2 x 8192 tokens, head_dim 64:
-// 0.43 and 0.92 ms.  fp32, 4096 tokens, 8 over 2 heads of 128: 0.63 and 0.95 ms = 82 and 73 TFLOP/s.
+// 2.70 ms = 815 of its four, join 0.06; with softcap 1.81 and 3.31.  2048 tokens: 58 + 100 + 20 + 8 us.  2 x 8192 tokens, head_dim 64:
+// 0.42 and 0.96 ms.  fp32, 4096 tokens, 8 over 2 heads of 128: 0.60 and 0.86 ms = 86 and 80 TFLOP/s.
 #include "attention_tiles.h"
 
 namespace {
@@ -275,7 +275,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void
 // dk, dv
 // ---------------------------------------------------------------------------------------------------------------
 // What a launch of the kernel forms.  At head_dim 256 the 256 accumulation registers of a lane hold dk and dv and nothing else, S and dP
-// spill: one launch for each there, which forms S twice (five products instead of four; 8192 tokens, 8 heads over 4: 1.03 + 0.48 ms, together 2.7).
+// spill: one launch for each there, which forms S twice (five products instead of four; 8192 tokens, 8 heads over 4: 0.79 + 0.47 ms, together 2.7).
 enum Grads { kDk = 1, kDv = 2, kBoth = 3 };
 
 template <typename T, int DP, int GRADS>
