@@ -8,6 +8,8 @@
 //
 // The accumulated O is only rescaled when a row's maximum grows by more than 2^8: until then P is at most 2^8 instead of 1,
 // which costs bf16 nothing and fp32 sums nothing, and the 64 multiplications per tile fall away in all but the first tiles.
+// What P refers to is the maximum rounded up to a whole power of two, so that rescaling is exact and commutes with P's rounding to
+// bf16: the walk that adds what that rounding left (kRest) forms P against the last maximum, whichever a tile was rounded against.
 //
 // Bound: the issue of vector instructions.  A wavefront's MFMAs keep the matrix pipe busy for 48 % of the cycles; its softmax takes a
 // vector instruction of every SIMD for as long again, and an MFMA occupies the port that issues them for about half its own time.
@@ -152,7 +154,7 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
     const typename Tl::Lane ln;
     const ScoreScale sc = score_scale<MODE>(a);
     f32x16_t o[kCols];
-    float top = -INFINITY, total = 0.f;  // running maximum that P refers to (log2 units), this lane's share of the sum
+    float top = -INFINITY, total = 0.f;  // what P refers to (log2 units, whole), this lane's share of the sum
 
     auto run = [&](auto which) __attribute__((always_inline)) {
         constexpr Walk kWalk = decltype(which)::value;
@@ -250,7 +252,7 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
                 mx = other_max(mx) * (MODE == kPlain ? sc.mul : 1.f);
                 if (kWalk != kRest && __any(mx > top + kLazy)) {
                     const float old = top;
-                    top = __builtin_fmaxf(top, mx);
+                    top = __builtin_fmaxf(top, __builtin_ceilf(mx));
                     const float shrink = __builtin_amdgcn_exp2f(old - (top == -INFINITY ? 0.f : top));
                     total *= shrink;
 #pragma unroll

@@ -1,0 +1,66 @@
+"""bf16 attention, rows of fewer than 128 keys: what the rounding of P and dx to bf16 leaves is added by a second walk.  The forward keeps
+out and what out's own rounding left, so that its sums can be looked at to 2^-16."""
+
+import pytest
+import torch
+
+from oracle import decoder_ops_oracle as O
+
+pytestmark = pytest.mark.gpu
+
+BF16 = torch.bfloat16
+
+
+def _inputs(seed, batch, q_len, kv_len, heads, kv_heads, D, size=1.0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    shapes = ((q_len, heads), (kv_len, kv_heads), (kv_len, kv_heads), (q_len, heads))
+    q, k, v, g = (torch.randn(batch, n, h, D, generator=gen, device="cuda") for n, h in shapes)
+    q, k = q * size, k * size
+    return [t.to(BF16).requires_grad_(True) for t in (q, k, v)], g.to(BF16)
+
+
+def _sums(out):
+    """out before its rounding, to 2^-16: what the forward keeps for the backward."""
+    residual = out.grad_fn.saved_tensors[4]
+    assert residual.dtype == BF16 and residual.shape == out.shape
+    return out.detach().double() + residual.double()
+
+
+# Terms that enter a sum in two parts are off by 2^-16 at most.  Rows whose maximum moves after a tile has been added form P of that tile a second
+# time, against the last maximum; the two differ by fp32 rounding, some 2^-22, which crosses one of bf16's rounding borders, 2^-7 apart, for one
+# of 2^15 terms, off by 2^-7 then.  Over many rows: sqrt(2^-32 + 2^-15 2^-14) = 2^-14.2 of the sums.  (Where the second forming is of another
+# number than the one that was rounded, 2^-9.3 of those terms is left: 2^-12 to 2^-13 of the sums of rows that cross a tile.)
+LEFT = 2.0 ** -14
+
+
+@pytest.mark.parametrize("window,size", [(20, 1.0), (20, 3.0), (60, 1.0), (60, 3.0), (100, 2.0)])
+@pytest.mark.parametrize("D,batch,q_len,kv_len", [(64, 1, 300, 300), (128, 2, 200, 457), (256, 1, 150, 150), (128, 3, 4, 330)])
+def test_windows_across_tiles(gpu, window, size, D, batch, q_len, kv_len):
+    """Rows whose keys lie in two tiles: their running maximum moves, and that of the rows beside them."""
+    (q, k, v), _ = _inputs(window + D, batch, q_len, kv_len, 4, 2, D, size)
+    out = _call(q, k, v, window=window)
+    value = O.attention(q.detach(), k.detach(), v.detach(), window=window)["out"][0]
+    last = torch.arange(q_len, device="cuda") + kv_len - q_len
+    first = (last - window + 1).clamp(min=0)
+    crossing = first // 64 != last // 64
+    off = _sums(out) - value
+    for rows in (crossing, ~crossing):
+        if rows.any():
+            assert off[:, rows].norm() <= LEFT * value[:, rows].norm(), float(off[:, rows].norm() / value[:, rows].norm())
+
+
+def _call(q, k, v, **options):
+    from picotron_amd import decoder_ops
+
+    return decoder_ops.attention(q, k, v, **options)
+
+
+@pytest.mark.parametrize("size", [1.0, 8.0, 30.0])
+def test_large_scores_in_bf16(gpu, size):
+    """Scores up to thousands: the running maximum is moved many times, by any factor."""
+    (q, k, v), g = _inputs(4, 1, 150, 150, 2, 1, 64, size)
+    out = _call(q, k, v)
+    want = O.attention(q.detach(), k.detach(), v.detach(), d_out=g)
+    for name, got in zip(("out", "dq", "dk", "dv"), (out.detach(), *torch.autograd.grad(out, (q, k, v), g))):
+        value, bound = want[name]
+        assert ((got.double() - value).abs() <= bound + 2.0 ** -126).all(), name
