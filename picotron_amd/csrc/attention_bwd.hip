@@ -549,9 +549,11 @@ __global__ __launch_bounds__(kThreads, (DkvShape<T, DP, GRADS>::kWavesPerSimd)) 
         __syncthreads();
     }
     if constexpr (sizeof(T) == 2) {
-        // without a narrow window only the first keys have such rows; the parts of a cut walk share them
+        // Without a narrow window only the first keys have such rows; the parts of a cut walk share them.  A query's interval grows with the
+        // query and, once its window has left the first key behind, shrinks (at the last keys): the shortest of a tile is at one of its ends.
         if (block0 < kFewKeys || (a.window > 0 && a.window < kFewKeys)) {
-            auto few = [&](int t, int d0, int d1) { return active(t, d0, d1) && hi_of(first_query(t)) - lo_of(first_query(t)) < kFewKeys - 1; };
+            auto keys_of = [&](int q) { return hi_of(q) - lo_of(q); };
+            auto few = [&](int t, int d0, int d1) { return active(t, d0, d1) && min(keys_of(first_query(t)), keys_of(last_query(t))) < kFewKeys - 1; };
             const int tiles = count_tiles(0, row_tiles, doc_min, doc_max, few), skip = tiles * split / share.parts;
             run(std::integral_constant<Walk, kRest>(), few, Share{share.parts, skip, tiles * (split + 1) / share.parts - skip});
         }

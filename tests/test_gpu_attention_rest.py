@@ -64,3 +64,23 @@ def test_large_scores_in_bf16(gpu, size):
     for name, got in zip(("out", "dq", "dk", "dv"), (out.detach(), *torch.autograd.grad(out, (q, k, v), g))):
         value, bound = want[name]
         assert ((got.double() - value).abs() <= bound + 2.0 ** -126).all(), name
+
+
+@pytest.mark.parametrize("S,window,heads,kv_heads,D", [(300, 100, 2, 2, 64), (300, 100, 4, 1, 128), (420, 90, 6, 2, 128), (290, 110, 1, 1, 256)])
+def test_last_rows_of_a_window_without_causality(gpu, S, window, heads, kv_heads, D):
+    """At the end of a sequence a window's rows see fewer and fewer keys: those of fewer than 128 alone have an output gradient, so that dk and dv are
+    their sums.  What is left of terms that enter in two parts, of fp32 sums and of d_out . out (2^-16) is a tenth of the rms of a gradient's own
+    rounding (2^-9.3); terms in one part would add another 2^-9.3."""
+    (q, k, v), g = _inputs(S, 1, S, S, heads, kv_heads, D)
+    p = torch.arange(S, device="cuda")
+    keys = (p + window - 1).clamp(max=S - 1) - (p - window + 1).clamp(min=0) + 1
+    few = (keys < 128) & (p > S // 2)
+    assert 0 < int(few.sum()) < 64
+    g = torch.where(few[None, :, None, None], g, torch.zeros((), device="cuda", dtype=BF16))
+    out = _call(q, k, v, window=window, causal=False)
+    grads = torch.autograd.grad(out, (q, k, v), g)
+    want = O.attention(q.detach(), k.detach(), v.detach(), d_out=g, window=window, causal=False)
+    for name, got in zip(("dq", "dk", "dv"), grads):
+        value = want[name][0]
+        rounding = (value.to(BF16).double() - value).norm()
+        assert (got.double() - value).norm() <= 1.2 * rounding, (name, float((got.double() - value).norm() / rounding))
