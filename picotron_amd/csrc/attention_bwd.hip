@@ -50,39 +50,12 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void
     const float slope2 = a.slopes ? a.slopes[head] * kLog2e : 0.f;
     const int64_t out_row = ((int64_t)b * a.q_len + s) * a.heads + head;
 
-    const bool some = key_span >= 0, few = sizeof(T) == 2 && __any(some && key_span < kFewKeys - 1);
-    Reach w;
-    w.lo_min = wave_min_i32(some ? span.lo : 0x7FFFFFFF);
-    w.hi_max = wave_max_i32(some ? span.hi : -1);
-    w.lo_max = wave_max_i32(some ? span.lo : 0x7FFFFFFF);
-    w.hi_min = wave_min_i32(some ? span.hi : -1);
-    w.doc_min = wave_min_i32(some ? span.doc : 0x7FFFFFFF);
-    w.doc_max = wave_max_i32(some ? span.doc : -1);
-    Reach blk = w;
-    int blk_few = few;
-    {
-        __shared__ int reach[kWaves][5];
-        if (lane == 0) {
-            reach[wave][0] = w.lo_min;
-            reach[wave][1] = w.hi_max;
-            reach[wave][2] = w.doc_min;
-            reach[wave][3] = w.doc_max;
-            reach[wave][4] = few;
-        }
-        __syncthreads();
-        for (int i = 0; i < kWaves; ++i) {
-            blk.lo_min = min(blk.lo_min, reach[i][0]);
-            blk.hi_max = max(blk.hi_max, reach[i][1]);
-            blk.doc_min = min(blk.doc_min, reach[i][2]);
-            blk.doc_max = max(blk.doc_max, reach[i][3]);
-            blk_few |= reach[i][4];
-        }
-        blk.lo_min = __builtin_amdgcn_readfirstlane(blk.lo_min);
-        blk.hi_max = __builtin_amdgcn_readfirstlane(blk.hi_max);
-        blk.doc_min = __builtin_amdgcn_readfirstlane(blk.doc_min);
-        blk.doc_max = __builtin_amdgcn_readfirstlane(blk.doc_max);
-        blk_few = __builtin_amdgcn_readfirstlane(blk_few);
-    }
+    const bool some = key_span >= 0, few = sizeof(T) == 2 && some && has_few(m, b, s, key_span);
+    const Reach w = wave_reach(some, span);
+    int blk_few = __any(few);
+    __shared__ BlockReach reach, few_reach;
+    const Reach blk = block_reach(w, blk_few, reach);
+    if (blk_few) keep_reach(wave_reach(few, span), few_reach);
     const int32_t* doc_min = a.docs ? m.key_docs.lowest + (int64_t)b * m.key_docs.tiles : nullptr;
     const int32_t* doc_max = a.docs ? m.key_docs.highest + (int64_t)b * m.key_docs.tiles : nullptr;
     const bool any = blk.hi_max >= blk.lo_min;
@@ -131,7 +104,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void
     const typename Tl::Lane ln;
     const ScoreScale sc = score_scale<MODE>(a);
     f32x16_t dq[kCols];
-    auto run = [&](auto which) __attribute__((always_inline)) {
+    Reach mine = w;  // the wavefront's rows, for kRest those with few keys
+    int first_tile = 0, last_tile = -1;  // that the walk has met
+    auto run = [&](auto which, auto active, int first, int end, Share share) __attribute__((always_inline)) {
         constexpr Walk kWalk = decltype(which)::value;
         if (kWalk != kRest) {
 #pragma unroll
@@ -141,24 +116,25 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void
         }
         TileWalk<decltype(active)> walk(first, end, doc_min, doc_max, active, share.skip, share.left);
         WalkTile cur = walk.next();
+        if (kWalk != kRest && cur.t >= 0) first_tile = cur.t;
         int buf = 0;
         if (cur.t >= 0) fetch(cur.t, 0);
         while (cur.t >= 0) {
             lds_loads_done();
             __syncthreads();
             const WalkTile following = walk.next();
+            if (kWalk != kRest) last_tile = cur.t;
             if (following.t >= 0) fetch(following.t, buf ^ 1);
             const char* kt = lds + buf * Sh::kBuf;
             const char* vt = kt + Sh::kTileBytes;
             const int32_t* docs = (const int32_t*)(vt + Sh::kTileBytes);
             const uint32_t ka = lds_address(kt), va = ka + Sh::kTileBytes;
             const int key0 = cur.t * Sh::kTile, key1 = key0 + Sh::kTile - 1;
-            bool in = key0 <= w.hi_max && key1 >= w.lo_min, full = key0 >= w.lo_max && key1 <= w.hi_min;
+            bool in = key0 <= mine.hi_max && key1 >= mine.lo_min, full = key0 >= w.lo_max && key1 <= w.hi_min;
             if (a.docs) {
-                in = in && cur.doc_max >= w.doc_min && cur.doc_min <= w.doc_max;
+                in = in && cur.doc_max >= mine.doc_min && cur.doc_min <= mine.doc_max;
                 full = full && cur.doc_min == cur.doc_max && cur.doc_min == w.doc_min && cur.doc_min == w.doc_max;
             }
-            if (kWalk == kRest) in = in && few;
             if (in) {
                 const typename Tl::Rows k_rows(ln, ka), v_rows(ln, va);
                 const typename Tl::Cols k_cols(ln, ka);
@@ -243,17 +219,24 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void
             buf ^= 1;
         }
     };
-    run(std::integral_constant<Walk, kMain>());
+    run(std::integral_constant<Walk, kMain>(), active, first, end, share);
     lds_loads_done();  // also where no tile was walked: nothing may land in LDS after the block is gone
     bool bad = false;
 #pragma unroll
     for (int t = 0; t < kCols; ++t) bad |= not_finite(dq[t]);
     if (__syncthreads_or(bad)) {
-        run(std::integral_constant<Walk, kCareful>());
+        run(std::integral_constant<Walk, kCareful>(), active, first, end, share);
         __syncthreads();
     }
     if constexpr (sizeof(T) == 2) {
-        if (blk_few) run(std::integral_constant<Walk, kRest>());
+        if (blk_few) {
+            mine = kept_reach(few_reach, wave, wave + 1);
+            // of the tiles walked those that the block's rows with few keys see
+            const Reach rest = kept_reach(few_reach, 0, kWaves);
+            auto seen = [&](int, int d0, int d1) { return !a.docs || (d1 >= rest.doc_min && d0 <= rest.doc_max); };
+            run(std::integral_constant<Walk, kRest>(), seen, max(first_tile, rest.lo_min / Sh::kTile), min(last_tile, rest.hi_max / Sh::kTile) + 1,
+                Share{1, 0, 0x7FFFFFFF});
+        }
     }
 
     if (!row_in) return;
@@ -398,7 +381,8 @@ __global__ __launch_bounds__(kThreads, (DkvShape<T, DP, GRADS>::kWavesPerSimd)) 
     const typename Sh::VTl::Rows v_rows(vl, vtile + wave * 32 * Tl::kRowBytes);
     const ScoreScale sc = score_scale<MODE>(a);
     f32x16_t dk[kCols], dv[kCols];
-    auto run = [&](auto which, auto active, Share share) __attribute__((always_inline)) {
+    int first_tile = 0, last_tile = -1;  // that the walk has met
+    auto run = [&](auto which, auto active, int first, int end, Share share) __attribute__((always_inline)) {
         constexpr Walk kWalk = decltype(which)::value;
         if (kWalk != kRest) {
 #pragma unroll
@@ -406,14 +390,16 @@ __global__ __launch_bounds__(kThreads, (DkvShape<T, DP, GRADS>::kWavesPerSimd)) 
 #pragma unroll
                 for (int i = 0; i < 16; ++i) dk[t][i] = dv[t][i] = 0.f;
         }
-        TileWalk<decltype(active)> walk(0, row_tiles, doc_min, doc_max, active, share.skip, share.left);
+        TileWalk<decltype(active)> walk(first, end, doc_min, doc_max, active, share.skip, share.left);
         WalkTile cur = walk.next();
+        if (kWalk != kRest && cur.t >= 0) first_tile = cur.t;
         int buf = 0;
         if (cur.t >= 0) fetch(cur.t, 0);
         while (cur.t >= 0) {
             lds_loads_done();
             __syncthreads();
             const WalkTile following = walk.next();
+            if (kWalk != kRest) last_tile = cur.t;
             if (following.t >= 0) fetch(following.t, buf ^ 1);
             const char* qt = lds + buf * kBuf;
             const char* gt = qt + Sh::kTileBytes;
@@ -539,23 +525,28 @@ __global__ __launch_bounds__(kThreads, (DkvShape<T, DP, GRADS>::kWavesPerSimd)) 
             buf ^= 1;
         }
     };
-    run(std::integral_constant<Walk, kMain>(), active, share);
+    run(std::integral_constant<Walk, kMain>(), active, 0, row_tiles, share);
     lds_loads_done();  // also where no tile was walked: nothing may land in LDS after the block is gone
     bool bad = false;
 #pragma unroll
     for (int t = 0; t < kCols; ++t) bad |= not_finite(dk[t]) || not_finite(dv[t]);
     if (__syncthreads_or(bad)) {
-        run(std::integral_constant<Walk, kCareful>(), active, share);
+        run(std::integral_constant<Walk, kCareful>(), active, 0, row_tiles, share);
         __syncthreads();
     }
     if constexpr (sizeof(T) == 2) {
-        // Without a narrow window only the first keys have such rows; the parts of a cut walk share them.  A query's interval grows with the
-        // query and, once its window has left the first key behind, shrinks (at the last keys): the shortest of a tile is at one of its ends.
-        if (block0 < kFewKeys || (a.window > 0 && a.window < kFewKeys)) {
+        // Without documents and a narrow window only the first keys have such rows.  A query's interval grows with the query and, once its window
+        // has left the first key behind, shrinks (at the last keys): the shortest of a tile is at one of its ends.  The parts of a cut walk take
+        // such tiles in turn, else the first part has all of them (2048 tokens: 106 us, in turn 97); with documents, where the tiles lie here
+        // and there, each those that it has met, else every part looks for them in all tiles (2 x 8192 tokens: 361 us, 331).
+        if (a.docs || block0 < kFewKeys || (a.window > 0 && a.window < kFewKeys)) {
             auto keys_of = [&](int q) { return hi_of(q) - lo_of(q); };
-            auto few = [&](int t, int d0, int d1) { return active(t, d0, d1) && min(keys_of(first_query(t)), keys_of(last_query(t))) < kFewKeys - 1; };
-            const int tiles = count_tiles(0, row_tiles, doc_min, doc_max, few), skip = tiles * split / share.parts;
-            run(std::integral_constant<Walk, kRest>(), few, Share{share.parts, skip, tiles * (split + 1) / share.parts - skip});
+            auto few = [&](int t, int d0, int d1) {
+                if ((!a.docs && share.parts > 1 && t % share.parts != split) || !active(t, d0, d1)) return false;
+                const int q0 = first_query(t), q1 = last_query(t);
+                return m.few ? any_has_few(m, b, q0, q1) : min(keys_of(q0), keys_of(q1)) < kFewKeys - 1;
+            };
+            run(std::integral_constant<Walk, kRest>(), few, a.docs ? first_tile : 0, a.docs ? last_tile + 1 : row_tiles, Share{1, 0, 0x7FFFFFFF});
         }
     }
 
@@ -614,11 +605,11 @@ __global__ __launch_bounds__(kThreads) void attention_grad_join_kernel(JoinArgs 
 // What the two kernels want to know of the rows, D = dO . (out + residual) among it -- a group of lanes per row of a key head, 16 bytes a
 // lane -- and the document ranges of the tiles
 constexpr int prepare_lanes(int DP, int per) { return (DP <= 128 ? 128 : DP) / per; }  // of a row
-template <typename T, int DP>
-__global__ __launch_bounds__(kThreads) void attention_prepare_kernel(MfmaArgs m, int delta_blocks, int key_tile, int row_tile, int key_blocks) {
+template <typename T, int DP, bool DOCS>
+__global__ __launch_bounds__(kThreads) void attention_prepare_kernel(MfmaArgs m, int delta_blocks, int key_tile, int row_tile, int key_blocks, int row_blocks) {
     const AttnArgs& a = m.a;
     constexpr int kPer = 16 / (int)sizeof(T), kLanes = prepare_lanes(DP, kPer), kRows = kThreads / kLanes;
-    if ((int)blockIdx.x < delta_blocks) {
+    if (!DOCS || (int)blockIdx.x < delta_blocks) {
         const int blocks = m.row_docs.tiles * 32 / kRows;  // of a key head
         const int bh = blockIdx.x / blocks, row = (blockIdx.x - bh * blocks) * kRows + threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
         const int at = row < m.rows ? row : m.rows - 1, b = bh / a.kv_heads, s = m.div(at), head = (bh - b * a.kv_heads) * a.group + at - s * a.group;
@@ -655,6 +646,8 @@ __global__ __launch_bounds__(kThreads) void attention_prepare_kernel(MfmaArgs m,
     if (block < key_blocks)
         document_range(a.docs, a.kv_len, block, key_tile, m.key_docs.tiles, a.kv_len, 0, GroupDiv{0u, 0}, (int32_t*)m.key_docs.lowest,
                        (int32_t*)m.key_docs.highest);
+    else if (block - key_blocks >= row_blocks)
+        few_queries(a, block - key_blocks - row_blocks, (uint64_t*)m.few);
     else
         document_range(a.docs, a.kv_len, block - key_blocks, row_tile, m.row_docs.tiles, m.rows, a.kv_len - a.q_len, m.div,
                        (int32_t*)m.row_docs.lowest, (int32_t*)m.row_docs.highest);
@@ -679,7 +672,7 @@ Cut cut(int64_t heads, int64_t blocks, int64_t tiles, int64_t shortest, int64_t 
 struct Plan {
     int key_tile, key_tiles, row_tiles;
     Cut dq, dkv;
-    int64_t key_docs, row_docs, stats_bytes, dq_parts, dkv_parts, dq_bytes, dkv_bytes;
+    int64_t key_docs, row_docs, few_bytes, stats_bytes, dq_parts, dkv_parts, dq_bytes, dkv_bytes;
 };
 Plan plan(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, int kv_heads, int head_dim) {
     Plan p;
@@ -696,6 +689,7 @@ Plan plan(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, 
     p.dkv = cut(heads, (kv_len + per - 1) / per, p.row_tiles, 16, 8 * resident);
     p.key_docs = round16(batch * p.key_tiles * 8);
     p.row_docs = round16(batch * p.row_tiles * 8);
+    p.few_bytes = dtype == PICOMOE_BF16 ? round16(batch * few_words(q_len) * 8) : 0;
     p.stats_bytes = heads * p.row_tiles * (kStats * 32 * 4);
     p.dq_parts = p.dq.splits > 1 ? round16(heads * p.dq.blocks * 4) : 0;
     p.dkv_parts = p.dkv.splits > 1 ? round16(heads * p.dkv.blocks * 4) : 0;
@@ -717,8 +711,10 @@ int launch(MfmaArgs m, const Plan& p, hipStream_t s) {
     const int64_t join_blocks = ((q_quads > k_quads ? q_quads : k_quads) + kThreads - 1) / kThreads;
     const int64_t delta_blocks = heads * p.row_tiles * 32 / (kThreads / prepare_lanes(DP, 16 / (int)sizeof(T)));
     const int64_t key_ranges = a.docs ? a.batch * range_blocks(p.key_tiles) : 0, row_ranges = a.docs ? a.batch * range_blocks(p.row_tiles) : 0;
+    const bool count_few = a.docs && sizeof(T) == 2;
+    const int64_t few_ranges = count_few ? a.batch * few_blocks(a.q_len) : 0, prepare_blocks = delta_blocks + key_ranges + row_ranges + few_ranges;
     if (heads * p.dq.blocks > 0x7FFFFFFF || heads * p.dkv.blocks > 0x7FFFFFFF || join_blocks > 0x7FFFFFFF ||
-        delta_blocks + key_ranges + row_ranges > 0x7FFFFFFF)
+        prepare_blocks > 0x7FFFFFFF)
         return PICOMOE_ERR_TOO_LARGE;
     char* ws = a.ws;
     auto take = [&](int64_t bytes) {
@@ -727,13 +723,16 @@ int launch(MfmaArgs m, const Plan& p, hipStream_t s) {
         return at;
     };
     int32_t *key_docs = (int32_t*)take(p.key_docs), *row_docs = (int32_t*)take(p.row_docs);
+    uint64_t* few = (uint64_t*)take(p.few_bytes);
     int32_t *dq_parts = (int32_t*)take(p.dq_parts), *dkv_parts = (int32_t*)take(p.dkv_parts);
     m.stats = (float*)take(p.stats_bytes);
     float *dq_sums = (float*)take(p.dq_bytes), *dkv_sums = (float*)take(p.dkv_bytes);
     m.key_docs = {key_docs, key_docs + a.batch * p.key_tiles, p.key_tiles};
     m.row_docs = {row_docs, row_docs + a.batch * p.row_tiles, p.row_tiles};
-    attention_prepare_kernel<T, DP><<<(unsigned)(delta_blocks + key_ranges + row_ranges), kThreads, 0, s>>>(m, (int)delta_blocks, p.key_tile, 32,
-                                                                                                        (int)key_ranges);
+    m.few = count_few ? few : nullptr;
+    m.few_words = few_words(a.q_len);
+    const auto prepare = a.docs ? attention_prepare_kernel<T, DP, true> : attention_prepare_kernel<T, DP, false>;
+    prepare<<<(unsigned)prepare_blocks, kThreads, 0, s>>>(m, (int)delta_blocks, p.key_tile, 32, (int)key_ranges, (int)row_ranges);
     auto use = [&](const Cut& c, int32_t* parts, float* sums) {
         m.blocks = c.blocks;
         m.splits = c.splits;
@@ -779,7 +778,7 @@ int launch_for(const MfmaArgs& m, const Plan& p, hipStream_t s) {
 
 int64_t attention_mfma_bwd_workspace(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, int kv_heads, int head_dim) {
     const Plan p = plan(dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim);
-    return p.key_docs + p.row_docs + p.stats_bytes + p.dq_parts + p.dkv_parts + p.dq_bytes + p.dkv_bytes + 16;
+    return p.key_docs + p.row_docs + p.few_bytes + p.stats_bytes + p.dq_parts + p.dkv_parts + p.dq_bytes + p.dkv_bytes + 16;
 }
 
 int attention_mfma_bwd(const AttnArgs& a, hipStream_t s) {

@@ -83,39 +83,13 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
 #pragma unroll
     for (int ks = 0; ks < kSteps; ++ks) qf[ks] = load_frag<T>(q, 16 * ks + 8 * hi, a.D);
 
-    const bool some = key_span >= 0, few = sizeof(T) == 2 && __any(some && key_span < kFewKeys - 1);
-    Reach w;
-    w.lo_min = wave_min_i32(some ? span.lo : 0x7FFFFFFF);
-    w.hi_max = wave_max_i32(some ? span.hi : -1);
-    w.lo_max = wave_max_i32(some ? span.lo : 0x7FFFFFFF);
-    w.hi_min = wave_min_i32(some ? span.hi : -1);
-    w.doc_min = wave_min_i32(some ? span.doc : 0x7FFFFFFF);
-    w.doc_max = wave_max_i32(some ? span.doc : -1);
+    const bool some = key_span >= 0, few = sizeof(T) == 2 && some && has_few(m, b, s, key_span);
+    const Reach w = wave_reach(some, span);
     Reach blk = w;
-    int blk_few = few;
-    if (!KEYS) {
-        __shared__ int reach[kWaves][5];
-        if (lane == 0) {
-            reach[wave][0] = w.lo_min;
-            reach[wave][1] = w.hi_max;
-            reach[wave][2] = w.doc_min;
-            reach[wave][3] = w.doc_max;
-            reach[wave][4] = few;
-        }
-        __syncthreads();
-        for (int i = 0; i < kWaves; ++i) {
-            blk.lo_min = min(blk.lo_min, reach[i][0]);
-            blk.hi_max = max(blk.hi_max, reach[i][1]);
-            blk.doc_min = min(blk.doc_min, reach[i][2]);
-            blk.doc_max = max(blk.doc_max, reach[i][3]);
-            blk_few |= reach[i][4];
-        }
-        blk.lo_min = __builtin_amdgcn_readfirstlane(blk.lo_min);
-        blk.hi_max = __builtin_amdgcn_readfirstlane(blk.hi_max);
-        blk.doc_min = __builtin_amdgcn_readfirstlane(blk.doc_min);
-        blk.doc_max = __builtin_amdgcn_readfirstlane(blk.doc_max);
-        blk_few = __builtin_amdgcn_readfirstlane(blk_few);
-    }
+    int blk_few = __any(few);
+    __shared__ BlockReach reach, few_reach;
+    if (!KEYS) blk = block_reach(w, blk_few, reach);
+    if (blk_few) keep_reach(wave_reach(few, span), few_reach);
     const int32_t* doc_min = a.docs ? m.key_docs.lowest + (int64_t)b * m.key_docs.tiles : nullptr;
     const int32_t* doc_max = a.docs ? m.key_docs.highest + (int64_t)b * m.key_docs.tiles : nullptr;
     const bool any = blk.hi_max >= blk.lo_min;
@@ -156,7 +130,9 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
     f32x16_t o[kCols];
     float top = -INFINITY, total = 0.f;  // what P refers to (log2 units, whole), this lane's share of the sum
 
-    auto run = [&](auto which) __attribute__((always_inline)) {
+    Reach mine = w;  // the wavefront's rows, for kRest those with few keys
+    int first_tile = 0, last_tile = -1;  // that the walk has met
+    auto run = [&](auto which, auto active, int first, int end, Share share) __attribute__((always_inline)) {
         constexpr Walk kWalk = decltype(which)::value;
         if (kWalk != kRest) {
             top = -INFINITY;
@@ -169,24 +145,25 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
 
         TileWalk<decltype(active)> walk(first, end, doc_min, doc_max, active, share.skip, share.left);
         WalkTile cur = walk.next();
+        if (kWalk != kRest && cur.t >= 0) first_tile = cur.t;
         int buf = 0;
         if (cur.t >= 0) fetch(cur.t, 0);
         while (cur.t >= 0) {
             lds_loads_done();
             __syncthreads();  // the tile is there, and every wave is done with the other buffer
             const WalkTile following = walk.next();
+            if (kWalk != kRest) last_tile = cur.t;
             if (Sh::kBuffers == 2 && following.t >= 0) fetch(following.t, buf ^ 1);
             const char* kt = lds + buf * Sh::kBuf;
             const char* vt = kt + Sh::kTileBytes;
             const int32_t* docs = (const int32_t*)(vt + Sh::kTileBytes);
             const uint32_t ka = lds_address(kt) + (KEYS ? wave * 32 * Tl::kRowBytes : 0), va = ka + Sh::kTileBytes;
             const int sub0 = KEYS ? wave * 32 : 0, key0 = cur.t * Sh::kTile + sub0, key1 = key0 + Sh::kWaveKeys - 1;
-            bool in = key0 <= w.hi_max && key1 >= w.lo_min, full = key0 >= w.lo_max && key1 <= w.hi_min;
+            bool in = key0 <= mine.hi_max && key1 >= mine.lo_min, full = key0 >= w.lo_max && key1 <= w.hi_min;
             if (a.docs) {
-                in = in && cur.doc_max >= w.doc_min && cur.doc_min <= w.doc_max;
+                in = in && cur.doc_max >= mine.doc_min && cur.doc_min <= mine.doc_max;
                 full = full && cur.doc_min == cur.doc_max && cur.doc_min == w.doc_min && cur.doc_min == w.doc_max;
             }
-            if (kWalk == kRest) in = in && few;
             if (in) {
                 const typename Tl::Rows k_rows(ln, ka);
                 const typename Tl::Cols v_cols(ln, va);
@@ -308,18 +285,23 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
             }
         }
     };
-    run(std::integral_constant<Walk, kMain>());
+    run(std::integral_constant<Walk, kMain>(), active, first, end, share);
     lds_loads_done();  // also where no tile was walked: nothing may land in LDS after the block is gone
     bool bad = false;
 #pragma unroll
     for (int t = 0; t < kCols; ++t) bad |= not_finite(o[t]);
     if (__syncthreads_or(bad)) {
-        run(std::integral_constant<Walk, kCareful>());
+        run(std::integral_constant<Walk, kCareful>(), active, first, end, share);
         __syncthreads();
     }
     if constexpr (sizeof(T) == 2) {
         if (blk_few) {
-            run(std::integral_constant<Walk, kRest>());
+            mine = kept_reach(few_reach, wave, wave + 1);
+            // of the tiles walked those that the block's rows with few keys see
+            const Reach rest = kept_reach(few_reach, 0, kWaves);
+            auto seen = [&](int, int d0, int d1) { return !a.docs || (d1 >= rest.doc_min && d0 <= rest.doc_max); };
+            run(std::integral_constant<Walk, kRest>(), seen, max(first_tile, rest.lo_min / Sh::kTile), min(last_tile, rest.hi_max / Sh::kTile) + 1,
+                Share{1, 0, 0x7FFFFFFF});
             __syncthreads();
         }
     }
@@ -424,9 +406,13 @@ __global__ __launch_bounds__(kThreads) void attention_join_kernel(MfmaArgs m, in
     }
 }
 
-__global__ __launch_bounds__(kThreads) void attention_documents_kernel(const int32_t* __restrict__ docs, int kv_len, int tile, int tiles,
-                                                                       int32_t* __restrict__ lowest, int32_t* __restrict__ highest) {
-    document_range(docs, kv_len, blockIdx.x, tile, tiles, kv_len, 0, GroupDiv{0u, 0}, lowest, highest);
+// What the kernel wants to know of the documents: the ranges of the key tiles, and (bf16) which queries have few keys
+__global__ __launch_bounds__(kThreads) void attention_documents_kernel(MfmaArgs m, int tile, int key_blocks) {
+    if ((int)blockIdx.x < key_blocks)
+        document_range(m.a.docs, m.a.kv_len, blockIdx.x, tile, m.key_docs.tiles, m.a.kv_len, 0, GroupDiv{0u, 0}, (int32_t*)m.key_docs.lowest,
+                       (int32_t*)m.key_docs.highest);
+    else
+        few_queries(m.a, blockIdx.x - key_blocks, (uint64_t*)m.few);
 }
 
 template <typename T, int DP, bool KEYS, int MODE>
@@ -460,7 +446,7 @@ int launch_for(const MfmaArgs& m, bool keys, hipStream_t s) {
 struct Plan {
     bool keys;  // the waves of a block share 32 rows
     int tile, blocks, key_tiles, splits, target;
-    int64_t doc_bytes, parts_bytes, out_bytes, lse_bytes;
+    int64_t doc_bytes, few_bytes, parts_bytes, out_bytes, lse_bytes;
 };
 int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 
@@ -479,6 +465,7 @@ Plan plan(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, 
     p.target = (int)(target < p.key_tiles || p.key_tiles == 0 ? target : p.key_tiles);
     p.splits = p.key_tiles > p.target ? (p.key_tiles + p.target - 1) / p.target : 1;
     p.doc_bytes = round16(batch * p.key_tiles * 8);
+    p.few_bytes = dtype == PICOMOE_BF16 ? round16(batch * few_words(q_len) * 8) : 0;
     p.parts_bytes = p.splits > 1 ? round16(heads * p.blocks * 4) : 0;
     p.out_bytes = p.splits > 1 ? round16((int64_t)p.splits * heads * rows * head_dim * 4) : 0;
     p.lse_bytes = p.splits > 1 ? round16((int64_t)p.splits * heads * rows * 4) : 0;
@@ -491,7 +478,7 @@ bool attention_mfma_supported(int dtype, int head_dim) { return head_dim <= (dty
 
 int64_t attention_mfma_fwd_workspace(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, int kv_heads, int head_dim) {
     const Plan p = plan(dtype, batch, q_len, kv_len, q_heads, kv_heads, head_dim);
-    return p.doc_bytes + p.parts_bytes + p.out_bytes + p.lse_bytes + 16;
+    return p.doc_bytes + p.few_bytes + p.parts_bytes + p.out_bytes + p.lse_bytes + 16;
 }
 
 int attention_mfma_fwd(const AttnArgs& a, hipStream_t s) {
@@ -503,15 +490,25 @@ int attention_mfma_fwd(const AttnArgs& a, hipStream_t s) {
     m.blocks = p.blocks;
     m.splits = p.splits;
     m.target = p.target;
-    int32_t* lowest = (int32_t*)a.ws;
+    char* ws = a.ws;
+    auto take = [&](int64_t bytes) {
+        char* at = ws;
+        ws += bytes;
+        return at;
+    };
+    int32_t* lowest = (int32_t*)take(p.doc_bytes);
     m.key_docs = {lowest, lowest + a.batch * p.key_tiles, p.key_tiles};
-    m.parts = (int32_t*)(a.ws + p.doc_bytes);
-    m.part_out = (float*)(a.ws + p.doc_bytes + p.parts_bytes);
-    m.part_lse = (float*)(a.ws + p.doc_bytes + p.parts_bytes + p.out_bytes);
+    const uint64_t* few = (const uint64_t*)take(p.few_bytes);
+    m.parts = (int32_t*)take(p.parts_bytes);
+    m.part_out = (float*)take(p.out_bytes);
+    m.part_lse = (float*)take(p.lse_bytes);
     if (a.docs && p.key_tiles > 0) {
-        const int64_t blocks = a.batch * range_blocks(p.key_tiles);
+        const bool count_few = a.dtype == PICOMOE_BF16;
+        const int64_t key_blocks = a.batch * range_blocks(p.key_tiles), blocks = key_blocks + (count_few ? a.batch * few_blocks(a.q_len) : 0);
         if (blocks > 0x7FFFFFFF) return PICOMOE_ERR_TOO_LARGE;
-        attention_documents_kernel<<<(unsigned)blocks, kThreads, 0, s>>>(a.docs, a.kv_len, p.tile, p.key_tiles, lowest, lowest + a.batch * p.key_tiles);
+        m.few = count_few ? few : nullptr;
+        m.few_words = few_words(a.q_len);
+        attention_documents_kernel<<<(unsigned)blocks, kThreads, 0, s>>>(m, p.tile, (int)key_blocks);
     }
     if (a.D > 128) return launch_for<__bf16, 256>(m, p.keys, s);
     if (a.dtype == PICOMOE_BF16) return a.D <= 64 ? launch_for<__bf16, 64>(m, p.keys, s) : launch_for<__bf16, 128>(m, p.keys, s);

@@ -68,9 +68,9 @@ __device__ __forceinline__ Frag<float> to_frag<float>(const f32x16_t& c, int hal
 
 // A kernel's walks over its tiles.  kMain.  kCareful, instead of it where its sums are not finite: values that are not finite are kept out
 // of the products, where 0 * inf would reach rows that do not see them, and added one by one to the rows that do.  kRest, bf16, after it:
-// rows with few keys -- the first ones of a sequence, narrow windows -- have a few large P and dx, whose rounding shows in the result as
-// it is, where the many of a long row average it out; what to_frag left of them is added.  6 batches of two tokens have dq to 0.0017 with
-// it, 0.0034 without (the rounding of dq itself: 0.0017).  Such rows have three tiles at most.
+// what to_frag left of P and dx is added for rows with few keys -- the first ones of a sequence or of a document, short documents, narrow
+// windows --, over the tiles that such rows see.  6 batches of two tokens have dq to 0.0017 with it, 0.0034 without (the rounding of dq
+// itself: 0.0017).
 enum Walk { kMain, kCareful, kRest };
 constexpr int kFewKeys = 128;
 __device__ __forceinline__ void take_rest(f32x16_t& c) {
@@ -481,6 +481,8 @@ struct MfmaArgs {
     float* part_out;
     float* part_lse;
     DocRanges key_docs, row_docs;
+    const uint64_t* few;  // bf16 with documents: a bit for each query, words of 64 per batch element (few_queries); else NULL
+    int few_words;
     float* stats;  // backward: [key heads][row tiles of 32][kStats][32], see RowStat
 };
 
@@ -488,10 +490,49 @@ struct MfmaArgs {
 // INT_MAX, kKeys 0 -- no key is that far -- and kLse2 +inf, which makes P zero.
 enum RowStat { kLse2, kDelta, kSlope2, kPos, kFirst, kKeys, kDoc, kStats = 8 };  // from kPos on: int32
 
-// what a set of query rows may see, and which documents it has
+// what a set of query rows may see, and which documents it has; of a wavefront's rows that are `in`
 struct Reach {
     int lo_min, lo_max, hi_min, hi_max, doc_min, doc_max;
 };
+__device__ __forceinline__ Reach wave_reach(bool in, const RowSpan& span) {
+    Reach w;
+    w.lo_min = wave_min_i32(in ? span.lo : 0x7FFFFFFF);
+    w.hi_max = wave_max_i32(in ? span.hi : -1);
+    w.lo_max = wave_max_i32(in ? span.lo : 0x7FFFFFFF);
+    w.hi_min = wave_min_i32(in ? span.hi : -1);
+    w.doc_min = wave_min_i32(in ? span.doc : 0x7FFFFFFF);
+    w.doc_max = wave_max_i32(in ? span.doc : -1);
+    return w;
+}
+// of all wavefronts of a block, lo_max and hi_min aside; and whether `flag` holds in one of them
+struct BlockReach {
+    int wave[kWaves][5];
+};
+__device__ __forceinline__ Reach block_reach(const Reach& w, int& flag, BlockReach& lds) {
+    const int at = wave_index();
+    if ((threadIdx.x & 63) == 0) {
+        lds.wave[at][0] = w.lo_min;
+        lds.wave[at][1] = w.hi_max;
+        lds.wave[at][2] = w.doc_min;
+        lds.wave[at][3] = w.doc_max;
+        lds.wave[at][4] = flag;
+    }
+    __syncthreads();
+    Reach blk = w;
+    for (int i = 0; i < kWaves; ++i) {
+        blk.lo_min = min(blk.lo_min, lds.wave[i][0]);
+        blk.hi_max = max(blk.hi_max, lds.wave[i][1]);
+        blk.doc_min = min(blk.doc_min, lds.wave[i][2]);
+        blk.doc_max = max(blk.doc_max, lds.wave[i][3]);
+        flag |= lds.wave[i][4];
+    }
+    blk.lo_min = __builtin_amdgcn_readfirstlane(blk.lo_min);
+    blk.hi_max = __builtin_amdgcn_readfirstlane(blk.hi_max);
+    blk.doc_min = __builtin_amdgcn_readfirstlane(blk.doc_min);
+    blk.doc_max = __builtin_amdgcn_readfirstlane(blk.doc_max);
+    flag = __builtin_amdgcn_readfirstlane(flag);
+    return blk;
+}
 
 // The walk over the tiles of [first, end) that pass `active(t, lowest document, highest document)`, 64 at a time, the first `skip` of
 // those left out and `left` taken; the same in every wave of a block.  The documents of a tile come with it: a load of them where
@@ -555,6 +596,82 @@ __device__ __forceinline__ void document_range(const int32_t* __restrict__ docs,
         lowest[(int64_t)b * tiles + tile] = lo;
         highest[(int64_t)b * tiles + tile] = hi;
     }
+}
+
+// The reach of the wavefronts' rows with few keys, kept in LDS until the second walk: the registers of the first one are full.
+__device__ __forceinline__ void keep_reach(const Reach& w, BlockReach& lds) {
+    const int at = wave_index();
+    if ((threadIdx.x & 63) == 0) {
+        lds.wave[at][0] = w.lo_min;
+        lds.wave[at][1] = w.hi_max;
+        lds.wave[at][2] = w.doc_min;
+        lds.wave[at][3] = w.doc_max;
+    }
+}
+__device__ __forceinline__ Reach kept_reach(const BlockReach& lds, int from, int to) {  // of wavefronts from .. to - 1
+    Reach r = {0x7FFFFFFF, 0, -1, 0, 0x7FFFFFFF, -1};
+    for (int i = from; i < to; ++i) {
+        r.lo_min = min(r.lo_min, lds.wave[i][0]);
+        r.hi_max = max(r.hi_max, lds.wave[i][1]);
+        r.doc_min = min(r.doc_min, lds.wave[i][2]);
+        r.doc_max = max(r.doc_max, lds.wave[i][3]);
+    }
+    r.lo_min = __builtin_amdgcn_readfirstlane(r.lo_min);
+    r.hi_max = __builtin_amdgcn_readfirstlane(r.hi_max);
+    r.doc_min = __builtin_amdgcn_readfirstlane(r.doc_min);
+    r.doc_max = __builtin_amdgcn_readfirstlane(r.doc_max);
+    return r;
+}
+
+// Which queries see fewer than kFewKeys keys where there are documents: without them the interval says it.  A wavefront looks at 64 queries and
+// counts the keys of their documents in their intervals, block by block of 64 from the queries' own positions to the front and then to the
+// back, until every query has enough, a block holds none of what those that lack some look for, or after kFewReach blocks.  Exact for
+// documents that lie in one piece; a query whose document goes on behind a gap, or is mixed with 8 and more others, may be taken to have
+// few, which costs a second walk and nothing else.  few_blocks(q_len) blocks per batch element.
+constexpr int kFewReach = 16;
+__host__ __device__ inline int few_words(int64_t q_len) { return (int)((q_len + 63) / 64); }
+__host__ __device__ inline int few_blocks(int64_t q_len) { return (few_words(q_len) + kWaves - 1) / kWaves; }
+__device__ __forceinline__ void few_queries(const AttnArgs& a, int block, uint64_t* __restrict__ few) {
+    const int words = few_words(a.q_len), per = few_blocks(a.q_len), b = block / per, lane = threadIdx.x & 63;
+    const int word = (block - b * per) * kWaves + (int)(threadIdx.x >> 6);
+    if (word >= words) return;
+    const int s = word * 64 + lane, pos0 = word * 64 + a.kv_len - a.q_len;
+    const RowSpan span = row_span(a, b, s < a.q_len ? s : a.q_len - 1);
+    const bool some = s < a.q_len && span.hi >= span.lo;
+    const uint32_t reach = some ? (uint32_t)(span.hi - span.lo) : 0u;
+    const int32_t* docs = a.docs + (int64_t)b * a.kv_len;
+    int n = 0;
+    for (int way = -1; way <= 1; way += 2) {
+        for (int i = way < 0 ? 0 : 1; i <= kFewReach; ++i) {
+            const int j0 = pos0 + 64 * way * i;
+            if (__ballot(some && n < kFewKeys && (way < 0 ? span.lo <= j0 + 63 : span.hi >= j0)) == 0) break;
+            const int doc = j0 + lane >= 0 && j0 + lane < a.kv_len ? docs[j0 + lane] : -1, doc0 = __builtin_amdgcn_readfirstlane(doc);
+            int here = 0;
+            if (__ballot(doc != doc0) == 0) {  // one document
+                here = doc0 == span.doc ? max(0, min(span.hi, j0 + 63) - max(span.lo, j0) + 1) : 0;
+            } else {
+                for (int u = 0; u < 64; ++u)
+                    here += __builtin_amdgcn_readlane(doc, u) == span.doc && (uint32_t)(j0 + u - span.lo) <= reach;
+            }
+            // the queries' own block holds them themselves
+            if (i > 0 && __ballot(some && n < kFewKeys && here > 0) == 0) break;
+            n += here;
+        }
+    }
+    const uint64_t bits = __ballot(some && n < kFewKeys);
+    if (lane == 0) few[(int64_t)b * words + word] = bits;
+}
+// whether query s, whose interval holds key_span + 1 keys, has few
+__device__ __forceinline__ bool has_few(const MfmaArgs& m, int b, int s, int key_span) {
+    if (!m.few) return key_span < kFewKeys - 1;
+    return m.few[(int64_t)b * m.few_words + (s >> 6)] >> (s & 63) & 1;
+}
+// whether one of queries q0 .. q1, at most 64, has
+__device__ __forceinline__ bool any_has_few(const MfmaArgs& m, int b, int q0, int q1) {
+    const uint64_t* words = m.few + (int64_t)b * m.few_words;
+    uint64_t bits = words[q0 >> 6] >> (q0 & 63);
+    if (q0 >> 6 != q1 >> 6) bits |= words[q1 >> 6] << (64 - (q0 & 63));  // q0 & 63 is not 0 then
+    return bits << (63 - (q1 - q0)) != 0;
 }
 
 // the tiles that a walk passes

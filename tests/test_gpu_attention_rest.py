@@ -84,3 +84,64 @@ def test_last_rows_of_a_window_without_causality(gpu, S, window, heads, kv_heads
         value = want[name][0]
         rounding = (value.to(BF16).double() - value).norm()
         assert (got.double() - value).norm() <= 1.2 * rounding, (name, float((got.double() - value).norm() / rounding))
+
+
+def _documents(kind, batch, length):
+    """[batch, length]: runs of tokens, some short, some begun inside a tile of 64, with padding among them; "scattered" has every document in two
+    pieces."""
+    lengths = {"short": [40, 5, 64, 1, 100, 30, 90, 127, 2, 60], "long": [300, 200, 140, 400, 129], "unequal": [700, 20, 128, 127, 3, 260]}[
+        "short" if kind == "scattered" else kind]
+    ids, number = [], 0
+    while len(ids) < length:
+        n = lengths[number % len(lengths)]
+        ids += [-7 if number % 6 == 4 else (number * 37 % 101 if kind != "scattered" else number // 4 * 2 + number % 2)] * n
+        number += 1
+    rows = [ids[:length], ids[-length:] if kind == "short" else ids[:length][::-1]]
+    return torch.tensor([rows[b % 2] for b in range(batch)], dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("kind,batch,q_len,kv_len,heads,kv_heads,D,options", [
+    ("short", 2, 700, 700, 4, 1, 128, {}), ("short", 1, 500, 500, 2, 2, 64, {"softcap": 20.0}), ("long", 1, 1000, 1000, 6, 2, 64, {}),
+    ("unequal", 2, 1200, 1200, 2, 1, 128, {"slopes": True}), ("short", 1, 300, 300, 2, 1, 256, {}), ("long", 1, 2600, 2600, 2, 1, 64, {}),
+    ("long", 2, 700, 700, 4, 2, 128, {"window": 150}), ("short", 2, 400, 400, 5, 1, 72, {"causal": False}), ("long", 1, 600, 600, 2, 1, 128, {"prefix": 350}),
+    ("scattered", 2, 600, 600, 4, 2, 128, {}), ("short", 2, 3, 700, 8, 2, 128, {}), ("unequal", 1, 200, 2000, 4, 2, 64, {}), ("short", 2, 150, 60, 4, 2, 64, {}),
+    ("long", 1, 1, 700, 1, 1, 64, {"softcap": 5.0})])
+def test_documents_in_a_row(gpu, kind, batch, q_len, kv_len, heads, kv_heads, D, options):
+    """The first tokens of a document, wherever it begins, and all of a short one see few keys.  Their rows of out, to 2^-16, and of dq; dk and dv with
+    an output gradient for them alone: each off by its own rounding, as above."""
+    (q, k, v), g = _inputs(q_len + kv_len, batch, q_len, kv_len, heads, kv_heads, D)
+    options = dict(options, document_ids=_documents(kind, batch, kv_len))
+    if options.pop("slopes", False):
+        options["slopes"] = 2.0 ** (-8.0 * torch.arange(1, heads + 1, device="cuda") / heads)
+    if "prefix" in options:
+        options["prefix_lengths"] = torch.full((batch,), options.pop("prefix"), dtype=torch.int32, device="cuda")
+    masks = {n: options.get(n) for n in ("window", "document_ids", "prefix_lengths")}
+    seen = O.seen(batch, q_len, kv_len, options.get("causal", True), masks["window"], masks["document_ids"], masks["prefix_lengths"], q.device).sum(-1)
+    few = (seen > 0) & (seen < 128)
+    assert few.any()
+    g = torch.where(few[..., None, None], g, torch.zeros((), device="cuda", dtype=BF16))
+    out = _call(q, k, v, **options)
+    sums = _sums(out)
+    grads = torch.autograd.grad(out, (q, k, v), g)
+    want = O.attention(q.detach(), k.detach(), v.detach(), d_out=g, **options)
+    value = want["out"][0]
+    assert (sums - value)[few].norm() <= LEFT * value[few].norm(), float((sums - value)[few].norm() / value[few].norm())
+    assert not out.detach()[seen == 0].any()
+    for name, got in zip(("dq", "dk", "dv"), grads):
+        value = want[name][0]
+        rounding = (value.to(BF16).double() - value).norm()
+        assert (got.double() - value).norm() <= 1.2 * rounding, (name, float((got.double() - value).norm() / rounding))
+
+
+def test_a_document_packed_is_as_exact_as_alone(gpu):
+    """40 tokens behind 500 others, and the same 40 alone: the same sums to 2^-16, the same gradients but for a rounding."""
+    (q, k, v), g = _inputs(3, 1, 540, 540, 4, 2, 128)
+    ids = torch.zeros(1, 540, dtype=torch.int32, device="cuda")
+    ids[:, 500:] = 1
+    last = [t.detach()[:, 500:].clone().requires_grad_(True) for t in (q, k, v)]
+    packed, alone = _call(q, k, v, document_ids=ids), _call(*last)
+    a, b = _sums(packed)[:, 500:], _sums(alone)
+    assert (a - b).norm() <= 2 * LEFT * b.norm()
+    for x, y in zip(torch.autograd.grad(packed, (q, k, v), g), torch.autograd.grad(alone, last, g[:, 500:].contiguous())):
+        x, y = x[:, 500:].double(), y.double()
+        assert ((x - y).abs() <= 2.0 ** -7 * y.abs() + 2.0 ** -12 * y.abs().max()).all()
