@@ -260,7 +260,7 @@ int picomoe_qk_norm_rope_bwd(const void* dq_out, const void* dk_out, const void*
  * bias and document, prefix and window masks.  q [batch, q_len, q_heads, head_dim], k and v [batch, kv_len, kv_heads, head_dim]
  * with element strides {batch, seq, head}; out dense like q; lse [batch, q_heads, q_len] fp32.  Query s stands at position
  * p = s + kv_len - q_len and head h reads key head h / (q_heads / kv_heads).  Scores: x = scale * q . k; with softcap > 0
- * softcap * tanh(x / softcap); with slopes [q_heads] (fp32) minus slopes[h] * |p - j|.  Key j is seen when: causal == 0 or
+ * softcap * tanh(x / softcap) (softcap at most 1e30, scale / softcap 0 or from 1.2e-38 to 1e38); with slopes [q_heads] (fp32) minus slopes[h] * |p - j|.  Key j is seen when: causal == 0 or
  * j <= p or j < prefix_lengths[batch] (needs causal); window == 0 or |p - j| < window; document_ids [batch, kv_len] is NULL or
  * document_ids[j] == document_ids[p] >= 0.  A query that sees nothing gets out 0 and lse -inf, and no gradient; what is not seen has no influence,
  * NaN and infinities included.  The backward call takes the forward's out and lse; d_out, dq, dk, dv are dense.  out_residual (bf16, dense like

@@ -24,8 +24,11 @@ bool tensor(AttnTensor* t, const void* p, const int64_t* strides, int dtype) {
 bool fill(AttnArgs* a, const void* q, const int64_t* qs, const void* k, const int64_t* ks, const void* v, const int64_t* vs, int dtype, int64_t batch,
           int64_t q_len, int64_t kv_len, int q_heads, int kv_heads, int head_dim, float scale, float softcap, int causal, int64_t window,
           const float* slopes, const int32_t* docs, const int32_t* prefix) {
-    if (!(softcap >= 0.f) || softcap > 3e38f || !(scale >= -3e38f && scale <= 3e38f) || window < 0 || (prefix && !causal)) return false;
-    if (softcap > 0.f && !((scale < 0.f ? -scale : scale) / softcap < 1e38f)) return false;  // the factor of q . k inside the cap, times 2 log2(e)
+    if (!(softcap >= 0.f) || softcap > 1e30f || !(scale >= -3e38f && scale <= 3e38f) || window < 0 || (prefix && !causal)) return false;
+    if (softcap > 0.f && scale != 0.f) {  // the factor of q . k inside the cap: normal, and finite times 2 log2(e)
+        const float inside = (scale < 0.f ? -scale : scale) / softcap;
+        if (!(inside >= 1.2e-38f && inside < 1e38f)) return false;
+    }
     if (!tensor(&a->q, q, qs, dtype)) return false;
     if (kv_len > 0 && (!tensor(&a->k, k, ks, dtype) || !tensor(&a->v, v, vs, dtype))) return false;
     a->dtype = dtype; a->causal = causal != 0; a->batch = batch;

@@ -303,7 +303,7 @@ def attention(q, k, v, *, causal=True, scale=None, softcap=0.0, window=0, slopes
     The queries are the last ones: query ``s`` stands at position ``p = s + kv_len - q_len`` (one new token over a cache: q_len 1).
 
     Scores, for key position ``j``: ``x = scale * q.k`` (``scale`` default ``head_dim ** -0.5``); ``softcap > 0``:
-    ``softcap * tanh(x / softcap)``; ``slopes`` (fp32 ``[heads]``): minus ``slopes[h] * |p - j|``.
+    ``softcap * tanh(x / softcap)`` (1e-30 to 1e30, and ``scale / softcap`` not below float32's normal numbers); ``slopes`` (fp32 ``[heads]``): minus ``slopes[h] * |p - j|``.
 
     A query sees key j when all of these hold: ``causal`` is off or ``j <= p`` or ``j < prefix_lengths[b]`` (int32 ``[batch]``); ``window``
     is 0 or ``|p - j| < window``; ``document_ids`` (int32 ``[batch, kv_len]``, in any order) is None or
@@ -327,8 +327,8 @@ def attention(q, k, v, *, causal=True, scale=None, softcap=0.0, window=0, slopes
                       RuntimeWarning, stacklevel=2)
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     softcap, window = float(softcap or 0.0), int(window or 0)
-    if not abs(scale) <= 3e38 or not (softcap == 0 or 1e-30 <= softcap <= 3e38) or window < 0:
-        _fail(f"{what}: scale {scale}, softcap {softcap} (0 or from 1e-30 on), window {window}")
+    if not abs(scale) <= 3e38 or not (softcap == 0 or 1e-30 <= softcap <= 1e30) or window < 0:
+        _fail(f"{what}: scale {scale}, softcap {softcap} (0 or from 1e-30 to 1e30), window {window}")
     window = min(window, Sq + Sk)  # no query is that far from a key
     if slopes is not None:
         if slopes.dtype != torch.float32 or slopes.shape != (H,):

@@ -98,6 +98,20 @@ def test_values_that_reach_no_kernel():
         assert lib.picomoe_embedding_bwd(P, 1, P, 4, 10, 64, scale, -1, P, P, 1 << 30, None) == 1
 
 
+def test_caps_beyond_the_factors_range():
+    """softcap log2(e) and scale / softcap are float32 factors: a cap that makes the first infinite or the second less than normal is refused."""
+    lib = _lib.load()
+
+    def refused(scale, softcap):
+        fwd = lib.picomoe_attention_fwd(P, STRIDES, P, STRIDES, P, STRIDES, 1, 2, 4, 4, 4, 4, 64, scale, softcap, 1, 0, None, None, None, P, None, P, P, 1 << 40, None)
+        bwd = lib.picomoe_attention_bwd(P, P, STRIDES, P, STRIDES, P, STRIDES, P, None, P, 1, 2, 4, 4, 4, 4, 64, scale, softcap, 1, 0, None, None, None, P, P, P, P, 1 << 40,
+                                        None)
+        return fwd == 1 and bwd == 1
+
+    for scale, softcap in ((0.125, 3e38), (0.125, 2.4e38), (0.125, 1e37), (0.125, 1.1e30), (1e-9, 1e30), (-1e-9, 1e30), (1e-38, 2.0), (0.0, 2e30)):
+        assert refused(scale, softcap), (scale, softcap)
+
+
 def test_cpu_tensors_are_refused():
     q = torch.zeros(1, 2, 2, 64)
     table = torch.zeros(4, 64)

@@ -145,3 +145,22 @@ def test_a_document_packed_is_as_exact_as_alone(gpu):
     for x, y in zip(torch.autograd.grad(packed, (q, k, v), g), torch.autograd.grad(alone, last, g[:, 500:].contiguous())):
         x, y = x[:, 500:].double(), y.double()
         assert ((x - y).abs() <= 2.0 ** -7 * y.abs() + 2.0 ** -12 * y.abs().max()).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+@pytest.mark.parametrize("scale,softcap", [(0.125, 1e30), (0.125, 1e20), (1e-7, 1e30), (0.0, 1e30), (1e-37, 2.0)])
+def test_the_largest_caps(gpu, dtype, scale, softcap):
+    """Caps up to the largest that is taken: far above every score they change nothing."""
+    from picotron_amd import _lib
+
+    (q, k, v), g = _inputs(8, 1, 90, 90, 2, 1, 64)
+    q, k, v = (t.detach().to(dtype).requires_grad_(True) for t in (q, k, v))
+    g = g.to(dtype)
+    out = _call(q, k, v, scale=scale, softcap=softcap)
+    want = O.attention(q.detach(), k.detach(), v.detach(), scale=scale, softcap=softcap, d_out=g)
+    for name, got in zip(("out", "dq", "dk", "dv"), (out.detach(), *torch.autograd.grad(out, (q, k, v), g))):
+        value, bound = want[name]
+        assert ((got.double() - value).abs() <= bound + 2.0 ** -126).all(), name
+    for bad in ((0.125, 3e38), (0.125, 1.1e30), (1e-9, 1e30)):
+        with pytest.raises(_lib.PicomoeError):
+            _call(q, k, v, scale=bad[0], softcap=bad[1])
