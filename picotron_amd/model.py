@@ -114,7 +114,7 @@ class Attention(nn.Module):
         elif bias != "distance":
             raise ValueError(f"attention_bias {bias!r}: 'distance' or none")
         # a plain attribute like the rotation tables (no state_dict entry)
-        self.slopes = 2.0 ** (-8.0 * torch.arange(1, self.num_heads + 1) / self.num_heads) if bias else None
+        self.slopes = 2.0 ** (-8.0 * torch.arange(1, self.num_heads + 1, dtype=torch.float32) / self.num_heads) if bias else None
         self.q_norm = self.k_norm = None
         if getattr(config, "qk_norm", False):
             self.q_norm, self.k_norm = (LlamaRMSNorm(self.head_dim, eps=config.rms_norm_eps) for _ in range(2))

@@ -149,3 +149,20 @@ def test_model_options():
         assert Llama(types.SimpleNamespace(**base, **option)).decoder_layers[0].attention.fused
     with pytest.raises(ValueError):
         Llama(types.SimpleNamespace(**base, attention_bias="alibi"))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float64])
+def test_slopes_are_float32_whatever_the_default_type(dtype):
+    """A model built with another default type has the fp32 slopes that the attention takes."""
+    from picotron_amd.model import Llama
+
+    config = types.SimpleNamespace(vocab_size=50, hidden_size=96, intermediate_size=32, num_attention_heads=12, num_key_value_heads=2, num_hidden_layers=1,
+                                   max_position_embeddings=8, rms_norm_eps=1e-5, rope_theta=10000.0, attention_bias="distance")
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(dtype)
+    try:
+        slopes = Llama(config).decoder_layers[0].attention.slopes
+    finally:
+        torch.set_default_dtype(before)
+    assert slopes.dtype == torch.float32
+    assert torch.equal(slopes, 2.0 ** (-8.0 * torch.arange(1, 13, dtype=torch.float32) / 12))
