@@ -19,6 +19,7 @@ for what the reference's decoder lacks (all optional, absent = the reference's b
 """
 
 import math
+import weakref
 
 import torch
 import torch.nn as nn
@@ -59,6 +60,30 @@ def rope_tables(seq_length, head_dim, base=500000.0):
     inv_freq = 1.0 / (base ** (torch.arange(0, head_dim, 2, dtype=torch.int64).float() / head_dim))
     angle = torch.arange(seq_length).float().unsqueeze(1) * inv_freq
     return torch.cos(angle).repeat(1, 2), torch.sin(angle).repeat(1, 2)
+
+
+class _Float32Tables:
+    """``rope_tables`` as the fused path reads them, in fp32: one copy per device, made when it is first asked for, for all layers."""
+
+    _all = weakref.WeakValueDictionary()   # by length, head size and base, as long as a layer holds them
+
+    def __init__(self, *key):
+        self.key, self.copies = key, {}
+
+    @classmethod
+    def of(cls, seq_length, head_dim, base):
+        key = (seq_length, head_dim, float(base))
+        found = cls._all.get(key)
+        if found is None:
+            found = cls._all[key] = cls(*key)
+        return found
+
+    def on(self, device):
+        if device not in self.copies:
+            with torch.device("cpu"):
+                tables = rope_tables(*self.key)
+            self.copies[device] = tuple(t.to(device) for t in tables)
+        return self.copies[device]
 
 
 def apply_rotary_pos_emb(x, cos, sin):
@@ -212,7 +237,7 @@ class DecoderLayer(nn.Module):
         self.cos, self.sin = rope_tables(
             config.max_position_embeddings, config.hidden_size // config.num_attention_heads, base=config.rope_theta
         )
-        self.tables_f32 = (self.cos, self.sin)  # of the fused path, moved to the activations' device on use
+        self.tables = _Float32Tables.of(config.max_position_embeddings, config.hidden_size // config.num_attention_heads, config.rope_theta)
 
     def _rope(self, x):
         if self.cos.device != x.device or self.cos.dtype != x.dtype:
@@ -222,9 +247,10 @@ class DecoderLayer(nn.Module):
 
     def _attend(self, n, attention_mask, position_ids, document_ids, prefix_lengths):
         if self.attention.fused or document_ids is not None or prefix_lengths is not None:
-            if self.tables_f32[0].device != n.device:
-                self.tables_f32 = tuple(t.to(n.device) for t in self.tables_f32)
-            return self.attention.forward_fused(n, *self.tables_f32, position_ids, document_ids, prefix_lengths)
+            cos, sin = self.tables.on(n.device)
+            if self.cos.device != n.device:   # this layer's host copy goes
+                self.cos, self.sin = cos, sin
+            return self.attention.forward_fused(n, cos, sin, position_ids, document_ids, prefix_lengths)
         cos, sin = self._rope(n)
         return self.attention(n, cos, sin, attention_mask, position_ids)
 

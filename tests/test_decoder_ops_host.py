@@ -1,8 +1,11 @@
 """Arguments of the decoder's operators that are refused before anything reaches the GPU: through the C ABI with pointers that are
 never dereferenced on the host, and through the Python wrappers with CPU tensors."""
 
+import copy
 import ctypes
+import gc
 import types
+import weakref
 
 import pytest
 import torch
@@ -166,3 +169,31 @@ def test_slopes_are_float32_whatever_the_default_type(dtype):
         torch.set_default_dtype(before)
     assert slopes.dtype == torch.float32
     assert torch.equal(slopes, 2.0 ** (-8.0 * torch.arange(1, 13, dtype=torch.float32) / 12))
+
+
+def test_no_layer_keeps_tables_that_it_does_not_read():
+    """A layer that rotates by tables of the activations' type holds no others once it has run; the fp32 tables of the fused path are one copy per
+    device for all layers, and go with the last of them."""
+    from picotron_amd.model import Llama, rope_tables
+
+    config = types.SimpleNamespace(vocab_size=50, hidden_size=64, intermediate_size=32, num_attention_heads=4, num_key_value_heads=2, num_hidden_layers=3,
+                                   max_position_embeddings=40, rms_norm_eps=1e-5, rope_theta=12345.0)
+    model = Llama(config)
+    layers = list(model.decoder_layers)
+    host = [weakref.ref(t) for layer in layers for t in (layer.cos, layer.sin)]
+    for layer in layers:
+        cos, sin = layer._rope(torch.zeros(1, 7, 64, dtype=torch.bfloat16))
+        assert cos.dtype == sin.dtype == torch.bfloat16 and cos.shape == (7, 16)
+    gc.collect()
+    assert all(t() is None for t in host)
+    cpu = torch.device("cpu")
+    shared = layers[0].tables.on(cpu)
+    assert all(layer.tables.on(cpu)[0] is shared[0] and layer.tables.on(cpu)[1] is shared[1] for layer in layers)
+    for a, b in zip(shared, rope_tables(40, 16, 12345.0)):
+        assert a.dtype == torch.float32 and torch.equal(a, b)
+    twin = copy.deepcopy(model)   # holds its own
+    assert torch.equal(twin.decoder_layers[1].tables.on(cpu)[0], shared[0])
+    gone = weakref.ref(shared[0])
+    del model, layers, layer, shared, a, b
+    gc.collect()
+    assert gone() is None

@@ -593,3 +593,19 @@ def test_decoder_with_everything(gpu, dtype):
         assert torch.allclose(packed[:, part], alone, **tol), float((packed[:, part] - alone).abs().max())
     prefix = model(ids, prefix_lengths=torch.tensor([40], device="cuda", dtype=torch.int32))
     assert torch.isfinite(prefix).all() and not torch.equal(prefix[:, :39], model(ids)[:, :39])
+
+
+def test_layers_share_their_tables(gpu):
+    """The fused path's fp32 tables are on the device once, and no layer holds a copy on the host after its first call; the plain path then still runs."""
+    model = _model(_config(fused_attention=True), FP32)
+    ids = torch.randint(0, 97, (2, 20), generator=_gen(5), device="cuda")
+    first = model(ids)
+    layers = list(model.decoder_layers)
+    assert all(layer.cos is layers[0].cos and layer.sin is layers[0].sin and layer.cos.is_cuda for layer in layers)
+    for layer in layers:
+        layer.attention.fused = False
+    plain = model(ids)
+    assert torch.allclose(first, plain, atol=2e-4, rtol=1e-4)   # fp32 rounding, as above
+    for layer in layers:
+        layer.attention.fused = True
+    assert torch.equal(model(ids), first)
