@@ -210,7 +210,7 @@ def qk_norm_rope(q, k, cos, sin, q_weight=None, k_weight=None, eps=1e-5, positio
 
     ``norm``: RMS norm over head_dim times the weight ``[head_dim]`` (None: no norm).  ``rotate``: rotate-half with the rows of
     the fp32 tables ``cos``, ``sin`` ``[n_positions, head_dim]`` (``model.rope_tables``) that ``positions`` (int64 or int32,
-    ``[batch, seq]`` or ``[seq]``; None: 0, 1, 2, ...) names.  fp32 arithmetic, rounded once.  Gradients for q, k and the weights."""
+    ``[batch, seq]``, ``[1, seq]`` or ``[seq]``; None: 0, 1, 2, ...) names.  fp32 arithmetic, rounded once.  Gradients for q, k and the weights."""
     what = "qk_norm_rope"
     _same_device(what, q, k, cos, sin, q_weight, k_weight, positions)
     if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3] or q.shape[2] < 1 or k.shape[2] < 1:
@@ -229,8 +229,8 @@ def qk_norm_rope(q, k, cos, sin, q_weight=None, k_weight=None, eps=1e-5, positio
         if t.requires_grad:
             _fail(f"{what}: no gradient for {name}")
     if positions is not None:
-        if positions.shape not in ((B, S), (S,)):
-            _fail(f"{what}: positions {tuple(positions.shape)}, [{B}, {S}] or [{S}] is needed")
+        if positions.shape not in ((B, S), (1, S), (S,)):
+            _fail(f"{what}: positions {tuple(positions.shape)}, [{B}, {S}], [1, {S}] or [{S}] is needed")
         positions = _integer(f"{what}: positions", positions.expand(B, S))
     elif S > cos.shape[0]:
         _fail(f"{what}: {S} tokens, tables of {cos.shape[0]} positions")

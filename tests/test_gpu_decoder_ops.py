@@ -609,3 +609,18 @@ def test_layers_share_their_tables(gpu):
     for layer in layers:
         layer.attention.fused = True
     assert torch.equal(model(ids), first)
+
+
+def test_positions_of_one_row_for_a_batch(gpu):
+    """[1, seq] positions serve every row of a batch, in the operator and through the model."""
+    gen = _gen(11)
+    q, k = _randn(gen, 3, 5, 4, 64), _randn(gen, 3, 5, 2, 64)
+    cos, sin = torch.rand(9, 64, generator=gen, device="cuda"), torch.rand(9, 64, generator=gen, device="cuda")
+    row = torch.tensor([[8, 0, 3, 3, 1]], device="cuda")
+    for at in (row, row.int(), row[0], row.expand(3, 5)):
+        for got, want in zip(_ops().qk_norm_rope(q, k, cos, sin, positions=at), _ops().qk_norm_rope(q, k, cos, sin, positions=row.repeat(3, 1))):
+            assert torch.equal(got, want)
+    model = _model(_config(fused_attention=True), FP32)
+    ids = torch.randint(0, 97, (2, 30), generator=gen, device="cuda")
+    row = torch.arange(30, device="cuda")[None] + 7
+    assert torch.equal(model(ids, position_ids=row), model(ids, position_ids=row.repeat(2, 1)))
