@@ -160,7 +160,8 @@ class Attention(nn.Module):
         q, k, v = heads(self.q_proj(x), self.num_heads), heads(self.k_proj(x), self.num_key_values), heads(self.v_proj(x), self.num_key_values)
         weights, eps = (None, None), 0.0
         if self.q_norm is not None:
-            weights, eps = (self.q_norm.weight, self.k_norm.weight), self.q_norm.variance_epsilon
+            # in the heads' type, which is another one under autocast
+            weights, eps = (self.q_norm.weight.to(q.dtype), self.k_norm.weight.to(q.dtype)), self.q_norm.variance_epsilon
         if self.slopes is not None and self.slopes.device != x.device:
             self.slopes = self.slopes.to(x.device)
         q, k = decoder_ops.qk_norm_rope(q, k, cos, sin, *weights, eps=eps, positions=position_ids)

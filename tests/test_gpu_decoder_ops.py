@@ -624,3 +624,29 @@ def test_positions_of_one_row_for_a_batch(gpu):
     ids = torch.randint(0, 97, (2, 30), generator=gen, device="cuda")
     row = torch.arange(30, device="cuda")[None] + 7
     assert torch.equal(model(ids, position_ids=row), model(ids, position_ids=row.repeat(2, 1)))
+
+
+def test_head_norms_under_autocast(gpu):
+    """fp32 parameters and bf16 heads: the norm weights are taken in the heads' type, their gradients come back in fp32."""
+    import torch.nn.functional as F
+
+    model = _model(_config(qk_norm=True), FP32)
+    layer = model.decoder_layers[0]
+    attention = layer.attention
+    cos, sin = layer.tables.on(torch.device("cuda", torch.cuda.current_device()))
+    x, g = torch.randn(2, 40, 256, generator=_gen(1), device="cuda"), _randn(_gen(2), 2, 40, 256)
+    leaves = [attention.q_norm.weight, attention.k_norm.weight]
+    with torch.autocast("cuda", dtype=BF16):
+        got = attention.forward_fused(x, cos, sin)
+    grads = torch.autograd.grad(got, leaves, g)
+    heads = [F.linear(x.to(BF16), p.weight.to(BF16)).view(2, 40, -1, 64) for p in (attention.q_proj, attention.k_proj, attention.v_proj)]
+    low = [w.detach().to(BF16).requires_grad_(True) for w in leaves]
+    q, k = _ops().qk_norm_rope(heads[0], heads[1], cos, sin, *low, eps=1e-5)
+    want = F.linear(_ops().attention(q, k, heads[2]).reshape(2, 40, 256), attention.out_proj.weight.to(BF16))
+    assert got.dtype == BF16 and torch.equal(got, want)
+    for a, b in zip(grads, torch.autograd.grad(want, low, g)):
+        assert a.dtype == FP32 and torch.equal(a, b.float())
+    with torch.autocast("cuda", dtype=BF16):
+        logits = model(torch.randint(0, 97, (2, 40), generator=_gen(3), device="cuda"))
+    logits.float().sum().backward()
+    assert all(p.grad is not None and p.grad.dtype == FP32 and torch.isfinite(p.grad).all() for p in leaves)
