@@ -26,7 +26,8 @@ namespace {
 constexpr float kLazy = 8.f;
 
 // KEYS: the four waves share 32 rows and split every tile's keys among them (few rows: one new token); otherwise every wave
-// has 32 rows of its own and all of the tile's keys.
+// has 32 rows of its own and all of the tile's keys.  The first, which waits for K and V and not for its products, takes P of all rows
+// in two bf16 parts; the second only those of rows with few keys, in a second walk (kRest).
 template <typename T, int DP, bool KEYS>
 struct FwdShape {
     static constexpr int kTile = KEYS ? 32 * kWaves : (sizeof(T) == 2 ? 64 : 32);  // keys of a tile
@@ -62,6 +63,7 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
     typedef FwdShape<T, DP, KEYS> Sh;
     typedef typename Sh::Tl Tl;
     constexpr int kSub = Sh::kWaveKeys / 32, kSteps = DP / 16, kCols = DP / 32;
+    constexpr bool kTwoParts = sizeof(T) == 2 && KEYS, kRestWalk = sizeof(T) == 2 && !KEYS;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const AttnArgs& a = m.a;
     const int lane = threadIdx.x & 63, wave = wave_index(), hi = lane >> 5;
@@ -83,7 +85,7 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
 #pragma unroll
     for (int ks = 0; ks < kSteps; ++ks) qf[ks] = load_frag<T>(q, 16 * ks + 8 * hi, a.D);
 
-    const bool some = key_span >= 0, few = sizeof(T) == 2 && some && has_few(m, b, s, key_span);
+    const bool some = key_span >= 0, few = kRestWalk && some && has_few(m, b, s, key_span);
     const Reach w = wave_reach(some, span);
     Reach blk = w;
     int blk_few = __any(few);
@@ -252,14 +254,17 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
 #pragma unroll
                 for (int st = 0; st < 2 * kSub; ++st) {
                     const Frag<T> p = to_frag<T>(x[st / 2], st & 1);
+                    Frag<T> rest;
+                    if constexpr (kTwoParts) rest = rest_frag(x[st / 2], st & 1);
 #pragma unroll
                     for (int t = 0; t < kCols; ++t) {
                         Frag<T> v = Tl::frag_t(v_cols, 16 * st, t);
                         if (kWalk != kMain) zero_not_finite(v);
                         mma(o[t], v, p);
+                        if constexpr (kTwoParts) mma(o[t], v, rest);
                     }
                 }
-                if (sizeof(T) == 2 && kWalk == kMain) read_ahead<2, 1, 2 * kSub * kCols, 2>();
+                if (sizeof(T) == 2 && kWalk == kMain) read_ahead<2, kTwoParts ? 2 : 1, 2 * kSub * kCols, 2>();
                 if (kWalk == kCareful) {
                     bool bad = false;
                     if (lane < Sh::kWaveKeys) bad = Tl::row_not_finite(vt, sub0 + lane);
@@ -294,7 +299,7 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
         run(std::integral_constant<Walk, kCareful>(), active, first, end, share);
         __syncthreads();
     }
-    if constexpr (sizeof(T) == 2) {
+    if constexpr (kRestWalk) {
         if (blk_few) {
             mine = kept_reach(few_reach, wave, wave + 1);
             // of the tiles walked those that the block's rows with few keys see
@@ -465,7 +470,7 @@ Plan plan(int dtype, int64_t batch, int64_t q_len, int64_t kv_len, int q_heads, 
     p.target = (int)(target < p.key_tiles || p.key_tiles == 0 ? target : p.key_tiles);
     p.splits = p.key_tiles > p.target ? (p.key_tiles + p.target - 1) / p.target : 1;
     p.doc_bytes = round16(batch * p.key_tiles * 8);
-    p.few_bytes = dtype == PICOMOE_BF16 ? round16(batch * few_words(q_len) * 8) : 0;
+    p.few_bytes = dtype == PICOMOE_BF16 && !p.keys ? round16(batch * few_words(q_len) * 8) : 0;
     p.parts_bytes = p.splits > 1 ? round16(heads * p.blocks * 4) : 0;
     p.out_bytes = p.splits > 1 ? round16((int64_t)p.splits * heads * rows * head_dim * 4) : 0;
     p.lse_bytes = p.splits > 1 ? round16((int64_t)p.splits * heads * rows * 4) : 0;
@@ -503,7 +508,7 @@ int attention_mfma_fwd(const AttnArgs& a, hipStream_t s) {
     m.part_out = (float*)take(p.out_bytes);
     m.part_lse = (float*)take(p.lse_bytes);
     if (a.docs && p.key_tiles > 0) {
-        const bool count_few = a.dtype == PICOMOE_BF16;
+        const bool count_few = p.few_bytes > 0;
         const int64_t key_blocks = a.batch * range_blocks(p.key_tiles), blocks = key_blocks + (count_few ? a.batch * few_blocks(a.q_len) : 0);
         if (blocks > 0x7FFFFFFF) return PICOMOE_ERR_TOO_LARGE;
         m.few = count_few ? few : nullptr;

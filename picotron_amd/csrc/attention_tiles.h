@@ -66,6 +66,17 @@ __device__ __forceinline__ Frag<float> to_frag<float>(const f32x16_t& c, int hal
     return f;
 }
 
+// what to_frag left of them, rounded to bf16 in turn: together they are off by 2^-16 of a term
+__device__ __forceinline__ Frag<__bf16> rest_frag(const f32x16_t& c, int half) {
+    u32x4_t w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float a = c[8 * half + 2 * i], b = c[8 * half + 2 * i + 1];
+        w[i] = pack_bf16x2(a - (float)(__bf16)a, b - (float)(__bf16)b);
+    }
+    return {__builtin_bit_cast(bf16x8_t, w)};
+}
+
 // A kernel's walks over its tiles.  kMain.  kCareful, instead of it where its sums are not finite: values that are not finite are kept out
 // of the products, where 0 * inf would reach rows that do not see them, and added one by one to the rows that do.  kRest, bf16, after it:
 // what to_frag left of P and dx is added for rows with few keys -- the first ones of a sequence or of a document, short documents, narrow

@@ -164,3 +164,20 @@ def test_the_largest_caps(gpu, dtype, scale, softcap):
     for bad in ((0.125, 3e38), (0.125, 1.1e30), (1e-9, 1e30)):
         with pytest.raises(_lib.PicomoeError):
             _call(q, k, v, scale=bad[0], softcap=bad[1])
+
+
+@pytest.mark.parametrize("batch,q_len,kv_len,heads,kv_heads,D,options", [
+    (1, 1, 3000, 4, 4, 64, {}), (8, 1, 4096, 32, 8, 128, {}), (2, 1, 20000, 2, 1, 128, {"softcap": 20.0}), (1, 5, 1003, 8, 2, 64, {"window": 400}),
+    (3, 2, 777, 6, 2, 72, {"slopes": True}), (1, 1, 700, 8, 2, 256, {}), (2, 7, 900, 4, 1, 128, {"documents": 150}), (1, 32, 500, 1, 1, 128, {"causal": False})])
+def test_a_few_tokens_over_a_cache(gpu, batch, q_len, kv_len, heads, kv_heads, D, options):
+    """Up to 32 rows of a key head take P in two parts whatever their number of keys: sums to 2^-16 of the terms."""
+    (q, k, v), _ = _inputs(kv_len, batch, q_len, kv_len, heads, kv_heads, D)
+    options = dict(options)
+    if options.pop("slopes", False):
+        options["slopes"] = 2.0 ** (-8.0 * torch.arange(1, heads + 1, device="cuda") / heads)
+    if "documents" in options:
+        options["document_ids"] = (torch.arange(kv_len, device="cuda") // options.pop("documents")).int().expand(batch, -1).contiguous()
+    out = _call(q, k, v, **options)
+    value = O.attention(q.detach(), k.detach(), v.detach(), **options)["out"][0]
+    off = _sums(out) - value
+    assert off.norm() <= LEFT * value.norm(), float(off.norm() / value.norm())
