@@ -8,8 +8,10 @@
 //
 // The accumulated O is only rescaled when a row's maximum grows by more than 2^8: until then P is at most 2^8 instead of 1,
 // which costs bf16 nothing and fp32 sums nothing, and the 64 multiplications per tile fall away in all but the first tiles.
-// What P refers to is the maximum rounded up to a whole power of two, so that rescaling is exact and commutes with P's rounding to
-// bf16: the walk that adds what that rounding left (kRest) forms P against the last maximum, whichever a tile was rounded against.
+// In rows with few keys P refers to the maximum rounded up to a whole power of two, so that rescaling is exact and commutes with P's
+// rounding to bf16: the walk that adds what that rounding left (kRest) forms P against the last maximum, whichever a tile was rounded
+// against.  In other rows it refers to the maximum itself, and the P of a key that outweighs the others is 1, which is not rounded (whole
+// powers there: dq under a distance bias of 2 a key is off by 2.9 times its own rounding, so by 1.4).
 //
 // Bound: the issue of vector instructions.  A wavefront's MFMAs keep the matrix pipe busy for 48 % of the cycles; its softmax takes a
 // vector instruction of every SIMD for as long again, and an MFMA occupies the port that issues them for about half its own time.
@@ -130,7 +132,7 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
     const typename Tl::Lane ln;
     const ScoreScale sc = score_scale<MODE>(a);
     f32x16_t o[kCols];
-    float top = -INFINITY, total = 0.f;  // what P refers to (log2 units, whole), this lane's share of the sum
+    float top = -INFINITY, total = 0.f;  // what P refers to (log2 units), this lane's share of the sum
 
     Reach mine = w;  // the wavefront's rows, for kRest those with few keys
     int first_tile = 0, last_tile = -1;  // that the walk has met
@@ -231,7 +233,7 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
                 mx = other_max(mx) * (MODE == kPlain ? sc.mul : 1.f);
                 if (kWalk != kRest && __any(mx > top + kLazy)) {
                     const float old = top;
-                    top = __builtin_fmaxf(top, __builtin_ceilf(mx));
+                    top = __builtin_fmaxf(top, few ? __builtin_ceilf(mx) : mx);
                     const float shrink = __builtin_amdgcn_exp2f(old - (top == -INFINITY ? 0.f : top));
                     total *= shrink;
 #pragma unroll
@@ -249,7 +251,11 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
                     }
                 if constexpr (kWalk == kRest) {
 #pragma unroll
-                    for (int u = 0; u < kSub; ++u) take_rest(x[u]);
+                    for (int u = 0; u < kSub; ++u) {
+                        take_rest(x[u]);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) x[u][i] = few ? x[u][i] : 0.f;
+                    }
                 }
 #pragma unroll
                 for (int st = 0; st < 2 * kSub; ++st) {

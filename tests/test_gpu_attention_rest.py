@@ -181,3 +181,19 @@ def test_a_few_tokens_over_a_cache(gpu, batch, q_len, kv_len, heads, kv_heads, D
     value = O.attention(q.detach(), k.detach(), v.detach(), **options)["out"][0]
     off = _sums(out) - value
     assert off.norm() <= LEFT * value.norm(), float(off.norm() / value.norm())
+
+
+@pytest.mark.parametrize("slope", [0.5, 1.0, 2.0, 4.0])
+@pytest.mark.parametrize("D,S", [(64, 800), (128, 800), (256, 400)])
+def test_one_key_that_outweighs_many(gpu, slope, D, S):
+    """Steep distance biases: every row sees hundreds of keys and one or two have all the weight.  Its P is 1, which bf16 holds; dx of the others, of
+    the order of their P, must not carry the rounding of the large one through d_out . out.  Three roundings of 2^-9.3 are left, of the gradient, of
+    dx, and of the lesser P in d_out . out: sqrt(3) times the gradient's own."""
+    (q, k, v), g = _inputs(5, 2, S, S, 4, 2, D)
+    options = {"slopes": torch.full((4,), slope, device="cuda")}
+    out = _call(q, k, v, **options)
+    want = O.attention(q.detach(), k.detach(), v.detach(), d_out=g, **options)
+    for name, got in zip(("dq", "dk", "dv"), torch.autograd.grad(out, (q, k, v), g)):
+        value = want[name][0]
+        rounding = (value.to(BF16).double() - value).norm()
+        assert (got.double() - value).norm() <= 3 ** 0.5 * rounding, (name, float((got.double() - value).norm() / rounding))
