@@ -10,8 +10,9 @@
 // which costs bf16 nothing and fp32 sums nothing, and the 64 multiplications per tile fall away in all but the first tiles.
 // In rows with few keys P refers to the maximum rounded up to a whole power of two, so that rescaling is exact and commutes with P's
 // rounding to bf16: the walk that adds what that rounding left (kRest) forms P against the last maximum, whichever a tile was rounded
-// against.  In other rows it refers to the maximum itself, and the P of a key that outweighs the others is 1, which is not rounded (whole
-// powers there: dq under a distance bias of 2 a key is off by 2.9 times its own rounding, so by 1.4).
+// against.  Other rows are divided by the sum of P and of what rounding added to the largest one: where a key outweighs the others, its
+// rounding then shows neither in out nor in the backward's D, beside which the others' dP - D are small (a key of 2^7.8 times the weight of
+// another, in a later tile: dq off by 0.22 without this, by 0.003 with it).
 //
 // Bound: the issue of vector instructions.  A wavefront's MFMAs keep the matrix pipe busy for 48 % of the cycles; its softmax takes a
 // vector instruction of every SIMD for as long again, and an MFMA occupies the port that issues them for about half its own time.
@@ -133,14 +134,15 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
     const ScoreScale sc = score_scale<MODE>(a);
     f32x16_t o[kCols];
     float top = -INFINITY, total = 0.f;  // what P refers to (log2 units), this lane's share of the sum
+    float largest = -INFINITY, over = 0.f;  // the maximum, and what the rounding of its P to bf16 added to it
 
     Reach mine = w;  // the wavefront's rows, for kRest those with few keys
     int first_tile = 0, last_tile = -1;  // that the walk has met
     auto run = [&](auto which, auto active, int first, int end, Share share) __attribute__((always_inline)) {
         constexpr Walk kWalk = decltype(which)::value;
         if (kWalk != kRest) {
-            top = -INFINITY;
-            total = 0.f;
+            top = largest = -INFINITY;
+            total = over = 0.f;
 #pragma unroll
             for (int t = 0; t < kCols; ++t)
 #pragma unroll
@@ -230,18 +232,25 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
                 for (int u = 0; u < kSub; ++u)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) mx = __builtin_fmaxf(mx, x[u][i]);
-                mx = other_max(mx) * (MODE == kPlain ? sc.mul : 1.f);
+                const float raw_mx = other_max(mx);
+                mx = raw_mx * (MODE == kPlain ? sc.mul : 1.f);
                 if (kWalk != kRest && __any(mx > top + kLazy)) {
                     const float old = top;
                     top = __builtin_fmaxf(top, few ? __builtin_ceilf(mx) : mx);
                     const float shrink = __builtin_amdgcn_exp2f(old - (top == -INFINITY ? 0.f : top));
                     total *= shrink;
+                    over *= shrink;
 #pragma unroll
                     for (int t = 0; t < kCols; ++t)
 #pragma unroll
                         for (int i = 0; i < 16; ++i) o[t][i] *= shrink;
                 }
                 const float base = top == -INFINITY ? 0.f : top;
+                if (kRestWalk && kWalk != kRest && __any(mx > largest)) {
+                    const float p = __builtin_amdgcn_exp2f(MODE == kPlain ? __builtin_fmaf(raw_mx, sc.mul, -base) : raw_mx - base);
+                    over = mx > largest ? (float)(__bf16)p - p : over;
+                    largest = __builtin_fmaxf(largest, mx);
+                }
 #pragma unroll
                 for (int u = 0; u < kSub; ++u)
 #pragma unroll
@@ -359,7 +368,7 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
             }
     }
 
-    const float inv = total == 0.f ? 0.f : 1.f / total;
+    const float inv = total == 0.f ? 0.f : 1.f / (few ? total : total + over);
     const float lse2 = total == 0.f ? -INFINITY : (top == -INFINITY ? 0.f : top) + log2f(total);
     if (!row_in) return;
     if (share.parts > 1) {

@@ -197,3 +197,22 @@ def test_one_key_that_outweighs_many(gpu, slope, D, S):
         value = want[name][0]
         rounding = (value.to(BF16).double() - value).norm()
         assert (got.double() - value).norm() <= 3 ** 0.5 * rounding, (name, float((got.double() - value).norm() / rounding))
+
+
+@pytest.mark.parametrize("gap", [5.3, 6.6, 7.8])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_a_later_key_that_outweighs_another(gpu, gap, D):
+    """Two keys count, key 3 and, 2^gap times its weight, key 140, in a tile of its own; the others are 2^-20 of it.  dP - D of the heavy key is 2^-gap of
+    dP: its P's rounding may not reach D.  dx of the two is off by its own rounding and by that of the light key's P in D, dq by its rounding
+    besides: three times 2^-8 at most (the rows' scores are nearly the same, and so are their roundings)."""
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    S, late = 250, 140
+    q, k, v, g = (torch.randn(1, S, n, D, generator=gen, device="cuda") for n in (2, 1, 1, 2))
+    q, k = q * 0.02, k * 0.02
+    q[..., 0], k[..., 0], k[:, 3, :, 0], k[:, late, :, 0] = D ** 0.5 * 0.6931, -20.0, 0.0, gap
+    q, k, v = (t.to(BF16).requires_grad_(True) for t in (q, k, v))
+    g = torch.where((torch.arange(S, device="cuda") >= late)[None, :, None, None], g, torch.zeros((), device="cuda")).to(BF16)
+    want = O.attention(q.detach(), k.detach(), v.detach(), d_out=g)
+    (dq,) = torch.autograd.grad(_call(q, k, v), q, g)
+    value = want["dq"][0]
+    assert (dq.double() - value).norm() <= 3 * 2.0 ** -8 * value.norm(), float((dq.double() - value).norm() / value.norm())
