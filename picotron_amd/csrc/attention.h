@@ -5,7 +5,7 @@
 //   x[j] = scale q . k[j]      y[j] = softcap tanh(x[j] / softcap)  (softcap 0: y = x)      z[j] = y[j] - slope[h] |p - j|
 //   P[j] = exp(z[j]) / sum exp(z)          out = sum P[j] v[j]          lse = log sum exp(z)
 //
-// and a query that sees no key gets out = 0, lse = -inf.  Which keys: an interval [lo, hi] (causal: j <= p, or j < prefix length;
+// and a query that sees no key -- or has only scores of -inf -- gets out = 0, lse = -inf.  Which keys: an interval [lo, hi] (causal: j <= p, or j < prefix length;
 // window: |p - j| < window), and of those the ones of the query's document (equal ids, not negative).  A key outside takes no
 // part at all: NaN or infinity in its k or v (or in the q or d_out of a query that does not see the key) reaches nothing.
 //

@@ -216,3 +216,19 @@ def test_a_later_key_that_outweighs_another(gpu, gap, D):
     (dq,) = torch.autograd.grad(_call(q, k, v), q, g)
     value = want["dq"][0]
     assert (dq.double() - value).norm() <= 3 * 2.0 ** -8 * value.norm(), float((dq.double() - value).norm() / value.norm())
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+@pytest.mark.parametrize("q_len", [1, 40])
+def test_scores_of_minus_infinity_weigh_nothing(gpu, dtype, q_len):
+    """A key whose score is -inf has no weight; a query that has only such scores gets zeros, like one that sees no key."""
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    q, k, v = (torch.randn(1, n, h, 64, generator=gen, device="cuda").to(dtype) for n, h in ((q_len, 2), (200, 1), (200, 1)))
+    q[..., 0] = 1.0
+    k[:, 50:100, :, 0] = -torch.inf
+    got = _call(q, k, v, causal=False)
+    keep = torch.cat([torch.arange(50), torch.arange(100, 200)]).cuda()
+    value, bound = O.attention(q, k[:, keep], v[:, keep], causal=False)["out"]
+    assert ((got.double() - value).abs() <= bound).all()
+    k[..., 0] = -torch.inf
+    assert not _call(q, k, v, causal=False).any()
