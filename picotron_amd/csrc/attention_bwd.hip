@@ -51,12 +51,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void
     const float slope2 = a.slopes ? a.slopes[head] * kLog2e : 0.f;
     const int64_t out_row = ((int64_t)b * a.q_len + s) * a.heads + head;
 
-    const bool some = key_span >= 0, few = sizeof(T) == 2 && some && has_few(m, b, s, key_span);
+    const bool some = key_span >= 0;
     const Reach w = wave_reach(some, span);
-    int blk_few = __any(few);
-    __shared__ BlockReach reach, few_reach;
-    const Reach blk = block_reach(w, blk_few, reach);
-    if (blk_few) keep_reach(wave_reach(few, span), few_reach);
+    bool two_parts = sizeof(T) == 2 && __any(some && has_few(m, b, s, key_span));
+    const Reach blk = block_reach(w, two_parts);
     const int32_t* doc_min = a.docs ? m.key_docs.lowest + (int64_t)b * m.key_docs.tiles : nullptr;
     const int32_t* doc_max = a.docs ? m.key_docs.highest + (int64_t)b * m.key_docs.tiles : nullptr;
     const bool any = blk.hi_max >= blk.lo_min;
@@ -105,35 +103,30 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void
     const typename Tl::Lane ln;
     const ScoreScale sc = score_scale<MODE>(a);
     f32x16_t dq[kCols];
-    Reach mine = w;  // the wavefront's rows, for kRest those with few keys
-    int first_tile = 0, last_tile = -1;  // that the walk has met
-    auto run = [&](auto which, auto active, int first, int end, Share share) __attribute__((always_inline)) {
+    auto run = [&](auto which, auto parts) __attribute__((always_inline)) {
         constexpr Walk kWalk = decltype(which)::value;
-        if (kWalk != kRest) {
+        constexpr int kParts = decltype(parts)::value;
 #pragma unroll
-            for (int t = 0; t < kCols; ++t)
+        for (int t = 0; t < kCols; ++t)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) dq[t][i] = 0.f;
-        }
+            for (int i = 0; i < 16; ++i) dq[t][i] = 0.f;
         TileWalk<decltype(active)> walk(first, end, doc_min, doc_max, active, share.skip, share.left);
         WalkTile cur = walk.next();
-        if (kWalk != kRest && cur.t >= 0) first_tile = cur.t;
         int buf = 0;
         if (cur.t >= 0) fetch(cur.t, 0);
         while (cur.t >= 0) {
             lds_loads_done();
             __syncthreads();
             const WalkTile following = walk.next();
-            if (kWalk != kRest) last_tile = cur.t;
             if (following.t >= 0) fetch(following.t, buf ^ 1);
             const char* kt = lds + buf * Sh::kBuf;
             const char* vt = kt + Sh::kTileBytes;
             const int32_t* docs = (const int32_t*)(vt + Sh::kTileBytes);
             const uint32_t ka = lds_address(kt), va = ka + Sh::kTileBytes;
             const int key0 = cur.t * Sh::kTile, key1 = key0 + Sh::kTile - 1;
-            bool in = key0 <= mine.hi_max && key1 >= mine.lo_min, full = key0 >= w.lo_max && key1 <= w.hi_min;
+            bool in = key0 <= w.hi_max && key1 >= w.lo_min, full = key0 >= w.lo_max && key1 <= w.hi_min;
             if (a.docs) {
-                in = in && cur.doc_max >= mine.doc_min && cur.doc_min <= mine.doc_max;
+                in = in && cur.doc_max >= w.doc_min && cur.doc_min <= w.doc_max;
                 full = full && cur.doc_min == cur.doc_max && cur.doc_min == w.doc_min && cur.doc_min == w.doc_max;
             }
             if (in) {
@@ -187,18 +180,20 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void
                             }
                         }
                     }
-                    if constexpr (kWalk == kRest) take_rest(x);
 #pragma unroll
                     for (int st = 0; st < 2; ++st) {
                         const Frag<T> dx = to_frag<T>(x, st);
+                        Frag<T> rest;
+                        if constexpr (kParts == 2) rest = rest_frag<T>(x, st);
 #pragma unroll
                         for (int t = 0; t < kCols; ++t) {
                             Frag<T> k = Tl::frag_t(k_cols, u * 32 + 16 * st, t);
-                            if (kWalk != kMain) zero_not_finite(k);
+                            if (kWalk == kCareful) zero_not_finite(k);
                             mma(dq[t], k, dx);
+                            if constexpr (kParts == 2) mma(dq[t], k, rest);
                         }
                     }
-                    if (sizeof(T) == 2 && kWalk == kMain) read_ahead<2, 1, 2 * kCols, 3>();
+                    if (sizeof(T) == 2 && kWalk != kCareful) read_ahead<2, kParts, 2 * kCols, 3>();
                 }
                 if (kWalk == kCareful) {
                     bool bad = false;
@@ -220,25 +215,20 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void
             buf ^= 1;
         }
     };
-    run(std::integral_constant<Walk, kMain>(), active, first, end, share);
+    auto walk_all = [&](auto which) __attribute__((always_inline)) {
+        if constexpr (sizeof(T) == 2) {
+            if (two_parts) run(which, std::integral_constant<int, 2>());
+            else run(which, std::integral_constant<int, 1>());
+        } else {
+            run(which, std::integral_constant<int, 1>());
+        }
+    };
+    walk_all(std::integral_constant<Walk, kMain>());
     lds_loads_done();  // also where no tile was walked: nothing may land in LDS after the block is gone
     bool bad = false;
 #pragma unroll
     for (int t = 0; t < kCols; ++t) bad |= not_finite(dq[t]);
-    if (__syncthreads_or(bad)) {
-        run(std::integral_constant<Walk, kCareful>(), active, first, end, share);
-        __syncthreads();
-    }
-    if constexpr (sizeof(T) == 2) {
-        if (blk_few) {
-            mine = kept_reach(few_reach, wave, wave + 1);
-            // of the tiles walked those that the block's rows with few keys see
-            const Reach rest = kept_reach(few_reach, 0, kWaves);
-            auto seen = [&](int, int d0, int d1) { return !a.docs || (d1 >= rest.doc_min && d0 <= rest.doc_max); };
-            run(std::integral_constant<Walk, kRest>(), seen, max(first_tile, rest.lo_min / Sh::kTile), min(last_tile, rest.hi_max / Sh::kTile) + 1,
-                Share{1, 0, 0x7FFFFFFF});
-        }
-    }
+    if (__syncthreads_or(bad)) walk_all(std::integral_constant<Walk, kCareful>());
 
     if (!row_in) return;
     T* to = (T*)a.dq + out_row * a.D;
@@ -382,7 +372,6 @@ __global__ __launch_bounds__(kThreads, (DkvShape<T, DP, GRADS>::kWavesPerSimd)) 
     const typename Sh::VTl::Rows v_rows(vl, vtile + wave * 32 * Tl::kRowBytes);
     const ScoreScale sc = score_scale<MODE>(a);
     f32x16_t dk[kCols], dv[kCols];
-    int first_tile = 0, last_tile = -1;  // that the walk has met
     auto run = [&](auto which, auto active, int first, int end, Share share) __attribute__((always_inline)) {
         constexpr Walk kWalk = decltype(which)::value;
         if (kWalk != kRest) {
@@ -393,14 +382,12 @@ __global__ __launch_bounds__(kThreads, (DkvShape<T, DP, GRADS>::kWavesPerSimd)) 
         }
         TileWalk<decltype(active)> walk(first, end, doc_min, doc_max, active, share.skip, share.left);
         WalkTile cur = walk.next();
-        if (kWalk != kRest && cur.t >= 0) first_tile = cur.t;
         int buf = 0;
         if (cur.t >= 0) fetch(cur.t, 0);
         while (cur.t >= 0) {
             lds_loads_done();
             __syncthreads();
             const WalkTile following = walk.next();
-            if (kWalk != kRest) last_tile = cur.t;
             if (following.t >= 0) fetch(following.t, buf ^ 1);
             const char* qt = lds + buf * kBuf;
             const char* gt = qt + Sh::kTileBytes;
@@ -538,8 +525,9 @@ __global__ __launch_bounds__(kThreads, (DkvShape<T, DP, GRADS>::kWavesPerSimd)) 
     if constexpr (sizeof(T) == 2) {
         // Without documents and a narrow window only the first keys have such rows.  A query's interval grows with the query and, once its window
         // has left the first key behind, shrinks (at the last keys): the shortest of a tile is at one of its ends.  The parts of a cut walk take
-        // such tiles in turn, else the first part has all of them (2048 tokens: 106 us, in turn 97); with documents, where the tiles lie here
-        // and there, each those that it has met, else every part looks for them in all tiles (2 x 8192 tokens: 361 us, 331).
+        // such tiles in turn, else the first part has them all (2048 tokens: 106 us instead of 97); with documents, where the tiles lie here and
+        // there, each looks for them among its own, else in all tiles (2 x 8192 tokens in documents of 1024: 363 us instead of 335).  Where its own
+        // tiles begin and end is looked up again here: kept in registers through the first walk it costs that up to 4 %.
         if (a.docs || block0 < kFewKeys || (a.window > 0 && a.window < kFewKeys)) {
             auto keys_of = [&](int q) { return hi_of(q) - lo_of(q); };
             auto few = [&](int t, int d0, int d1) {
@@ -547,7 +535,14 @@ __global__ __launch_bounds__(kThreads, (DkvShape<T, DP, GRADS>::kWavesPerSimd)) 
                 const int q0 = first_query(t), q1 = last_query(t);
                 return m.few ? any_has_few(m, b, q0, q1) : min(keys_of(q0), keys_of(q1)) < kFewKeys - 1;
             };
-            run(std::integral_constant<Walk, kRest>(), few, a.docs ? first_tile : 0, a.docs ? last_tile + 1 : row_tiles, Share{1, 0, 0x7FFFFFFF});
+            int first = 0, end = row_tiles;
+            if (a.docs && share.parts > 1) {
+                TileWalk<decltype(active)> from(0, row_tiles, doc_min, doc_max, active, share.skip, 1);
+                first = max(0, from.next().t);
+                TileWalk<decltype(active)> to(first, row_tiles, doc_min, doc_max, active, share.left - 1, 1);
+                end = to.next().t + 1;
+            }
+            run(std::integral_constant<Walk, kRest>(), few, first, end, Share{1, 0, 0x7FFFFFFF});
         }
     }
 

@@ -8,10 +8,7 @@
 //
 // The accumulated O is only rescaled when a row's maximum grows by more than 2^8: until then P is at most 2^8 instead of 1,
 // which costs bf16 nothing and fp32 sums nothing, and the 64 multiplications per tile fall away in all but the first tiles.
-// In rows with few keys P refers to the maximum rounded up to a whole power of two, so that rescaling is exact and commutes with P's
-// rounding to bf16: the walk that adds what that rounding left (kRest) forms P against the last maximum, whichever a tile was rounded
-// against.  Other rows are divided by the sum of P and of what rounding added to the largest one: where a key outweighs the others, its
-// rounding then shows neither in out nor in the backward's D, beside which the others' dP - D are small (a key of 2^7.8 times the weight of
+// bf16: in blocks that hold rows with few keys, and in the form for few rows, P enters the products in two parts.  Other rows are divided by the sum of P and of what rounding added to the largest one: where a key outweighs the others, its rounding then shows neither in out nor in the backward's D, beside which the others' dP - D are small (a key of 2^7.8 times the weight of
 // another, in a later tile: dq off by 0.22 without this, by 0.003 with it).
 //
 // Bound: the issue of vector instructions.  A wavefront's MFMAs keep the matrix pipe busy for 47 % of the cycles; its softmax takes a
@@ -32,7 +29,7 @@ constexpr float kLazy = 8.f;
 
 // KEYS: the four waves share 32 rows and split every tile's keys among them (few rows: one new token); otherwise every wave
 // has 32 rows of its own and all of the tile's keys.  The first, which waits for K and V and not for its products, takes P of all rows
-// in two bf16 parts; the second only those of rows with few keys, in a second walk (kRest).
+// in two bf16 parts.
 template <typename T, int DP, bool KEYS>
 struct FwdShape {
     static constexpr int kTile = KEYS ? 32 * kWaves : (sizeof(T) == 2 ? 64 : 32);  // keys of a tile
@@ -68,7 +65,6 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
     typedef FwdShape<T, DP, KEYS> Sh;
     typedef typename Sh::Tl Tl;
     constexpr int kSub = Sh::kWaveKeys / 32, kSteps = DP / 16, kCols = DP / 32;
-    constexpr bool kTwoParts = sizeof(T) == 2 && KEYS, kRestWalk = sizeof(T) == 2 && !KEYS;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const AttnArgs& a = m.a;
     const int lane = threadIdx.x & 63, wave = wave_index(), hi = lane >> 5;
@@ -90,13 +86,10 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
 #pragma unroll
     for (int ks = 0; ks < kSteps; ++ks) qf[ks] = load_frag<T>(q, 16 * ks + 8 * hi, a.D);
 
-    const bool some = key_span >= 0, few = kRestWalk && some && has_few(m, b, s, key_span);
+    const bool some = key_span >= 0;
     const Reach w = wave_reach(some, span);
-    Reach blk = w;
-    int blk_few = __any(few);
-    __shared__ BlockReach reach, few_reach;
-    if (!KEYS) blk = block_reach(w, blk_few, reach);
-    if (blk_few) keep_reach(wave_reach(few, span), few_reach);
+    bool two_parts = sizeof(T) == 2 && !KEYS && __any(some && has_few(m, b, s, key_span));
+    const Reach blk = KEYS ? w : block_reach(w, two_parts);
     const int32_t* doc_min = a.docs ? m.key_docs.lowest + (int64_t)b * m.key_docs.tiles : nullptr;
     const int32_t* doc_max = a.docs ? m.key_docs.highest + (int64_t)b * m.key_docs.tiles : nullptr;
     const bool any = blk.hi_max >= blk.lo_min;
@@ -138,38 +131,34 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
     float top = -INFINITY, total = 0.f;  // what P refers to (log2 units), this lane's share of the sum
     float largest = -INFINITY, over = 0.f;  // the maximum, and what the rounding of its P to bf16 added to it
 
-    Reach mine = w;  // the wavefront's rows, for kRest those with few keys
-    int first_tile = 0, last_tile = -1;  // that the walk has met
-    auto run = [&](auto which, auto active, int first, int end, Share share) __attribute__((always_inline)) {
+    auto run = [&](auto which, auto parts) __attribute__((always_inline)) {
         constexpr Walk kWalk = decltype(which)::value;
-        if (kWalk != kRest) {
-            top = largest = -INFINITY;
-            total = over = 0.f;
+        constexpr int kParts = decltype(parts)::value;
+        constexpr bool kOneRounded = sizeof(T) == 2 && kParts == 1;
+        top = largest = -INFINITY;
+        total = over = 0.f;
 #pragma unroll
-            for (int t = 0; t < kCols; ++t)
+        for (int t = 0; t < kCols; ++t)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
-        }
+            for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
 
         TileWalk<decltype(active)> walk(first, end, doc_min, doc_max, active, share.skip, share.left);
         WalkTile cur = walk.next();
-        if (kWalk != kRest && cur.t >= 0) first_tile = cur.t;
         int buf = 0;
         if (cur.t >= 0) fetch(cur.t, 0);
         while (cur.t >= 0) {
             lds_loads_done();
             __syncthreads();  // the tile is there, and every wave is done with the other buffer
             const WalkTile following = walk.next();
-            if (kWalk != kRest) last_tile = cur.t;
             if (Sh::kBuffers == 2 && following.t >= 0) fetch(following.t, buf ^ 1);
             const char* kt = lds + buf * Sh::kBuf;
             const char* vt = kt + Sh::kTileBytes;
             const int32_t* docs = (const int32_t*)(vt + Sh::kTileBytes);
             const uint32_t ka = lds_address(kt) + (KEYS ? wave * 32 * Tl::kRowBytes : 0), va = ka + Sh::kTileBytes;
             const int sub0 = KEYS ? wave * 32 : 0, key0 = cur.t * Sh::kTile + sub0, key1 = key0 + Sh::kWaveKeys - 1;
-            bool in = key0 <= mine.hi_max && key1 >= mine.lo_min, full = key0 >= w.lo_max && key1 <= w.hi_min;
+            bool in = key0 <= w.hi_max && key1 >= w.lo_min, full = key0 >= w.lo_max && key1 <= w.hi_min;
             if (a.docs) {
-                in = in && cur.doc_max >= mine.doc_min && cur.doc_min <= mine.doc_max;
+                in = in && cur.doc_max >= w.doc_min && cur.doc_min <= w.doc_max;
                 full = full && cur.doc_min == cur.doc_max && cur.doc_min == w.doc_min && cur.doc_min == w.doc_max;
             }
             if (in) {
@@ -236,19 +225,19 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
                     for (int i = 0; i < 16; ++i) mx = __builtin_fmaxf(mx, x[u][i]);
                 const float raw_mx = other_max(mx);
                 mx = raw_mx * (MODE == kPlain ? sc.mul : 1.f);
-                if (kWalk != kRest && __any(mx > top + kLazy)) {
+                if (__any(mx > top + kLazy)) {
                     const float old = top;
-                    top = __builtin_fmaxf(top, few ? __builtin_ceilf(mx) : mx);
+                    top = __builtin_fmaxf(top, mx);
                     const float shrink = __builtin_amdgcn_exp2f(old - (top == -INFINITY ? 0.f : top));
                     total *= shrink;
-                    over *= shrink;
+                    if constexpr (kOneRounded) over *= shrink;
 #pragma unroll
                     for (int t = 0; t < kCols; ++t)
 #pragma unroll
                         for (int i = 0; i < 16; ++i) o[t][i] *= shrink;
                 }
                 const float base = top == -INFINITY ? 0.f : top;
-                if (kRestWalk && kWalk != kRest && __any(mx > largest)) {
+                if (kOneRounded && __any(mx > largest)) {
                     const float p = __builtin_amdgcn_exp2f(MODE == kPlain ? __builtin_fmaf(raw_mx, sc.mul, -base) : raw_mx - base);
                     over = mx > largest ? (float)(__bf16)p - p : over;
                     largest = __builtin_fmaxf(largest, mx);
@@ -258,30 +247,22 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         x[u][i] = __builtin_amdgcn_exp2f(MODE == kPlain ? __builtin_fmaf(x[u][i], sc.mul, -base) : x[u][i] - base);
-                        if (kWalk != kRest) total += x[u][i];
+                        total += x[u][i];
                     }
-                if constexpr (kWalk == kRest) {
-#pragma unroll
-                    for (int u = 0; u < kSub; ++u) {
-                        take_rest(x[u]);
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) x[u][i] = few ? x[u][i] : 0.f;
-                    }
-                }
 #pragma unroll
                 for (int st = 0; st < 2 * kSub; ++st) {
                     const Frag<T> p = to_frag<T>(x[st / 2], st & 1);
                     Frag<T> rest;
-                    if constexpr (kTwoParts) rest = rest_frag(x[st / 2], st & 1);
+                    if constexpr (kParts == 2) rest = rest_frag<T>(x[st / 2], st & 1);
 #pragma unroll
                     for (int t = 0; t < kCols; ++t) {
                         Frag<T> v = Tl::frag_t(v_cols, 16 * st, t);
-                        if (kWalk != kMain) zero_not_finite(v);
+                        if (kWalk == kCareful) zero_not_finite(v);
                         mma(o[t], v, p);
-                        if constexpr (kTwoParts) mma(o[t], v, rest);
+                        if constexpr (kParts == 2) mma(o[t], v, rest);
                     }
                 }
-                if (sizeof(T) == 2 && kWalk == kMain) read_ahead<2, kTwoParts ? 2 : 1, 2 * kSub * kCols, 2>();
+                if (sizeof(T) == 2 && kWalk != kCareful) read_ahead<2, kParts, 2 * kSub * kCols, 2>();
                 if (kWalk == kCareful) {
                     bool bad = false;
                     if (lane < Sh::kWaveKeys) bad = Tl::row_not_finite(vt, sub0 + lane);
@@ -307,25 +288,26 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
             }
         }
     };
-    run(std::integral_constant<Walk, kMain>(), active, first, end, share);
+    typedef std::integral_constant<int, 1> One;
+    typedef std::integral_constant<int, 2> Two;
+    auto walk_all = [&](auto which) __attribute__((always_inline)) {
+        if constexpr (sizeof(T) == 4) {
+            run(which, One());
+        } else if constexpr (KEYS) {
+            run(which, Two());
+        } else {
+            if (two_parts) run(which, Two());
+            else run(which, One());
+        }
+    };
+    walk_all(std::integral_constant<Walk, kMain>());
     lds_loads_done();  // also where no tile was walked: nothing may land in LDS after the block is gone
     bool bad = false;
 #pragma unroll
     for (int t = 0; t < kCols; ++t) bad |= not_finite(o[t]);
     if (__syncthreads_or(bad)) {
-        run(std::integral_constant<Walk, kCareful>(), active, first, end, share);
+        walk_all(std::integral_constant<Walk, kCareful>());
         __syncthreads();
-    }
-    if constexpr (kRestWalk) {
-        if (blk_few) {
-            mine = kept_reach(few_reach, wave, wave + 1);
-            // of the tiles walked those that the block's rows with few keys see
-            const Reach rest = kept_reach(few_reach, 0, kWaves);
-            auto seen = [&](int, int d0, int d1) { return !a.docs || (d1 >= rest.doc_min && d0 <= rest.doc_max); };
-            run(std::integral_constant<Walk, kRest>(), seen, max(first_tile, rest.lo_min / Sh::kTile), min(last_tile, rest.hi_max / Sh::kTile) + 1,
-                Share{1, 0, 0x7FFFFFFF});
-            __syncthreads();
-        }
     }
     total = other_sum(total);
 
@@ -370,7 +352,7 @@ __global__ __launch_bounds__(kThreads, (FwdShape<T, DP, KEYS>::kWavesPerSimd)) v
             }
     }
 
-    const float inv = total == 0.f ? 0.f : 1.f / (few ? total : total + over);
+    const float inv = total == 0.f ? 0.f : 1.f / (total + over);
     const float lse2 = total == 0.f ? -INFINITY : (top == -INFINITY ? 0.f : top) + log2f(total);
     if (!row_in) return;
     if (share.parts > 1) {

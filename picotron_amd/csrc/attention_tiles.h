@@ -67,7 +67,9 @@ __device__ __forceinline__ Frag<float> to_frag<float>(const f32x16_t& c, int hal
 }
 
 // what to_frag left of them, rounded to bf16 in turn: together they are off by 2^-16 of a term
-__device__ __forceinline__ Frag<__bf16> rest_frag(const f32x16_t& c, int half) {
+template <typename T>
+__device__ __forceinline__ Frag<T> rest_frag(const f32x16_t& c, int half) {
+    static_assert(sizeof(T) == 2);
     u32x4_t w;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -77,11 +79,11 @@ __device__ __forceinline__ Frag<__bf16> rest_frag(const f32x16_t& c, int half) {
     return {__builtin_bit_cast(bf16x8_t, w)};
 }
 
-// A kernel's walks over its tiles.  kMain.  kCareful, instead of it where its sums are not finite: values that are not finite are kept out
-// of the products, where 0 * inf would reach rows that do not see them, and added one by one to the rows that do.  kRest, bf16, after it:
-// what to_frag left of P and dx is added for rows with few keys -- the first ones of a sequence or of a document, short documents, narrow
-// windows --, over the tiles that such rows see.  6 batches of two tokens have dq to 0.0017 with it, 0.0034 without (the rounding of dq
-// itself: 0.0017).
+// A kernel's walk over its tiles.  kMain.  kCareful, instead of it where its sums are not finite: values that are not finite are kept out of the
+// products, where 0 * inf would reach rows that do not see them, and added one by one to the rows that do.  Both, in bf16, take P and dx in two
+// parts (to_frag and rest_frag) in blocks that hold rows with few keys -- the first ones of a sequence or of a document, short documents,
+// narrow windows --: 6 batches of two tokens have dq to 0.0017 with it, 0.0034 without (the rounding of dq itself: 0.0017).  dk / dv, whose
+// registers two parts would spill (650 and more), adds what to_frag left in a second walk over the tiles of such rows, kRest.
 enum Walk { kMain, kCareful, kRest };
 constexpr int kFewKeys = 128;
 __device__ __forceinline__ void take_rest(f32x16_t& c) {
@@ -516,32 +518,31 @@ __device__ __forceinline__ Reach wave_reach(bool in, const RowSpan& span) {
     return w;
 }
 // of all wavefronts of a block, lo_max and hi_min aside; and whether `flag` holds in one of them
-struct BlockReach {
-    int wave[kWaves][5];
-};
-__device__ __forceinline__ Reach block_reach(const Reach& w, int& flag, BlockReach& lds) {
+__device__ __forceinline__ Reach block_reach(const Reach& w, bool& flag) {
+    __shared__ int lds[kWaves][5];
     const int at = wave_index();
     if ((threadIdx.x & 63) == 0) {
-        lds.wave[at][0] = w.lo_min;
-        lds.wave[at][1] = w.hi_max;
-        lds.wave[at][2] = w.doc_min;
-        lds.wave[at][3] = w.doc_max;
-        lds.wave[at][4] = flag;
+        lds[at][0] = w.lo_min;
+        lds[at][1] = w.hi_max;
+        lds[at][2] = w.doc_min;
+        lds[at][3] = w.doc_max;
+        lds[at][4] = flag;
     }
     __syncthreads();
     Reach blk = w;
+    int any = 0;
     for (int i = 0; i < kWaves; ++i) {
-        blk.lo_min = min(blk.lo_min, lds.wave[i][0]);
-        blk.hi_max = max(blk.hi_max, lds.wave[i][1]);
-        blk.doc_min = min(blk.doc_min, lds.wave[i][2]);
-        blk.doc_max = max(blk.doc_max, lds.wave[i][3]);
-        flag |= lds.wave[i][4];
+        blk.lo_min = min(blk.lo_min, lds[i][0]);
+        blk.hi_max = max(blk.hi_max, lds[i][1]);
+        blk.doc_min = min(blk.doc_min, lds[i][2]);
+        blk.doc_max = max(blk.doc_max, lds[i][3]);
+        any |= lds[i][4];
     }
     blk.lo_min = __builtin_amdgcn_readfirstlane(blk.lo_min);
     blk.hi_max = __builtin_amdgcn_readfirstlane(blk.hi_max);
     blk.doc_min = __builtin_amdgcn_readfirstlane(blk.doc_min);
     blk.doc_max = __builtin_amdgcn_readfirstlane(blk.doc_max);
-    flag = __builtin_amdgcn_readfirstlane(flag);
+    flag = __builtin_amdgcn_readfirstlane(any) != 0;
     return blk;
 }
 
@@ -607,31 +608,6 @@ __device__ __forceinline__ void document_range(const int32_t* __restrict__ docs,
         lowest[(int64_t)b * tiles + tile] = lo;
         highest[(int64_t)b * tiles + tile] = hi;
     }
-}
-
-// The reach of the wavefronts' rows with few keys, kept in LDS until the second walk: the registers of the first one are full.
-__device__ __forceinline__ void keep_reach(const Reach& w, BlockReach& lds) {
-    const int at = wave_index();
-    if ((threadIdx.x & 63) == 0) {
-        lds.wave[at][0] = w.lo_min;
-        lds.wave[at][1] = w.hi_max;
-        lds.wave[at][2] = w.doc_min;
-        lds.wave[at][3] = w.doc_max;
-    }
-}
-__device__ __forceinline__ Reach kept_reach(const BlockReach& lds, int from, int to) {  // of wavefronts from .. to - 1
-    Reach r = {0x7FFFFFFF, 0, -1, 0, 0x7FFFFFFF, -1};
-    for (int i = from; i < to; ++i) {
-        r.lo_min = min(r.lo_min, lds.wave[i][0]);
-        r.hi_max = max(r.hi_max, lds.wave[i][1]);
-        r.doc_min = min(r.doc_min, lds.wave[i][2]);
-        r.doc_max = max(r.doc_max, lds.wave[i][3]);
-    }
-    r.lo_min = __builtin_amdgcn_readfirstlane(r.lo_min);
-    r.hi_max = __builtin_amdgcn_readfirstlane(r.hi_max);
-    r.doc_min = __builtin_amdgcn_readfirstlane(r.doc_min);
-    r.doc_max = __builtin_amdgcn_readfirstlane(r.doc_max);
-    return r;
 }
 
 // Which queries see fewer than kFewKeys keys where there are documents: without them the interval says it.  A wavefront looks at 64 queries and
