@@ -7,14 +7,14 @@
 // into parts (MfmaArgs) whose fp32 sums a last launch adds in order; a first one forms D = dO . out.  Both kinds of blocks in one
 // launch were slower (8.3 ms for what then took 4.7 + 2.3): the registers of the two spill more together.
 //
-// Bound: dq as the forward (MFMAs 55 % of the cycles).  dk / dv, which reads three LDS fragments for two MFMAs and has a tile of 32 rows
-// between barriers, is at 39 %; its loads, which mostly miss the L2, are not what holds it (walks from the last
+// Bound: dq as the forward (MFMAs 59 % of the cycles).  dk / dv, which reads three LDS fragments for two MFMAs and has a tile of 32 rows
+// between barriers, is at 40 %; its loads, which mostly miss the L2, are not what holds it (walks from the last
 // tile on, in step over an XCD's blocks so that they share them: -1.5 % at 16384 tokens, +4 % with documents).  Tiles of 64 rows with eight wavefronts
 // take 2 % less at 16384 tokens and 23 % more at 4096.
-// Measured, bf16, 16384 causal tokens, 16 over 4 heads of 128: prepare 0.03, dq 1.45 ms = 1135 TFLOP/s of its three products, dk / dv
-// 2.50 ms = 880 of its four, join 0.06; with softcap 1.78 and 3.11.  2048 tokens: 57 + 100 + 20 + 7 us.  2 x 8192 tokens, head_dim 64:
-// 0.41 and 0.85 ms.  fp32, 4096 tokens, 8 over 2 heads of 128: 0.58 and 0.83 ms = 89 and 83 TFLOP/s.  2 x 8192 tokens: documents of 1024
-// 0.18 and 0.35 ms, of 40 0.114 and 0.173 (0.081 and 0.125 without the second walk); 16384 tokens, window 64: 0.12 and 0.24 ms.
+// Measured, bf16, 16384 causal tokens, 16 over 4 heads of 128: prepare 0.03, dq 1.39 ms = 1190 TFLOP/s of its three products, dk / dv
+// 2.45 ms = 895 of its four, join 0.06; with softcap 1.69 and 3.10.  2048 tokens: 56 + 100 + 20 + 7 us.  2 x 8192 tokens, head_dim 64:
+// 0.40 and 0.86 ms.  fp32, 4096 tokens, 8 over 2 heads of 128: 0.60 and 0.82 ms = 86 and 83 TFLOP/s.  2 x 8192 tokens: documents of 1024
+// 0.18 and 0.35 ms, of 40 0.078 and 0.197 (dk / dv without its second walk: two thirds of that); 16384 tokens, window 64: 0.08 and 0.24 ms.
 #include "attention_tiles.h"
 
 namespace {
@@ -249,7 +249,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 128 ? 2 : 1) void
 // dk, dv
 // ---------------------------------------------------------------------------------------------------------------
 // What a launch of the kernel forms.  At head_dim 256 the 256 accumulation registers of a lane hold dk and dv and nothing else, S and dP
-// spill: one launch for each there, which forms S twice (five products instead of four; 8192 tokens, 8 heads over 4: 0.79 + 0.47 ms, together 2.7).
+// spill: one launch for each there, which forms S twice (five products instead of four; 8192 tokens, 8 heads over 4: 0.74 + 0.44 ms, together 2.7).
 enum Grads { kDk = 1, kDv = 2, kBoth = 3 };
 
 template <typename T, int DP, int GRADS>

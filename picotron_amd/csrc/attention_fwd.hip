@@ -8,17 +8,19 @@
 //
 // The accumulated O is only rescaled when a row's maximum grows by more than 2^8: until then P is at most 2^8 instead of 1,
 // which costs bf16 nothing and fp32 sums nothing, and the 64 multiplications per tile fall away in all but the first tiles.
-// bf16: in blocks that hold rows with few keys, and in the form for few rows, P enters the products in two parts.  Other rows are divided by the sum of P and of what rounding added to the largest one: where a key outweighs the others, its rounding then shows neither in out nor in the backward's D, beside which the others' dP - D are small (a key of 2^7.8 times the weight of
-// another, in a later tile: dq off by 0.22 without this, by 0.003 with it).
+// bf16: in blocks that hold rows with few keys, and in the form for few rows, P enters the products in two parts.  Other rows are divided by
+// the sum of P and of what rounding added to the largest one: where a key outweighs the others, its rounding then shows neither in out nor in
+// the backward's D, beside which the others' dP - D are small (a key of 2^7.8 times the weight of another, in a later tile: dq off by 0.22
+// without this, by 0.003 with it).
 //
-// Bound: the issue of vector instructions.  A wavefront's MFMAs keep the matrix pipe busy for 47 % of the cycles; its softmax takes a
+// Bound: the issue of vector instructions.  A wavefront's MFMAs keep the matrix pipe busy for 50 % of the cycles; its softmax takes a
 // vector instruction of every SIMD for as long again, and an MFMA occupies the port that issues them for about half its own time.
-// Measured, causal, 16 query over 4 key heads, bf16: 16384 tokens, head_dim 128: 1.08 ms = 1015 TFLOP/s (a library GEMM of 8192^3:
-// 1155), with softcap 1.37 ms; 2 x 8192 tokens, head_dim 64: 0.33 ms = 830; 8192 tokens, 8 over 4 heads of 256: 0.48 ms = 575 (512
-// registers, one wavefront per SIMD).  fp32, 4096 tokens, 8 over 2 heads of 128: 0.46 ms = 75 (GEMM: 153).  One new token for each of 8
-// sequences over 32768 keys, 32 over 8 heads: 0.217 ms = 5.0 TB/s of K and V (a copy: 4.9 read and written), + 7 us for the join; P in two
-// parts is 1 % of that.  2 x 8192 tokens: documents of 1024 0.160 ms, of 40, where every row has few keys, 0.113 (0.081 without the second
-// walk); 16384 tokens, window 64: 0.160 ms, window 1024: 0.213.
+// Measured, causal, 16 query over 4 key heads, bf16: 16384 tokens, head_dim 128: 1.05 ms = 1045 TFLOP/s (a library GEMM of 8192^3:
+// 1157), with softcap 1.33 ms; 2 x 8192 tokens, head_dim 64: 0.32 ms = 865; 8192 tokens, 8 over 4 heads of 256: 0.40 ms = 690 (512
+// registers, one wavefront per SIMD).  fp32, 4096 tokens, 8 over 2 heads of 128: 0.46 ms = 75 (GEMM: 154).  One new token for each of 8
+// sequences over 32768 keys, 32 over 8 heads: 0.210 ms = 5.1 TB/s of K and V (a copy: 4.9 read and written), + 7 us for the join; P in two
+// parts is 1 % of that.  2 x 8192 tokens: documents of 1024 0.154 ms, of 40, where every row has few keys, 0.081; 16384 tokens, window 64:
+// 0.135 ms, window 1024: 0.220.
 // Tried and slower: tiles of 128 keys; of 32 keys with three wavefronts per SIMD (1.32 ms); blocks of eight wavefronts; a higher
 // priority for the wavefront in its MFMAs (+7 %); the panel tiles of the backward (one token: 239 us).
 #include "attention_tiles.h"

@@ -614,7 +614,7 @@ __device__ __forceinline__ void document_range(const int32_t* __restrict__ docs,
 // counts the keys of their documents in their intervals, block by block of 64 from the queries' own positions to the front and then to the
 // back, until every query has enough, a block holds none of what those that lack some look for, or after kFewReach blocks.  Exact for
 // documents that lie in one piece; a query whose document goes on behind a gap, or is mixed with 8 and more others, may be taken to have
-// few, which costs a second walk and nothing else.  few_blocks(q_len) blocks per batch element.
+// few, which costs time and nothing else.  few_blocks(q_len) blocks per batch element.
 constexpr int kFewReach = 16;
 __host__ __device__ inline int few_words(int64_t q_len) { return (int)((q_len + 63) / 64); }
 __host__ __device__ inline int few_blocks(int64_t q_len) { return (few_words(q_len) + kWaves - 1) / kWaves; }

@@ -1,5 +1,5 @@
-"""bf16 attention, rows of fewer than 128 keys: what the rounding of P and dx to bf16 leaves is added by a second walk.  The forward keeps
-out and what out's own rounding left, so that its sums can be looked at to 2^-16."""
+"""bf16 attention, rows of fewer than 128 keys: P and dx enter the products in two parts, so that what their rounding to bf16 leaves is added.  The
+forward keeps out and what out's own rounding left, so that its sums can be looked at to 2^-16."""
 
 import pytest
 import torch
