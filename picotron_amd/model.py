@@ -80,9 +80,9 @@ class _Float32Tables:
 
     def on(self, device):
         if device not in self.copies:
-            with torch.device("cpu"):
-                tables = rope_tables(*self.key)
-            self.copies[device] = tuple(t.to(device) for t in tables)
+            # ordinary tensors, also where the first call that asks is one of inference: a later one trains with them
+            with torch.inference_mode(False), torch.device("cpu"):
+                self.copies[device] = tuple(t.to(device) for t in rope_tables(*self.key))
         return self.copies[device]
 
 
@@ -163,7 +163,8 @@ class Attention(nn.Module):
             # in the heads' type, which is another one under autocast
             weights, eps = (self.q_norm.weight.to(q.dtype), self.k_norm.weight.to(q.dtype)), self.q_norm.variance_epsilon
         if self.slopes is not None and self.slopes.device != x.device:
-            self.slopes = self.slopes.to(x.device)
+            with torch.inference_mode(False):   # as the tables
+                self.slopes = self.slopes.to(x.device)
         q, k = decoder_ops.qk_norm_rope(q, k, cos, sin, *weights, eps=eps, positions=position_ids)
         out = decoder_ops.attention(q, k, v, softcap=self.softcap, window=self.window, slopes=self.slopes, document_ids=document_ids,
                                     prefix_lengths=prefix_lengths)
@@ -242,7 +243,8 @@ class DecoderLayer(nn.Module):
 
     def _rope(self, x):
         if self.cos.device != x.device or self.cos.dtype != x.dtype:
-            self.cos, self.sin = self.cos.to(x.device, x.dtype), self.sin.to(x.device, x.dtype)
+            with torch.inference_mode(False):   # as _Float32Tables.on
+                self.cos, self.sin = self.cos.to(x.device, x.dtype), self.sin.to(x.device, x.dtype)
         S = x.shape[1]
         return self.cos[:S], self.sin[:S]
 

@@ -197,3 +197,18 @@ def test_no_layer_keeps_tables_that_it_does_not_read():
     del model, layers, layer, shared, a, b
     gc.collect()
     assert gone() is None
+
+
+def test_tables_of_a_first_call_under_inference_mode_can_be_trained_with():
+    from picotron_amd.model import Llama
+
+    config = types.SimpleNamespace(vocab_size=50, hidden_size=64, intermediate_size=32, num_attention_heads=4, num_key_value_heads=2, num_hidden_layers=1,
+                                   max_position_embeddings=40, rms_norm_eps=1e-5, rope_theta=54321.0)
+    layer = Llama(config).decoder_layers[0]
+    with torch.inference_mode():
+        cos, sin = layer._rope(torch.zeros(1, 7, 64, dtype=torch.bfloat16))
+        shared = layer.tables.on(torch.device("cpu"))
+    for t in (layer.cos, layer.sin, *shared):
+        assert not t.is_inference()
+        x = torch.ones(t.shape, requires_grad=True)
+        (x * t).sum().backward()

@@ -650,3 +650,15 @@ def test_head_norms_under_autocast(gpu):
         logits = model(torch.randint(0, 97, (2, 40), generator=_gen(3), device="cuda"))
     logits.float().sum().backward()
     assert all(p.grad is not None and p.grad.dtype == FP32 and torch.isfinite(p.grad).all() for p in leaves)
+
+
+def test_training_after_inference(gpu):
+    """A model whose first call ran under inference mode trains afterwards: what the layers keep from that call are ordinary tensors."""
+    for kw in ({}, dict(qk_norm=True, attention_bias="distance", embedding_scale=2.0)):
+        model = _model(_config(rope_theta=4321.0, num_experts=1, num_shared_experts=0, **kw), FP32)
+        ids = torch.randint(0, 97, (2, 20), generator=_gen(6), device="cuda")
+        with torch.inference_mode():
+            first = model(ids)
+        logits = model(ids)
+        logits.sum().backward()
+        assert torch.equal(logits, first) and all(p.grad is not None for p in model.parameters())
