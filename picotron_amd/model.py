@@ -248,21 +248,22 @@ class DecoderLayer(nn.Module):
         S = x.shape[1]
         return self.cos[:S], self.sin[:S]
 
-    def _attend(self, n, attention_mask, position_ids, document_ids, prefix_lengths):
+    def _attend(self, x, n, attention_mask, position_ids, document_ids, prefix_lengths):
+        """The attention of n, the norm of the layer's input x, whose type the plain path's tables are in."""
         if self.attention.fused or document_ids is not None or prefix_lengths is not None:
             cos, sin = self.tables.on(n.device)
             if self.cos.device != n.device:   # this layer's host copy goes
                 self.cos, self.sin = cos, sin
             return self.attention.forward_fused(n, cos, sin, position_ids, document_ids, prefix_lengths)
-        cos, sin = self._rope(n)
+        cos, sin = self._rope(x)
         return self.attention(n, cos, sin, attention_mask, position_ids)
 
     def forward(self, x, attention_mask=None, position_ids=None, document_ids=None, prefix_lengths=None):
         masks = (attention_mask, position_ids, document_ids, prefix_lengths)
         if self.parallel_block:
             n = self.input_layernorm(x)
-            return x + self._attend(n, *masks) + self.mlp(n)
-        x = x + self._attend(self.input_layernorm(x), *masks)
+            return x + self._attend(x, n, *masks) + self.mlp(n)
+        x = x + self._attend(x, self.input_layernorm(x), *masks)
         return x + self.mlp(self.post_attention_layernorm(x))
 
 

@@ -212,3 +212,18 @@ def test_tables_of_a_first_call_under_inference_mode_can_be_trained_with():
         assert not t.is_inference()
         x = torch.ones(t.shape, requires_grad=True)
         (x * t).sum().backward()
+
+
+@pytest.mark.parametrize("parallel", [False, True])
+def test_the_plain_paths_tables_are_in_the_type_of_the_layers_input(parallel):
+    """Norm weights kept in fp32 make the norm's output fp32; the rotation tables stay in the type of the hidden states."""
+    from picotron_amd.model import Llama
+
+    config = types.SimpleNamespace(vocab_size=50, hidden_size=64, intermediate_size=32, num_attention_heads=4, num_key_value_heads=2, num_hidden_layers=1,
+                                   max_position_embeddings=40, rms_norm_eps=1e-5, rope_theta=10000.0, parallel_block=parallel)
+    layer = Llama(config).decoder_layers[0]
+    seen = []
+    layer.attention.forward = lambda n, cos, sin, *rest: seen.append((n.dtype, cos.dtype, sin.dtype)) or torch.zeros_like(n)
+    layer.mlp.forward = torch.zeros_like
+    layer(torch.ones(1, 5, 64, dtype=torch.bfloat16))
+    assert seen == [(torch.float32, torch.bfloat16, torch.bfloat16)]
